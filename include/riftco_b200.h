@@ -304,6 +304,105 @@ B2_API int32_t b2_paged_decode_attention_noalloc(
     uint32_t head_width, uint32_t block_size, uint64_t physical_blocks, uint32_t max_blocks,
     uint32_t max_seq_len, uint32_t* status, void* stream);
 
+/* ---- 4-bit paged K/V cache ----------------------------------------------- */
+/*
+ * The paged cache above in 4.5 bits a value instead of 32, for keys and values
+ * alike, and the attention that reads it. The reference keeps its pages in FP32
+ * (src/core/backend/attention/contracts.hpp:88-106) and has neither.
+ *
+ * Format. One uint8 pool [physical_blocks, kv_heads, block_size / 16,
+ * 18 * head_width]; a tile holds 16 consecutive slots of one head: 9 * head_width
+ * bytes of keys, then as many of values, each
+ *   codes  [head_width / 32][16 slots][16 bytes], byte j of a row = channels 2j
+ *          (low nibble, as in the packed NF4 weights) and 2j + 1 of the 32
+ *   pairs  [16 slots][head_width / 64] of fp16 (scale, base)
+ * and value = base + scale * code, one pair for 64 channels of one token. A group
+ * x is stored, in FP32 with every operation rounded to nearest even, as
+ *   base = f16(min x)   scale = f16((max x - base) / 15)
+ *   code = clamp(rint((x - base) * (1 / scale)), 0, 15), 0 where scale is 0
+ * A group that holds a NaN, an infinity or a magnitude above 65000 is stored as
+ * scale = base = NaN (codes 0): it reads back as NaN, and attention over its
+ * keys reports B2_ATTN_STATUS_NAN_OR_POS_INF.
+ * head_width is 64, 128 or 256, block_size any multiple of 16.
+ */
+typedef struct b2_kv4_cache {
+    void* pages;                  /* the pool, 16-byte aligned                  */
+    const uint32_t* block_tables; /* [n_seq, max_blocks]                        */
+    uint64_t physical_blocks;
+    uint32_t n_seq, max_blocks, kv_heads, head_width, block_size;
+    uint32_t reserved;            /* must be 0                                  */
+} b2_kv4_cache;
+
+/* What is done to a score s = q . k / sqrt(head_width) before the softmax, in this
+ * order; a NULL pointer or zeros mean plain scores. position is the query's own.
+ *   softcap > 0:   s = softcap * tanh(s / softcap)
+ *   alibi_slopes:  s -= alibi_slopes[query head] * |position - t|   (device float[q_heads])
+ *   window > 0:    token t is seen only if t > position - window */
+typedef struct b2_kv4_score_rules {
+    float softcap;
+    uint32_t window;
+    const float* alibi_slopes;
+} b2_kv4_score_rules;
+
+/* b2_rope_append_kv(_tokens) into the 4-bit cache: rotates q and k at positions[t]
+ * (the same rotation; q_out may be q), and stores rotated k and v in slot
+ * positions[t] of sequence token_seq[t], or of sequence t where token_seq is NULL
+ * (n_tokens == n_seq then). q, q_out [n_tokens, q_heads, d], k, v [n_tokens, kv_heads, d],
+ * FP32, 16-byte aligned. A token with position 0xFFFFFFFF is padding: nothing of it
+ * is read or written. A position, sequence or block id outside the cache stores
+ * nothing (q is still rotated) and sets B2_ATTN_STATUS_BAD_BLOCK. The (sequence,
+ * position) pairs of one call must be distinct: of two tokens that share a slot,
+ * parts of either may be stored. */
+B2_API int32_t b2_rope_append_kv4(const b2_kv4_cache* cache, const float* q, float* q_out, const float* k,
+                                  const float* v, const uint32_t* positions, const uint32_t* token_seq,
+                                  uint32_t n_tokens, uint32_t q_heads, float theta, uint32_t* status,
+                                  void* stream);
+
+/* The stored keys and values of the same tokens, as FP32 [n_tokens, kv_heads, d]
+ * (base + scale * code with one rounding): the cache's counterpart of
+ * b2_nf4_dequantize. Padding tokens and ones outside the cache (flagged as above)
+ * leave their rows as they were. */
+B2_API int32_t b2_kv4_dequantize(const b2_kv4_cache* cache, const uint32_t* positions, const uint32_t* token_seq,
+                                 uint32_t n_tokens, float* k_out, float* v_out, uint32_t* status, void* stream);
+
+/* b2_paged_decode_attention over the 4-bit cache: one query token per sequence, at
+ * position seq_lens[s] - 1. q [n_seq, q_heads, d] FP32; ctx the same in FP32 and / or
+ * ctx_bf16 rounded from it (either may be NULL, not both); all 16-byte aligned.
+ * q_heads is any multiple of kv_heads. Scores, softmax statistics and sums are FP32,
+ * the products exact to 22 bits. A sequence of length 0 sees nothing and gets zeros.
+ * Errors go to the status word: NaN or +infinite scores, every score of a head
+ * -infinite (zeros), a block id outside the pool (its page is read as page 0), a
+ * length above max_seq_len (read up to max_seq_len; BAD_BLOCK).
+ * Workspace as for b2_paged_decode_attention: at least the bytes below (NULL: the
+ * library's arena), 16-byte aligned, not shared by calls that may overlap on the GPU. */
+B2_API size_t b2_paged_decode_kv4_workspace_bytes(uint32_t n_seq, uint32_t q_heads, uint32_t kv_heads,
+                                                  uint32_t head_width, uint32_t max_seq_len);
+B2_API int32_t b2_paged_decode_attention_kv4(const b2_kv4_cache* cache, const b2_kv4_score_rules* rules,
+                                             const float* q, const uint32_t* seq_lens, float* ctx, void* ctx_bf16,
+                                             uint32_t q_heads, uint32_t max_seq_len, void* workspace,
+                                             size_t workspace_bytes, uint32_t* status, void* stream);
+
+/* Several new query tokens per sequence (a prompt, a part of one, drafted tokens),
+ * already appended to the cache. Tokens chunk_starts[s] .. chunk_starts[s + 1] - 1
+ * of q [n_tokens, q_heads, d] are the LAST ones of sequence s, whose length with
+ * them is seq_lens[s]; chunk_starts is uint32[n_seq + 1], rising. The token at
+ * position p sees t < max(p + 1, prefix_lens[s]) (prefix_lens may be NULL: causal;
+ * a prefix is seen from anywhere in it, the window and the sequence's end still
+ * apply). max_chunk and max_seq_len bound the chunk lengths and seq_lens. The
+ * context is written in bf16, the form the output projection reads
+ * (b2_nf4_linear_forward_multi_bf16). Rows behind chunk_starts[n_seq] are left as
+ * they were; a chunk longer than its sequence is flagged BAD_BLOCK and the
+ * tokens that would lie before position 0 get zeros. Other errors and the
+ * workspace as above. */
+B2_API size_t b2_paged_chunk_kv4_workspace_bytes(uint32_t n_seq, uint32_t n_tokens, uint32_t q_heads,
+                                                 uint32_t kv_heads, uint32_t head_width, uint32_t max_chunk,
+                                                 uint32_t max_seq_len);
+B2_API int32_t b2_paged_chunk_attention_kv4(const b2_kv4_cache* cache, const b2_kv4_score_rules* rules,
+                                            const uint32_t* prefix_lens, const float* q, const uint32_t* seq_lens,
+                                            const uint32_t* chunk_starts, void* ctx_bf16, uint32_t n_tokens,
+                                            uint32_t q_heads, uint32_t max_chunk, uint32_t max_seq_len,
+                                            void* workspace, size_t workspace_bytes, uint32_t* status, void* stream);
+
 /* ---- decode-step glue ---------------------------------------------------- */
 /*
  * The small operators either side of the linears and the attention in one
@@ -431,6 +530,7 @@ B2_API int32_t b2_check_device_errors(void);
 #define B2_ROUTE_GENERIC 7          /* FP32 SIMT kernels, any shape */
 #define B2_ROUTE_ATTENTION_BULK 8   /* head_width 128, block_size 16, rep in {1,2,4,8} */
 #define B2_ROUTE_ATTENTION_GENERIC 9
+#define B2_ROUTE_ATTENTION_KV4 10   /* 4-bit cache, each query row on its own */
 B2_API int32_t b2_last_route(void);
 
 /* ---- host-buffer seam --------------------------------------------------- */

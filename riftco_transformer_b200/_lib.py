@@ -49,6 +49,32 @@ class Nf4WeightStruct(C.Structure):
     ]
 
 
+class Kv4CacheStruct(C.Structure):
+    """b2_kv4_cache."""
+
+    _fields_ = [
+        ("pages", C.c_void_p),
+        ("block_tables", C.c_void_p),
+        ("physical_blocks", C.c_uint64),
+        ("n_seq", C.c_uint32),
+        ("max_blocks", C.c_uint32),
+        ("kv_heads", C.c_uint32),
+        ("head_width", C.c_uint32),
+        ("block_size", C.c_uint32),
+        ("reserved", C.c_uint32),
+    ]
+
+
+class Kv4ScoreRulesStruct(C.Structure):
+    """b2_kv4_score_rules."""
+
+    _fields_ = [
+        ("softcap", C.c_float),
+        ("window", C.c_uint32),
+        ("alibi_slopes", C.c_void_p),
+    ]
+
+
 # name -> (restype, argtypes); every symbol the public header declares.
 _W = C.POINTER(Nf4WeightStruct)
 _vp, _u32, _u64, _sz, _i32 = C.c_void_p, C.c_uint32, C.c_uint64, C.c_size_t, C.c_int32
@@ -85,6 +111,13 @@ SIGNATURES = {
                                  C.c_float, _vp, _vp]),
     "b2_rope_append_kv_tokens": (_i32, [_vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _u32, _u32, _u32, _u32, _u32, _u64,
                                         _u32, C.c_float, _vp, _vp]),
+    "b2_rope_append_kv4": (_i32, [_vp, _vp, _vp, _vp, _vp, _vp, _vp, _u32, _u32, C.c_float, _vp, _vp]),
+    "b2_kv4_dequantize": (_i32, [_vp, _vp, _vp, _u32, _vp, _vp, _vp, _vp]),
+    "b2_paged_decode_kv4_workspace_bytes": (_sz, [_u32, _u32, _u32, _u32, _u32]),
+    "b2_paged_decode_attention_kv4": (_i32, [_vp, _vp, _vp, _vp, _vp, _vp, _u32, _u32, _vp, _sz, _vp, _vp]),
+    "b2_paged_chunk_kv4_workspace_bytes": (_sz, [_u32, _u32, _u32, _u32, _u32, _u32, _u32]),
+    "b2_paged_chunk_attention_kv4": (_i32, [_vp, _vp, _vp, _vp, _vp, _vp, _vp, _u32, _u32, _u32, _u32, _vp, _sz, _vp,
+                                            _vp]),
     "b2_silu_mul": (_i32, [_vp, _vp, _vp, _u64, _vp]),
     "b2_add": (_i32, [_vp, _vp, _vp, _u64, _vp]),
     "b2_gather_rows": (_i32, [_vp, _vp, _vp, _u32, _u32, _u32, _vp, _vp]),

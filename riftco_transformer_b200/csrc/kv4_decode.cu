@@ -1,0 +1,763 @@
+// Attention over the 4-bit paged cache, each query row on its own: the single-token decode step, and a
+// few new tokens of a sequence (kv4_chunk.cu takes over where there are enough to fill a tile of rows).
+//
+// For one row of head h, over the cached tokens t it sees:
+//   s_t = q . k_t / sqrt(d)      cap:  s = cap * tanh(s / cap)      bias:  s -= slope_h * |position - t|
+//   ctx = sum_t softmax(s)_t v_t
+// A code leaves its packed word as the fp16 number a = code - 8: one AND-OR makes 1024 + code (or 1024 +
+// 16 code of the next nibble) of two codes at once, one fp16 add (or multiply-add) takes the 1032 off, both
+// exact; nine instructions for eight codes. With value = base + scale * code = (base + 8 scale) + scale * a,
+// in groups of 64 channels, both products become products with numbers that a tensor core takes exactly:
+//   q . k_t     = sum_g scale_tg (sum_{c in g} q_c a_tc) + (base_tg + 8 scale_tg) (sum_{c in g} q_c)
+//   sum_t p_t v = sum_t (p_t scale_tg) a_tc + sum_t p_t (base_tg + 8 scale_tg)
+// so no value is ever rounded to 16 bits. Cheaper forms of a lose accuracy, because the tensor core cuts its
+// sums off instead of rounding them: fp16 subnormals (an AND alone, five instructions for eight) are aligned
+// to the nominal exponent and drop ten bits of the accumulator, 4e-5 off; 1 + code / 64 (seven) has an offset
+// whose cut-off part adds up over the tokens, 1.5e-4 off at 2049 tokens of zero mean. Centred, the
+// sums stay small and so does what is cut off. The other operand is an FP32 number (q, or p * scale) split into two fp16 parts,
+// 22 bits, that sit in adjacent columns of the eight of mma.m16n8k16 (up to four query heads: the second
+// part costs nothing) or in a second instruction (five to eight heads). Scores, softmax statistics and
+// accumulators are FP32, and the result agrees with FP32 arithmetic to about 1e-6.
+//
+// Bound by HBM: 9d/8 bytes per token and K/V head against 8d of the FP32 cache. mma.sync rather than
+// tcgen05: a row tile has at most 8 live rows, M = 64 or 128 would be idle lanes, and the operands come
+// from registers without a trip through shared or tensor memory.
+#include "kv4.cuh"
+#include "sm100_ptx.cuh"
+
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
+
+#include <cmath>
+
+namespace b2 {
+namespace {
+
+constexpr int kWarps = 4;
+constexpr int kSlots = 4;             // tiles in flight per warp
+constexpr float kLog2e = 1.4426950408889634f;
+constexpr float kNoMax = -FLT_MAX;    // running maximum before the first score (log2 units)
+constexpr float kSlack = 2.0f;        // p may reach 2^kSlack before the maximum is moved
+
+__device__ __forceinline__ float ex2(float x) {
+    float y;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+__device__ __forceinline__ void ldsm4(uint32_t (&r)[4], uint32_t addr) {
+    asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0,%1,%2,%3}, [%4];"
+                 : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
+                 : "r"(addr)
+                 : "memory");
+}
+__device__ __forceinline__ void ldsm4_trans(uint32_t (&r)[4], uint32_t addr) {
+    asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0,%1,%2,%3}, [%4];"
+                 : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
+                 : "r"(addr)
+                 : "memory");
+}
+__device__ __forceinline__ void mma16816(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3,
+                                         uint32_t b0, uint32_t b1) {
+    asm volatile(
+        "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+        : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+        : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+__device__ __forceinline__ uint32_t lds32(uint32_t addr) {
+    uint32_t v;
+    asm volatile("ld.shared.u32 %0, [%1];" : "=r"(v) : "r"(addr) : "memory");
+    return v;
+}
+// N consecutive words (N = 1, 2, 4 or 8), `addr` aligned to min(N, 4) words.
+template <int N>
+__device__ __forceinline__ void lds_words(uint32_t (&v)[N], uint32_t addr) {
+    if constexpr (N == 1) {
+        v[0] = lds32(addr);
+    } else if constexpr (N == 2) {
+        asm volatile("ld.shared.v2.u32 {%0,%1}, [%2];" : "=r"(v[0]), "=r"(v[1]) : "r"(addr) : "memory");
+    } else {
+#pragma unroll
+        for (int i = 0; i < N; i += 4) {
+            asm volatile("ld.shared.v4.u32 {%0,%1,%2,%3}, [%4];"
+                         : "=r"(v[i]), "=r"(v[i + 1]), "=r"(v[i + 2]), "=r"(v[i + 3])
+                         : "r"(addr + 4u * i)
+                         : "memory");
+        }
+    }
+}
+__device__ __forceinline__ float low_half(uint32_t pair) { return __low2float(*reinterpret_cast<__half2*>(&pair)); }
+__device__ __forceinline__ float high_half(uint32_t pair) { return __high2float(*reinterpret_cast<__half2*>(&pair)); }
+__device__ __forceinline__ uint32_t pack_half(float lo, float hi) {
+    const __half2 h = __floats2half2_rn(lo, hi);
+    return *reinterpret_cast<const uint32_t*>(&h);
+}
+// Two codes of a word, 16 bits apart, as fp16 numbers code - 8 (exact: 1024 + 16 * 15 fits 11 bits).
+template <int NIBBLE>
+__device__ __forceinline__ uint32_t codes_of(uint32_t word) {
+    constexpr uint32_t k1024 = 0x64006400u;
+    if (NIBBLE >= 2) word >>= 8;
+    if (NIBBLE % 2 == 0) {
+        uint32_t x = (word & 0x000F000Fu) | k1024;
+        const __half2 y = __hadd2(*reinterpret_cast<__half2*>(&x), __half2half2(__ushort_as_half(0xE408)));   // -1032
+        return *reinterpret_cast<const uint32_t*>(&y);
+    }
+    uint32_t x = (word & 0x00F000F0u) | k1024;
+    const __half2 y = __hfma2(*reinterpret_cast<__half2*>(&x), __half2half2(__ushort_as_half(0x2C00)),   // 1/16
+                              __half2half2(__ushort_as_half(0xD480)));                                    // -72
+    return *reinterpret_cast<const uint32_t*>(&y);
+}
+// The first 11 bits of x; x minus it is exact.
+__device__ __forceinline__ float first_part(float x) { return __uint_as_float(__float_as_uint(x) & 0xFFFFE000u); }
+
+__device__ __forceinline__ void bulk_load(uint32_t dst32, const void* src, uint32_t bytes, uint64_t* bar) {
+    asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];"
+                 ::"r"(dst32), "l"(src), "r"(bytes), "r"(sm100::smem_u32(bar))
+                 : "memory");
+}
+
+// What a row sees: tokens [begin, end) of sequence `seq`, its own position, and whether the caller's
+// lengths were out of bounds.
+struct RowSpan {
+    uint32_t seq, position, begin, end;
+    bool bad;
+    bool owned;   // false: a row behind the last sequence, which is left as it was
+};
+__device__ __forceinline__ RowSpan row_span(const Kv4AttentionArgs& a, uint32_t row) {
+    RowSpan r{row, 0, 0, 0, false, true};
+    uint32_t back = 0;   // tokens after this one
+    if (a.chunk_starts != nullptr) {
+        uint32_t lo = 0, hi = a.cache.n_seq;   // the last sequence that starts at or before `row`
+        while (lo + 1u < hi) {
+            const uint32_t mid = (lo + hi) / 2u;
+            if (__ldg(a.chunk_starts + mid) <= row) lo = mid; else hi = mid;
+        }
+        r.seq = lo;
+        const uint32_t first = __ldg(a.chunk_starts + lo), last = __ldg(a.chunk_starts + lo + 1u);
+        r.owned = row >= first && row < last;
+        if (!r.owned) return r;
+        back = last - 1u - row;
+    }
+    uint32_t len = __ldg(a.seq_lens + r.seq);
+    if (len > a.max_seq_len) {
+        len = a.max_seq_len;
+        r.bad = true;
+    }
+    if (back >= len) {
+        r.bad = r.bad || a.chunk_starts != nullptr;   // more new tokens than the sequence holds
+        return r;
+    }
+    r.position = len - 1u - back;
+    r.end = r.position + 1u;
+    if (a.rules.prefix_lens != nullptr) r.end = max(r.end, min(len, __ldg(a.rules.prefix_lens + r.seq)));
+    if (a.rules.window != 0u && r.position >= a.rules.window) r.begin = r.position - a.rules.window + 1u;
+    return r;
+}
+
+struct SplitPlan {
+    uint32_t splits;          // most splits of a row
+    uint32_t tiles_per_split;
+};
+
+template <int D, int HC>   // HC: query heads of one K/V head worked on together (4 or 8)
+__global__ void __launch_bounds__(kWarps * 32)
+kv4_decode_kernel(const Kv4AttentionArgs a, float* __restrict__ partials, const SplitPlan plan) {
+    using namespace sm100;
+    pdl_launch_dependents();
+    constexpr int G = D / 64, kChunks = D / 32;
+    constexpr int HL = HC / 4;            // heads of a lane in the score layout
+    constexpr uint32_t kTileBytes = kv4_tile_bytes(D);
+    constexpr float kWTop = 8192.0f;      // p * scale likewise: p <= 4 keeps it below 65504
+
+    const uint32_t rep = a.q_heads / a.cache.kv_heads;
+    const uint32_t head_chunks = (rep + HC - 1u) / HC;
+    uint32_t block = blockIdx.x;
+    const uint32_t split = block % plan.splits;
+    block /= plan.splits;
+    const uint32_t chunk = block % head_chunks;
+    block /= head_chunks;
+    const uint32_t kvh = block % a.cache.kv_heads;
+    const uint32_t row = block / a.cache.kv_heads;
+
+    const RowSpan span = row_span(a, row);
+    const uint32_t tile0 = span.begin / kKv4Tile;
+    const uint32_t tiles = span.end > span.begin ? (span.end - 1u) / kKv4Tile + 1u - tile0 : 0u;
+    const uint32_t n_splits = max(1u, (tiles + plan.tiles_per_split - 1u) / plan.tiles_per_split);
+    if (split >= n_splits || !span.owned) return;
+
+    extern __shared__ __align__(128) uint8_t ring_raw[];
+    __shared__ __align__(8) uint64_t bars[kWarps][kSlots];
+    __shared__ uint32_t s_abort;
+    __shared__ float s_m[kWarps][HC], s_l[kWarps][HC];
+
+    const uint32_t lane = threadIdx.x & 31u, warp = threadIdx.x >> 5;
+    const uint32_t g = lane >> 2, t = lane & 3u;
+    const uint32_t first_head = kvh * rep + chunk * HC;
+    const uint32_t live_heads = min(static_cast<uint32_t>(HC), rep - chunk * HC);
+    volatile uint32_t* abort = &s_abort;
+    uint32_t flags = span.bad ? B2_ATTN_STATUS_BAD_BLOCK : 0u;
+
+    if (threadIdx.x == 0) s_abort = 0;
+    if (lane == 0) {
+        for (int i = 0; i < kSlots; ++i) mbar_init(&bars[warp][i], 1);
+        mbar_fence_init();
+    }
+    __syncthreads();
+
+    const uint32_t ring32 = smem_u32(ring_raw) + warp * (kSlots * kTileBytes);
+    const uint32_t my_first = tile0 + split * plan.tiles_per_split + warp;
+    const uint32_t my_end = tile0 + min(tiles, (split + 1u) * plan.tiles_per_split);
+    const uint32_t my_tiles = my_first < my_end ? (my_end - my_first + kWarps - 1u) / kWarps : 0u;
+    const uint32_t* table = a.cache.block_tables + static_cast<uint64_t>(span.seq) * a.cache.max_blocks;
+
+    // Byte offsets of the warp's next 32 tiles, one per lane.
+    uint64_t tile_offset = 0;
+    auto look_up = [&](uint32_t i0) {
+        const uint32_t i = i0 + lane;
+        if (i < my_tiles) {
+            const uint32_t tile = my_first + i * kWarps;
+            uint64_t phys = __ldg(table + tile / a.cache.tiles_per_block);
+            if (phys >= a.cache.physical_blocks) {
+                phys = 0;
+                flags |= B2_ATTN_STATUS_BAD_BLOCK;
+            }
+            tile_offset = kv4_tile_offset(a.cache, phys, kvh, tile % a.cache.tiles_per_block);
+        }
+    };
+    auto issue = [&](uint32_t i) {   // the whole warp: tile i of its list into slot i % kSlots
+        if ((i & 31u) == 0u) look_up(i);
+        const uint64_t offset = __shfl_sync(0xFFFFFFFFu, tile_offset, i & 31u);
+        if (lane == 0) {
+            fence_proxy_async_smem();
+            mbar_expect_tx(&bars[warp][i % kSlots], kTileBytes);
+            bulk_load(ring32 + (i % kSlots) * kTileBytes, a.cache.pages + offset, kTileBytes, &bars[warp][i % kSlots]);
+        }
+    };
+    for (uint32_t i = 0; i < kSlots && i < my_tiles; ++i) issue(i);
+
+    // ---- q: scaled by a power of two, split into two fp16 parts, in the order the codes come out ----
+    // Column n of the products is head n/2, part n%2 (HC = 4), or head n with the parts in two
+    // instructions (HC = 8). A chunk of 32 channels takes two k16 steps; in step u the lane's four k
+    // positions are channels 8t + 2u, 8t + 2u + 4, then 8t + 2u + 1, 8t + 2u + 5.
+    const uint32_t col_head = HC == 4 ? g >> 1 : g;
+    const bool col_live = col_head < live_heads;
+    const float* qp = a.q + (static_cast<uint64_t>(row) * a.q_heads + first_head + (col_live ? col_head : 0u)) * D;
+    uint32_t qf[kChunks][2][2][HL];   // [chunk][step][register][part, HC = 8]
+    float q_unscale;                  // of column head
+    float q_sum[G];
+    {
+        float x[kChunks][8];
+        float top = 0.0f;
+#pragma unroll
+        for (int j = 0; j < kChunks; ++j) {
+            const float4 u0 = __ldg(reinterpret_cast<const float4*>(qp + 32 * j + 8 * t));
+            const float4 u1 = __ldg(reinterpret_cast<const float4*>(qp + 32 * j + 8 * t + 4));
+            x[j][0] = u0.x; x[j][1] = u0.y; x[j][2] = u0.z; x[j][3] = u0.w;
+            x[j][4] = u1.x; x[j][5] = u1.y; x[j][6] = u1.z; x[j][7] = u1.w;
+#pragma unroll
+            for (int e = 0; e < 8; ++e) {
+                if (!col_live) x[j][e] = 0.0f;
+                top = fmaxf(top, fabsf(x[j][e]));
+            }
+        }
+        top = fmaxf(top, __shfl_xor_sync(0xFFFFFFFFu, top, 1));
+        top = fmaxf(top, __shfl_xor_sync(0xFFFFFFFFu, top, 2));
+        // 2^e with top * 2^e in [2^13, 2^14); a head of zeros or beyond 2^113 keeps a bounded factor
+        int e = 13 - (static_cast<int>((__float_as_uint(top) >> 23) & 255u) - 127);
+        e = max(-100, min(100, e));
+        const float up = __uint_as_float(static_cast<uint32_t>(e + 127) << 23);
+        q_unscale = __uint_as_float(static_cast<uint32_t>(127 - e) << 23);
+#pragma unroll
+        for (int gr = 0; gr < G; ++gr) {
+            float s = 0.0f;
+#pragma unroll
+            for (int j = 2 * gr; j < 2 * gr + 2; ++j)
+#pragma unroll
+                for (int c = 0; c < 8; ++c) s += x[j][c];
+            s += __shfl_xor_sync(0xFFFFFFFFu, s, 1);
+            s += __shfl_xor_sync(0xFFFFFFFFu, s, 2);
+            q_sum[gr] = s;
+        }
+        const bool second = HC == 4 && (g & 1u) != 0u;
+#pragma unroll
+        for (int j = 0; j < kChunks; ++j)
+#pragma unroll
+            for (int u = 0; u < 2; ++u)
+#pragma unroll
+                for (int w = 0; w < 2; ++w) {
+                    const float v0 = x[j][2 * u + w] * up, v1 = x[j][2 * u + w + 4] * up;
+                    const float h0 = first_part(v0), h1 = first_part(v1);
+                    if (HC == 4) {
+                        qf[j][u][w][0] = second ? pack_half(v0 - h0, v1 - h1) : pack_half(h0, h1);
+                    } else {
+                        qf[j][u][w][0] = pack_half(h0, h1);
+                        qf[j][u][w][HL - 1] = pack_half(v0 - h0, v1 - h1);
+                    }
+                }
+    }
+    // Score layout: a lane holds tokens g and g + 8 of heads t (HC = 4) or 2t, 2t + 1 (HC = 8).
+    const float inv_sqrt = 1.0f / sqrtf(static_cast<float>(D));
+    float code_factor[HL];   // 1 / q's power of two / sqrt(d)
+    float base_factor[HL][G];
+    float slope[HL];
+#pragma unroll
+    for (int h = 0; h < HL; ++h) {
+        const int src = HC == 4 ? static_cast<int>(t) * 8 : static_cast<int>(2 * t + h) * 4;   // lane of column head
+        code_factor[h] = __shfl_sync(0xFFFFFFFFu, q_unscale, src) * inv_sqrt;
+#pragma unroll
+        for (int gr = 0; gr < G; ++gr) base_factor[h][gr] = __shfl_sync(0xFFFFFFFFu, q_sum[gr], src) * inv_sqrt;
+        const uint32_t head = HC == 4 ? t : 2 * t + h;
+        slope[h] = a.rules.alibi_slopes != nullptr && head < live_heads ? __ldg(a.rules.alibi_slopes + first_head + head) : 0.0f;
+    }
+
+    float m[HL], l[HL], base_acc[HL][G];
+    float acc[kChunks][2][4];
+#pragma unroll
+    for (int h = 0; h < HL; ++h) {
+        m[h] = kNoMax;
+        l[h] = 0.0f;
+#pragma unroll
+        for (int gr = 0; gr < G; ++gr) base_acc[h][gr] = 0.0f;
+    }
+#pragma unroll
+    for (int j = 0; j < kChunks; ++j)
+#pragma unroll
+        for (int u = 0; u < 2; ++u)
+#pragma unroll
+            for (int c = 0; c < 4; ++c) acc[j][u][c] = 0.0f;
+    // p * scale is brought to fp16's range by a power of two over the largest value scale met so far.
+    float scale_top = 0.0f;      // power of two at or above it (0: none yet)
+    float weight_factor = 0.0f;  // kWTop / scale_top
+
+    for (uint32_t i = 0; i < my_tiles; ++i) {
+        const uint32_t token0 = (my_first + i * kWarps) * kKv4Tile;
+        const uint32_t slot32 = ring32 + (i % kSlots) * kTileBytes;
+        mbar_wait(&bars[warp][i % kSlots], (i / kSlots) & 1u, abort);
+
+        // ---- scores ----
+        float s[2][HL];   // [token g, g + 8]
+        {
+            float total[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+            uint32_t kp0[G], kp1[G];
+            float k_base0[G], k_base1[G];
+            lds_words<G>(kp0, slot32 + 8u * D + g * (4u * G));
+            lds_words<G>(kp1, slot32 + 8u * D + (g + 8u) * (4u * G));
+#pragma unroll
+            for (int gr = 0; gr < G; ++gr) {
+                uint32_t r[4];   // chunk 2gr: tokens g, g + 8; chunk 2gr + 1: the same
+                ldsm4(r, slot32 + gr * 512u + lane * 16u);
+                float c[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+                for (int j = 0; j < 2; ++j)
+#pragma unroll
+                    for (int u = 0; u < 2; ++u) {
+                        const uint32_t a0 = u == 0 ? codes_of<0>(r[2 * j]) : codes_of<2>(r[2 * j]);
+                        const uint32_t a1 = u == 0 ? codes_of<0>(r[2 * j + 1]) : codes_of<2>(r[2 * j + 1]);
+                        const uint32_t a2 = u == 0 ? codes_of<1>(r[2 * j]) : codes_of<3>(r[2 * j]);
+                        const uint32_t a3 = u == 0 ? codes_of<1>(r[2 * j + 1]) : codes_of<3>(r[2 * j + 1]);
+#pragma unroll
+                        for (int part = 0; part < HL; ++part) {
+                            mma16816(c, a0, a1, a2, a3, qf[2 * gr + j][u][0][part], qf[2 * gr + j][u][1][part]);
+                        }
+                    }
+                const float s0 = low_half(kp0[gr]), s1 = low_half(kp1[gr]);
+                k_base0[gr] = fmaf(8.0f, s0, high_half(kp0[gr]));
+                k_base1[gr] = fmaf(8.0f, s1, high_half(kp1[gr]));
+                total[0] = fmaf(s0, c[0], total[0]);
+                total[1] = fmaf(s0, c[1], total[1]);
+                total[2] = fmaf(s1, c[2], total[2]);
+                total[3] = fmaf(s1, c[3], total[3]);
+            }
+#pragma unroll
+            for (int h = 0; h < HL; ++h) {
+                // HC = 4: columns 2t, 2t + 1 are the two parts of head t; HC = 8: two heads
+                s[0][h] = HC == 4 ? total[0] + total[1] : total[h];
+                s[1][h] = HC == 4 ? total[2] + total[3] : total[2 + h];
+                s[0][h] *= code_factor[h];
+                s[1][h] *= code_factor[h];
+#pragma unroll
+                for (int gr = 0; gr < G; ++gr) {
+                    s[0][h] = fmaf(k_base0[gr], base_factor[h][gr], s[0][h]);
+                    s[1][h] = fmaf(k_base1[gr], base_factor[h][gr], s[1][h]);
+                }
+            }
+        }
+        bool seen[2];
+#pragma unroll
+        for (int k = 0; k < 2; ++k) {
+            const uint32_t token = token0 + g + 8u * k;
+            seen[k] = token >= span.begin && token < span.end;
+#pragma unroll
+            for (int h = 0; h < HL; ++h) {
+                float x = s[k][h];
+                if (a.rules.softcap != 0.0f) x = a.rules.softcap * tanhf(x / a.rules.softcap);
+                if (a.rules.alibi_slopes != nullptr) {
+                    const uint32_t far = span.position >= token ? span.position - token : token - span.position;
+                    x = fmaf(-slope[h], static_cast<float>(far), x);
+                }
+                const uint32_t head = HC == 4 ? t : 2 * t + h;
+                if (seen[k] && !(x < INFINITY) && head < live_heads) flags |= B2_ATTN_STATUS_NAN_OR_POS_INF;
+                s[k][h] = seen[k] ? x * kLog2e : -INFINITY;   // log2 units from here
+            }
+        }
+
+        // ---- maximum: moved only when a score passes it by kSlack, or a value scale its bound ----
+        const uint32_t v32 = slot32 + kv4_half_bytes(D);
+        uint32_t vq0[G], vq1[G];   // pairs of tokens g, g + 8
+        lds_words<G>(vq0, v32 + 8u * D + g * (4u * G));
+        lds_words<G>(vq1, v32 + 8u * D + (g + 8u) * (4u * G));
+        float scale_max;   // over the tokens the row sees: other slots may hold anything
+        {
+            __half2 top0 = *reinterpret_cast<__half2*>(&vq0[0]), top1 = *reinterpret_cast<__half2*>(&vq1[0]);
+#pragma unroll
+            for (int gr = 1; gr < G; ++gr) {
+                top0 = __hmax2(top0, *reinterpret_cast<__half2*>(&vq0[gr]));
+                top1 = __hmax2(top1, *reinterpret_cast<__half2*>(&vq1[gr]));
+            }
+            scale_max = fmaxf(seen[0] ? __low2float(top0) : 0.0f, seen[1] ? __low2float(top1) : 0.0f);
+        }
+        bool move = scale_max > scale_top;
+#pragma unroll
+        for (int h = 0; h < HL; ++h) move = move || fmaxf(s[0][h], s[1][h]) > m[h] + kSlack;
+        if (__any_sync(0xFFFFFFFFu, move)) {
+            scale_max = fmaxf(scale_max, __shfl_xor_sync(0xFFFFFFFFu, scale_max, 4));
+            scale_max = fmaxf(scale_max, __shfl_xor_sync(0xFFFFFFFFu, scale_max, 8));
+            scale_max = fmaxf(scale_max, __shfl_xor_sync(0xFFFFFFFFu, scale_max, 16));
+            float shrink = 1.0f;
+            if (scale_max > scale_top) {
+                // the power of two at or above scale_max (fp16, so at least 2^-24 and at most 2^14)
+                const float top = __uint_as_float((__float_as_uint(scale_max) + 0x007FFFFFu) & 0x7F800000u);
+                shrink = scale_top / top;   // both powers of two; 0 the first time
+                scale_top = top;
+                weight_factor = kWTop / top;
+            }
+            float factor[HL];
+#pragma unroll
+            for (int h = 0; h < HL; ++h) {
+                float top = fmaxf(m[h], fmaxf(s[0][h], s[1][h]));
+                top = fmaxf(top, __shfl_xor_sync(0xFFFFFFFFu, top, 4));
+                top = fmaxf(top, __shfl_xor_sync(0xFFFFFFFFu, top, 8));
+                top = fmaxf(top, __shfl_xor_sync(0xFFFFFFFFu, top, 16));
+                factor[h] = ex2(m[h] - top);
+                m[h] = top;
+                l[h] *= factor[h];
+#pragma unroll
+                for (int gr = 0; gr < G; ++gr) base_acc[h][gr] *= factor[h];
+            }
+            // accumulator columns 2t, 2t + 1 belong to the same heads as this lane's scores
+#pragma unroll
+            for (int j = 0; j < kChunks; ++j)
+#pragma unroll
+                for (int u = 0; u < 2; ++u)
+#pragma unroll
+                    for (int c = 0; c < 4; ++c) acc[j][u][c] *= factor[(c & 1) * (HL - 1)] * shrink;
+        }
+
+        // ---- weights ----
+        float p[2][HL];
+#pragma unroll
+        for (int h = 0; h < HL; ++h) {
+            p[0][h] = ex2(s[0][h] - m[h]);
+            p[1][h] = ex2(s[1][h] - m[h]);
+            l[h] += p[0][h] + p[1][h];
+        }
+#pragma unroll
+        for (int gr = 0; gr < G; ++gr) {
+            const float b0 = seen[0] ? fmaf(8.0f, low_half(vq0[gr]), high_half(vq0[gr])) : 0.0f;
+            const float b1 = seen[1] ? fmaf(8.0f, low_half(vq1[gr]), high_half(vq1[gr])) : 0.0f;
+#pragma unroll
+            for (int h = 0; h < HL; ++h) {
+                base_acc[h][gr] = fmaf(p[0][h], b0, base_acc[h][gr]);
+                base_acc[h][gr] = fmaf(p[1][h], b1, base_acc[h][gr]);
+            }
+        }
+        // To the layout of the second product's B operand: column g, tokens 2t, 2t + 1, 2t + 8, 2t + 9.
+        float w[4];
+        {
+            const int src0 = static_cast<int>(2 * t) * 4 + static_cast<int>(g >> 1), src1 = src0 + 4;
+#pragma unroll
+            for (int k = 0; k < 2; ++k) {
+                float a0 = __shfl_sync(0xFFFFFFFFu, p[k][0], src0), a1 = __shfl_sync(0xFFFFFFFFu, p[k][0], src1);
+                if (HC == 8) {   // heads 2t, 2t + 1 of the source lane: the odd columns take the second
+                    const float o0 = __shfl_sync(0xFFFFFFFFu, p[k][HL - 1], src0);
+                    const float o1 = __shfl_sync(0xFFFFFFFFu, p[k][HL - 1], src1);
+                    if (g & 1u) {
+                        a0 = o0;
+                        a1 = o1;
+                    }
+                }
+                w[2 * k] = a0 * weight_factor;
+                w[2 * k + 1] = a1 * weight_factor;
+            }
+        }
+        // ---- values ----
+        uint32_t vp_low[2 * G], vp_high[2 * G];   // pairs of tokens 2t, 2t + 1 and 2t + 8, 2t + 9
+        lds_words<2 * G>(vp_low, v32 + 8u * D + (2u * t) * (4u * G));
+        lds_words<2 * G>(vp_high, v32 + 8u * D + (2u * t + 8u) * (4u * G));
+#pragma unroll
+        for (int gr = 0; gr < G; ++gr) {
+            uint32_t b[2][HL];   // [register][part, HC = 8]
+#pragma unroll
+            for (int k = 0; k < 2; ++k) {
+                const uint32_t p0 = k == 0 ? vp_low[gr] : vp_high[gr], p1 = k == 0 ? vp_low[G + gr] : vp_high[G + gr];
+                // a weight of zero may be an unseen slot's, which may hold anything, NaN included
+                const float w0 = w[2 * k] != 0.0f ? w[2 * k] * low_half(p0) : 0.0f;
+                const float w1 = w[2 * k + 1] != 0.0f ? w[2 * k + 1] * low_half(p1) : 0.0f;
+                const float h0 = first_part(w0), h1 = first_part(w1);
+                if (HC == 4) {
+                    b[k][0] = (g & 1u) ? pack_half(w0 - h0, w1 - h1) : pack_half(h0, h1);
+                } else {
+                    b[k][0] = pack_half(h0, h1);
+                    b[k][HL - 1] = pack_half(w0 - h0, w1 - h1);
+                }
+            }
+            uint32_t r[4];   // chunk 2gr: tokens (2t, 2t+1), (2t+8, 2t+9); chunk 2gr + 1: the same
+            ldsm4_trans(r, v32 + gr * 512u + lane * 16u);
+#pragma unroll
+            for (int j = 0; j < 2; ++j)
+#pragma unroll
+                for (int u = 0; u < 2; ++u) {
+                    // rows g and g + 8 are channels 4g + 2u and 4g + 2u + 1 of the chunk
+                    const uint32_t a0 = u == 0 ? codes_of<0>(r[2 * j]) : codes_of<2>(r[2 * j]);
+                    const uint32_t a1 = u == 0 ? codes_of<1>(r[2 * j]) : codes_of<3>(r[2 * j]);
+                    const uint32_t a2 = u == 0 ? codes_of<0>(r[2 * j + 1]) : codes_of<2>(r[2 * j + 1]);
+                    const uint32_t a3 = u == 0 ? codes_of<1>(r[2 * j + 1]) : codes_of<3>(r[2 * j + 1]);
+#pragma unroll
+                    for (int part = 0; part < HL; ++part) {
+                        mma16816(acc[2 * gr + j][u], a0, a1, a2, a3, b[0][part], b[1][part]);
+                    }
+                }
+        }
+        __syncwarp();   // every lane has read the slot
+        if (i + kSlots < my_tiles) issue(i + kSlots);
+    }
+
+    // ---- join the warps (the ring is free: it holds their accumulators) ----
+    if (lane == 0 && *abort != 0) flags |= B2_ATTN_STATUS_TIMEOUT;
+    if (flags != 0u) kv4_flag(a.status, flags);
+    __syncthreads();
+    float* s_acc = reinterpret_cast<float*>(ring_raw);   // [warp][HC][D]
+    const float undo = scale_top / kWTop;
+#pragma unroll
+    for (int h = 0; h < HL; ++h) {
+        l[h] += __shfl_xor_sync(0xFFFFFFFFu, l[h], 4);
+        l[h] += __shfl_xor_sync(0xFFFFFFFFu, l[h], 8);
+        l[h] += __shfl_xor_sync(0xFFFFFFFFu, l[h], 16);
+        const uint32_t head = HC == 4 ? t : 2 * t + h;
+        if (g == 0) {
+            s_m[warp][head] = m[h];
+            s_l[warp][head] = l[h];
+        }
+#pragma unroll
+        for (int gr = 0; gr < G; ++gr) {
+            float b = base_acc[h][gr];
+            b += __shfl_xor_sync(0xFFFFFFFFu, b, 4);
+            b += __shfl_xor_sync(0xFFFFFFFFu, b, 8);
+            b += __shfl_xor_sync(0xFFFFFFFFu, b, 16);
+#pragma unroll
+            for (int j = 2 * gr; j < 2 * gr + 2; ++j) {
+                float o[4];   // channels 32j + 4g + 0..3
+#pragma unroll
+                for (int u = 0; u < 2; ++u) {
+                    const float even = HC == 4 ? acc[j][u][0] + acc[j][u][1] : acc[j][u][h];
+                    const float odd = HC == 4 ? acc[j][u][2] + acc[j][u][3] : acc[j][u][2 + h];
+                    o[2 * u] = fmaf(even, undo, b);
+                    o[2 * u + 1] = fmaf(odd, undo, b);
+                }
+                *reinterpret_cast<float4*>(&s_acc[(warp * HC + head) * D + 32 * j + 4 * g]) =
+                    make_float4(o[0], o[1], o[2], o[3]);
+            }
+        }
+    }
+    __syncthreads();
+    for (uint32_t i = threadIdx.x; i < live_heads * (D / 4u); i += kWarps * 32u) {
+        const uint32_t head = i / (D / 4u), c = (i % (D / 4u)) * 4u;
+        float mm = s_m[0][head];
+#pragma unroll
+        for (int wv = 1; wv < kWarps; ++wv) mm = fmaxf(mm, s_m[wv][head]);
+        float ll = 0.0f;
+        float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+        for (int wv = 0; wv < kWarps; ++wv) {
+            const float f = ex2(s_m[wv][head] - mm);
+            const float4 x = *reinterpret_cast<const float4*>(&s_acc[(wv * HC + head) * D + c]);
+            ll = fmaf(s_l[wv][head], f, ll);
+            o.x = fmaf(x.x, f, o.x);
+            o.y = fmaf(x.y, f, o.y);
+            o.z = fmaf(x.z, f, o.z);
+            o.w = fmaf(x.w, f, o.w);
+        }
+        const uint64_t out_head = static_cast<uint64_t>(row) * a.q_heads + first_head + head;
+        if (n_splits > 1u) {
+            float* dst = partials + (out_head * plan.splits + split) * (D + 4u);
+            *reinterpret_cast<float4*>(dst + 4u + c) = o;
+            if (c == 0) {
+                dst[0] = mm;
+                dst[1] = ll;
+            }
+            continue;
+        }
+        if (ll == 0.0f) {   // nothing seen, or every score -infinity
+            if (tiles != 0u && c == 0) kv4_flag(a.status, B2_ATTN_STATUS_ALL_NEG_INF);
+            o = make_float4(0.f, 0.f, 0.f, 0.f);
+            ll = 1.0f;
+        }
+        o = make_float4(o.x / ll, o.y / ll, o.z / ll, o.w / ll);
+        if (a.ctx != nullptr) *reinterpret_cast<float4*>(a.ctx + out_head * D + c) = o;
+        if (a.ctx16 != nullptr) {
+            const __nv_bfloat162 lo = __floats2bfloat162_rn(o.x, o.y), hi = __floats2bfloat162_rn(o.z, o.w);
+            uint2 packed;
+            packed.x = *reinterpret_cast<const uint32_t*>(&lo);
+            packed.y = *reinterpret_cast<const uint32_t*>(&hi);
+            *reinterpret_cast<uint2*>(static_cast<__nv_bfloat16*>(a.ctx16) + out_head * D + c) = packed;
+        }
+    }
+}
+
+// Joins the splits of every (row, query head) that has more than one.
+template <int D>
+__global__ void __launch_bounds__(D / 4)
+kv4_merge_kernel(const Kv4AttentionArgs a, const float* __restrict__ partials, const SplitPlan plan) {
+    sm100::pdl_launch_dependents();
+    const uint64_t out_head = blockIdx.x;
+    const uint32_t row = static_cast<uint32_t>(out_head / a.q_heads);
+    const RowSpan span = row_span(a, row);   // inputs of the call, not of the kernel before
+    const uint32_t tile0 = span.begin / kKv4Tile;
+    const uint32_t tiles = span.end > span.begin ? (span.end - 1u) / kKv4Tile + 1u - tile0 : 0u;
+    const uint32_t n_splits = max(1u, (tiles + plan.tiles_per_split - 1u) / plan.tiles_per_split);
+    sm100::pdl_wait();   // every CTA waits, so that this grid never ends before the one it follows
+    if (n_splits <= 1u || !span.owned) return;
+    const float* src = partials + out_head * plan.splits * (D + 4u);
+    const uint32_t c = threadIdx.x * 4u;
+    float mm = kNoMax, ll = 0.0f;
+    float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
+    for (uint32_t s0 = 0; s0 < n_splits; s0 += 8u) {
+        float2 ml[8];
+        float4 x[8];
+#pragma unroll
+        for (uint32_t u = 0; u < 8u; ++u) {   // all loads before the first use
+            const bool live = s0 + u < n_splits;
+            const float* part = src + (s0 + u) * (D + 4u);
+            ml[u] = live ? *reinterpret_cast<const float2*>(part) : make_float2(kNoMax, 0.0f);
+            x[u] = live ? *reinterpret_cast<const float4*>(part + 4u + c) : make_float4(0.f, 0.f, 0.f, 0.f);
+        }
+        float top = mm;
+#pragma unroll
+        for (uint32_t u = 0; u < 8u; ++u) top = fmaxf(top, ml[u].x);
+        const float keep = ex2(mm - top);
+        mm = top;
+        ll *= keep;
+        o = make_float4(o.x * keep, o.y * keep, o.z * keep, o.w * keep);
+#pragma unroll
+        for (uint32_t u = 0; u < 8u; ++u) {   // in split order
+            const float f = ex2(ml[u].x - mm);
+            ll = fmaf(ml[u].y, f, ll);
+            o.x = fmaf(x[u].x, f, o.x);
+            o.y = fmaf(x[u].y, f, o.y);
+            o.z = fmaf(x[u].z, f, o.z);
+            o.w = fmaf(x[u].w, f, o.w);
+        }
+    }
+    if (ll == 0.0f) {
+        if (c == 0) kv4_flag(a.status, B2_ATTN_STATUS_ALL_NEG_INF);
+        o = make_float4(0.f, 0.f, 0.f, 0.f);
+        ll = 1.0f;
+    }
+    o = make_float4(o.x / ll, o.y / ll, o.z / ll, o.w / ll);
+    if (a.ctx != nullptr) *reinterpret_cast<float4*>(a.ctx + out_head * D + c) = o;
+    if (a.ctx16 != nullptr) {
+        const __nv_bfloat162 lo = __floats2bfloat162_rn(o.x, o.y), hi = __floats2bfloat162_rn(o.z, o.w);
+        uint2 packed;
+        packed.x = *reinterpret_cast<const uint32_t*>(&lo);
+        packed.y = *reinterpret_cast<const uint32_t*>(&hi);
+        *reinterpret_cast<uint2*>(static_cast<__nv_bfloat16*>(a.ctx16) + out_head * D + c) = packed;
+    }
+}
+
+uint32_t heads_together(uint32_t rep) { return rep <= 4u ? 4u : 8u; }
+
+// Tiles of one CTA. Split finer while the card is not filled (four CTAs for every SM), but never below
+// 16 tiles: a CTA's own set-up and the join cost about as much as four tiles a warp.
+SplitPlan split_plan(int sm_count, uint64_t rows, uint32_t q_heads, uint32_t kv_heads, uint32_t max_seq_len) {
+    const uint32_t rep = q_heads / kv_heads;
+    const uint64_t sms = sm_count > 0 ? static_cast<uint64_t>(sm_count) : 148u;
+    const uint64_t lists = rows * kv_heads * ((rep + heads_together(rep) - 1u) / heads_together(rep));
+    const uint64_t tiles = (static_cast<uint64_t>(max_seq_len) + kKv4Tile - 1u) / kKv4Tile;
+    const uint64_t wanted = 4u * sms;   // CTAs
+    uint64_t per = tiles;
+    if (lists < wanted) per = (tiles * lists + wanted - 1u) / wanted;
+    if (per < 16u) per = 16u;
+    if (per > 128u) per = 128u;
+    return SplitPlan{static_cast<uint32_t>((tiles + per - 1u) / per), static_cast<uint32_t>(per)};
+}
+
+template <int D, int HC>
+int32_t launch_one(const DeviceContext& ctx, const Kv4AttentionArgs& a, float* partials, const SplitPlan& plan,
+                   unsigned blocks, cudaStream_t stream) {
+    constexpr int kRing = kWarps * kSlots * static_cast<int>(kv4_tile_bytes(D));
+    static PerDeviceOnce configured;
+    B2_TRY(once_per_device(configured, ctx.device, []() -> int32_t {
+        B2_CUDA_TRY(cudaFuncSetAttribute(kv4_decode_kernel<D, HC>, cudaFuncAttributeMaxDynamicSharedMemorySize, kRing));
+        return B2_STATUS_OK;
+    }));
+    kv4_decode_kernel<D, HC><<<blocks, kWarps * 32, kRing, stream>>>(a, partials, plan);
+    B2_CUDA_TRY(cudaGetLastError());
+    return B2_STATUS_OK;
+}
+
+template <int D>
+int32_t launch_merge(const Kv4AttentionArgs& a, const float* partials, const SplitPlan& plan, cudaStream_t stream) {
+    cudaLaunchConfig_t config{};
+    config.gridDim = dim3(static_cast<unsigned>(static_cast<uint64_t>(a.rows) * a.q_heads));
+    config.blockDim = dim3(D / 4);
+    config.stream = stream;
+    cudaLaunchAttribute attribute[1];
+    attribute[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attribute[0].val.programmaticStreamSerializationAllowed = 1;
+    config.attrs = attribute;
+    config.numAttrs = 1;
+    B2_CUDA_TRY(cudaLaunchKernelEx(&config, kv4_merge_kernel<D>, a, partials, plan));
+    return B2_STATUS_OK;
+}
+
+}  // namespace
+
+size_t kv4_decode_workspace_bytes(int sm_count, uint64_t rows, uint32_t q_heads, uint32_t kv_heads, uint32_t head_width,
+                                  uint32_t max_seq_len) {
+    const SplitPlan plan = split_plan(sm_count, rows, q_heads, kv_heads, max_seq_len);
+    if (plan.splits <= 1u) return 0;
+    return static_cast<size_t>(rows) * q_heads * plan.splits * (head_width + 4u) * sizeof(float);
+}
+
+int32_t launch_kv4_decode(const DeviceContext& ctx, const Kv4AttentionArgs& a, void* workspace, size_t workspace_bytes,
+                          cudaStream_t stream) {
+    const size_t need = kv4_decode_workspace_bytes(ctx.sm_count, a.rows, a.q_heads, a.cache.kv_heads,
+                                                   a.cache.head_width, a.max_seq_len);
+    if (need > workspace_bytes) {
+        return fail(B2_STATUS_INVALID_ARGUMENT, "paged attention workspace too small: need %zu bytes, got %zu", need,
+                    workspace_bytes);
+    }
+    const SplitPlan plan = split_plan(ctx.sm_count, a.rows, a.q_heads, a.cache.kv_heads, a.max_seq_len);
+    const uint32_t rep = a.q_heads / a.cache.kv_heads, together = heads_together(rep);
+    const uint64_t blocks = static_cast<uint64_t>(a.rows) * a.cache.kv_heads * ((rep + together - 1u) / together) *
+                            plan.splits;
+    const uint64_t merges = static_cast<uint64_t>(a.rows) * a.q_heads;
+    if (blocks > 0x7FFFFFFFull || merges > 0x7FFFFFFFull) return fail(B2_STATUS_OVERFLOW, "paged attention batch too large");
+    float* partials = static_cast<float*>(workspace);
+    const unsigned n = static_cast<unsigned>(blocks);
+    switch (a.cache.head_width) {
+    case 64:
+        B2_TRY(together == 4u ? (launch_one<64, 4>(ctx, a, partials, plan, n, stream))
+                              : (launch_one<64, 8>(ctx, a, partials, plan, n, stream)));
+        return plan.splits > 1u ? launch_merge<64>(a, partials, plan, stream) : B2_STATUS_OK;
+    case 128:
+        B2_TRY(together == 4u ? (launch_one<128, 4>(ctx, a, partials, plan, n, stream))
+                              : (launch_one<128, 8>(ctx, a, partials, plan, n, stream)));
+        return plan.splits > 1u ? launch_merge<128>(a, partials, plan, stream) : B2_STATUS_OK;
+    default:
+        B2_TRY(together == 4u ? (launch_one<256, 4>(ctx, a, partials, plan, n, stream))
+                              : (launch_one<256, 8>(ctx, a, partials, plan, n, stream)));
+        return plan.splits > 1u ? launch_merge<256>(a, partials, plan, stream) : B2_STATUS_OK;
+    }
+}
+
+}  // namespace b2
