@@ -34,7 +34,9 @@ namespace b2 {
 namespace {
 
 constexpr int kWarps = 4;
-constexpr int kSlots = 4;             // tiles in flight per warp
+constexpr int kPair = 2;              // tiles a warp works on at once: 32 tokens, one for each lane to guard
+// Pairs a warp holds in shared memory, one being worked on and the rest in flight.
+__host__ __device__ constexpr int slots_of(int d) { return d == 64 ? 4 : 2; }
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kNoMax = -FLT_MAX;    // running maximum before the first score (log2 units)
 constexpr float kSlack = 2.0f;        // p may reach 2^kSlack before the maximum is moved
@@ -62,6 +64,9 @@ __device__ __forceinline__ void mma16816(float (&c)[4], uint32_t a0, uint32_t a1
         "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
         : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
         : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+__device__ __forceinline__ void sts32(uint32_t addr, uint32_t v) {
+    asm volatile("st.shared.u32 [%0], %1;" ::"r"(addr), "r"(v) : "memory");
 }
 __device__ __forceinline__ uint32_t lds32(uint32_t addr) {
     uint32_t v;
@@ -185,6 +190,8 @@ kv4_decode_kernel(const Kv4AttentionArgs a, float* __restrict__ partials, const 
     if (split >= n_splits || !span.owned) return;
 
     extern __shared__ __align__(128) uint8_t ring_raw[];
+    constexpr int kSlots = slots_of(D);
+    constexpr uint32_t kPairBytes = kPair * kTileBytes;
     __shared__ __align__(8) uint64_t bars[kWarps][kSlots];
     __shared__ uint32_t s_abort;
     __shared__ float s_m[kWarps][HC], s_l[kWarps][HC];
@@ -203,18 +210,18 @@ kv4_decode_kernel(const Kv4AttentionArgs a, float* __restrict__ partials, const 
     }
     __syncthreads();
 
-    const uint32_t ring32 = smem_u32(ring_raw) + warp * (kSlots * kTileBytes);
-    const uint32_t my_first = tile0 + split * plan.tiles_per_split + warp;
-    const uint32_t my_end = tile0 + min(tiles, (split + 1u) * plan.tiles_per_split);
-    const uint32_t my_tiles = my_first < my_end ? (my_end - my_first + kWarps - 1u) / kWarps : 0u;
+    const uint32_t ring32 = smem_u32(ring_raw) + warp * (kSlots * kPairBytes);
+    const uint32_t my_first = tile0 + split * plan.tiles_per_split + warp * kPair;
+    const uint32_t tile_end = tile0 + min(tiles, (split + 1u) * plan.tiles_per_split);
+    constexpr uint32_t kStride = kWarps * kPair;
+    const uint32_t my_pairs = my_first < tile_end ? (tile_end - my_first + kStride - 1u) / kStride : 0u;
     const uint32_t* table = a.cache.block_tables + static_cast<uint64_t>(span.seq) * a.cache.max_blocks;
 
-    // Byte offsets of the warp's next 32 tiles, one per lane.
+    // Byte offsets of the tiles of the warp's next 16 pairs, one per lane.
     uint64_t tile_offset = 0;
     auto look_up = [&](uint32_t i0) {
-        const uint32_t i = i0 + lane;
-        if (i < my_tiles) {
-            const uint32_t tile = my_first + i * kWarps;
+        const uint32_t tile = my_first + (i0 + lane / kPair) * kStride + lane % kPair;
+        if (tile < tile_end) {
             uint64_t phys = __ldg(table + tile / a.cache.tiles_per_block);
             if (phys >= a.cache.physical_blocks) {
                 phys = 0;
@@ -223,16 +230,23 @@ kv4_decode_kernel(const Kv4AttentionArgs a, float* __restrict__ partials, const 
             tile_offset = kv4_tile_offset(a.cache, phys, kvh, tile % a.cache.tiles_per_block);
         }
     };
-    auto issue = [&](uint32_t i) {   // the whole warp: tile i of its list into slot i % kSlots
-        if ((i & 31u) == 0u) look_up(i);
-        const uint64_t offset = __shfl_sync(0xFFFFFFFFu, tile_offset, i & 31u);
-        if (lane == 0) {
+    // The whole warp: pair i of its list into slot i % kSlots (lanes 2(i % 16) and the next hold its offsets).
+    auto issue = [&](uint32_t i) {
+        if ((i & 15u) == 0u) look_up(i);
+        const uint32_t slot = i % kSlots;
+        if (lane / kPair == (i & 15u)) {
+            const uint32_t which = lane % kPair, tile = my_first + i * kStride + which;
             fence_proxy_async_smem();
-            mbar_expect_tx(&bars[warp][i % kSlots], kTileBytes);
-            bulk_load(ring32 + (i % kSlots) * kTileBytes, a.cache.pages + offset, kTileBytes, &bars[warp][i % kSlots]);
+            if (which == 0u) {
+                mbar_expect_tx(&bars[warp][slot], tile + 1u < tile_end ? kPairBytes : kTileBytes);
+            }
+            if (tile < tile_end) {
+                bulk_load(ring32 + slot * kPairBytes + which * kTileBytes, a.cache.pages + tile_offset, kTileBytes,
+                          &bars[warp][slot]);
+            }
         }
     };
-    for (uint32_t i = 0; i < kSlots && i < my_tiles; ++i) issue(i);
+    for (uint32_t i = 0; i < kSlots && i < my_pairs; ++i) issue(i);
 
     // ---- q: scaled by a power of two, split into two fp16 parts, in the order the codes come out ----
     // Column n of the products is head n/2, part n%2 (HC = 4), or head n with the parts in two
@@ -296,17 +310,21 @@ kv4_decode_kernel(const Kv4AttentionArgs a, float* __restrict__ partials, const 
     }
     // Score layout: a lane holds tokens g and g + 8 of heads t (HC = 4) or 2t, 2t + 1 (HC = 8).
     const float inv_sqrt = 1.0f / sqrtf(static_cast<float>(D));
-    float code_factor[HL];   // 1 / q's power of two / sqrt(d)
+    // Scores come out in log2 units, or, where they are capped, divided by the cap.
+    const bool capped = a.rules.softcap != 0.0f;
+    const float unit = capped ? 1.0f / a.rules.softcap : kLog2e;
+    const float cap_log2 = a.rules.softcap * kLog2e;
+    float code_factor[HL];   // unit / q's power of two / sqrt(d)
     float base_factor[HL][G];
     float slope[HL];
 #pragma unroll
     for (int h = 0; h < HL; ++h) {
         const int src = HC == 4 ? static_cast<int>(t) * 8 : static_cast<int>(2 * t + h) * 4;   // lane of column head
-        code_factor[h] = __shfl_sync(0xFFFFFFFFu, q_unscale, src) * inv_sqrt;
+        code_factor[h] = __shfl_sync(0xFFFFFFFFu, q_unscale, src) * (inv_sqrt * unit);
 #pragma unroll
-        for (int gr = 0; gr < G; ++gr) base_factor[h][gr] = __shfl_sync(0xFFFFFFFFu, q_sum[gr], src) * inv_sqrt;
+        for (int gr = 0; gr < G; ++gr) base_factor[h][gr] = __shfl_sync(0xFFFFFFFFu, q_sum[gr], src) * (inv_sqrt * unit);
         const uint32_t head = HC == 4 ? t : 2 * t + h;
-        slope[h] = a.rules.alibi_slopes != nullptr && head < live_heads ? __ldg(a.rules.alibi_slopes + first_head + head) : 0.0f;
+        slope[h] = a.rules.alibi_slopes != nullptr && head < live_heads ? __ldg(a.rules.alibi_slopes + first_head + head) * kLog2e : 0.0f;
     }
 
     float m[HL], l[HL], base_acc[HL][G];
@@ -328,23 +346,49 @@ kv4_decode_kernel(const Kv4AttentionArgs a, float* __restrict__ partials, const 
     float scale_top = 0.0f;      // power of two at or above it (0: none yet)
     float weight_factor = 0.0f;  // kWTop / scale_top
 
-    for (uint32_t i = 0; i < my_tiles; ++i) {
-        const uint32_t token0 = (my_first + i * kWarps) * kKv4Tile;
-        const uint32_t slot32 = ring32 + (i % kSlots) * kTileBytes;
+    // This lane's part of a weight: the first 11 bits (even columns) or the rest (odd ones) of w, as
+    // w * part_of + ((w & first 11 bits) ^ part_sign).
+    const float part_of = (g & 1u) ? 1.0f : 0.0f;
+    const uint32_t part_sign = (g & 1u) ? 0x80000000u : 0u;
+
+    for (uint32_t i = 0; i < my_pairs; ++i) {
+        const uint32_t token0 = (my_first + i * kStride) * kKv4Tile;
+        const uint32_t slot32 = ring32 + (i % kSlots) * kPairBytes;
+        // Only the first and the last tiles hold tokens that are not seen (or no tile at all).
+        const bool whole = token0 >= span.begin && token0 + kPair * kKv4Tile <= span.end &&
+                           my_first + i * kStride + kPair <= tile_end;
         mbar_wait(&bars[warp][i % kSlots], (i / kSlots) & 1u, abort);
+        if (!whole) {
+            // Lane l guards token l of the pair: a slot that is not seen may hold anything, NaN included.
+            const uint32_t token = token0 + lane;
+            if (token < span.begin || token >= span.end || token / kKv4Tile >= tile_end) {
+                const uint32_t at = slot32 + (lane / kKv4Tile) * kTileBytes + 8u * D + (lane % kKv4Tile) * (4u * G);
+#pragma unroll
+                for (int gr = 0; gr < G; ++gr) {
+                    sts32(at + 4u * gr, 0u);
+                    sts32(at + 4u * gr + kv4_half_bytes(D), 0u);
+                }
+            }
+            fence_proxy_async_smem();   // the slot is next written by a bulk copy
+            __syncwarp();
+        }
 
         // ---- scores ----
-        float s[2][HL];   // [token g, g + 8]
-        {
+        float s[2 * kPair][HL];   // tokens g, g + 8 of both tiles
+#pragma unroll
+        for (int w = 0; w < kPair; ++w) {
+            const uint32_t k32 = slot32 + w * kTileBytes;
             float total[4] = {0.0f, 0.0f, 0.0f, 0.0f};
             uint32_t kp0[G], kp1[G];
-            float k_base0[G], k_base1[G];
-            lds_words<G>(kp0, slot32 + 8u * D + g * (4u * G));
-            lds_words<G>(kp1, slot32 + 8u * D + (g + 8u) * (4u * G));
+            lds_words<G>(kp0, k32 + 8u * D + g * (4u * G));
+            lds_words<G>(kp1, k32 + 8u * D + (g + 8u) * (4u * G));
+            float base0[HL], base1[HL];
+#pragma unroll
+            for (int h = 0; h < HL; ++h) base0[h] = base1[h] = 0.0f;
 #pragma unroll
             for (int gr = 0; gr < G; ++gr) {
                 uint32_t r[4];   // chunk 2gr: tokens g, g + 8; chunk 2gr + 1: the same
-                ldsm4(r, slot32 + gr * 512u + lane * 16u);
+                ldsm4(r, k32 + gr * 512u + lane * 16u);
                 float c[4] = {0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
                 for (int j = 0; j < 2; ++j)
@@ -360,71 +404,72 @@ kv4_decode_kernel(const Kv4AttentionArgs a, float* __restrict__ partials, const 
                         }
                     }
                 const float s0 = low_half(kp0[gr]), s1 = low_half(kp1[gr]);
-                k_base0[gr] = fmaf(8.0f, s0, high_half(kp0[gr]));
-                k_base1[gr] = fmaf(8.0f, s1, high_half(kp1[gr]));
+                const float k_base0 = fmaf(8.0f, s0, high_half(kp0[gr]));
+                const float k_base1 = fmaf(8.0f, s1, high_half(kp1[gr]));
                 total[0] = fmaf(s0, c[0], total[0]);
                 total[1] = fmaf(s0, c[1], total[1]);
                 total[2] = fmaf(s1, c[2], total[2]);
                 total[3] = fmaf(s1, c[3], total[3]);
+#pragma unroll
+                for (int h = 0; h < HL; ++h) {
+                    base0[h] = fmaf(k_base0, base_factor[h][gr], base0[h]);
+                    base1[h] = fmaf(k_base1, base_factor[h][gr], base1[h]);
+                }
             }
 #pragma unroll
             for (int h = 0; h < HL; ++h) {
                 // HC = 4: columns 2t, 2t + 1 are the two parts of head t; HC = 8: two heads
-                s[0][h] = HC == 4 ? total[0] + total[1] : total[h];
-                s[1][h] = HC == 4 ? total[2] + total[3] : total[2 + h];
-                s[0][h] *= code_factor[h];
-                s[1][h] *= code_factor[h];
-#pragma unroll
-                for (int gr = 0; gr < G; ++gr) {
-                    s[0][h] = fmaf(k_base0[gr], base_factor[h][gr], s[0][h]);
-                    s[1][h] = fmaf(k_base1[gr], base_factor[h][gr], s[1][h]);
-                }
+                s[2 * w][h] = fmaf(HC == 4 ? total[0] + total[1] : total[h], code_factor[h], base0[h]);
+                s[2 * w + 1][h] = fmaf(HC == 4 ? total[2] + total[3] : total[2 + h], code_factor[h], base1[h]);
             }
         }
-        bool seen[2];
+        if (capped) {
 #pragma unroll
-        for (int k = 0; k < 2; ++k) {
-            const uint32_t token = token0 + g + 8u * k;
-            seen[k] = token >= span.begin && token < span.end;
+            for (int k = 0; k < 2 * kPair; ++k)
 #pragma unroll
-            for (int h = 0; h < HL; ++h) {
-                float x = s[k][h];
-                if (a.rules.softcap != 0.0f) x = a.rules.softcap * tanhf(x / a.rules.softcap);
-                if (a.rules.alibi_slopes != nullptr) {
-                    const uint32_t far = span.position >= token ? span.position - token : token - span.position;
-                    x = fmaf(-slope[h], static_cast<float>(far), x);
+                for (int h = 0; h < HL; ++h) s[k][h] = cap_log2 * tanhf(s[k][h]);
+        }
+        if (a.rules.alibi_slopes != nullptr) {
+#pragma unroll
+            for (int k = 0; k < 2 * kPair; ++k) {
+                const float away = fabsf(static_cast<float>(static_cast<int>(span.position - (token0 + g + 8u * k))));
+#pragma unroll
+                for (int h = 0; h < HL; ++h) s[k][h] = fmaf(-slope[h], away, s[k][h]);
+            }
+        }
+        if (!whole) {
+#pragma unroll
+            for (int k = 0; k < 2 * kPair; ++k) {
+                const uint32_t token = token0 + g + 8u * k;
+                if (token < span.begin || token >= span.end || token / kKv4Tile >= tile_end) {
+#pragma unroll
+                    for (int h = 0; h < HL; ++h) s[k][h] = -INFINITY;
                 }
-                const uint32_t head = HC == 4 ? t : 2 * t + h;
-                if (seen[k] && !(x < INFINITY) && head < live_heads) flags |= B2_ATTN_STATUS_NAN_OR_POS_INF;
-                s[k][h] = seen[k] ? x * kLog2e : -INFINITY;   // log2 units from here
             }
         }
 
         // ---- maximum: moved only when a score passes it by kSlack, or a value scale its bound ----
-        const uint32_t v32 = slot32 + kv4_half_bytes(D);
-        uint32_t vq0[G], vq1[G];   // pairs of tokens g, g + 8
-        lds_words<G>(vq0, v32 + 8u * D + g * (4u * G));
-        lds_words<G>(vq1, v32 + 8u * D + (g + 8u) * (4u * G));
-        float scale_max;   // over the tokens the row sees: other slots may hold anything
-        {
-            __half2 top0 = *reinterpret_cast<__half2*>(&vq0[0]), top1 = *reinterpret_cast<__half2*>(&vq1[0]);
+        uint32_t vq[2 * kPair][G];   // pairs of the values of tokens g, g + 8 of both tiles
+        __half2 top2 = __half2half2(__ushort_as_half(0));
 #pragma unroll
-            for (int gr = 1; gr < G; ++gr) {
-                top0 = __hmax2(top0, *reinterpret_cast<__half2*>(&vq0[gr]));
-                top1 = __hmax2(top1, *reinterpret_cast<__half2*>(&vq1[gr]));
-            }
-            scale_max = fmaxf(seen[0] ? __low2float(top0) : 0.0f, seen[1] ? __low2float(top1) : 0.0f);
+        for (int k = 0; k < 2 * kPair; ++k) {
+            lds_words<G>(vq[k], slot32 + (k / 2) * kTileBytes + kv4_half_bytes(D) + 8u * D + (g + 8u * (k % 2)) * (4u * G));
+#pragma unroll
+            for (int gr = 0; gr < G; ++gr) top2 = __hmax2(top2, *reinterpret_cast<__half2*>(&vq[k][gr]));
         }
+        float scale_max = __low2float(top2);
         bool move = scale_max > scale_top;
 #pragma unroll
-        for (int h = 0; h < HL; ++h) move = move || fmaxf(s[0][h], s[1][h]) > m[h] + kSlack;
+        for (int h = 0; h < HL; ++h) {
+            move = move || fmaxf(fmaxf(s[0][h], s[1][h]), fmaxf(s[2][h], s[3][h])) > m[h] + kSlack;
+        }
         if (__any_sync(0xFFFFFFFFu, move)) {
             scale_max = fmaxf(scale_max, __shfl_xor_sync(0xFFFFFFFFu, scale_max, 4));
             scale_max = fmaxf(scale_max, __shfl_xor_sync(0xFFFFFFFFu, scale_max, 8));
             scale_max = fmaxf(scale_max, __shfl_xor_sync(0xFFFFFFFFu, scale_max, 16));
             float shrink = 1.0f;
             if (scale_max > scale_top) {
-                // the power of two at or above scale_max (fp16, so at least 2^-24 and at most 2^14)
+                // the power of two at or above scale_max (fp16, so at least 2^-24 and at most 2^16)
                 const float top = __uint_as_float((__float_as_uint(scale_max) + 0x007FFFFFu) & 0x7F800000u);
                 shrink = scale_top / top;   // both powers of two; 0 the first time
                 scale_top = top;
@@ -433,7 +478,7 @@ kv4_decode_kernel(const Kv4AttentionArgs a, float* __restrict__ partials, const 
             float factor[HL];
 #pragma unroll
             for (int h = 0; h < HL; ++h) {
-                float top = fmaxf(m[h], fmaxf(s[0][h], s[1][h]));
+                float top = fmaxf(m[h], fmaxf(fmaxf(s[0][h], s[1][h]), fmaxf(s[2][h], s[3][h])));
                 top = fmaxf(top, __shfl_xor_sync(0xFFFFFFFFu, top, 4));
                 top = fmaxf(top, __shfl_xor_sync(0xFFFFFFFFu, top, 8));
                 top = fmaxf(top, __shfl_xor_sync(0xFFFFFFFFu, top, 16));
@@ -453,87 +498,90 @@ kv4_decode_kernel(const Kv4AttentionArgs a, float* __restrict__ partials, const 
         }
 
         // ---- weights ----
-        float p[2][HL];
+        float p[2 * kPair][HL];
 #pragma unroll
-        for (int h = 0; h < HL; ++h) {
-            p[0][h] = ex2(s[0][h] - m[h]);
-            p[1][h] = ex2(s[1][h] - m[h]);
-            l[h] += p[0][h] + p[1][h];
-        }
-#pragma unroll
-        for (int gr = 0; gr < G; ++gr) {
-            const float b0 = seen[0] ? fmaf(8.0f, low_half(vq0[gr]), high_half(vq0[gr])) : 0.0f;
-            const float b1 = seen[1] ? fmaf(8.0f, low_half(vq1[gr]), high_half(vq1[gr])) : 0.0f;
+        for (int k = 0; k < 2 * kPair; ++k)
 #pragma unroll
             for (int h = 0; h < HL; ++h) {
-                base_acc[h][gr] = fmaf(p[0][h], b0, base_acc[h][gr]);
-                base_acc[h][gr] = fmaf(p[1][h], b1, base_acc[h][gr]);
+                p[k][h] = ex2(s[k][h] - m[h]);
+                l[h] += p[k][h];
             }
-        }
-        // To the layout of the second product's B operand: column g, tokens 2t, 2t + 1, 2t + 8, 2t + 9.
-        float w[4];
-        {
-            const int src0 = static_cast<int>(2 * t) * 4 + static_cast<int>(g >> 1), src1 = src0 + 4;
 #pragma unroll
-            for (int k = 0; k < 2; ++k) {
-                float a0 = __shfl_sync(0xFFFFFFFFu, p[k][0], src0), a1 = __shfl_sync(0xFFFFFFFFu, p[k][0], src1);
-                if (HC == 8) {   // heads 2t, 2t + 1 of the source lane: the odd columns take the second
-                    const float o0 = __shfl_sync(0xFFFFFFFFu, p[k][HL - 1], src0);
-                    const float o1 = __shfl_sync(0xFFFFFFFFu, p[k][HL - 1], src1);
-                    if (g & 1u) {
-                        a0 = o0;
-                        a1 = o1;
+        for (int k = 0; k < 2 * kPair; ++k)
+#pragma unroll
+            for (int gr = 0; gr < G; ++gr) {
+                const float b = fmaf(8.0f, low_half(vq[k][gr]), high_half(vq[k][gr]));
+#pragma unroll
+                for (int h = 0; h < HL; ++h) base_acc[h][gr] = fmaf(p[k][h], b, base_acc[h][gr]);
+            }
+#pragma unroll
+        for (int w = 0; w < kPair; ++w) {
+            const uint32_t v32 = slot32 + w * kTileBytes + kv4_half_bytes(D);
+            // To the layout of the second product's B operand: column g, tokens 2t, 2t + 1, 2t + 8, 2t + 9.
+            float wt[4];
+            {
+                const int src0 = static_cast<int>(2 * t) * 4 + static_cast<int>(g >> 1), src1 = src0 + 4;
+#pragma unroll
+                for (int k = 0; k < 2; ++k) {
+                    float a0 = __shfl_sync(0xFFFFFFFFu, p[2 * w + k][0], src0);
+                    float a1 = __shfl_sync(0xFFFFFFFFu, p[2 * w + k][0], src1);
+                    if (HC == 8) {   // heads 2t, 2t + 1 of the source lane: the odd columns take the second
+                        const float o0 = __shfl_sync(0xFFFFFFFFu, p[2 * w + k][HL - 1], src0);
+                        const float o1 = __shfl_sync(0xFFFFFFFFu, p[2 * w + k][HL - 1], src1);
+                        if (g & 1u) {
+                            a0 = o0;
+                            a1 = o1;
+                        }
+                    }
+                    wt[2 * k] = a0 * weight_factor;
+                    wt[2 * k + 1] = a1 * weight_factor;
+                }
+            }
+            // ---- values ----
+            uint32_t vp_low[2 * G], vp_high[2 * G];   // pairs of tokens 2t, 2t + 1 and 2t + 8, 2t + 9
+            lds_words<2 * G>(vp_low, v32 + 8u * D + (2u * t) * (4u * G));
+            lds_words<2 * G>(vp_high, v32 + 8u * D + (2u * t + 8u) * (4u * G));
+#pragma unroll
+            for (int gr = 0; gr < G; ++gr) {
+                uint32_t b[2][HL];   // [register][part, HC = 8]
+#pragma unroll
+                for (int k = 0; k < 2; ++k) {
+                    const uint32_t p0 = k == 0 ? vp_low[gr] : vp_high[gr], p1 = k == 0 ? vp_low[G + gr] : vp_high[G + gr];
+                    const float w0 = wt[2 * k] * low_half(p0), w1 = wt[2 * k + 1] * low_half(p1);
+                    if (HC == 4) {
+                        const float x0 = __uint_as_float((__float_as_uint(w0) & 0xFFFFE000u) ^ part_sign);
+                        const float x1 = __uint_as_float((__float_as_uint(w1) & 0xFFFFE000u) ^ part_sign);
+                        b[k][0] = pack_half(fmaf(w0, part_of, x0), fmaf(w1, part_of, x1));
+                    } else {
+                        const float h0 = first_part(w0), h1 = first_part(w1);
+                        b[k][0] = pack_half(h0, h1);
+                        b[k][HL - 1] = pack_half(w0 - h0, w1 - h1);
                     }
                 }
-                w[2 * k] = a0 * weight_factor;
-                w[2 * k + 1] = a1 * weight_factor;
-            }
-        }
-        // ---- values ----
-        uint32_t vp_low[2 * G], vp_high[2 * G];   // pairs of tokens 2t, 2t + 1 and 2t + 8, 2t + 9
-        lds_words<2 * G>(vp_low, v32 + 8u * D + (2u * t) * (4u * G));
-        lds_words<2 * G>(vp_high, v32 + 8u * D + (2u * t + 8u) * (4u * G));
+                uint32_t r[4];   // chunk 2gr: tokens (2t, 2t+1), (2t+8, 2t+9); chunk 2gr + 1: the same
+                ldsm4_trans(r, v32 + gr * 512u + lane * 16u);
 #pragma unroll
-        for (int gr = 0; gr < G; ++gr) {
-            uint32_t b[2][HL];   // [register][part, HC = 8]
+                for (int j = 0; j < 2; ++j)
 #pragma unroll
-            for (int k = 0; k < 2; ++k) {
-                const uint32_t p0 = k == 0 ? vp_low[gr] : vp_high[gr], p1 = k == 0 ? vp_low[G + gr] : vp_high[G + gr];
-                // a weight of zero may be an unseen slot's, which may hold anything, NaN included
-                const float w0 = w[2 * k] != 0.0f ? w[2 * k] * low_half(p0) : 0.0f;
-                const float w1 = w[2 * k + 1] != 0.0f ? w[2 * k + 1] * low_half(p1) : 0.0f;
-                const float h0 = first_part(w0), h1 = first_part(w1);
-                if (HC == 4) {
-                    b[k][0] = (g & 1u) ? pack_half(w0 - h0, w1 - h1) : pack_half(h0, h1);
-                } else {
-                    b[k][0] = pack_half(h0, h1);
-                    b[k][HL - 1] = pack_half(w0 - h0, w1 - h1);
-                }
-            }
-            uint32_t r[4];   // chunk 2gr: tokens (2t, 2t+1), (2t+8, 2t+9); chunk 2gr + 1: the same
-            ldsm4_trans(r, v32 + gr * 512u + lane * 16u);
+                    for (int u = 0; u < 2; ++u) {
+                        // rows g and g + 8 are channels 4g + 2u and 4g + 2u + 1 of the chunk
+                        const uint32_t a0 = u == 0 ? codes_of<0>(r[2 * j]) : codes_of<2>(r[2 * j]);
+                        const uint32_t a1 = u == 0 ? codes_of<1>(r[2 * j]) : codes_of<3>(r[2 * j]);
+                        const uint32_t a2 = u == 0 ? codes_of<0>(r[2 * j + 1]) : codes_of<2>(r[2 * j + 1]);
+                        const uint32_t a3 = u == 0 ? codes_of<1>(r[2 * j + 1]) : codes_of<3>(r[2 * j + 1]);
 #pragma unroll
-            for (int j = 0; j < 2; ++j)
-#pragma unroll
-                for (int u = 0; u < 2; ++u) {
-                    // rows g and g + 8 are channels 4g + 2u and 4g + 2u + 1 of the chunk
-                    const uint32_t a0 = u == 0 ? codes_of<0>(r[2 * j]) : codes_of<2>(r[2 * j]);
-                    const uint32_t a1 = u == 0 ? codes_of<1>(r[2 * j]) : codes_of<3>(r[2 * j]);
-                    const uint32_t a2 = u == 0 ? codes_of<0>(r[2 * j + 1]) : codes_of<2>(r[2 * j + 1]);
-                    const uint32_t a3 = u == 0 ? codes_of<1>(r[2 * j + 1]) : codes_of<3>(r[2 * j + 1]);
-#pragma unroll
-                    for (int part = 0; part < HL; ++part) {
-                        mma16816(acc[2 * gr + j][u], a0, a1, a2, a3, b[0][part], b[1][part]);
+                        for (int part = 0; part < HL; ++part) {
+                            mma16816(acc[2 * gr + j][u], a0, a1, a2, a3, b[0][part], b[1][part]);
+                        }
                     }
-                }
+            }
         }
         __syncwarp();   // every lane has read the slot
-        if (i + kSlots < my_tiles) issue(i + kSlots);
+        if (i + kSlots < my_pairs) issue(i + kSlots);
     }
 
     // ---- join the warps (the ring is free: it holds their accumulators) ----
     if (lane == 0 && *abort != 0) flags |= B2_ATTN_STATUS_TIMEOUT;
-    if (flags != 0u) kv4_flag(a.status, flags);
     __syncthreads();
     float* s_acc = reinterpret_cast<float*>(ring_raw);   // [warp][HC][D]
     const float undo = scale_top / kWTop;
@@ -543,6 +591,8 @@ kv4_decode_kernel(const Kv4AttentionArgs a, float* __restrict__ partials, const 
         l[h] += __shfl_xor_sync(0xFFFFFFFFu, l[h], 8);
         l[h] += __shfl_xor_sync(0xFFFFFFFFu, l[h], 16);
         const uint32_t head = HC == 4 ? t : 2 * t + h;
+        // a NaN or +infinite score left a NaN weight, and nothing else does
+        if (isnan(l[h]) && head < live_heads) flags |= B2_ATTN_STATUS_NAN_OR_POS_INF;
         if (g == 0) {
             s_m[warp][head] = m[h];
             s_l[warp][head] = l[h];
@@ -568,6 +618,7 @@ kv4_decode_kernel(const Kv4AttentionArgs a, float* __restrict__ partials, const 
             }
         }
     }
+    if (flags != 0u) kv4_flag(a.status, flags);
     __syncthreads();
     for (uint32_t i = threadIdx.x; i < live_heads * (D / 4u); i += kWarps * 32u) {
         const uint32_t head = i / (D / 4u), c = (i % (D / 4u)) * 4u;
@@ -687,13 +738,14 @@ SplitPlan split_plan(int sm_count, uint64_t rows, uint32_t q_heads, uint32_t kv_
     if (lists < wanted) per = (tiles * lists + wanted - 1u) / wanted;
     if (per < 16u) per = 16u;
     if (per > 128u) per = 128u;
+    per = (per + kPair - 1u) / kPair * kPair;
     return SplitPlan{static_cast<uint32_t>((tiles + per - 1u) / per), static_cast<uint32_t>(per)};
 }
 
 template <int D, int HC>
 int32_t launch_one(const DeviceContext& ctx, const Kv4AttentionArgs& a, float* partials, const SplitPlan& plan,
                    unsigned blocks, cudaStream_t stream) {
-    constexpr int kRing = kWarps * kSlots * static_cast<int>(kv4_tile_bytes(D));
+    constexpr int kRing = kWarps * slots_of(D) * kPair * static_cast<int>(kv4_tile_bytes(D));
     static PerDeviceOnce configured;
     B2_TRY(once_per_device(configured, ctx.device, []() -> int32_t {
         B2_CUDA_TRY(cudaFuncSetAttribute(kv4_decode_kernel<D, HC>, cudaFuncAttributeMaxDynamicSharedMemorySize, kRing));
