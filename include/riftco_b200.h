@@ -531,6 +531,7 @@ B2_API int32_t b2_check_device_errors(void);
 #define B2_ROUTE_ATTENTION_BULK 8   /* head_width 128, block_size 16, rep in {1,2,4,8} */
 #define B2_ROUTE_ATTENTION_GENERIC 9
 #define B2_ROUTE_ATTENTION_KV4 10   /* 4-bit cache, each query row on its own */
+#define B2_ROUTE_ATTENTION_KV4_TILES 11   /* 4-bit cache, tiles of 128 query rows on tcgen05 */
 B2_API int32_t b2_last_route(void);
 
 /* ---- host-buffer seam --------------------------------------------------- */

@@ -79,7 +79,7 @@ def check_device_errors() -> None:
 
 
 ROUTES = ("none", "decode_tmem", "gemv_tma", "gemv_tile", "gemm_tmem", "gemm_smem", "backward_dense",
-          "generic", "attention_bulk", "attention_generic", "attention_kv4")
+          "generic", "attention_bulk", "attention_generic", "attention_kv4", "attention_kv4_tiles")
 
 
 def last_route() -> str:

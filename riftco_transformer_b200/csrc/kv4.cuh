@@ -13,6 +13,13 @@
 
 #include "b2_common.cuh"
 
+#if defined(__CUDACC__)
+#include "sm100_ptx.cuh"
+
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
+#endif
+
 namespace b2 {
 
 constexpr uint32_t kKv4Tile = 16;          // slots of a tile
@@ -83,6 +90,13 @@ size_t kv4_decode_workspace_bytes(int sm_count, uint64_t rows, uint32_t q_heads,
 int32_t launch_kv4_decode(const DeviceContext& ctx, const Kv4AttentionArgs& args, void* workspace,
                           size_t workspace_bytes, cudaStream_t stream);
 
+// kv4_chunk.cu - tiles of 128 query rows on the tcgen05 tensor cores, bf16 contexts.
+bool kv4_chunk_supported(uint32_t head_width, uint32_t q_heads, uint32_t kv_heads, uint32_t max_chunk);
+size_t kv4_chunk_workspace_bytes(int sm_count, uint32_t n_seq, uint64_t rows, uint32_t q_heads, uint32_t kv_heads,
+                                 uint32_t head_width, uint32_t max_chunk, uint32_t max_seq_len);
+int32_t launch_kv4_chunk(const DeviceContext& ctx, const Kv4AttentionArgs& args, void* workspace,
+                         size_t workspace_bytes, cudaStream_t stream);
+
 #if defined(__CUDACC__)
 
 // Adds `bits` to the caller's status word.
@@ -107,6 +121,119 @@ __device__ __forceinline__ bool kv4_locate(const Kv4View& c, uint32_t seq, uint3
     if (seq >= c.n_seq || logical >= c.max_blocks) return false;
     *phys = c.block_tables[static_cast<uint64_t>(seq) * c.max_blocks + logical];
     return *phys < c.physical_blocks;
+}
+
+
+// ---- shared by the two attention kernels ------------------------------------------------------
+
+constexpr float kLog2e = 1.4426950408889634f;
+constexpr float kNoMax = -FLT_MAX;    // running maximum before the first score (log2 units)
+
+__device__ __forceinline__ float ex2(float x) {
+    float y;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+__device__ __forceinline__ float low_half(uint32_t pair) { return __low2float(*reinterpret_cast<__half2*>(&pair)); }
+__device__ __forceinline__ float high_half(uint32_t pair) { return __high2float(*reinterpret_cast<__half2*>(&pair)); }
+__device__ __forceinline__ uint32_t pack_half(float lo, float hi) {
+    const __half2 h = __floats2half2_rn(lo, hi);
+    return *reinterpret_cast<const uint32_t*>(&h);
+}
+__device__ __forceinline__ void bulk_load(uint32_t dst32, const void* src, uint32_t bytes, uint64_t* bar) {
+    asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];"
+                 ::"r"(dst32), "l"(src), "r"(bytes), "r"(sm100::smem_u32(bar))
+                 : "memory");
+}
+
+// What a row sees: tokens [begin, end) of sequence `seq`, its own position, and whether the caller's
+// lengths were out of bounds.
+struct RowSpan {
+    uint32_t seq, position, begin, end;
+    bool bad;
+    bool owned;   // false: a row behind the last sequence, which is left as it was
+};
+__device__ __forceinline__ RowSpan row_span(const Kv4AttentionArgs& a, uint32_t row) {
+    RowSpan r{row, 0, 0, 0, false, true};
+    uint32_t back = 0;   // tokens after this one
+    if (a.chunk_starts != nullptr) {
+        uint32_t lo = 0, hi = a.cache.n_seq;   // the last sequence that starts at or before `row`
+        while (lo + 1u < hi) {
+            const uint32_t mid = (lo + hi) / 2u;
+            if (__ldg(a.chunk_starts + mid) <= row) lo = mid; else hi = mid;
+        }
+        r.seq = lo;
+        const uint32_t first = __ldg(a.chunk_starts + lo), last = __ldg(a.chunk_starts + lo + 1u);
+        r.owned = row >= first && row < last;
+        if (!r.owned) return r;
+        back = last - 1u - row;
+    }
+    uint32_t len = __ldg(a.seq_lens + r.seq);
+    if (len > a.max_seq_len) {
+        len = a.max_seq_len;
+        r.bad = true;
+    }
+    if (back >= len) {
+        r.bad = r.bad || a.chunk_starts != nullptr;   // more new tokens than the sequence holds
+        return r;
+    }
+    r.position = len - 1u - back;
+    r.end = r.position + 1u;
+    if (a.rules.prefix_lens != nullptr) r.end = max(r.end, min(len, __ldg(a.rules.prefix_lens + r.seq)));
+    if (a.rules.window != 0u && r.position >= a.rules.window) r.begin = r.position - a.rules.window + 1u;
+    return r;
+}
+
+// Four channels of a context, o / l; zeros where nothing was seen (l = 0).
+template <int D>
+__device__ __forceinline__ void put_context(const Kv4AttentionArgs& a, uint64_t out_head, uint32_t c, float4 o, float l) {
+    o = l == 0.0f ? make_float4(0.f, 0.f, 0.f, 0.f) : make_float4(o.x / l, o.y / l, o.z / l, o.w / l);
+    if (a.ctx != nullptr) *reinterpret_cast<float4*>(a.ctx + out_head * D + c) = o;
+    if (a.ctx16 != nullptr) {
+        const __nv_bfloat162 lo = __floats2bfloat162_rn(o.x, o.y), hi = __floats2bfloat162_rn(o.z, o.w);
+        uint2 packed;
+        packed.x = *reinterpret_cast<const uint32_t*>(&lo);
+        packed.y = *reinterpret_cast<const uint32_t*>(&hi);
+        *reinterpret_cast<uint2*>(static_cast<__nv_bfloat16*>(a.ctx16) + out_head * D + c) = packed;
+    }
+}
+
+// Joins `n_splits` partial results of one (row, query head), each [maximum (log2 units), sum of weights, -, -,
+// D sums], for the channels c .. c + 3 of this thread, in split order.
+template <int D>
+__device__ __forceinline__ void join_splits(const Kv4AttentionArgs& a, const float* src, uint64_t out_head,
+                                            uint32_t n_splits, uint32_t c, bool sees_any) {
+    float mm = kNoMax, ll = 0.0f;
+    float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
+    for (uint32_t s0 = 0; s0 < n_splits; s0 += 8u) {
+        float2 ml[8];
+        float4 x[8];
+#pragma unroll
+        for (uint32_t u = 0; u < 8u; ++u) {   // all loads before the first use
+            const bool live = s0 + u < n_splits;
+            const float* part = src + (s0 + u) * (D + 4u);
+            ml[u] = live ? *reinterpret_cast<const float2*>(part) : make_float2(kNoMax, 0.0f);
+            x[u] = live ? *reinterpret_cast<const float4*>(part + 4u + c) : make_float4(0.f, 0.f, 0.f, 0.f);
+        }
+        float top = mm;
+#pragma unroll
+        for (uint32_t u = 0; u < 8u; ++u) top = fmaxf(top, ml[u].x);
+        const float keep = ex2(mm - top);
+        mm = top;
+        ll *= keep;
+        o = make_float4(o.x * keep, o.y * keep, o.z * keep, o.w * keep);
+#pragma unroll
+        for (uint32_t u = 0; u < 8u; ++u) {   // in split order
+            const float f = ex2(ml[u].x - mm);
+            ll = fmaf(ml[u].y, f, ll);
+            o.x = fmaf(x[u].x, f, o.x);
+            o.y = fmaf(x[u].y, f, o.y);
+            o.z = fmaf(x[u].z, f, o.z);
+            o.w = fmaf(x[u].w, f, o.w);
+        }
+    }
+    if (ll == 0.0f && sees_any && c == 0) kv4_flag(a.status, B2_ATTN_STATUS_ALL_NEG_INF);
+    put_context<D>(a, out_head, c, o, ll);
 }
 
 #endif  // __CUDACC__

@@ -165,6 +165,13 @@ DeviceContext* query_context(uint32_t rows, uint32_t q_heads, uint32_t kv_heads,
     return ctx;
 }
 
+size_t chunk_workspace(const DeviceContext& ctx, uint32_t n_seq, uint32_t n_tokens, uint32_t q_heads, uint32_t kv_heads,
+                       uint32_t head_width, uint32_t max_chunk, uint32_t max_seq_len) {
+    return kv4_chunk_supported(head_width, q_heads, kv_heads, max_chunk)
+               ? kv4_chunk_workspace_bytes(ctx.sm_count, n_seq, n_tokens, q_heads, kv_heads, head_width, max_chunk, max_seq_len)
+               : kv4_decode_workspace_bytes(ctx.sm_count, n_tokens, q_heads, kv_heads, head_width, max_seq_len);
+}
+
 }  // namespace
 }  // namespace b2
 
@@ -264,7 +271,7 @@ size_t b2_paged_chunk_kv4_workspace_bytes(uint32_t n_seq, uint32_t n_tokens, uin
     if (n_seq == 0 || max_chunk == 0) return 0;
     DeviceContext* ctx = query_context(n_tokens, q_heads, kv_heads, head_width, max_seq_len);
     return ctx == nullptr ? 0
-                          : kv4_decode_workspace_bytes(ctx->sm_count, n_tokens, q_heads, kv_heads, head_width, max_seq_len);
+                          : chunk_workspace(*ctx, n_seq, n_tokens, q_heads, kv_heads, head_width, max_chunk, max_seq_len);
 }
 
 int32_t b2_paged_chunk_attention_kv4(const b2_kv4_cache* cache, const b2_kv4_score_rules* rules,
@@ -287,9 +294,14 @@ int32_t b2_paged_chunk_attention_kv4(const b2_kv4_cache* cache, const b2_kv4_sco
     if (max_chunk > max_seq_len || max_chunk > n_tokens) {
         return fail(B2_STATUS_INVALID_ARGUMENT, "paged attention chunk is longer than its sequence or the call's tokens");
     }
-    B2_TRY(take_workspace(ctx, kv4_decode_workspace_bytes(ctx->sm_count, n_tokens, q_heads, args.cache.kv_heads,
-                                                          args.cache.head_width, max_seq_len),
+    const uint32_t kv_heads = args.cache.kv_heads, head_width = args.cache.head_width;
+    B2_TRY(take_workspace(ctx, chunk_workspace(*ctx, args.cache.n_seq, n_tokens, q_heads, kv_heads, head_width, max_chunk,
+                                               max_seq_len),
                           &workspace, &workspace_bytes, stream));
+    if (kv4_chunk_supported(head_width, q_heads, kv_heads, max_chunk)) {
+        note_route(B2_ROUTE_ATTENTION_KV4_TILES);
+        return launch_kv4_chunk(*ctx, args, workspace, workspace_bytes, stream);
+    }
     note_route(B2_ROUTE_ATTENTION_KV4);
     return launch_kv4_decode(*ctx, args, workspace, workspace_bytes, stream);
 }

@@ -1,0 +1,711 @@
+// Attention of several new tokens per sequence over the 4-bit paged cache, on the tcgen05 tensor cores.
+//
+// A row is (new token, query head of one K/V head): token i and head h of the group are row i * rep + h, so
+// that any number of query heads per K/V head fills whole tiles. A CTA takes 256 rows (two tiles of 128
+// = two M of tcgen05.mma) of one K/V head and walks the cached tokens they see in blocks of 128:
+//   S = Q K^T          [128 x 128], A and B in shared memory, FP32 in tensor memory
+//   P = 2^(S - m)      fp16, written over S
+//   O += P V           A = P in tensor memory, B = V^T in shared memory, FP32 in tensor memory
+// Unlike in the single-row kernel (kv4_decode.cu) a block of K and V serves 256 rows, so its codes are expanded
+// to fp16 once, by four warps, into swizzled shared-memory tiles: value = scale * code + base with one rounding.
+// The contraction order inside eight channels follows the nibbles (0 4 1 5 2 6 3 7; Q is staged to match); V is
+// transposed on the way, since its contraction is over tokens: two tokens' words are merged so that one
+// AND-OR yields two tokens' codes of one channel.
+//
+// Roundings: Q, K, V and P are fp16 (2^-12 of each value; Q is first scaled by a power of two per row), sums,
+// maxima and O are FP32, and the context is bf16 (2^-9), which is the larger error. The maximum m is moved, and O
+// rescaled in tensor memory, only when a score passes it by 8 in log2 units: P may reach 2^8, and a row
+// sum of 2^8 * 10^5 tokens stays far inside FP32.
+//
+// What bounds it: for a block and a tile the two products take 128 * 128 * D * 2 / 4096 = 1024 cycles of the
+// tensor core at D = 128, the 16384 exponentials as many of the 16-per-cycle unit: the two tiles alternate so
+// that one's products run under the other's softmax.
+//
+// Roles (14 warps): 0-3 and 4-7 softmax and epilogue of the two tiles (thread = row = tensor-memory lane), 8-11
+// expansion, 12 bulk copies of raw tiles, 13 the tcgen05 issue. Every wait is bounded.
+#include "kv4.cuh"
+
+#include <cmath>
+
+namespace b2 {
+namespace {
+
+using namespace sm100;
+
+constexpr uint32_t kRows = 256, kBlock = 128, kHalf = 64;   // rows of a CTA, tokens of a block and of half of one
+constexpr uint32_t kBlockTiles = kBlock / kKv4Tile, kHalfTiles = kHalf / kKv4Tile;
+constexpr uint32_t kSoftmaxWarps = 8, kExpandWarps = 4;
+constexpr uint32_t kLoadWarp = 12, kIssueWarp = 13;
+constexpr uint32_t kThreads = 14 * 32;
+constexpr uint32_t kRawSlots = 3, kStages = 2;
+constexpr uint32_t kTmemColumns = 512, kTmemTile = 256, kTmemO = 128;   // a tile's S (and P) and its O
+constexpr float kSlack = 8.0f;
+
+template <int D>
+struct Layout {
+    static constexpr uint32_t kQ = kRows * D * 2, kKStage = kBlock * D * 2, kVStage = kBlock * D * 2;
+    // 16 bytes apart, so that the same word of four tiles lies in different banks
+    static constexpr uint32_t kRawTile = kv4_tile_bytes(D) + 16u;
+    static constexpr uint32_t kRawSlot = kHalfTiles * kRawTile;
+    static constexpr uint32_t kTotal = kQ + kStages * (kKStage + kVStage) + kRawSlots * kRawSlot + 1024u;
+};
+
+struct Barriers {
+    uint64_t raw_full[kRawSlots], raw_empty[kRawSlots];
+    uint64_t k_full[kStages], k_empty[kStages], v_full[kStages], v_empty[kStages];
+    uint64_t s_full[2], p_full[2], o_full[2];
+    uint32_t tmem_base;
+    uint32_t abort;
+};
+
+struct ChunkPlan {
+    uint32_t row_tiles;         // CTAs of 256 rows a sequence may need
+    uint32_t splits;            // most splits of the blocks of one of them
+    uint32_t blocks_per_split;
+};
+
+// What the 256 rows from `row0` of a sequence's n * rep rows see together.
+struct TileSpan {
+    uint32_t first;          // row of q of the sequence's first new token
+    uint32_t tokens;         // new tokens n
+    uint32_t rows;           // n * rep
+    uint32_t len;
+    uint32_t prefix;
+    int64_t position0;       // position of new token 0: negative where the chunk is longer than the sequence
+    uint32_t begin, end;     // tokens any row sees
+    bool bad;
+};
+__device__ __forceinline__ TileSpan tile_span(const Kv4AttentionArgs& a, uint32_t seq, uint32_t rep, uint32_t row0) {
+    TileSpan s{};
+    uint32_t first = __ldg(a.chunk_starts + seq), last = __ldg(a.chunk_starts + seq + 1u);
+    first = min(first, a.rows);
+    last = min(last, a.rows);
+    s.first = first;
+    s.tokens = last > first ? last - first : 0u;
+    if (s.tokens > a.max_chunk) {   // the grid holds max_chunk of them
+        s.bad = true;
+        s.tokens = a.max_chunk;
+    }
+    s.rows = s.tokens * rep;
+    if (row0 >= s.rows) return s;
+    s.len = __ldg(a.seq_lens + seq);
+    if (s.len > a.max_seq_len) {
+        s.len = a.max_seq_len;
+        s.bad = true;
+    }
+    s.position0 = static_cast<int64_t>(s.len) - (last - first);
+    s.bad = s.bad || s.position0 < 0;
+    s.prefix = a.rules.prefix_lens != nullptr ? min(s.len, __ldg(a.rules.prefix_lens + seq)) : 0u;
+    const uint32_t token_lo = row0 / rep, token_hi = min(s.tokens - 1u, (row0 + kRows - 1u) / rep);
+    const int64_t lowest = max(static_cast<int64_t>(0), s.position0 + token_lo), highest = s.position0 + token_hi;
+    if (highest < 0) return s;
+    s.end = max(static_cast<uint32_t>(highest) + 1u, s.prefix);
+    if (a.rules.window != 0u && lowest >= a.rules.window) s.begin = static_cast<uint32_t>(lowest) - a.rules.window + 1u;
+    return s;
+}
+
+__device__ __forceinline__ float rcp(float x) {
+    float y;
+    asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+__device__ __forceinline__ bool elect_one() {
+    uint32_t pred;
+    asm volatile("{ .reg .pred p; elect.sync _|p, 0xFFFFFFFF; selp.u32 %0, 1, 0, p; }" : "=r"(pred));
+    return pred != 0;
+}
+__device__ __forceinline__ uint32_t lds32(uint32_t addr) {
+    uint32_t v;
+    asm volatile("ld.shared.u32 %0, [%1];" : "=r"(v) : "r"(addr) : "memory");
+    return v;
+}
+__device__ __forceinline__ uint4 lds128(uint32_t addr) {
+    uint4 v;
+    asm volatile("ld.shared.v4.u32 {%0,%1,%2,%3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(addr) : "memory");
+    return v;
+}
+__device__ __forceinline__ void sts128(uint32_t addr, uint32_t x, uint32_t y, uint32_t z, uint32_t w) {
+    asm volatile("st.shared.v4.u32 [%0], {%1,%2,%3,%4};" ::"r"(addr), "r"(x), "r"(y), "r"(z), "r"(w) : "memory");
+}
+__device__ __forceinline__ void tmem_st_32(uint32_t taddr, const uint32_t* r) {
+    asm volatile(
+        "tcgen05.st.sync.aligned.32x32b.x32.b32 [%0], "
+        "{%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,"
+        "%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31,%32};"
+        ::"r"(taddr), "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]),
+          "r"(r[8]), "r"(r[9]), "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15]), "r"(r[16]),
+          "r"(r[17]), "r"(r[18]), "r"(r[19]), "r"(r[20]), "r"(r[21]), "r"(r[22]), "r"(r[23]), "r"(r[24]),
+          "r"(r[25]), "r"(r[26]), "r"(r[27]), "r"(r[28]), "r"(r[29]), "r"(r[30]), "r"(r[31])
+        : "memory");
+}
+__device__ __forceinline__ void tmem_st_wait() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
+__device__ __forceinline__ void umma_ss(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t accumulate) {
+    asm volatile(
+        "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
+        "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}"
+        ::"r"(d), "l"(a), "l"(b), "r"(idesc), "r"(accumulate)
+        : "memory");
+}
+__device__ __forceinline__ void umma_ts(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, uint32_t accumulate) {
+    asm volatile(
+        "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
+        "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}"
+        ::"r"(d), "r"(a), "l"(b), "r"(idesc), "r"(accumulate)
+        : "memory");
+}
+// kind::f16, fp16 x fp16 -> FP32, both operands K-major, M = 128.
+__host__ __device__ constexpr uint32_t idesc_f16(uint32_t n) { return (1u << 4) | ((n >> 3) << 17) | ((128u >> 4) << 24); }
+
+// scale * code + base of the two codes that nibble N of both halves of `word` holds; the scales and bases
+// are those of the two. 1024 + code and 1024 + 16 code are exact, so is taking the 1024 off.
+template <int N>
+__device__ __forceinline__ uint32_t expand(uint32_t word, __half2 scale, __half2 base) {
+    if (N >= 2) word >>= 8;
+    __half2 c;
+    if (N % 2 == 0) {
+        uint32_t x = (word & 0x000F000Fu) | 0x64006400u;
+        c = __hadd2(*reinterpret_cast<__half2*>(&x), __half2half2(__ushort_as_half(0xE400)));   // -1024
+    } else {
+        uint32_t x = (word & 0x00F000F0u) | 0x64006400u;
+        c = __hfma2(*reinterpret_cast<__half2*>(&x), __half2half2(__ushort_as_half(0x2C00)),    // 1/16
+                    __half2half2(__ushort_as_half(0xD400)));                                     // -64
+    }
+    c = __hfma2(c, scale, base);
+    return *reinterpret_cast<const uint32_t*>(&c);
+}
+__device__ __forceinline__ __half2 as_half2(uint32_t x) { return *reinterpret_cast<__half2*>(&x); }
+// Whether the scale or the base of a pair is an infinity or a NaN.
+__device__ __forceinline__ bool not_finite(uint32_t pair) {
+    return (pair & 0x7C00u) == 0x7C00u || (pair & 0x7C000000u) == 0x7C000000u;
+}
+
+// Half a block (64 tokens) of keys: 32 channels of one token per step and thread, rows of the tile in token order.
+template <int D>
+__device__ __forceinline__ void expand_keys(uint32_t raw32, uint32_t stage32, uint32_t half, uint32_t tid, uint32_t token0,
+                                            uint32_t begin, uint32_t end) {
+    constexpr uint32_t G = D / 64;
+#pragma unroll
+    for (uint32_t u = tid; u < kHalf * (D / 32); u += kExpandWarps * 32u) {
+        const uint32_t tk = u % kHalf, j = u / kHalf;   // lanes: consecutive tokens
+        const uint32_t tile32 = raw32 + (tk / 16u) * Layout<D>::kRawTile;
+        const uint32_t at = (tk % 16u) * (4u * G);
+        uint32_t pair = lds32(tile32 + 8u * D + at + (j / 2u) * 4u);
+        const uint32_t token = token0 + tk;
+        if (token < begin || token >= end) {
+            pair = 0u;
+        } else if (j == 0u) {
+            // A value that is not finite must not meet the zero weight of a row that does not see it: its group
+            // is expanded as zeros (expand_values), and the token's scores, which such a row masks, become NaN.
+            for (uint32_t gr = 0; gr < G; ++gr) {
+                if (not_finite(lds32(tile32 + kv4_half_bytes(D) + 8u * D + at + gr * 4u))) pair = 0x7FFF7FFFu;
+            }
+        }
+        const uint4 raw = lds128(tile32 + j * 256u + (tk % 16u) * 16u);
+        const __half2 scale = __half2half2(__low2half(as_half2(pair))), base = __half2half2(__high2half(as_half2(pair)));
+        const uint32_t row = half * kHalf + tk;
+        const uint32_t row32 = stage32 + (j / 2u) * (kBlock * 128u) + row * 128u;
+        const uint32_t words[4] = {raw.x, raw.y, raw.z, raw.w};
+#pragma unroll
+        for (uint32_t w = 0; w < 4u; ++w) {
+            const uint32_t unit = (j % 2u) * 4u + w;
+            sts128(row32 + ((unit ^ (row & 7u)) << 4), expand<0>(words[w], scale, base), expand<1>(words[w], scale, base),
+                   expand<2>(words[w], scale, base), expand<3>(words[w], scale, base));
+        }
+    }
+}
+
+// Half a block of values, transposed: eight channels of eight tokens per step and thread, rows of the tile are channels.
+template <int D>
+__device__ __forceinline__ void expand_values(uint32_t raw32, uint32_t stage32, uint32_t half, uint32_t tid,
+                                              uint32_t token0, uint32_t begin, uint32_t end) {
+    constexpr uint32_t G = D / 64;
+    if (tid >= D) return;
+    const uint32_t octet = tid % 8u, word = tid / 8u;   // tokens 8 octet.., channels 8 word..
+    const uint32_t j = word / 4u;
+    const uint32_t tile32 = raw32 + (octet / 2u) * Layout<D>::kRawTile + kv4_half_bytes(D);
+    const uint32_t slot0 = (octet & 1u) * 8u;
+    uint32_t scale[4], base[4], lo[4], hi[4];
+#pragma unroll
+    for (uint32_t k = 0; k < 4u; ++k) {
+        uint32_t pair[2], code[2];
+#pragma unroll
+        for (uint32_t e = 0; e < 2u; ++e) {
+            const uint32_t slot = slot0 + 2u * k + e, token = token0 + octet * 8u + 2u * k + e;
+            pair[e] = lds32(tile32 + 8u * D + slot * (4u * G) + (j / 2u) * 4u);
+            if (token < begin || token >= end || not_finite(pair[e])) pair[e] = 0u;
+            code[e] = lds32(tile32 + j * 256u + slot * 16u + (word % 4u) * 4u);
+        }
+        scale[k] = __byte_perm(pair[0], pair[1], 0x5410);
+        base[k] = __byte_perm(pair[0], pair[1], 0x7632);
+        lo[k] = __byte_perm(code[0], code[1], 0x5410);   // channels 0..3 of both tokens
+        hi[k] = __byte_perm(code[0], code[1], 0x7632);   // channels 4..7
+    }
+    const uint32_t column32 = stage32 + half * (D * 128u) + word * 1024u;
+    auto put = [&](uint32_t n, uint32_t x0, uint32_t x1, uint32_t x2, uint32_t x3) {
+        sts128(column32 + n * 128u + ((octet ^ n) << 4), x0, x1, x2, x3);
+    };
+#define B2_KV4_PUT(N, SRC)                                                                                    \
+    put(N, expand<(N) % 4>(SRC[0], as_half2(scale[0]), as_half2(base[0])),                                    \
+        expand<(N) % 4>(SRC[1], as_half2(scale[1]), as_half2(base[1])),                                       \
+        expand<(N) % 4>(SRC[2], as_half2(scale[2]), as_half2(base[2])),                                       \
+        expand<(N) % 4>(SRC[3], as_half2(scale[3]), as_half2(base[3])))
+    B2_KV4_PUT(0, lo);
+    B2_KV4_PUT(1, lo);
+    B2_KV4_PUT(2, lo);
+    B2_KV4_PUT(3, lo);
+    B2_KV4_PUT(4, hi);
+    B2_KV4_PUT(5, hi);
+    B2_KV4_PUT(6, hi);
+    B2_KV4_PUT(7, hi);
+#undef B2_KV4_PUT
+}
+
+template <int D>
+__global__ void __launch_bounds__(kThreads, 1)
+kv4_chunk_kernel(const Kv4AttentionArgs a, float* __restrict__ partials, const ChunkPlan plan) {
+    using L = Layout<D>;
+    constexpr uint32_t kChannels8 = D / 8;
+    pdl_launch_dependents();
+    extern __shared__ __align__(1024) uint8_t smem_raw[];
+    __shared__ __align__(8) Barriers bars;
+    __shared__ float s_factor[kRows];
+
+    const uint32_t rep = a.q_heads / a.cache.kv_heads;
+    uint32_t block = blockIdx.x;
+    const uint32_t split = block % plan.splits;
+    block /= plan.splits;
+    const uint32_t kvh = block % a.cache.kv_heads;
+    block /= a.cache.kv_heads;
+    const uint32_t seq = block % a.cache.n_seq;
+    // the last rows see the most tokens: they start first
+    const uint32_t row0 = (plan.row_tiles - 1u - block / a.cache.n_seq) * kRows;
+    const TileSpan span = tile_span(a, seq, rep, row0);
+    if (row0 >= span.rows) return;
+    const uint32_t rows = min(kRows, span.rows - row0);
+    const uint32_t tile0 = span.begin / kKv4Tile;
+    const uint32_t tiles = span.end > span.begin ? (span.end - 1u) / kKv4Tile + 1u - tile0 : 0u;
+    const uint32_t blocks = (tiles + kBlockTiles - 1u) / kBlockTiles;
+    const uint32_t n_splits = max(1u, (blocks + plan.blocks_per_split - 1u) / plan.blocks_per_split);
+    if (split >= n_splits) return;
+    const uint32_t block0 = split * plan.blocks_per_split;
+    const uint32_t n_blocks = min(plan.blocks_per_split, blocks - block0);   // 0 where nothing is seen
+    const uint32_t first_tile = tile0 + block0 * kBlockTiles;
+    const uint32_t end_tile = min(tile0 + tiles, first_tile + n_blocks * kBlockTiles);
+    const uint32_t n_tiles = rows > 128u ? 2u : 1u;   // row tiles with a live row
+
+    const uint32_t smem32 = (smem_u32(smem_raw) + 1023u) & ~1023u;
+    const uint32_t q32 = smem32, k32 = q32 + L::kQ, v32 = k32 + kStages * L::kKStage, raw32 = v32 + kStages * L::kVStage;
+    const uint32_t tid = threadIdx.x, lane = tid & 31u, warp = tid >> 5;
+    volatile uint32_t* abort = &bars.abort;
+    uint32_t flags = span.bad ? B2_ATTN_STATUS_BAD_BLOCK : 0u;
+
+    if (warp == kIssueWarp) {
+        if (lane == 0) {
+            for (uint32_t i = 0; i < kRawSlots; ++i) {
+                mbar_init(&bars.raw_full[i], 1);
+                mbar_init(&bars.raw_empty[i], kExpandWarps);
+            }
+            for (uint32_t i = 0; i < kStages; ++i) {
+                mbar_init(&bars.k_full[i], kExpandWarps);
+                mbar_init(&bars.v_full[i], kExpandWarps);
+                mbar_init(&bars.k_empty[i], 1);
+                mbar_init(&bars.v_empty[i], 1);
+            }
+            for (uint32_t i = 0; i < 2u; ++i) {
+                mbar_init(&bars.s_full[i], 1);
+                mbar_init(&bars.p_full[i], 4);
+                mbar_init(&bars.o_full[i], 1);
+            }
+            bars.abort = 0;
+            mbar_fence_init();
+        }
+        __syncwarp();
+        tmem_alloc(&bars.tmem_base, kTmemColumns);
+    }
+
+    // ---- Q: scaled to a largest magnitude in [2^9, 2^10) per row, fp16, in the order the codes come out ----
+    const float unit = a.rules.softcap != 0.0f ? 1.0f / a.rules.softcap : kLog2e;
+    const float to_unit = unit / sqrtf(static_cast<float>(D));
+    for (uint32_t i = tid; i < kRows * kChannels8; i += kThreads) {   // whole warps: kRows * kChannels8 % 32 == 0
+        const uint32_t r = i / kChannels8, c8 = i % kChannels8;
+        float x[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+        if (r < rows) {
+            const uint32_t gr = row0 + r;
+            const float* src = a.q + (static_cast<uint64_t>(span.first + gr / rep) * a.q_heads + kvh * rep + gr % rep) * D + c8 * 8u;
+            const float4 u0 = __ldg(reinterpret_cast<const float4*>(src)), u1 = __ldg(reinterpret_cast<const float4*>(src) + 1);
+            x[0] = u0.x; x[1] = u0.y; x[2] = u0.z; x[3] = u0.w;
+            x[4] = u1.x; x[5] = u1.y; x[6] = u1.z; x[7] = u1.w;
+        }
+        float top = 0.0f;
+#pragma unroll
+        for (int e = 0; e < 8; ++e) top = fmaxf(top, fabsf(x[e]));
+#pragma unroll
+        for (uint32_t o = kChannels8 / 2u; o > 0u; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xFFFFFFFFu, top, o));
+        int e = 9 - (static_cast<int>((__float_as_uint(top) >> 23) & 255u) - 127);
+        e = max(-100, min(100, e));   // a row of zeros or beyond 2^109 keeps a bounded factor
+        const float up = __uint_as_float(static_cast<uint32_t>(e + 127) << 23);
+        if (c8 == 0u) s_factor[r] = __uint_as_float(static_cast<uint32_t>(127 - e) << 23) * to_unit;
+        const uint32_t dst = q32 + (r / 128u) * (128u * D * 2u) + (c8 / 8u) * 16384u + (r % 128u) * 128u + (((c8 % 8u) ^ (r & 7u)) << 4);
+        sts128(dst, pack_half(x[0] * up, x[4] * up), pack_half(x[1] * up, x[5] * up), pack_half(x[2] * up, x[6] * up),
+               pack_half(x[3] * up, x[7] * up));
+    }
+    fence_proxy_async_smem();
+    tcgen05_fence_before_sync();
+    __syncthreads();
+    tcgen05_fence_after_sync();
+    const uint32_t tmem = bars.tmem_base;
+
+    if (warp == kLoadWarp) {
+        // ---- raw tiles, half a block at a time ----
+        const uint32_t* table = a.cache.block_tables + static_cast<uint64_t>(seq) * a.cache.max_blocks;
+        uint64_t offset = 0;
+        for (uint32_t hb = 0; hb < 2u * n_blocks; ++hb) {
+            const uint32_t first = first_tile + hb * kHalfTiles;
+            if (hb % 8u == 0u) {   // one lane for each of the next 32 tiles
+                const uint32_t tile = first + lane;
+                if (tile < end_tile) {
+                    uint64_t phys = __ldg(table + tile / a.cache.tiles_per_block);
+                    if (phys >= a.cache.physical_blocks) {
+                        phys = 0;
+                        flags |= B2_ATTN_STATUS_BAD_BLOCK;
+                    }
+                    offset = kv4_tile_offset(a.cache, phys, kvh, tile % a.cache.tiles_per_block);
+                }
+            }
+            const uint32_t slot = hb % kRawSlots;
+            if (hb >= kRawSlots) mbar_wait(&bars.raw_empty[slot], (hb / kRawSlots - 1u) & 1u, abort);
+            const uint32_t live = first < end_tile ? min(kHalfTiles, end_tile - first) : 0u;
+            if (lane == 0) mbar_expect_tx(&bars.raw_full[slot], live * kv4_tile_bytes(D));
+            __syncwarp();
+            const uint32_t mine = lane - (hb % 8u) * kHalfTiles;   // wraps for lanes of other halves
+            if (mine < live) {
+                fence_proxy_async_smem();
+                bulk_load(raw32 + slot * L::kRawSlot + mine * L::kRawTile, a.cache.pages + offset, kv4_tile_bytes(D),
+                          &bars.raw_full[slot]);
+            }
+            __syncwarp();
+        }
+    } else if (warp >= kSoftmaxWarps && warp < kSoftmaxWarps + kExpandWarps) {
+        // ---- expansion ----
+        const uint32_t et = tid - kSoftmaxWarps * 32u;
+        for (uint32_t jb = 0; jb < n_blocks; ++jb) {
+            const uint32_t stage = jb % kStages, use = jb / kStages;
+            const uint32_t token0 = (first_tile + jb * kBlockTiles) * kKv4Tile;
+            if (use > 0) mbar_wait(&bars.k_empty[stage], (use - 1u) & 1u, abort);
+#pragma unroll 1
+            for (uint32_t half = 0; half < 2u; ++half) {
+                const uint32_t hb = 2u * jb + half, slot = hb % kRawSlots;
+                mbar_wait(&bars.raw_full[slot], (hb / kRawSlots) & 1u, abort);
+                expand_keys<D>(raw32 + slot * L::kRawSlot, k32 + stage * L::kKStage, half, et, token0 + half * kHalf,
+                               span.begin, span.end);
+            }
+            fence_proxy_async_smem();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&bars.k_full[stage]);
+            if (use > 0) mbar_wait(&bars.v_empty[stage], (use - 1u) & 1u, abort);
+#pragma unroll 1
+            for (uint32_t half = 0; half < 2u; ++half) {
+                const uint32_t hb = 2u * jb + half, slot = hb % kRawSlots;
+                expand_values<D>(raw32 + slot * L::kRawSlot, v32 + stage * L::kVStage, half, et, token0 + half * kHalf,
+                                 span.begin, span.end);
+                fence_proxy_async_smem();
+                __syncwarp();
+                if (lane == 0) mbar_arrive(&bars.raw_empty[slot]);
+            }
+            if (lane == 0) mbar_arrive(&bars.v_full[stage]);
+        }
+    } else if (warp == kIssueWarp) {
+        // ---- tcgen05 issue: for every block, each row tile's P V of the block before, then its Q K^T ----
+        const uint64_t dq = umma_desc_k_major_sw128(q32), dk = umma_desc_k_major_sw128(k32), dv = umma_desc_k_major_sw128(v32);
+        auto issue_pv = [&](uint32_t i, uint32_t jb) {
+            const uint64_t b = dv + ((jb % kStages) * L::kVStage >> 4);
+#pragma unroll
+            for (uint32_t kk = 0; kk < kBlock / 16u; ++kk) {
+                umma_ts(tmem + i * kTmemTile + kTmemO, tmem + i * kTmemTile + kk * 8u,
+                        b + (kk / 4u) * (D * 128u >> 4) + (kk % 4u) * 2u, idesc_f16(D), (jb | kk) != 0u ? 1u : 0u);
+            }
+        };
+        for (uint32_t jb = 0; jb <= n_blocks && n_blocks != 0u; ++jb) {
+            for (uint32_t i = 0; i < n_tiles; ++i) {
+                if (jb > 0u) {
+                    if (i == 0u) mbar_wait(&bars.v_full[(jb - 1u) % kStages], ((jb - 1u) / kStages) & 1u, abort);
+                    mbar_wait(&bars.p_full[i], (jb - 1u) & 1u, abort);
+                    tcgen05_fence_after_sync();
+                    if (elect_one()) {
+                        issue_pv(i, jb - 1u);
+                        if (i + 1u == n_tiles) umma_commit(&bars.v_empty[(jb - 1u) % kStages]);
+                        if (jb == n_blocks) umma_commit(&bars.o_full[i]);
+                    }
+                    __syncwarp();
+                }
+                if (jb < n_blocks) {
+                    if (i == 0u) {
+                        mbar_wait(&bars.k_full[jb % kStages], (jb / kStages) & 1u, abort);
+                        tcgen05_fence_after_sync();
+                    }
+                    if (elect_one()) {
+                        const uint64_t qa = dq + (i * (128u * D * 2u) >> 4), kb = dk + ((jb % kStages) * L::kKStage >> 4);
+#pragma unroll
+                        for (uint32_t kk = 0; kk < D / 16u; ++kk) {
+                            const uint64_t step = (kk / 4u) * (16384u >> 4) + (kk % 4u) * 2u;
+                            umma_ss(tmem + i * kTmemTile, qa + step, kb + step, idesc_f16(kBlock), kk != 0u ? 1u : 0u);
+                        }
+                        umma_commit(&bars.s_full[i]);
+                        if (i + 1u == n_tiles) umma_commit(&bars.k_empty[jb % kStages]);
+                    }
+                    __syncwarp();
+                }
+            }
+        }
+    } else if (warp / 4u < n_tiles) {
+        // ---- softmax: a thread is a row ----
+        const uint32_t i = warp / 4u;
+        const uint32_t r = i * 128u + (warp % 4u) * 32u + lane, gr = row0 + r;
+        const bool live = r < rows;
+        const uint32_t lane_base = tmem + i * kTmemTile + (((warp % 4u) * 32u) << 16);
+        const int64_t position64 = span.position0 + gr / rep;
+        uint32_t position = 0, begin = 0, end = 0;
+        if (live && position64 >= 0) {
+            position = static_cast<uint32_t>(position64);
+            end = max(position + 1u, span.prefix);
+            if (a.rules.window != 0u && position >= a.rules.window) begin = position - a.rules.window + 1u;
+        }
+        // every row of the warp sees tokens [all_begin, all_end); rows that are not live do not count
+        const uint32_t all_begin = __reduce_max_sync(0xFFFFFFFFu, live ? begin : 0u);
+        const uint32_t all_end = __reduce_min_sync(0xFFFFFFFFu, live ? end : 0xFFFFFFFFu);
+        const bool capped = a.rules.softcap != 0.0f, biased = a.rules.alibi_slopes != nullptr;
+        const float cap_log2 = a.rules.softcap * kLog2e;
+        const float slope = biased && live ? __ldg(a.rules.alibi_slopes + kvh * rep + gr % rep) * kLog2e : 0.0f;
+        const float row_factor = s_factor[r];
+        const float factor = capped || biased ? 1.0f : row_factor;   // of what fetch() leaves
+        float m = kNoMax, l = 0.0f;
+
+        for (uint32_t jb = 0; jb < n_blocks; ++jb) {
+            const uint32_t token0 = (first_tile + jb * kBlockTiles) * kKv4Tile;
+            mbar_wait(&bars.s_full[i], jb & 1u, abort);
+            tcgen05_fence_after_sync();
+            const bool masked = token0 < all_begin || token0 + kBlock > all_end;   // the same for the whole warp
+            // 32 scores of the row: raw products, or finished scores in log2 units where they are capped or biased
+            auto fetch = [&](uint32_t c, float (&x)[32]) {
+                uint32_t raw[32];
+                tmem_ld_32x32(lane_base + c * 32u, raw);
+                tmem_ld_wait();
+#pragma unroll
+                for (int e = 0; e < 32; ++e) x[e] = __uint_as_float(raw[e]);
+                if (capped) {
+#pragma unroll
+                    for (int e = 0; e < 32; ++e) {
+                        // tanh y = 1 - 2 / (1 + e^2y): exact at both ends, 2^-22 absolute between
+                        const float y = ex2(x[e] * (row_factor * (2.0f * kLog2e)));
+                        x[e] = fmaf(-2.0f * cap_log2, rcp(1.0f + y), cap_log2);
+                    }
+                } else if (biased) {
+#pragma unroll
+                    for (int e = 0; e < 32; ++e) x[e] *= row_factor;
+                }
+                if (biased) {
+                    const float away0 = static_cast<float>(static_cast<int>(position - (token0 + c * 32u)));
+#pragma unroll
+                    for (int e = 0; e < 32; ++e) x[e] = fmaf(-slope, fabsf(away0 - static_cast<float>(e)), x[e]);
+                }
+                if (masked) {
+                    const uint32_t t0 = token0 + c * 32u;
+#pragma unroll
+                    for (int e = 0; e < 32; ++e) {
+                        if (t0 + e < begin || t0 + e >= end) x[e] = -INFINITY;
+                    }
+                }
+            };
+            uint32_t p[64];
+            float sum, top;
+            auto weigh = [&]() {
+                sum = 0.0f;
+                top = -INFINITY;
+#pragma unroll
+                for (uint32_t c = 0; c < 4u; ++c) {
+                    float x[32];
+                    fetch(c, x);
+#pragma unroll
+                    for (int e = 0; e < 32; ++e) top = fmaxf(top, x[e]);
+#pragma unroll
+                    for (int e = 0; e < 32; e += 2) {
+                        const float p0 = ex2(fmaf(x[e], factor, -m)), p1 = ex2(fmaf(x[e + 1], factor, -m));
+                        sum += p0 + p1;
+                        p[c * 16u + e / 2] = pack_half(p0, p1);
+                    }
+                }
+                top *= factor;
+            };
+            weigh();
+            if (__any_sync(0xFFFFFFFFu, top > m + kSlack)) {
+                const float moved = fmaxf(m, top);
+                const float shrink = ex2(m - moved);
+                m = moved;
+                l *= shrink;
+                if (jb > 0u) {
+                    // P V of the block before completed before this block's scores did: O is at rest
+#pragma unroll 1
+                    for (uint32_t c = 0; c < D / 32u; ++c) {
+                        uint32_t o[32];
+                        tmem_ld_32x32(lane_base + kTmemO + c * 32u, o);
+                        tmem_ld_wait();
+#pragma unroll
+                        for (int e = 0; e < 32; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * shrink);
+                        tmem_st_32(lane_base + kTmemO + c * 32u, o);
+                    }
+                }
+                weigh();
+            }
+            l += sum;
+            tmem_st_32(lane_base, p);
+            tmem_st_32(lane_base + 32u, p + 32);
+            tmem_st_wait();
+            tcgen05_fence_before_sync();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&bars.p_full[i]);
+        }
+
+        // ---- epilogue ----
+        if (live && isnan(l)) flags |= B2_ATTN_STATUS_NAN_OR_POS_INF;
+        if (n_blocks != 0u) {
+            mbar_wait(&bars.o_full[i], 0u, abort);
+            tcgen05_fence_after_sync();
+        }
+        if (lane == 0 && *abort != 0) flags |= B2_ATTN_STATUS_TIMEOUT;
+        const uint64_t out_head = static_cast<uint64_t>(span.first + (live ? gr / rep : 0u)) * a.q_heads + kvh * rep + (live ? gr % rep : 0u);
+        const bool whole = n_splits == 1u;
+        if (whole && live && l == 0.0f && end > begin) flags |= B2_ATTN_STATUS_ALL_NEG_INF;
+        float* part = partials + (out_head * plan.splits + split) * (D + 4u);
+        if (!whole && live) *reinterpret_cast<float2*>(part) = make_float2(m, l);
+        const float inv = l == 0.0f ? 0.0f : 1.0f / l;
+#pragma unroll 1
+        for (uint32_t c = 0; c < D / 32u; ++c) {
+            uint32_t raw[32];
+            if (n_blocks != 0u) {
+                tmem_ld_32x32(lane_base + kTmemO + c * 32u, raw);
+                tmem_ld_wait();
+            }
+            if (!live) continue;
+            float o[32];
+#pragma unroll
+            for (int e = 0; e < 32; ++e) o[e] = l == 0.0f ? 0.0f : __uint_as_float(raw[e]);
+            if (whole) {
+                uint4* dst = reinterpret_cast<uint4*>(static_cast<__nv_bfloat16*>(a.ctx16) + out_head * D + c * 32u);
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    uint32_t w[4];
+#pragma unroll
+                    for (int k = 0; k < 4; ++k) {
+                        const __nv_bfloat162 b = __floats2bfloat162_rn(o[8 * e + 2 * k] * inv, o[8 * e + 2 * k + 1] * inv);
+                        w[k] = *reinterpret_cast<const uint32_t*>(&b);
+                    }
+                    dst[e] = make_uint4(w[0], w[1], w[2], w[3]);
+                }
+            } else {
+                float4* dst = reinterpret_cast<float4*>(part + 4u + c * 32u);
+#pragma unroll
+                for (int e = 0; e < 8; ++e) dst[e] = make_float4(o[4 * e], o[4 * e + 1], o[4 * e + 2], o[4 * e + 3]);
+            }
+        }
+    }
+    if (flags != 0u) kv4_flag(a.status, flags);
+    tcgen05_fence_before_sync();
+    __syncthreads();
+    if (warp == kIssueWarp) tmem_dealloc(tmem, kTmemColumns);
+}
+
+// Joins the splits of every (row, query head) that has more than one.
+template <int D>
+__global__ void __launch_bounds__(D / 4)
+kv4_chunk_merge_kernel(const Kv4AttentionArgs a, const float* __restrict__ partials, const ChunkPlan plan) {
+    pdl_launch_dependents();
+    const uint64_t out_head = blockIdx.x;
+    const uint32_t row = static_cast<uint32_t>(out_head / a.q_heads), rep = a.q_heads / a.cache.kv_heads;
+    const uint32_t head = static_cast<uint32_t>(out_head % a.q_heads) % rep;
+    const RowSpan mine = row_span(a, row);   // inputs of the call, not of the kernel before
+    uint32_t n_splits = 0;
+    if (mine.owned) {
+        const uint32_t first = min(__ldg(a.chunk_starts + mine.seq), a.rows);
+        const TileSpan span = tile_span(a, mine.seq, rep, ((row - first) * rep + head) / kRows * kRows);
+        if ((row - first) < span.tokens) {
+            const uint32_t tile0 = span.begin / kKv4Tile;
+            const uint32_t tiles = span.end > span.begin ? (span.end - 1u) / kKv4Tile + 1u - tile0 : 0u;
+            n_splits = ((tiles + kBlockTiles - 1u) / kBlockTiles + plan.blocks_per_split - 1u) / plan.blocks_per_split;
+        }
+    }
+    pdl_wait();   // every CTA waits, so that this grid never ends before the one it follows
+    if (n_splits <= 1u) return;
+    join_splits<D>(a, partials + out_head * plan.splits * (D + 4u), out_head, n_splits, threadIdx.x * 4u,
+                   mine.end > mine.begin);
+}
+
+// One CTA holds an SM. Where the row tiles leave SMs idle, the blocks of each are split over several CTAs, down to
+// four blocks, below which a CTA's own set-up costs as much as its blocks.
+ChunkPlan chunk_plan(int sm_count, uint32_t n_seq, uint32_t q_heads, uint32_t kv_heads, uint32_t max_chunk, uint32_t max_seq_len) {
+    const uint64_t rep = q_heads / kv_heads;
+    const uint64_t sms = sm_count > 0 ? static_cast<uint64_t>(sm_count) : 148u;
+    const uint64_t row_tiles = (max_chunk * rep + kRows - 1u) / kRows;
+    const uint64_t blocks = (static_cast<uint64_t>(max_seq_len) + kBlock - 1u) / kBlock + 1u;   // a window may start inside a tile
+    const uint64_t ctas = row_tiles * n_seq * kv_heads;
+    uint64_t per = blocks;
+    if (ctas < sms) per = (blocks * ctas + sms - 1u) / sms;
+    if (per < 4u) per = 4u;
+    return ChunkPlan{static_cast<uint32_t>(row_tiles), static_cast<uint32_t>((blocks + per - 1u) / per), static_cast<uint32_t>(per)};
+}
+
+template <int D>
+int32_t launch_one(const DeviceContext& ctx, const Kv4AttentionArgs& a, float* partials, const ChunkPlan& plan,
+                   cudaStream_t stream) {
+    static PerDeviceOnce configured;
+    B2_TRY(once_per_device(configured, ctx.device, []() -> int32_t {
+        B2_CUDA_TRY(cudaFuncSetAttribute(kv4_chunk_kernel<D>, cudaFuncAttributeMaxDynamicSharedMemorySize, Layout<D>::kTotal));
+        return B2_STATUS_OK;
+    }));
+    const uint64_t ctas = static_cast<uint64_t>(plan.row_tiles) * a.cache.n_seq * a.cache.kv_heads * plan.splits;
+    const uint64_t merges = static_cast<uint64_t>(a.rows) * a.q_heads;
+    if (ctas > 0x7FFFFFFFull || merges > 0x7FFFFFFFull) return fail(B2_STATUS_OVERFLOW, "paged attention batch too large");
+    kv4_chunk_kernel<D><<<static_cast<unsigned>(ctas), kThreads, Layout<D>::kTotal, stream>>>(a, partials, plan);
+    B2_CUDA_TRY(cudaGetLastError());
+    if (plan.splits <= 1u) return B2_STATUS_OK;
+    cudaLaunchConfig_t config{};
+    config.gridDim = dim3(static_cast<unsigned>(merges));
+    config.blockDim = dim3(D / 4);
+    config.stream = stream;
+    cudaLaunchAttribute attribute[1];
+    attribute[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attribute[0].val.programmaticStreamSerializationAllowed = 1;
+    config.attrs = attribute;
+    config.numAttrs = 1;
+    B2_CUDA_TRY(cudaLaunchKernelEx(&config, kv4_chunk_merge_kernel<D>, a, const_cast<const float*>(partials), plan));
+    return B2_STATUS_OK;
+}
+
+}  // namespace
+
+bool kv4_chunk_supported(uint32_t head_width, uint32_t q_heads, uint32_t kv_heads, uint32_t max_chunk) {
+    const uint64_t rows = static_cast<uint64_t>(max_chunk) * (q_heads / kv_heads);
+    return (head_width == 64u || head_width == 128u) && rows >= 16u && rows <= 0x7FFFFF00u;
+}
+
+size_t kv4_chunk_workspace_bytes(int sm_count, uint32_t n_seq, uint64_t rows, uint32_t q_heads, uint32_t kv_heads,
+                                 uint32_t head_width, uint32_t max_chunk, uint32_t max_seq_len) {
+    const ChunkPlan plan = chunk_plan(sm_count, n_seq, q_heads, kv_heads, max_chunk, max_seq_len);
+    if (plan.splits <= 1u) return 0;
+    return static_cast<size_t>(rows) * q_heads * plan.splits * (head_width + 4u) * sizeof(float);
+}
+
+int32_t launch_kv4_chunk(const DeviceContext& ctx, const Kv4AttentionArgs& a, void* workspace, size_t workspace_bytes,
+                         cudaStream_t stream) {
+    const size_t need = kv4_chunk_workspace_bytes(ctx.sm_count, a.cache.n_seq, a.rows, a.q_heads, a.cache.kv_heads,
+                                                  a.cache.head_width, a.max_chunk, a.max_seq_len);
+    if (need > workspace_bytes) {
+        return fail(B2_STATUS_INVALID_ARGUMENT, "paged attention workspace too small: need %zu bytes, got %zu", need,
+                    workspace_bytes);
+    }
+    const ChunkPlan plan = chunk_plan(ctx.sm_count, a.cache.n_seq, a.q_heads, a.cache.kv_heads, a.max_chunk, a.max_seq_len);
+    float* partials = static_cast<float*>(workspace);
+    return a.cache.head_width == 64u ? launch_one<64>(ctx, a, partials, plan, stream)
+                                     : launch_one<128>(ctx, a, partials, plan, stream);
+}
+
+}  // namespace b2

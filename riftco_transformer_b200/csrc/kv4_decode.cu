@@ -37,15 +37,8 @@ constexpr int kWarps = 4;
 constexpr int kPair = 2;              // tiles a warp works on at once: 32 tokens, one for each lane to guard
 // Pairs a warp holds in shared memory, one being worked on and the rest in flight.
 __host__ __device__ constexpr int slots_of(int d) { return d == 64 ? 4 : 2; }
-constexpr float kLog2e = 1.4426950408889634f;
-constexpr float kNoMax = -FLT_MAX;    // running maximum before the first score (log2 units)
 constexpr float kSlack = 2.0f;        // p may reach 2^kSlack before the maximum is moved
 
-__device__ __forceinline__ float ex2(float x) {
-    float y;
-    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
-    return y;
-}
 __device__ __forceinline__ void ldsm4(uint32_t (&r)[4], uint32_t addr) {
     asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0,%1,%2,%3}, [%4];"
                  : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
@@ -90,12 +83,6 @@ __device__ __forceinline__ void lds_words(uint32_t (&v)[N], uint32_t addr) {
         }
     }
 }
-__device__ __forceinline__ float low_half(uint32_t pair) { return __low2float(*reinterpret_cast<__half2*>(&pair)); }
-__device__ __forceinline__ float high_half(uint32_t pair) { return __high2float(*reinterpret_cast<__half2*>(&pair)); }
-__device__ __forceinline__ uint32_t pack_half(float lo, float hi) {
-    const __half2 h = __floats2half2_rn(lo, hi);
-    return *reinterpret_cast<const uint32_t*>(&h);
-}
 // Two codes of a word, 16 bits apart, as fp16 numbers code - 8 (exact: 1024 + 16 * 15 fits 11 bits).
 template <int NIBBLE>
 __device__ __forceinline__ uint32_t codes_of(uint32_t word) {
@@ -113,50 +100,6 @@ __device__ __forceinline__ uint32_t codes_of(uint32_t word) {
 }
 // The first 11 bits of x; x minus it is exact.
 __device__ __forceinline__ float first_part(float x) { return __uint_as_float(__float_as_uint(x) & 0xFFFFE000u); }
-
-__device__ __forceinline__ void bulk_load(uint32_t dst32, const void* src, uint32_t bytes, uint64_t* bar) {
-    asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];"
-                 ::"r"(dst32), "l"(src), "r"(bytes), "r"(sm100::smem_u32(bar))
-                 : "memory");
-}
-
-// What a row sees: tokens [begin, end) of sequence `seq`, its own position, and whether the caller's
-// lengths were out of bounds.
-struct RowSpan {
-    uint32_t seq, position, begin, end;
-    bool bad;
-    bool owned;   // false: a row behind the last sequence, which is left as it was
-};
-__device__ __forceinline__ RowSpan row_span(const Kv4AttentionArgs& a, uint32_t row) {
-    RowSpan r{row, 0, 0, 0, false, true};
-    uint32_t back = 0;   // tokens after this one
-    if (a.chunk_starts != nullptr) {
-        uint32_t lo = 0, hi = a.cache.n_seq;   // the last sequence that starts at or before `row`
-        while (lo + 1u < hi) {
-            const uint32_t mid = (lo + hi) / 2u;
-            if (__ldg(a.chunk_starts + mid) <= row) lo = mid; else hi = mid;
-        }
-        r.seq = lo;
-        const uint32_t first = __ldg(a.chunk_starts + lo), last = __ldg(a.chunk_starts + lo + 1u);
-        r.owned = row >= first && row < last;
-        if (!r.owned) return r;
-        back = last - 1u - row;
-    }
-    uint32_t len = __ldg(a.seq_lens + r.seq);
-    if (len > a.max_seq_len) {
-        len = a.max_seq_len;
-        r.bad = true;
-    }
-    if (back >= len) {
-        r.bad = r.bad || a.chunk_starts != nullptr;   // more new tokens than the sequence holds
-        return r;
-    }
-    r.position = len - 1u - back;
-    r.end = r.position + 1u;
-    if (a.rules.prefix_lens != nullptr) r.end = max(r.end, min(len, __ldg(a.rules.prefix_lens + r.seq)));
-    if (a.rules.window != 0u && r.position >= a.rules.window) r.begin = r.position - a.rules.window + 1u;
-    return r;
-}
 
 struct SplitPlan {
     uint32_t splits;          // most splits of a row
@@ -647,20 +590,8 @@ kv4_decode_kernel(const Kv4AttentionArgs a, float* __restrict__ partials, const 
             }
             continue;
         }
-        if (ll == 0.0f) {   // nothing seen, or every score -infinity
-            if (tiles != 0u && c == 0) kv4_flag(a.status, B2_ATTN_STATUS_ALL_NEG_INF);
-            o = make_float4(0.f, 0.f, 0.f, 0.f);
-            ll = 1.0f;
-        }
-        o = make_float4(o.x / ll, o.y / ll, o.z / ll, o.w / ll);
-        if (a.ctx != nullptr) *reinterpret_cast<float4*>(a.ctx + out_head * D + c) = o;
-        if (a.ctx16 != nullptr) {
-            const __nv_bfloat162 lo = __floats2bfloat162_rn(o.x, o.y), hi = __floats2bfloat162_rn(o.z, o.w);
-            uint2 packed;
-            packed.x = *reinterpret_cast<const uint32_t*>(&lo);
-            packed.y = *reinterpret_cast<const uint32_t*>(&hi);
-            *reinterpret_cast<uint2*>(static_cast<__nv_bfloat16*>(a.ctx16) + out_head * D + c) = packed;
-        }
+        if (ll == 0.0f && tiles != 0u && c == 0) kv4_flag(a.status, B2_ATTN_STATUS_ALL_NEG_INF);
+        put_context<D>(a, out_head, c, o, ll);
     }
 }
 
@@ -677,51 +608,7 @@ kv4_merge_kernel(const Kv4AttentionArgs a, const float* __restrict__ partials, c
     const uint32_t n_splits = max(1u, (tiles + plan.tiles_per_split - 1u) / plan.tiles_per_split);
     sm100::pdl_wait();   // every CTA waits, so that this grid never ends before the one it follows
     if (n_splits <= 1u || !span.owned) return;
-    const float* src = partials + out_head * plan.splits * (D + 4u);
-    const uint32_t c = threadIdx.x * 4u;
-    float mm = kNoMax, ll = 0.0f;
-    float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
-    for (uint32_t s0 = 0; s0 < n_splits; s0 += 8u) {
-        float2 ml[8];
-        float4 x[8];
-#pragma unroll
-        for (uint32_t u = 0; u < 8u; ++u) {   // all loads before the first use
-            const bool live = s0 + u < n_splits;
-            const float* part = src + (s0 + u) * (D + 4u);
-            ml[u] = live ? *reinterpret_cast<const float2*>(part) : make_float2(kNoMax, 0.0f);
-            x[u] = live ? *reinterpret_cast<const float4*>(part + 4u + c) : make_float4(0.f, 0.f, 0.f, 0.f);
-        }
-        float top = mm;
-#pragma unroll
-        for (uint32_t u = 0; u < 8u; ++u) top = fmaxf(top, ml[u].x);
-        const float keep = ex2(mm - top);
-        mm = top;
-        ll *= keep;
-        o = make_float4(o.x * keep, o.y * keep, o.z * keep, o.w * keep);
-#pragma unroll
-        for (uint32_t u = 0; u < 8u; ++u) {   // in split order
-            const float f = ex2(ml[u].x - mm);
-            ll = fmaf(ml[u].y, f, ll);
-            o.x = fmaf(x[u].x, f, o.x);
-            o.y = fmaf(x[u].y, f, o.y);
-            o.z = fmaf(x[u].z, f, o.z);
-            o.w = fmaf(x[u].w, f, o.w);
-        }
-    }
-    if (ll == 0.0f) {
-        if (c == 0) kv4_flag(a.status, B2_ATTN_STATUS_ALL_NEG_INF);
-        o = make_float4(0.f, 0.f, 0.f, 0.f);
-        ll = 1.0f;
-    }
-    o = make_float4(o.x / ll, o.y / ll, o.z / ll, o.w / ll);
-    if (a.ctx != nullptr) *reinterpret_cast<float4*>(a.ctx + out_head * D + c) = o;
-    if (a.ctx16 != nullptr) {
-        const __nv_bfloat162 lo = __floats2bfloat162_rn(o.x, o.y), hi = __floats2bfloat162_rn(o.z, o.w);
-        uint2 packed;
-        packed.x = *reinterpret_cast<const uint32_t*>(&lo);
-        packed.y = *reinterpret_cast<const uint32_t*>(&hi);
-        *reinterpret_cast<uint2*>(static_cast<__nv_bfloat16*>(a.ctx16) + out_head * D + c) = packed;
-    }
+    join_splits<D>(a, partials + out_head * plan.splits * (D + 4u), out_head, n_splits, threadIdx.x * 4u, true);
 }
 
 uint32_t heads_together(uint32_t rep) { return rep <= 4u ? 4u : 8u; }
