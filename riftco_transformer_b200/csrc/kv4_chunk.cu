@@ -2,8 +2,8 @@
 //
 // A row is (new token, query head of one K/V head): token i and head h of the group are row i * rep + h, so
 // that any number of query heads per K/V head fills whole tiles. A CTA takes 256 rows (two tiles of 128
-// = two M of tcgen05.mma) of one K/V head and walks the cached tokens they see in blocks of 128:
-//   S = Q K^T          [128 x 128], A and B in shared memory, FP32 in tensor memory
+// = two M of tcgen05.mma) of one K/V head and walks the cached tokens they see in blocks of 64:
+//   S = Q K^T          [128 x 64], A and B in shared memory, FP32 in tensor memory
 //   P = 2^(S - m)      fp16, written over S
 //   O += P V           A = P in tensor memory, B = V^T in shared memory, FP32 in tensor memory
 // Unlike in the single-row kernel (kv4_decode.cu) a block of K and V serves 256 rows, so its codes are expanded
@@ -17,12 +17,15 @@
 // rescaled in tensor memory, only when a score passes it by 8 in log2 units: P may reach 2^8, and a row
 // sum of 2^8 * 10^5 tokens stays far inside FP32.
 //
-// What bounds it: for a block and a tile the two products take 128 * 128 * D * 2 / 4096 = 1024 cycles of the
-// tensor core at D = 128, the 16384 exponentials as many of the 16-per-cycle unit: the two tiles alternate so
-// that one's products run under the other's softmax.
+// What bounds it: per 64 tokens and row tile (D = 128) the two products take 400 + 256 cycles of the tensor core
+// (N = 64 reads Q faster than it multiplies) and the exponentials 512 of the 16-per-cycle unit, that is 1312 and 1024
+// for the CTA. A row tile has two S buffers, so that the next scores are made while these are weighed: with blocks of
+// 128 tokens, whose S and O fill tensor memory, softmax and products of a tile took turns and a 4096-token prompt
+// 203 us.
 //
-// Roles (14 warps): 0-3 and 4-7 softmax and epilogue of the two tiles (thread = row = tensor-memory lane), 8-11
-// expansion, 12 bulk copies of raw tiles, 13 the tcgen05 issue. Every wait is bounded.
+// Roles (20 warps): 0-3 and 4-7 softmax and epilogue of the two tiles (thread = row = tensor-memory lane), 8-11
+// and 12-15 expansion of keys and of values, 16 bulk copies of raw tiles, 17 and 18 the tcgen05 issue of a
+// tile each (19 completes the warpgroup whose registers go to the softmax). Every wait is bounded.
 #include "kv4.cuh"
 
 #include <cmath>
@@ -32,13 +35,18 @@ namespace {
 
 using namespace sm100;
 
-constexpr uint32_t kRows = 256, kBlock = 128, kHalf = 64;   // rows of a CTA, tokens of a block and of half of one
-constexpr uint32_t kBlockTiles = kBlock / kKv4Tile, kHalfTiles = kHalf / kKv4Tile;
-constexpr uint32_t kSoftmaxWarps = 8, kExpandWarps = 4;
-constexpr uint32_t kLoadWarp = 12, kIssueWarp = 13;
-constexpr uint32_t kThreads = 14 * 32;
-constexpr uint32_t kRawSlots = 3, kStages = 2;
-constexpr uint32_t kTmemColumns = 512, kTmemTile = 256, kTmemO = 128;   // a tile's S (and P) and its O
+constexpr uint32_t kRows = 256, kBlock = 64;   // rows of a CTA, tokens of a block
+constexpr uint32_t kBlockTiles = kBlock / kKv4Tile;
+constexpr uint32_t kExpandWarps = 4;   // for keys and for values each
+constexpr uint32_t kKeyWarp = 8, kValueWarp = 12, kLoadWarp = 16, kIssueWarp = 17;   // and 18
+constexpr uint32_t kThreads = 20 * 32;
+// Registers of a thread by warpgroup, against 96 at the launch (the most that 20 warps of 640 threads can have):
+// softmax 2 x 128 x 136 + expansion 2 x 128 x 80 + the last 128 x 48 = 640 x 96, what the launch holds.
+constexpr int kSoftmaxRegisters = 136, kExpandRegisters = 80, kOtherRegisters = 48;
+static_assert(256 * kSoftmaxRegisters + 256 * kExpandRegisters + 128 * kOtherRegisters <= 640 * 96, "more than the launch holds");
+constexpr uint32_t kRawSlots = 3;
+constexpr uint32_t kStages = 4;   // of expanded keys and of values
+constexpr uint32_t kTmemColumns = 512, kTmemTile = 256, kTmemO = 128;   // a tile's two S (and P) of 64 columns, its O
 constexpr float kSlack = 8.0f;
 
 template <int D>
@@ -46,14 +54,17 @@ struct Layout {
     static constexpr uint32_t kQ = kRows * D * 2, kKStage = kBlock * D * 2, kVStage = kBlock * D * 2;
     // 16 bytes apart, so that the same word of four tiles lies in different banks
     static constexpr uint32_t kRawTile = kv4_tile_bytes(D) + 16u;
-    static constexpr uint32_t kRawSlot = kHalfTiles * kRawTile;
+    static constexpr uint32_t kRawSlot = kBlockTiles * kRawTile;
     static constexpr uint32_t kTotal = kQ + kStages * (kKStage + kVStage) + kRawSlots * kRawSlot + 1024u;
 };
 
 struct Barriers {
     uint64_t raw_full[kRawSlots], raw_empty[kRawSlots];
     uint64_t k_full[kStages], k_empty[kStages], v_full[kStages], v_empty[kStages];
-    uint64_t s_full[2], p_full[2], o_full[2];
+    uint64_t s_full[2][2], p_full[2][2];   // [tile][buffer]
+    // P V of a block and of the last one. Whoever waits for o_done knows that the one before has completed (the
+    // scores it has seen were issued after it), so that a parity tells; at the end only two before that is known.
+    uint64_t o_done[2], o_full[2];
     uint32_t tmem_base;
     uint32_t abort;
 };
@@ -104,6 +115,10 @@ __device__ __forceinline__ TileSpan tile_span(const Kv4AttentionArgs& a, uint32_
     return s;
 }
 
+template <int N>
+__device__ __forceinline__ void registers_up() { asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(N)); }
+template <int N>
+__device__ __forceinline__ void registers_down() { asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(N)); }
 __device__ __forceinline__ float rcp(float x) {
     float y;
     asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
@@ -174,73 +189,85 @@ __device__ __forceinline__ uint32_t expand(uint32_t word, __half2 scale, __half2
     return *reinterpret_cast<const uint32_t*>(&c);
 }
 __device__ __forceinline__ __half2 as_half2(uint32_t x) { return *reinterpret_cast<__half2*>(&x); }
-// Whether the scale or the base of a pair is an infinity or a NaN.
-__device__ __forceinline__ bool not_finite(uint32_t pair) {
-    return (pair & 0x7C00u) == 0x7C00u || (pair & 0x7C000000u) == 0x7C000000u;
-}
+// Nonzero where the scale or the base of a pair is an infinity or a NaN.
+__device__ __forceinline__ uint32_t not_finite(uint32_t pair) { return ((pair & 0x7C007C00u) + 0x04000400u) & 0x80008000u; }
 
-// Half a block (64 tokens) of keys: 32 channels of one token per step and thread, rows of the tile in token order.
+// A block of keys: 32 channels of one token per step and thread, rows of the tile in token order. `whole`: every
+// one of the tokens is seen by some row.
 template <int D>
-__device__ __forceinline__ void expand_keys(uint32_t raw32, uint32_t stage32, uint32_t half, uint32_t tid, uint32_t token0,
+__device__ __forceinline__ void expand_keys(uint32_t raw32, uint32_t stage32, uint32_t tid, uint32_t token0, bool whole,
                                             uint32_t begin, uint32_t end) {
-    constexpr uint32_t G = D / 64;
+    constexpr uint32_t G = D / 64, kSteps = kBlock * (D / 32) / (kExpandWarps * 32u);
+    const uint32_t tk = tid % kBlock;   // lanes: consecutive tokens
+    const uint32_t tile32 = raw32 + (tk / 16u) * Layout<D>::kRawTile;
+    const uint32_t row32 = stage32 + tk * 128u;
+    uint32_t pair[kSteps];
+    uint4 raw[kSteps];
 #pragma unroll
-    for (uint32_t u = tid; u < kHalf * (D / 32); u += kExpandWarps * 32u) {
-        const uint32_t tk = u % kHalf, j = u / kHalf;   // lanes: consecutive tokens
-        const uint32_t tile32 = raw32 + (tk / 16u) * Layout<D>::kRawTile;
-        const uint32_t at = (tk % 16u) * (4u * G);
-        uint32_t pair = lds32(tile32 + 8u * D + at + (j / 2u) * 4u);
-        const uint32_t token = token0 + tk;
-        if (token < begin || token >= end) {
-            pair = 0u;
-        } else if (j == 0u) {
-            // A value that is not finite must not meet the zero weight of a row that does not see it: its group
-            // is expanded as zeros (expand_values), and the token's scores, which such a row masks, become NaN.
-            for (uint32_t gr = 0; gr < G; ++gr) {
-                if (not_finite(lds32(tile32 + kv4_half_bytes(D) + 8u * D + at + gr * 4u))) pair = 0x7FFF7FFFu;
-            }
+    for (uint32_t n = 0; n < kSteps; ++n) {   // chunk of 32 channels j = tid / 64 + 2n, group j / 2 = n
+        pair[n] = lds32(tile32 + 8u * D + (tk % 16u) * (4u * G) + n * 4u);
+        raw[n] = lds128(tile32 + (tid / kBlock + 2u * n) * 256u + (tk % 16u) * 16u);
+    }
+    // A value that is not finite must not meet the zero weight of a row that does not see it: its group is
+    // expanded as zeros (expand_values), and the token's scores, which such a row masks, become NaN.
+    if (tid < kBlock) {
+#pragma unroll
+        for (uint32_t gr = 0; gr < G; ++gr) {
+            if (not_finite(lds32(tile32 + kv4_half_bytes(D) + 8u * D + (tk % 16u) * (4u * G) + gr * 4u))) pair[0] = 0x7FFF7FFFu;
         }
-        const uint4 raw = lds128(tile32 + j * 256u + (tk % 16u) * 16u);
-        const __half2 scale = __half2half2(__low2half(as_half2(pair))), base = __half2half2(__high2half(as_half2(pair)));
-        const uint32_t row = half * kHalf + tk;
-        const uint32_t row32 = stage32 + (j / 2u) * (kBlock * 128u) + row * 128u;
-        const uint32_t words[4] = {raw.x, raw.y, raw.z, raw.w};
+    }
+    if (!whole && (token0 + tk < begin || token0 + tk >= end)) {
+#pragma unroll
+        for (uint32_t n = 0; n < kSteps; ++n) pair[n] = 0u;
+    }
+#pragma unroll
+    for (uint32_t n = 0; n < kSteps; ++n) {
+        const __half2 scale = __half2half2(__low2half(as_half2(pair[n]))), base = __half2half2(__high2half(as_half2(pair[n])));
+        const uint32_t words[4] = {raw[n].x, raw[n].y, raw[n].z, raw[n].w};
 #pragma unroll
         for (uint32_t w = 0; w < 4u; ++w) {
-            const uint32_t unit = (j % 2u) * 4u + w;
-            sts128(row32 + ((unit ^ (row & 7u)) << 4), expand<0>(words[w], scale, base), expand<1>(words[w], scale, base),
-                   expand<2>(words[w], scale, base), expand<3>(words[w], scale, base));
+            const uint32_t unit = (tid / kBlock) * 4u + w;
+            sts128(row32 + n * (kBlock * 128u) + ((unit ^ (tk & 7u)) << 4), expand<0>(words[w], scale, base),
+                   expand<1>(words[w], scale, base), expand<2>(words[w], scale, base), expand<3>(words[w], scale, base));
         }
     }
 }
 
-// Half a block of values, transposed: eight channels of eight tokens per step and thread, rows of the tile are channels.
+// A block of values, transposed: eight channels of eight tokens per thread, rows of the tile are channels.
 template <int D>
-__device__ __forceinline__ void expand_values(uint32_t raw32, uint32_t stage32, uint32_t half, uint32_t tid,
-                                              uint32_t token0, uint32_t begin, uint32_t end) {
+__device__ __forceinline__ void expand_values(uint32_t raw32, uint32_t stage32, uint32_t tid, uint32_t token0, bool whole,
+                                              uint32_t begin, uint32_t end) {
     constexpr uint32_t G = D / 64;
     if (tid >= D) return;
     const uint32_t octet = tid % 8u, word = tid / 8u;   // tokens 8 octet.., channels 8 word..
     const uint32_t j = word / 4u;
     const uint32_t tile32 = raw32 + (octet / 2u) * Layout<D>::kRawTile + kv4_half_bytes(D);
     const uint32_t slot0 = (octet & 1u) * 8u;
+    uint32_t pair[8], code[8];
+#pragma unroll
+    for (uint32_t e = 0; e < 8u; ++e) {
+        pair[e] = lds32(tile32 + 8u * D + (slot0 + e) * (4u * G) + (j / 2u) * 4u);
+        code[e] = lds32(tile32 + j * 256u + (slot0 + e) * 16u + (word % 4u) * 4u);
+    }
+    uint32_t bad = whole ? 0u : 1u;
+#pragma unroll
+    for (uint32_t e = 0; e < 8u; ++e) bad |= not_finite(pair[e]);
+    if (bad != 0u) {
+#pragma unroll
+        for (uint32_t e = 0; e < 8u; ++e) {
+            const uint32_t token = token0 + octet * 8u + e;
+            if (token < begin || token >= end || not_finite(pair[e])) pair[e] = 0u;
+        }
+    }
     uint32_t scale[4], base[4], lo[4], hi[4];
 #pragma unroll
     for (uint32_t k = 0; k < 4u; ++k) {
-        uint32_t pair[2], code[2];
-#pragma unroll
-        for (uint32_t e = 0; e < 2u; ++e) {
-            const uint32_t slot = slot0 + 2u * k + e, token = token0 + octet * 8u + 2u * k + e;
-            pair[e] = lds32(tile32 + 8u * D + slot * (4u * G) + (j / 2u) * 4u);
-            if (token < begin || token >= end || not_finite(pair[e])) pair[e] = 0u;
-            code[e] = lds32(tile32 + j * 256u + slot * 16u + (word % 4u) * 4u);
-        }
-        scale[k] = __byte_perm(pair[0], pair[1], 0x5410);
-        base[k] = __byte_perm(pair[0], pair[1], 0x7632);
-        lo[k] = __byte_perm(code[0], code[1], 0x5410);   // channels 0..3 of both tokens
-        hi[k] = __byte_perm(code[0], code[1], 0x7632);   // channels 4..7
+        scale[k] = __byte_perm(pair[2 * k], pair[2 * k + 1], 0x5410);
+        base[k] = __byte_perm(pair[2 * k], pair[2 * k + 1], 0x7632);
+        lo[k] = __byte_perm(code[2 * k], code[2 * k + 1], 0x5410);   // channels 0..3 of both tokens
+        hi[k] = __byte_perm(code[2 * k], code[2 * k + 1], 0x7632);   // channels 4..7
     }
-    const uint32_t column32 = stage32 + half * (D * 128u) + word * 1024u;
+    const uint32_t column32 = stage32 + word * 1024u;
     auto put = [&](uint32_t n, uint32_t x0, uint32_t x1, uint32_t x2, uint32_t x3) {
         sts128(column32 + n * 128u + ((octet ^ n) << 4), x0, x1, x2, x3);
     };
@@ -258,6 +285,76 @@ __device__ __forceinline__ void expand_values(uint32_t raw32, uint32_t stage32, 
     B2_KV4_PUT(6, hi);
     B2_KV4_PUT(7, hi);
 #undef B2_KV4_PUT
+}
+
+// Two FP32 operations in one instruction.
+__device__ __forceinline__ uint64_t two(float x, float y) {
+    uint64_t r;
+    asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(x), "f"(y));
+    return r;
+}
+__device__ __forceinline__ void parts(uint64_t r, float& x, float& y) { asm("mov.b64 {%0, %1}, %2;" : "=f"(x), "=f"(y) : "l"(r)); }
+__device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
+    uint64_t r;
+    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+    return r;
+}
+__device__ __forceinline__ uint64_t mul2(uint64_t a, uint64_t b) {
+    uint64_t r;
+    asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+    return r;
+}
+__device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
+    uint64_t r;
+    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+    return r;
+}
+
+// Waits for this thread's tensor-memory loads; x is what the last of them wrote, named so that no use of it is
+// moved before the wait.
+__device__ __forceinline__ void tmem_ld_ready(uint32_t* x) {
+    asm volatile("tcgen05.wait::ld.sync.aligned;"
+                 : "+r"(x[0]), "+r"(x[1]), "+r"(x[2]), "+r"(x[3]), "+r"(x[4]), "+r"(x[5]), "+r"(x[6]), "+r"(x[7]),
+                   "+r"(x[8]), "+r"(x[9]), "+r"(x[10]), "+r"(x[11]), "+r"(x[12]), "+r"(x[13]), "+r"(x[14]),
+                   "+r"(x[15]), "+r"(x[16]), "+r"(x[17]), "+r"(x[18]), "+r"(x[19]), "+r"(x[20]), "+r"(x[21]),
+                   "+r"(x[22]), "+r"(x[23]), "+r"(x[24]), "+r"(x[25]), "+r"(x[26]), "+r"(x[27]), "+r"(x[28]),
+                   "+r"(x[29]), "+r"(x[30]), "+r"(x[31])
+                 :
+                 : "memory");
+}
+__device__ __forceinline__ void tmem_ld_32(uint32_t taddr, uint32_t* x) { tmem_ld_32x32(taddr, *reinterpret_cast<uint32_t(*)[32]>(x)); }
+
+// cap * tanh(x * f) for 64 values. Up to |y| = 0.7, where capped scores mostly are, y times a polynomial in y^2
+// (least-squares fit of tanh y / y, weighted to even out its largest error: 5e-8); beyond, 1 - 2 / (1 + e^2y). On the
+// exponential unit alone a capped block would take three times as long as its matrix products.
+__device__ __forceinline__ void cap_scores(uint32_t (&x)[64], float f, float cap) {
+    float most = 0.0f;
+#pragma unroll
+    for (int e = 0; e < 64; e += 2) {
+        most = fmaxf(most, fmaxf(fabsf(__uint_as_float(x[e])), fabsf(__uint_as_float(x[e + 1]))));
+    }
+    if (__any_sync(0xFFFFFFFFu, !(most * f <= 0.7f))) {
+#pragma unroll
+        for (int e = 0; e < 64; ++e) {
+            const float y = ex2(__uint_as_float(x[e]) * (f * (2.0f * kLog2e)));
+            x[e] = __float_as_uint(fmaf(-2.0f * cap, rcp(1.0f + y), cap));
+        }
+        return;
+    }
+    const uint64_t f2 = two(f, f), cap2 = two(cap, cap);
+    const float c[6] = {1.0f, -0.3333314061164856f, 0.13328571617603302f, -0.053534939885139465f,
+                        0.020045235753059387f, -0.005105267278850079f};
+#pragma unroll
+    for (int e = 0; e < 64; e += 2) {
+        const uint64_t y = mul2(two(__uint_as_float(x[e]), __uint_as_float(x[e + 1])), f2), z = mul2(y, y);
+        uint64_t r = two(c[5], c[5]);
+#pragma unroll
+        for (int k = 4; k >= 0; --k) r = fma2(r, z, two(c[k], c[k]));
+        float lo, hi;
+        parts(mul2(mul2(r, y), cap2), lo, hi);
+        x[e] = __float_as_uint(lo);
+        x[e + 1] = __float_as_uint(hi);
+    }
 }
 
 template <int D>
@@ -303,17 +400,20 @@ kv4_chunk_kernel(const Kv4AttentionArgs a, float* __restrict__ partials, const C
         if (lane == 0) {
             for (uint32_t i = 0; i < kRawSlots; ++i) {
                 mbar_init(&bars.raw_full[i], 1);
-                mbar_init(&bars.raw_empty[i], kExpandWarps);
+                mbar_init(&bars.raw_empty[i], 2u * kExpandWarps);
             }
             for (uint32_t i = 0; i < kStages; ++i) {
                 mbar_init(&bars.k_full[i], kExpandWarps);
                 mbar_init(&bars.v_full[i], kExpandWarps);
-                mbar_init(&bars.k_empty[i], 1);
-                mbar_init(&bars.v_empty[i], 1);
+                mbar_init(&bars.k_empty[i], n_tiles);
+                mbar_init(&bars.v_empty[i], n_tiles);
             }
             for (uint32_t i = 0; i < 2u; ++i) {
-                mbar_init(&bars.s_full[i], 1);
-                mbar_init(&bars.p_full[i], 4);
+                for (uint32_t b = 0; b < 2u; ++b) {
+                    mbar_init(&bars.s_full[i][b], 1);
+                    mbar_init(&bars.p_full[i][b], 4);
+                }
+                mbar_init(&bars.o_done[i], 1);
                 mbar_init(&bars.o_full[i], 1);
             }
             bars.abort = 0;
@@ -353,116 +453,117 @@ kv4_chunk_kernel(const Kv4AttentionArgs a, float* __restrict__ partials, const C
     tcgen05_fence_before_sync();
     __syncthreads();
     tcgen05_fence_after_sync();
-    const uint32_t tmem = bars.tmem_base;
 
-    if (warp == kLoadWarp) {
-        // ---- raw tiles, half a block at a time ----
-        const uint32_t* table = a.cache.block_tables + static_cast<uint64_t>(seq) * a.cache.max_blocks;
-        uint64_t offset = 0;
-        for (uint32_t hb = 0; hb < 2u * n_blocks; ++hb) {
-            const uint32_t first = first_tile + hb * kHalfTiles;
-            if (hb % 8u == 0u) {   // one lane for each of the next 32 tiles
-                const uint32_t tile = first + lane;
-                if (tile < end_tile) {
-                    uint64_t phys = __ldg(table + tile / a.cache.tiles_per_block);
-                    if (phys >= a.cache.physical_blocks) {
-                        phys = 0;
-                        flags |= B2_ATTN_STATUS_BAD_BLOCK;
+    // (a warpgroup's four warps take its registers with one instruction, ahead of their own branches)
+    if (warp >= kLoadWarp) {
+        registers_down<kOtherRegisters>();
+        if (warp == kLoadWarp) {
+            // ---- raw tiles ----
+            const uint32_t* table = a.cache.block_tables + static_cast<uint64_t>(seq) * a.cache.max_blocks;
+            uint64_t offset = 0;
+            for (uint32_t jb = 0; jb < n_blocks; ++jb) {
+                const uint32_t first = first_tile + jb * kBlockTiles;
+                if (jb % 8u == 0u) {   // one lane for each of the next 32 tiles
+                    const uint32_t tile = first + lane;
+                    if (tile < end_tile) {
+                        uint64_t phys = __ldg(table + tile / a.cache.tiles_per_block);
+                        if (phys >= a.cache.physical_blocks) {
+                            phys = 0;
+                            flags |= B2_ATTN_STATUS_BAD_BLOCK;
+                        }
+                        offset = kv4_tile_offset(a.cache, phys, kvh, tile % a.cache.tiles_per_block);
                     }
-                    offset = kv4_tile_offset(a.cache, phys, kvh, tile % a.cache.tiles_per_block);
+                }
+                const uint32_t slot = jb % kRawSlots;
+                if (jb >= kRawSlots) mbar_wait(&bars.raw_empty[slot], (jb / kRawSlots - 1u) & 1u, abort);
+                const uint32_t live = min(kBlockTiles, end_tile - first);
+                if (lane == 0) mbar_expect_tx(&bars.raw_full[slot], live * kv4_tile_bytes(D));
+                __syncwarp();
+                const uint32_t mine = lane - (jb % 8u) * kBlockTiles;   // wraps for lanes of other blocks
+                if (mine < live) {
+                    fence_proxy_async_smem();
+                    bulk_load(raw32 + slot * L::kRawSlot + mine * L::kRawTile, a.cache.pages + offset, kv4_tile_bytes(D),
+                              &bars.raw_full[slot]);
+                }
+                __syncwarp();
+            }
+        } else if (warp - kIssueWarp < n_tiles) {
+            // ---- tcgen05 issue: round jb makes a tile's scores of block jb, then its P V of block jb - 1 ----
+            // One warp for each tile: an issued MMA is hardly queued, so that what one warp spends on its barriers (75
+            // cycles a wait) would leave the tensor core idle, were it not for the other's MMAs. Tensor memory starts at
+            // column 0, this CTA holds all of it.
+            const uint32_t i = warp - kIssueWarp;
+            const uint64_t dq = umma_desc_k_major_sw128(q32 + i * (128u * D * 2u));
+            const uint64_t dk = umma_desc_k_major_sw128(k32), dv = umma_desc_k_major_sw128(v32);
+            for (uint32_t jb = 0; jb <= n_blocks && n_blocks != 0u; ++jb) {
+                if (jb < n_blocks) {
+                    const uint32_t stage = jb % kStages;
+                    mbar_wait(&bars.k_full[stage], (jb / kStages) & 1u, abort);
+                    tcgen05_fence_after_sync();
+                    const uint64_t kb = dk + (stage * L::kKStage >> 4);
+                    const uint32_t d = i * kTmemTile + (jb & 1u) * kBlock;   // its P was read by P V of block jb - 2
+                    if (elect_one()) {
+#pragma unroll
+                        for (uint32_t kk = 0; kk < D / 16u; ++kk) {
+                            umma_ss(d, dq + (kk / 4u) * (16384u >> 4) + (kk % 4u) * 2u,
+                                    kb + (kk / 4u) * (kBlock * 128u >> 4) + (kk % 4u) * 2u, idesc_f16(kBlock), kk != 0u ? 1u : 0u);
+                        }
+                        umma_commit(&bars.s_full[i][jb & 1u]);
+                        umma_commit(&bars.k_empty[stage]);
+                    }
+                    __syncwarp();
+                }
+                if (jb > 0u) {
+                    const uint32_t before = jb - 1u, stage = before % kStages;
+                    mbar_wait(&bars.v_full[stage], (before / kStages) & 1u, abort);
+                    mbar_wait(&bars.p_full[i][before & 1u], (before / 2u) & 1u, abort);
+                    tcgen05_fence_after_sync();
+                    const uint64_t b = dv + (stage * L::kVStage >> 4);
+                    const uint32_t w = i * kTmemTile + (before & 1u) * kBlock;
+                    if (elect_one()) {
+#pragma unroll
+                        for (uint32_t kk = 0; kk < kBlock / 16u; ++kk) {
+                            umma_ts(i * kTmemTile + kTmemO, w + kk * 8u, b + kk * 2u, idesc_f16(D), kk != 0u ? 1u : before);
+                        }
+                        umma_commit(jb == n_blocks ? &bars.o_full[i] : &bars.o_done[i]);
+                        umma_commit(&bars.v_empty[stage]);
+                    }
+                    __syncwarp();
                 }
             }
-            const uint32_t slot = hb % kRawSlots;
-            if (hb >= kRawSlots) mbar_wait(&bars.raw_empty[slot], (hb / kRawSlots - 1u) & 1u, abort);
-            const uint32_t live = first < end_tile ? min(kHalfTiles, end_tile - first) : 0u;
-            if (lane == 0) mbar_expect_tx(&bars.raw_full[slot], live * kv4_tile_bytes(D));
-            __syncwarp();
-            const uint32_t mine = lane - (hb % 8u) * kHalfTiles;   // wraps for lanes of other halves
-            if (mine < live) {
-                fence_proxy_async_smem();
-                bulk_load(raw32 + slot * L::kRawSlot + mine * L::kRawTile, a.cache.pages + offset, kv4_tile_bytes(D),
-                          &bars.raw_full[slot]);
-            }
-            __syncwarp();
         }
-    } else if (warp >= kSoftmaxWarps && warp < kSoftmaxWarps + kExpandWarps) {
+    } else if (warp >= kKeyWarp) {
         // ---- expansion ----
-        const uint32_t et = tid - kSoftmaxWarps * 32u;
+        registers_down<kExpandRegisters>();
+        const bool keys = warp < kValueWarp;
+        const uint32_t et = tid - (keys ? kKeyWarp : kValueWarp) * 32u;
+        uint64_t* const empty = keys ? bars.k_empty : bars.v_empty;
+        uint64_t* const full = keys ? bars.k_full : bars.v_full;
         for (uint32_t jb = 0; jb < n_blocks; ++jb) {
-            const uint32_t stage = jb % kStages, use = jb / kStages;
+            const uint32_t stage = jb % kStages, use = jb / kStages, slot = jb % kRawSlots;
             const uint32_t token0 = (first_tile + jb * kBlockTiles) * kKv4Tile;
-            if (use > 0) mbar_wait(&bars.k_empty[stage], (use - 1u) & 1u, abort);
-#pragma unroll 1
-            for (uint32_t half = 0; half < 2u; ++half) {
-                const uint32_t hb = 2u * jb + half, slot = hb % kRawSlots;
-                mbar_wait(&bars.raw_full[slot], (hb / kRawSlots) & 1u, abort);
-                expand_keys<D>(raw32 + slot * L::kRawSlot, k32 + stage * L::kKStage, half, et, token0 + half * kHalf,
-                               span.begin, span.end);
+            const bool whole = token0 >= span.begin && token0 + kBlock <= span.end;
+            if (use > 0) mbar_wait(&empty[stage], (use - 1u) & 1u, abort);
+            mbar_wait(&bars.raw_full[slot], (jb / kRawSlots) & 1u, abort);
+            if (keys) {
+                expand_keys<D>(raw32 + slot * L::kRawSlot, k32 + stage * L::kKStage, et, token0, whole, span.begin, span.end);
+            } else {
+                expand_values<D>(raw32 + slot * L::kRawSlot, v32 + stage * L::kVStage, et, token0, whole, span.begin, span.end);
             }
             fence_proxy_async_smem();
             __syncwarp();
-            if (lane == 0) mbar_arrive(&bars.k_full[stage]);
-            if (use > 0) mbar_wait(&bars.v_empty[stage], (use - 1u) & 1u, abort);
-#pragma unroll 1
-            for (uint32_t half = 0; half < 2u; ++half) {
-                const uint32_t hb = 2u * jb + half, slot = hb % kRawSlots;
-                expand_values<D>(raw32 + slot * L::kRawSlot, v32 + stage * L::kVStage, half, et, token0 + half * kHalf,
-                                 span.begin, span.end);
-                fence_proxy_async_smem();
-                __syncwarp();
-                if (lane == 0) mbar_arrive(&bars.raw_empty[slot]);
-            }
-            if (lane == 0) mbar_arrive(&bars.v_full[stage]);
-        }
-    } else if (warp == kIssueWarp) {
-        // ---- tcgen05 issue: for every block, each row tile's P V of the block before, then its Q K^T ----
-        const uint64_t dq = umma_desc_k_major_sw128(q32), dk = umma_desc_k_major_sw128(k32), dv = umma_desc_k_major_sw128(v32);
-        auto issue_pv = [&](uint32_t i, uint32_t jb) {
-            const uint64_t b = dv + ((jb % kStages) * L::kVStage >> 4);
-#pragma unroll
-            for (uint32_t kk = 0; kk < kBlock / 16u; ++kk) {
-                umma_ts(tmem + i * kTmemTile + kTmemO, tmem + i * kTmemTile + kk * 8u,
-                        b + (kk / 4u) * (D * 128u >> 4) + (kk % 4u) * 2u, idesc_f16(D), (jb | kk) != 0u ? 1u : 0u);
-            }
-        };
-        for (uint32_t jb = 0; jb <= n_blocks && n_blocks != 0u; ++jb) {
-            for (uint32_t i = 0; i < n_tiles; ++i) {
-                if (jb > 0u) {
-                    if (i == 0u) mbar_wait(&bars.v_full[(jb - 1u) % kStages], ((jb - 1u) / kStages) & 1u, abort);
-                    mbar_wait(&bars.p_full[i], (jb - 1u) & 1u, abort);
-                    tcgen05_fence_after_sync();
-                    if (elect_one()) {
-                        issue_pv(i, jb - 1u);
-                        if (i + 1u == n_tiles) umma_commit(&bars.v_empty[(jb - 1u) % kStages]);
-                        if (jb == n_blocks) umma_commit(&bars.o_full[i]);
-                    }
-                    __syncwarp();
-                }
-                if (jb < n_blocks) {
-                    if (i == 0u) {
-                        mbar_wait(&bars.k_full[jb % kStages], (jb / kStages) & 1u, abort);
-                        tcgen05_fence_after_sync();
-                    }
-                    if (elect_one()) {
-                        const uint64_t qa = dq + (i * (128u * D * 2u) >> 4), kb = dk + ((jb % kStages) * L::kKStage >> 4);
-#pragma unroll
-                        for (uint32_t kk = 0; kk < D / 16u; ++kk) {
-                            const uint64_t step = (kk / 4u) * (16384u >> 4) + (kk % 4u) * 2u;
-                            umma_ss(tmem + i * kTmemTile, qa + step, kb + step, idesc_f16(kBlock), kk != 0u ? 1u : 0u);
-                        }
-                        umma_commit(&bars.s_full[i]);
-                        if (i + 1u == n_tiles) umma_commit(&bars.k_empty[jb % kStages]);
-                    }
-                    __syncwarp();
-                }
+            if (lane == 0) {
+                mbar_arrive(&bars.raw_empty[slot]);
+                mbar_arrive(&full[stage]);
             }
         }
     } else if (warp / 4u < n_tiles) {
         // ---- softmax: a thread is a row ----
+        registers_up<kSoftmaxRegisters>();
         const uint32_t i = warp / 4u;
         const uint32_t r = i * 128u + (warp % 4u) * 32u + lane, gr = row0 + r;
         const bool live = r < rows;
-        const uint32_t lane_base = tmem + i * kTmemTile + (((warp % 4u) * 32u) << 16);
+        const uint32_t lane_base = i * kTmemTile + (((warp % 4u) * 32u) << 16);
         const int64_t position64 = span.position0 + gr / rep;
         uint32_t position = 0, begin = 0, end = 0;
         if (live && position64 >= 0) {
@@ -477,92 +578,85 @@ kv4_chunk_kernel(const Kv4AttentionArgs a, float* __restrict__ partials, const C
         const float cap_log2 = a.rules.softcap * kLog2e;
         const float slope = biased && live ? __ldg(a.rules.alibi_slopes + kvh * rep + gr % rep) * kLog2e : 0.0f;
         const float row_factor = s_factor[r];
-        const float factor = capped || biased ? 1.0f : row_factor;   // of what fetch() leaves
         float m = kNoMax, l = 0.0f;
 
         for (uint32_t jb = 0; jb < n_blocks; ++jb) {
             const uint32_t token0 = (first_tile + jb * kBlockTiles) * kKv4Tile;
-            mbar_wait(&bars.s_full[i], jb & 1u, abort);
+            const uint32_t buffer = lane_base + (jb & 1u) * kBlock;
+            mbar_wait(&bars.s_full[i][jb & 1u], (jb / 2u) & 1u, abort);
             tcgen05_fence_after_sync();
             const bool masked = token0 < all_begin || token0 + kBlock > all_end;   // the same for the whole warp
-            // 32 scores of the row: raw products, or finished scores in log2 units where they are capped or biased
-            auto fetch = [&](uint32_t c, float (&x)[32]) {
-                uint32_t raw[32];
-                tmem_ld_32x32(lane_base + c * 32u, raw);
-                tmem_ld_wait();
-#pragma unroll
-                for (int e = 0; e < 32; ++e) x[e] = __uint_as_float(raw[e]);
+            uint32_t x[64];
+            tmem_ld_32(buffer, x);
+            tmem_ld_32(buffer + 32u, x + 32);
+            tmem_ld_ready(x);
+            tmem_ld_ready(x + 32);
+            float factor = row_factor;
+            if (capped || biased) {   // scores in log2 units instead of raw products
+                factor = 1.0f;
                 if (capped) {
+                    cap_scores(x, row_factor, cap_log2);
+                } else {
 #pragma unroll
-                    for (int e = 0; e < 32; ++e) {
-                        // tanh y = 1 - 2 / (1 + e^2y): exact at both ends, 2^-22 absolute between
-                        const float y = ex2(x[e] * (row_factor * (2.0f * kLog2e)));
-                        x[e] = fmaf(-2.0f * cap_log2, rcp(1.0f + y), cap_log2);
-                    }
-                } else if (biased) {
-#pragma unroll
-                    for (int e = 0; e < 32; ++e) x[e] *= row_factor;
+                    for (int e = 0; e < 64; ++e) x[e] = __float_as_uint(__uint_as_float(x[e]) * row_factor);
                 }
                 if (biased) {
-                    const float away0 = static_cast<float>(static_cast<int>(position - (token0 + c * 32u)));
+                    const float away0 = static_cast<float>(static_cast<int>(position - token0));
 #pragma unroll
-                    for (int e = 0; e < 32; ++e) x[e] = fmaf(-slope, fabsf(away0 - static_cast<float>(e)), x[e]);
-                }
-                if (masked) {
-                    const uint32_t t0 = token0 + c * 32u;
-#pragma unroll
-                    for (int e = 0; e < 32; ++e) {
-                        if (t0 + e < begin || t0 + e >= end) x[e] = -INFINITY;
+                    for (int e = 0; e < 64; ++e) {
+                        x[e] = __float_as_uint(fmaf(-slope, fabsf(away0 - static_cast<float>(e)), __uint_as_float(x[e])));
                     }
                 }
-            };
-            uint32_t p[64];
-            float sum, top;
-            auto weigh = [&]() {
-                sum = 0.0f;
-                top = -INFINITY;
+            }
+            if (masked) {
 #pragma unroll
-                for (uint32_t c = 0; c < 4u; ++c) {
-                    float x[32];
-                    fetch(c, x);
-#pragma unroll
-                    for (int e = 0; e < 32; ++e) top = fmaxf(top, x[e]);
-#pragma unroll
-                    for (int e = 0; e < 32; e += 2) {
-                        const float p0 = ex2(fmaf(x[e], factor, -m)), p1 = ex2(fmaf(x[e + 1], factor, -m));
-                        sum += p0 + p1;
-                        p[c * 16u + e / 2] = pack_half(p0, p1);
-                    }
+                for (int e = 0; e < 64; ++e) {
+                    if (token0 + e < begin || token0 + e >= end) x[e] = 0xFF800000u;   // -infinity
                 }
-                top *= factor;
-            };
-            weigh();
+            }
+            float top4[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+#pragma unroll
+            for (int e = 0; e < 64; ++e) top4[e % 4] = fmaxf(top4[e % 4], __uint_as_float(x[e]));
+            const float top = fmaxf(fmaxf(top4[0], top4[1]), fmaxf(top4[2], top4[3])) * factor;
             if (__any_sync(0xFFFFFFFFu, top > m + kSlack)) {
                 const float moved = fmaxf(m, top);
                 const float shrink = ex2(m - moved);
                 m = moved;
                 l *= shrink;
                 if (jb > 0u) {
-                    // P V of the block before completed before this block's scores did: O is at rest
+                    mbar_wait(&bars.o_done[i], (jb - 1u) & 1u, abort);   // P V of the block before: O is at rest
+                    tcgen05_fence_after_sync();
 #pragma unroll 1
                     for (uint32_t c = 0; c < D / 32u; ++c) {
                         uint32_t o[32];
-                        tmem_ld_32x32(lane_base + kTmemO + c * 32u, o);
-                        tmem_ld_wait();
+                        tmem_ld_32(lane_base + kTmemO + c * 32u, o);
+                        tmem_ld_ready(o);
 #pragma unroll
                         for (int e = 0; e < 32; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * shrink);
                         tmem_st_32(lane_base + kTmemO + c * 32u, o);
                     }
                 }
-                weigh();
             }
-            l += sum;
-            tmem_st_32(lane_base, p);
-            tmem_st_32(lane_base + 32u, p + 32);
+            const uint64_t factor2 = two(factor, factor), minus_m = two(-m, -m);
+            uint64_t sums[2] = {0ull, 0ull};
+            uint32_t p[32];
+#pragma unroll
+            for (int e = 0; e < 64; e += 2) {
+                float a0, a1;
+                parts(fma2(two(__uint_as_float(x[e]), __uint_as_float(x[e + 1])), factor2, minus_m), a0, a1);
+                a0 = ex2(a0);
+                a1 = ex2(a1);
+                sums[(e / 2) & 1] = add2(sums[(e / 2) & 1], two(a0, a1));
+                p[e / 2] = pack_half(a0, a1);
+            }
+            tmem_st_32(buffer, p);
+            float s0, s1;
+            parts(add2(sums[0], sums[1]), s0, s1);
+            l += s0 + s1;
             tmem_st_wait();
             tcgen05_fence_before_sync();
             __syncwarp();
-            if (lane == 0) mbar_arrive(&bars.p_full[i]);
+            if (lane == 0) mbar_arrive(&bars.p_full[i][jb & 1u]);
         }
 
         // ---- epilogue ----
@@ -582,8 +676,8 @@ kv4_chunk_kernel(const Kv4AttentionArgs a, float* __restrict__ partials, const C
         for (uint32_t c = 0; c < D / 32u; ++c) {
             uint32_t raw[32];
             if (n_blocks != 0u) {
-                tmem_ld_32x32(lane_base + kTmemO + c * 32u, raw);
-                tmem_ld_wait();
+                tmem_ld_32(lane_base + kTmemO + c * 32u, raw);
+                tmem_ld_ready(raw);
             }
             if (!live) continue;
             float o[32];
@@ -611,7 +705,7 @@ kv4_chunk_kernel(const Kv4AttentionArgs a, float* __restrict__ partials, const C
     if (flags != 0u) kv4_flag(a.status, flags);
     tcgen05_fence_before_sync();
     __syncthreads();
-    if (warp == kIssueWarp) tmem_dealloc(tmem, kTmemColumns);
+    if (warp == kIssueWarp) tmem_dealloc(bars.tmem_base, kTmemColumns);
 }
 
 // Joins the splits of every (row, query head) that has more than one.
@@ -640,7 +734,7 @@ kv4_chunk_merge_kernel(const Kv4AttentionArgs a, const float* __restrict__ parti
 }
 
 // One CTA holds an SM. Where the row tiles leave SMs idle, the blocks of each are split over several CTAs, down to
-// four blocks, below which a CTA's own set-up costs as much as its blocks.
+// eight blocks, below which a CTA's own set-up costs as much as its blocks.
 ChunkPlan chunk_plan(int sm_count, uint32_t n_seq, uint32_t q_heads, uint32_t kv_heads, uint32_t max_chunk, uint32_t max_seq_len) {
     const uint64_t rep = q_heads / kv_heads;
     const uint64_t sms = sm_count > 0 ? static_cast<uint64_t>(sm_count) : 148u;
@@ -649,7 +743,7 @@ ChunkPlan chunk_plan(int sm_count, uint32_t n_seq, uint32_t q_heads, uint32_t kv
     const uint64_t ctas = row_tiles * n_seq * kv_heads;
     uint64_t per = blocks;
     if (ctas < sms) per = (blocks * ctas + sms - 1u) / sms;
-    if (per < 4u) per = 4u;
+    if (per < 8u) per = 8u;
     return ChunkPlan{static_cast<uint32_t>(row_tiles), static_cast<uint32_t>((blocks + per - 1u) / per), static_cast<uint32_t>(per)};
 }
 
