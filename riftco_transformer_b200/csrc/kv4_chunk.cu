@@ -65,6 +65,7 @@ struct Barriers {
     // P V of a block and of the last one. Whoever waits for o_done knows that the one before has completed (the
     // scores it has seen were issued after it), so that a parity tells; at the end only two before that is known.
     uint64_t o_done[2], o_full[2];
+    uint64_t q_full[2];   // a tile's rows of Q are staged
     uint32_t tmem_base;
     uint32_t abort;
 };
@@ -365,7 +366,6 @@ kv4_chunk_kernel(const Kv4AttentionArgs a, float* __restrict__ partials, const C
     pdl_launch_dependents();
     extern __shared__ __align__(1024) uint8_t smem_raw[];
     __shared__ __align__(8) Barriers bars;
-    __shared__ float s_factor[kRows];
 
     const uint32_t rep = a.q_heads / a.cache.kv_heads;
     uint32_t block = blockIdx.x;
@@ -415,44 +415,13 @@ kv4_chunk_kernel(const Kv4AttentionArgs a, float* __restrict__ partials, const C
                 }
                 mbar_init(&bars.o_done[i], 1);
                 mbar_init(&bars.o_full[i], 1);
+                mbar_init(&bars.q_full[i], 4);
             }
             bars.abort = 0;
             mbar_fence_init();
         }
-        __syncwarp();
-        tmem_alloc(&bars.tmem_base, kTmemColumns);
     }
-
-    // ---- Q: scaled to a largest magnitude in [2^9, 2^10) per row, fp16, in the order the codes come out ----
-    const float unit = a.rules.softcap != 0.0f ? 1.0f / a.rules.softcap : kLog2e;
-    const float to_unit = unit / sqrtf(static_cast<float>(D));
-    for (uint32_t i = tid; i < kRows * kChannels8; i += kThreads) {   // whole warps: kRows * kChannels8 % 32 == 0
-        const uint32_t r = i / kChannels8, c8 = i % kChannels8;
-        float x[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
-        if (r < rows) {
-            const uint32_t gr = row0 + r;
-            const float* src = a.q + (static_cast<uint64_t>(span.first + gr / rep) * a.q_heads + kvh * rep + gr % rep) * D + c8 * 8u;
-            const float4 u0 = __ldg(reinterpret_cast<const float4*>(src)), u1 = __ldg(reinterpret_cast<const float4*>(src) + 1);
-            x[0] = u0.x; x[1] = u0.y; x[2] = u0.z; x[3] = u0.w;
-            x[4] = u1.x; x[5] = u1.y; x[6] = u1.z; x[7] = u1.w;
-        }
-        float top = 0.0f;
-#pragma unroll
-        for (int e = 0; e < 8; ++e) top = fmaxf(top, fabsf(x[e]));
-#pragma unroll
-        for (uint32_t o = kChannels8 / 2u; o > 0u; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xFFFFFFFFu, top, o));
-        int e = 9 - (static_cast<int>((__float_as_uint(top) >> 23) & 255u) - 127);
-        e = max(-100, min(100, e));   // a row of zeros or beyond 2^109 keeps a bounded factor
-        const float up = __uint_as_float(static_cast<uint32_t>(e + 127) << 23);
-        if (c8 == 0u) s_factor[r] = __uint_as_float(static_cast<uint32_t>(127 - e) << 23) * to_unit;
-        const uint32_t dst = q32 + (r / 128u) * (128u * D * 2u) + (c8 / 8u) * 16384u + (r % 128u) * 128u + (((c8 % 8u) ^ (r & 7u)) << 4);
-        sts128(dst, pack_half(x[0] * up, x[4] * up), pack_half(x[1] * up, x[5] * up), pack_half(x[2] * up, x[6] * up),
-               pack_half(x[3] * up, x[7] * up));
-    }
-    fence_proxy_async_smem();
-    tcgen05_fence_before_sync();
     __syncthreads();
-    tcgen05_fence_after_sync();
 
     // (a warpgroup's four warps take its registers with one instruction, ahead of their own branches)
     if (warp >= kLoadWarp) {
@@ -493,6 +462,11 @@ kv4_chunk_kernel(const Kv4AttentionArgs a, float* __restrict__ partials, const C
             // cycles a wait) would leave the tensor core idle, were it not for the other's MMAs. Tensor memory starts at
             // column 0, this CTA holds all of it.
             const uint32_t i = warp - kIssueWarp;
+            if (i == 0u) tmem_alloc(&bars.tmem_base, kTmemColumns);
+            // the other tile's warp must not be ahead of the allocation
+            asm volatile("bar.sync 1, %0;" ::"r"(n_tiles * 32u) : "memory");
+            tcgen05_fence_after_sync();
+            mbar_wait(&bars.q_full[i], 0u, abort);
             const uint64_t dq = umma_desc_k_major_sw128(q32 + i * (128u * D * 2u));
             const uint64_t dk = umma_desc_k_major_sw128(k32), dv = umma_desc_k_major_sw128(v32);
             for (uint32_t jb = 0; jb <= n_blocks && n_blocks != 0u; ++jb) {
@@ -577,7 +551,55 @@ kv4_chunk_kernel(const Kv4AttentionArgs a, float* __restrict__ partials, const C
         const bool capped = a.rules.softcap != 0.0f, biased = a.rules.alibi_slopes != nullptr;
         const float cap_log2 = a.rules.softcap * kLog2e;
         const float slope = biased && live ? __ldg(a.rules.alibi_slopes + kvh * rep + gr % rep) * kLog2e : 0.0f;
-        const float row_factor = s_factor[r];
+        // Q: scaled to a largest magnitude in [2^9, 2^10) per row, fp16, in the order the codes come out. A warp stages
+        // its own 32 rows, kChannels8 lanes a row, with all loads of eight steps before their first use.
+        const float to_unit = (capped ? 1.0f / a.rules.softcap : kLog2e) / sqrtf(static_cast<float>(D));
+        constexpr uint32_t kRowsAtOnce = 32u / kChannels8, kSteps = 32u / kRowsAtOnce;
+        const uint32_t warp_row = i * 128u + (warp % 4u) * 32u, c8 = lane % kChannels8;
+        const uint32_t my_out = static_cast<uint32_t>(gr / rep), my_head = gr % rep;
+        float row_factor = 0.0f;
+#pragma unroll 1
+        for (uint32_t n0 = 0; n0 < kSteps; n0 += 8u) {
+            float y[8][8];
+#pragma unroll
+            for (uint32_t n = 0; n < 8u; ++n) {
+                const uint32_t mine = (n0 + n) * kRowsAtOnce + lane / kChannels8;   // of the warp's 32 rows
+                const uint32_t token = __shfl_sync(0xFFFFFFFFu, my_out, mine), head = __shfl_sync(0xFFFFFFFFu, my_head, mine);
+                float4 u0 = make_float4(0.f, 0.f, 0.f, 0.f), u1 = u0;
+                if (warp_row + mine < rows) {
+                    const float* src = a.q + (static_cast<uint64_t>(span.first + token) * a.q_heads + kvh * rep + head) * D + c8 * 8u;
+                    u0 = __ldg(reinterpret_cast<const float4*>(src));
+                    u1 = __ldg(reinterpret_cast<const float4*>(src) + 1);
+                }
+                y[n][0] = u0.x; y[n][1] = u0.y; y[n][2] = u0.z; y[n][3] = u0.w;
+                y[n][4] = u1.x; y[n][5] = u1.y; y[n][6] = u1.z; y[n][7] = u1.w;
+            }
+#pragma unroll
+            for (uint32_t n = 0; n < 8u; ++n) {
+                const uint32_t mine = (n0 + n) * kRowsAtOnce + lane / kChannels8, tile_row = (warp % 4u) * 32u + mine;
+                float top = 0.0f;
+#pragma unroll
+                for (int e = 0; e < 8; ++e) top = fmaxf(top, fabsf(y[n][e]));
+#pragma unroll
+                for (uint32_t o = kChannels8 / 2u; o > 0u; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xFFFFFFFFu, top, o));
+                int e = 9 - (static_cast<int>((__float_as_uint(top) >> 23) & 255u) - 127);
+                e = max(-100, min(100, e));   // a row of zeros or beyond 2^109 keeps a bounded factor
+                const float up = __uint_as_float(static_cast<uint32_t>(e + 127) << 23);
+                const float down = __uint_as_float(static_cast<uint32_t>(127 - e) << 23) * to_unit;
+                // to the lane whose row it is
+#pragma unroll
+                for (uint32_t k = 0; k < kRowsAtOnce; ++k) {
+                    const float f = __shfl_sync(0xFFFFFFFFu, down, k * kChannels8);
+                    if (lane == (n0 + n) * kRowsAtOnce + k) row_factor = f;
+                }
+                const uint32_t dst = q32 + i * (128u * D * 2u) + (c8 / 8u) * 16384u + tile_row * 128u + (((c8 % 8u) ^ (tile_row & 7u)) << 4);
+                sts128(dst, pack_half(y[n][0] * up, y[n][4] * up), pack_half(y[n][1] * up, y[n][5] * up),
+                       pack_half(y[n][2] * up, y[n][6] * up), pack_half(y[n][3] * up, y[n][7] * up));
+            }
+        }
+        fence_proxy_async_smem();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&bars.q_full[i]);
         float m = kNoMax, l = 0.0f;
 
         for (uint32_t jb = 0; jb < n_blocks; ++jb) {
@@ -614,10 +636,30 @@ kv4_chunk_kernel(const Kv4AttentionArgs a, float* __restrict__ partials, const C
                     if (token0 + e < begin || token0 + e >= end) x[e] = 0xFF800000u;   // -infinity
                 }
             }
-            float top4[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+            // The weights are made against the maximum so far, while the block's own is found; where it passes that by
+            // more than kSlack (the first block, hardly ever later) they are made again.
+            uint32_t p[32];
+            float sum, top;
+            auto weigh = [&]() {
+                const uint64_t factor2 = two(factor, factor), minus_m = two(-m, -m);
+                uint64_t sums[2] = {0ull, 0ull};
+                float top4[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
 #pragma unroll
-            for (int e = 0; e < 64; ++e) top4[e % 4] = fmaxf(top4[e % 4], __uint_as_float(x[e]));
-            const float top = fmaxf(fmaxf(top4[0], top4[1]), fmaxf(top4[2], top4[3])) * factor;
+                for (int e = 0; e < 64; e += 2) {
+                    float a0, a1;
+                    parts(fma2(two(__uint_as_float(x[e]), __uint_as_float(x[e + 1])), factor2, minus_m), a0, a1);
+                    a0 = ex2(a0);
+                    a1 = ex2(a1);
+                    top4[(e / 2) & 3] = fmaxf(fmaxf(top4[(e / 2) & 3], __uint_as_float(x[e])), __uint_as_float(x[e + 1]));
+                    sums[(e / 2) & 1] = add2(sums[(e / 2) & 1], two(a0, a1));
+                    p[e / 2] = pack_half(a0, a1);
+                }
+                float s0, s1;
+                parts(add2(sums[0], sums[1]), s0, s1);
+                sum = s0 + s1;
+                top = fmaxf(fmaxf(top4[0], top4[1]), fmaxf(top4[2], top4[3])) * factor;
+            };
+            weigh();
             if (__any_sync(0xFFFFFFFFu, top > m + kSlack)) {
                 const float moved = fmaxf(m, top);
                 const float shrink = ex2(m - moved);
@@ -628,31 +670,17 @@ kv4_chunk_kernel(const Kv4AttentionArgs a, float* __restrict__ partials, const C
                     tcgen05_fence_after_sync();
 #pragma unroll 1
                     for (uint32_t c = 0; c < D / 32u; ++c) {
-                        uint32_t o[32];
-                        tmem_ld_32(lane_base + kTmemO + c * 32u, o);
-                        tmem_ld_ready(o);
+                        tmem_ld_32(lane_base + kTmemO + c * 32u, p);
+                        tmem_ld_ready(p);
 #pragma unroll
-                        for (int e = 0; e < 32; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * shrink);
-                        tmem_st_32(lane_base + kTmemO + c * 32u, o);
+                        for (int e = 0; e < 32; ++e) p[e] = __float_as_uint(__uint_as_float(p[e]) * shrink);
+                        tmem_st_32(lane_base + kTmemO + c * 32u, p);
                     }
                 }
+                weigh();
             }
-            const uint64_t factor2 = two(factor, factor), minus_m = two(-m, -m);
-            uint64_t sums[2] = {0ull, 0ull};
-            uint32_t p[32];
-#pragma unroll
-            for (int e = 0; e < 64; e += 2) {
-                float a0, a1;
-                parts(fma2(two(__uint_as_float(x[e]), __uint_as_float(x[e + 1])), factor2, minus_m), a0, a1);
-                a0 = ex2(a0);
-                a1 = ex2(a1);
-                sums[(e / 2) & 1] = add2(sums[(e / 2) & 1], two(a0, a1));
-                p[e / 2] = pack_half(a0, a1);
-            }
+            l += sum;
             tmem_st_32(buffer, p);
-            float s0, s1;
-            parts(add2(sums[0], sums[1]), s0, s1);
-            l += s0 + s1;
             tmem_st_wait();
             tcgen05_fence_before_sync();
             __syncwarp();
@@ -664,41 +692,58 @@ kv4_chunk_kernel(const Kv4AttentionArgs a, float* __restrict__ partials, const C
         if (n_blocks != 0u) {
             mbar_wait(&bars.o_full[i], 0u, abort);
             tcgen05_fence_after_sync();
+        } else {
+            mbar_wait(&bars.q_full[i], 0u, abort);   // the other warps' staging, which the rows below are written over
         }
         if (lane == 0 && *abort != 0) flags |= B2_ATTN_STATUS_TIMEOUT;
-        const uint64_t out_head = static_cast<uint64_t>(span.first + (live ? gr / rep : 0u)) * a.q_heads + kvh * rep + (live ? gr % rep : 0u);
+        const uint64_t out_head = static_cast<uint64_t>(span.first + my_out) * a.q_heads + kvh * rep + my_head;
         const bool whole = n_splits == 1u;
         if (whole && live && l == 0.0f && end > begin) flags |= B2_ATTN_STATUS_ALL_NEG_INF;
         float* part = partials + (out_head * plan.splits + split) * (D + 4u);
         if (!whole && live) *reinterpret_cast<float2*>(part) = make_float2(m, l);
-        const float inv = l == 0.0f ? 0.0f : 1.0f / l;
+        const float inv = whole ? (l == 0.0f ? 0.0f : 1.0f / l) : 1.0f;
+        // The tile's Q is not needed any more: its 2 D bytes a row take the warp's bf16 rows, so that they leave in whole
+        // rows instead of 16 bytes of 32 different ones.
+        const uint32_t stage32 = q32 + i * (128u * D * 2u) + (warp % 4u) * (32u * D * 2u);
 #pragma unroll 1
         for (uint32_t c = 0; c < D / 32u; ++c) {
-            uint32_t raw[32];
+            uint32_t o[32];
             if (n_blocks != 0u) {
-                tmem_ld_32(lane_base + kTmemO + c * 32u, raw);
-                tmem_ld_ready(raw);
+                tmem_ld_32(lane_base + kTmemO + c * 32u, o);
+                tmem_ld_ready(o);
             }
-            if (!live) continue;
-            float o[32];
 #pragma unroll
-            for (int e = 0; e < 32; ++e) o[e] = l == 0.0f ? 0.0f : __uint_as_float(raw[e]);
+            for (int e = 0; e < 32; ++e) o[e] = l == 0.0f ? 0u : __float_as_uint(__uint_as_float(o[e]) * inv);
             if (whole) {
-                uint4* dst = reinterpret_cast<uint4*>(static_cast<__nv_bfloat16*>(a.ctx16) + out_head * D + c * 32u);
 #pragma unroll
-                for (int e = 0; e < 4; ++e) {
+                for (uint32_t e = 0; e < 4u; ++e) {
                     uint32_t w[4];
 #pragma unroll
-                    for (int k = 0; k < 4; ++k) {
-                        const __nv_bfloat162 b = __floats2bfloat162_rn(o[8 * e + 2 * k] * inv, o[8 * e + 2 * k + 1] * inv);
+                    for (uint32_t k = 0; k < 4u; ++k) {
+                        const __nv_bfloat162 b = __floats2bfloat162_rn(__uint_as_float(o[8 * e + 2 * k]), __uint_as_float(o[8 * e + 2 * k + 1]));
                         w[k] = *reinterpret_cast<const uint32_t*>(&b);
                     }
-                    dst[e] = make_uint4(w[0], w[1], w[2], w[3]);
+                    sts128(stage32 + lane * (D * 2u) + (((c * 4u + e) ^ (lane & 7u)) << 4), w[0], w[1], w[2], w[3]);
                 }
-            } else {
+            } else if (live) {
                 float4* dst = reinterpret_cast<float4*>(part + 4u + c * 32u);
 #pragma unroll
-                for (int e = 0; e < 8; ++e) dst[e] = make_float4(o[4 * e], o[4 * e + 1], o[4 * e + 2], o[4 * e + 3]);
+                for (int e = 0; e < 8; ++e) {
+                    dst[e] = make_float4(__uint_as_float(o[4 * e]), __uint_as_float(o[4 * e + 1]), __uint_as_float(o[4 * e + 2]),
+                                         __uint_as_float(o[4 * e + 3]));
+                }
+            }
+        }
+        if (whole) {
+            __syncwarp();
+#pragma unroll 4
+            for (uint32_t n = 0; n < kSteps; ++n) {
+                const uint32_t mine = n * kRowsAtOnce + lane / kChannels8;
+                const uint64_t head = __shfl_sync(0xFFFFFFFFu, out_head, mine);
+                const uint4 v = lds128(stage32 + mine * (D * 2u) + ((c8 ^ (mine & 7u)) << 4));
+                if (warp_row + mine < rows) {
+                    reinterpret_cast<uint4*>(static_cast<__nv_bfloat16*>(a.ctx16) + head * D)[c8] = v;
+                }
             }
         }
     }
