@@ -85,8 +85,8 @@ int32_t launch_kv4_append(const DeviceContext& ctx, const Kv4AppendArgs& args, c
 int32_t launch_kv4_read(const DeviceContext& ctx, const Kv4ReadArgs& args, cudaStream_t stream);
 
 // kv4_decode.cu - every row on its own: one token per sequence, or a few tokens of each.
-size_t kv4_decode_workspace_bytes(int sm_count, uint64_t rows, uint32_t q_heads, uint32_t kv_heads, uint32_t head_width,
-                                  uint32_t max_seq_len);
+int32_t kv4_decode_workspace_bytes(const DeviceContext& ctx, uint64_t rows, uint32_t q_heads, uint32_t kv_heads,
+                                   uint32_t head_width, uint32_t max_seq_len, size_t* bytes);
 int32_t launch_kv4_decode(const DeviceContext& ctx, const Kv4AttentionArgs& args, void* workspace,
                           size_t workspace_bytes, cudaStream_t stream);
 
@@ -133,6 +133,20 @@ __device__ __forceinline__ float ex2(float x) {
     float y;
     asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
     return y;
+}
+// fp16 numbers 1024 + code (or 1024 + 16 code) of two codes of a word, 16 bits apart: (word & MASK) | k1024 in one
+// instruction. k1024 comes from opaque_1024() once per thread: an instruction holds one immediate, and given two
+// constants the compiler takes an AND and an OR (a sixth of the decode kernel's instructions).
+template <uint32_t MASK>
+__device__ __forceinline__ uint32_t codes_1024(uint32_t word, uint32_t k1024) {
+    uint32_t r;
+    asm("lop3.b32 %0, %1, %2, %3, 0xEA;" : "=r"(r) : "r"(word), "n"(MASK), "r"(k1024));
+    return r;
+}
+__device__ __forceinline__ uint32_t opaque_1024() {
+    uint32_t r;
+    asm volatile("mov.b32 %0, 0x64006400;" : "=r"(r));
+    return r;
 }
 __device__ __forceinline__ float low_half(uint32_t pair) { return __low2float(*reinterpret_cast<__half2*>(&pair)); }
 __device__ __forceinline__ float high_half(uint32_t pair) { return __high2float(*reinterpret_cast<__half2*>(&pair)); }
@@ -198,42 +212,47 @@ __device__ __forceinline__ void put_context(const Kv4AttentionArgs& a, uint64_t 
     }
 }
 
-// Joins `n_splits` partial results of one (row, query head), each [maximum (log2 units), sum of weights, -, -,
-// D sums], for the channels c .. c + 3 of this thread, in split order.
-template <int D>
-__device__ __forceinline__ void join_splits(const Kv4AttentionArgs& a, const float* src, uint64_t out_head,
-                                            uint32_t n_splits, uint32_t c, bool sees_any) {
-    float mm = kNoMax, ll = 0.0f;
-    float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
-    for (uint32_t s0 = 0; s0 < n_splits; s0 += 8u) {
+struct Joined {
+    float m, l;   // maximum (log2 units), sum of weights
+    float4 o;     // sums of four channels
+};
+// Joins `n` partial results of one (row, query head), each [m, l, -, -, sums of the channels], for the channels
+// c .. c + 3 of this thread, in order: the first at `first`, the others `stride` floats apart from `rest`.
+__device__ __forceinline__ Joined join_run(const float* first, const float* rest, uint64_t stride, uint32_t n, uint32_t c) {
+    Joined j{kNoMax, 0.0f, make_float4(0.f, 0.f, 0.f, 0.f)};
+    for (uint32_t s0 = 0; s0 < n; s0 += 8u) {
         float2 ml[8];
         float4 x[8];
 #pragma unroll
         for (uint32_t u = 0; u < 8u; ++u) {   // all loads before the first use
-            const bool live = s0 + u < n_splits;
-            const float* part = src + (s0 + u) * (D + 4u);
+            const bool live = s0 + u < n;
+            const float* part = s0 + u == 0u ? first : rest + (s0 + u - 1u) * stride;
             ml[u] = live ? *reinterpret_cast<const float2*>(part) : make_float2(kNoMax, 0.0f);
             x[u] = live ? *reinterpret_cast<const float4*>(part + 4u + c) : make_float4(0.f, 0.f, 0.f, 0.f);
         }
-        float top = mm;
+        float top = j.m;
 #pragma unroll
         for (uint32_t u = 0; u < 8u; ++u) top = fmaxf(top, ml[u].x);
-        const float keep = ex2(mm - top);
-        mm = top;
-        ll *= keep;
-        o = make_float4(o.x * keep, o.y * keep, o.z * keep, o.w * keep);
+        const float keep = ex2(j.m - top);
+        j.m = top;
+        j.l *= keep;
+        j.o = make_float4(j.o.x * keep, j.o.y * keep, j.o.z * keep, j.o.w * keep);
 #pragma unroll
-        for (uint32_t u = 0; u < 8u; ++u) {   // in split order
-            const float f = ex2(ml[u].x - mm);
-            ll = fmaf(ml[u].y, f, ll);
-            o.x = fmaf(x[u].x, f, o.x);
-            o.y = fmaf(x[u].y, f, o.y);
-            o.z = fmaf(x[u].z, f, o.z);
-            o.w = fmaf(x[u].w, f, o.w);
+        for (uint32_t u = 0; u < 8u; ++u) {
+            const float f = ex2(ml[u].x - j.m);
+            j.l = fmaf(ml[u].y, f, j.l);
+            j.o.x = fmaf(x[u].x, f, j.o.x);
+            j.o.y = fmaf(x[u].y, f, j.o.y);
+            j.o.z = fmaf(x[u].z, f, j.o.z);
+            j.o.w = fmaf(x[u].w, f, j.o.w);
         }
     }
-    if (ll == 0.0f && sees_any && c == 0) kv4_flag(a.status, B2_ATTN_STATUS_ALL_NEG_INF);
-    put_context<D>(a, out_head, c, o, ll);
+    return j;
+}
+template <int D>
+__device__ __forceinline__ void finish(const Kv4AttentionArgs& a, const Joined& j, uint64_t out_head, uint32_t c, bool sees_any) {
+    if (j.l == 0.0f && sees_any && c == 0u) kv4_flag(a.status, B2_ATTN_STATUS_ALL_NEG_INF);
+    put_context<D>(a, out_head, c, j.o, j.l);
 }
 
 #endif  // __CUDACC__

@@ -159,17 +159,20 @@ DeviceContext* query_context(uint32_t rows, uint32_t q_heads, uint32_t kv_heads,
     int32_t status = B2_STATUS_OK;
     DeviceContext* ctx = device_context(&status);
     clear_error();
-    if (rows == 0 || q_heads == 0 || kv_heads == 0 || q_heads % kv_heads != 0 || head_width == 0 || max_seq_len == 0) {
+    if (rows == 0 || q_heads == 0 || kv_heads == 0 || q_heads % kv_heads != 0 || max_seq_len == 0 ||
+        (head_width != 64 && head_width != 128 && head_width != 256)) {
         return nullptr;
     }
     return ctx;
 }
 
-size_t chunk_workspace(const DeviceContext& ctx, uint32_t n_seq, uint32_t n_tokens, uint32_t q_heads, uint32_t kv_heads,
-                       uint32_t head_width, uint32_t max_chunk, uint32_t max_seq_len) {
-    return kv4_chunk_supported(head_width, q_heads, kv_heads, max_chunk)
-               ? kv4_chunk_workspace_bytes(ctx.sm_count, n_seq, n_tokens, q_heads, kv_heads, head_width, max_chunk, max_seq_len)
-               : kv4_decode_workspace_bytes(ctx.sm_count, n_tokens, q_heads, kv_heads, head_width, max_seq_len);
+int32_t chunk_workspace(const DeviceContext& ctx, uint32_t n_seq, uint32_t n_tokens, uint32_t q_heads, uint32_t kv_heads,
+                        uint32_t head_width, uint32_t max_chunk, uint32_t max_seq_len, size_t* bytes) {
+    if (!kv4_chunk_supported(head_width, q_heads, kv_heads, max_chunk)) {
+        return kv4_decode_workspace_bytes(ctx, n_tokens, q_heads, kv_heads, head_width, max_seq_len, bytes);
+    }
+    *bytes = kv4_chunk_workspace_bytes(ctx.sm_count, n_seq, n_tokens, q_heads, kv_heads, head_width, max_chunk, max_seq_len);
+    return B2_STATUS_OK;
 }
 
 }  // namespace
@@ -242,7 +245,12 @@ int32_t b2_kv4_dequantize(const b2_kv4_cache* cache, const uint32_t* positions, 
 size_t b2_paged_decode_kv4_workspace_bytes(uint32_t n_seq, uint32_t q_heads, uint32_t kv_heads, uint32_t head_width,
                                            uint32_t max_seq_len) {
     DeviceContext* ctx = query_context(n_seq, q_heads, kv_heads, head_width, max_seq_len);
-    return ctx == nullptr ? 0 : kv4_decode_workspace_bytes(ctx->sm_count, n_seq, q_heads, kv_heads, head_width, max_seq_len);
+    size_t bytes = 0;
+    if (ctx == nullptr || kv4_decode_workspace_bytes(*ctx, n_seq, q_heads, kv_heads, head_width, max_seq_len, &bytes) != B2_STATUS_OK) {
+        bytes = 0;
+    }
+    clear_error();
+    return bytes;
 }
 
 int32_t b2_paged_decode_attention_kv4(const b2_kv4_cache* cache, const b2_kv4_score_rules* rules, const float* q,
@@ -259,9 +267,9 @@ int32_t b2_paged_decode_attention_kv4(const b2_kv4_cache* cache, const b2_kv4_sc
                              status_word};
     Kv4AttentionArgs args;
     B2_TRY(attention_args(call, &args));
-    B2_TRY(take_workspace(ctx, kv4_decode_workspace_bytes(ctx->sm_count, args.rows, q_heads, args.cache.kv_heads,
-                                                          args.cache.head_width, max_seq_len),
-                          &workspace, &workspace_bytes, stream));
+    size_t need = 0;
+    B2_TRY(kv4_decode_workspace_bytes(*ctx, args.rows, q_heads, args.cache.kv_heads, args.cache.head_width, max_seq_len, &need));
+    B2_TRY(take_workspace(ctx, need, &workspace, &workspace_bytes, stream));
     note_route(B2_ROUTE_ATTENTION_KV4);
     return launch_kv4_decode(*ctx, args, workspace, workspace_bytes, stream);
 }
@@ -270,8 +278,13 @@ size_t b2_paged_chunk_kv4_workspace_bytes(uint32_t n_seq, uint32_t n_tokens, uin
                                           uint32_t head_width, uint32_t max_chunk, uint32_t max_seq_len) {
     if (n_seq == 0 || max_chunk == 0) return 0;
     DeviceContext* ctx = query_context(n_tokens, q_heads, kv_heads, head_width, max_seq_len);
-    return ctx == nullptr ? 0
-                          : chunk_workspace(*ctx, n_seq, n_tokens, q_heads, kv_heads, head_width, max_chunk, max_seq_len);
+    size_t bytes = 0;
+    if (ctx == nullptr ||
+        chunk_workspace(*ctx, n_seq, n_tokens, q_heads, kv_heads, head_width, max_chunk, max_seq_len, &bytes) != B2_STATUS_OK) {
+        bytes = 0;
+    }
+    clear_error();
+    return bytes;
 }
 
 int32_t b2_paged_chunk_attention_kv4(const b2_kv4_cache* cache, const b2_kv4_score_rules* rules,
@@ -295,9 +308,9 @@ int32_t b2_paged_chunk_attention_kv4(const b2_kv4_cache* cache, const b2_kv4_sco
         return fail(B2_STATUS_INVALID_ARGUMENT, "paged attention chunk is longer than its sequence or the call's tokens");
     }
     const uint32_t kv_heads = args.cache.kv_heads, head_width = args.cache.head_width;
-    B2_TRY(take_workspace(ctx, chunk_workspace(*ctx, args.cache.n_seq, n_tokens, q_heads, kv_heads, head_width, max_chunk,
-                                               max_seq_len),
-                          &workspace, &workspace_bytes, stream));
+    size_t need = 0;
+    B2_TRY(chunk_workspace(*ctx, args.cache.n_seq, n_tokens, q_heads, kv_heads, head_width, max_chunk, max_seq_len, &need));
+    B2_TRY(take_workspace(ctx, need, &workspace, &workspace_bytes, stream));
     if (kv4_chunk_supported(head_width, q_heads, kv_heads, max_chunk)) {
         note_route(B2_ROUTE_ATTENTION_KV4_TILES);
         return launch_kv4_chunk(*ctx, args, workspace, workspace_bytes, stream);

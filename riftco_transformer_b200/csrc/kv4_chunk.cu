@@ -175,14 +175,14 @@ __host__ __device__ constexpr uint32_t idesc_f16(uint32_t n) { return (1u << 4) 
 // scale * code + base of the two codes that nibble N of both halves of `word` holds; the scales and bases
 // are those of the two. 1024 + code and 1024 + 16 code are exact, so is taking the 1024 off.
 template <int N>
-__device__ __forceinline__ uint32_t expand(uint32_t word, __half2 scale, __half2 base) {
+__device__ __forceinline__ uint32_t expand(uint32_t word, __half2 scale, __half2 base, uint32_t k1024) {
     if (N >= 2) word >>= 8;
     __half2 c;
     if (N % 2 == 0) {
-        uint32_t x = (word & 0x000F000Fu) | 0x64006400u;
+        uint32_t x = codes_1024<0x000F000Fu>(word, k1024);
         c = __hadd2(*reinterpret_cast<__half2*>(&x), __half2half2(__ushort_as_half(0xE400)));   // -1024
     } else {
-        uint32_t x = (word & 0x00F000F0u) | 0x64006400u;
+        uint32_t x = codes_1024<0x00F000F0u>(word, k1024);
         c = __hfma2(*reinterpret_cast<__half2*>(&x), __half2half2(__ushort_as_half(0x2C00)),    // 1/16
                     __half2half2(__ushort_as_half(0xD400)));                                     // -64
     }
@@ -197,7 +197,7 @@ __device__ __forceinline__ uint32_t not_finite(uint32_t pair) { return ((pair & 
 // one of the tokens is seen by some row.
 template <int D>
 __device__ __forceinline__ void expand_keys(uint32_t raw32, uint32_t stage32, uint32_t tid, uint32_t token0, bool whole,
-                                            uint32_t begin, uint32_t end) {
+                                            uint32_t begin, uint32_t end, uint32_t k1024) {
     constexpr uint32_t G = D / 64, kSteps = kBlock * (D / 32) / (kExpandWarps * 32u);
     const uint32_t tk = tid % kBlock;   // lanes: consecutive tokens
     const uint32_t tile32 = raw32 + (tk / 16u) * Layout<D>::kRawTile;
@@ -228,8 +228,8 @@ __device__ __forceinline__ void expand_keys(uint32_t raw32, uint32_t stage32, ui
 #pragma unroll
         for (uint32_t w = 0; w < 4u; ++w) {
             const uint32_t unit = (tid / kBlock) * 4u + w;
-            sts128(row32 + n * (kBlock * 128u) + ((unit ^ (tk & 7u)) << 4), expand<0>(words[w], scale, base),
-                   expand<1>(words[w], scale, base), expand<2>(words[w], scale, base), expand<3>(words[w], scale, base));
+            sts128(row32 + n * (kBlock * 128u) + ((unit ^ (tk & 7u)) << 4), expand<0>(words[w], scale, base, k1024),
+                   expand<1>(words[w], scale, base, k1024), expand<2>(words[w], scale, base, k1024), expand<3>(words[w], scale, base, k1024));
         }
     }
 }
@@ -237,7 +237,7 @@ __device__ __forceinline__ void expand_keys(uint32_t raw32, uint32_t stage32, ui
 // A block of values, transposed: eight channels of eight tokens per thread, rows of the tile are channels.
 template <int D>
 __device__ __forceinline__ void expand_values(uint32_t raw32, uint32_t stage32, uint32_t tid, uint32_t token0, bool whole,
-                                              uint32_t begin, uint32_t end) {
+                                              uint32_t begin, uint32_t end, uint32_t k1024) {
     constexpr uint32_t G = D / 64;
     if (tid >= D) return;
     const uint32_t octet = tid % 8u, word = tid / 8u;   // tokens 8 octet.., channels 8 word..
@@ -273,10 +273,10 @@ __device__ __forceinline__ void expand_values(uint32_t raw32, uint32_t stage32, 
         sts128(column32 + n * 128u + ((octet ^ n) << 4), x0, x1, x2, x3);
     };
 #define B2_KV4_PUT(N, SRC)                                                                                    \
-    put(N, expand<(N) % 4>(SRC[0], as_half2(scale[0]), as_half2(base[0])),                                    \
-        expand<(N) % 4>(SRC[1], as_half2(scale[1]), as_half2(base[1])),                                       \
-        expand<(N) % 4>(SRC[2], as_half2(scale[2]), as_half2(base[2])),                                       \
-        expand<(N) % 4>(SRC[3], as_half2(scale[3]), as_half2(base[3])))
+    put(N, expand<(N) % 4>(SRC[0], as_half2(scale[0]), as_half2(base[0]), k1024),                                    \
+        expand<(N) % 4>(SRC[1], as_half2(scale[1]), as_half2(base[1]), k1024),                                       \
+        expand<(N) % 4>(SRC[2], as_half2(scale[2]), as_half2(base[2]), k1024),                                       \
+        expand<(N) % 4>(SRC[3], as_half2(scale[3]), as_half2(base[3]), k1024))
     B2_KV4_PUT(0, lo);
     B2_KV4_PUT(1, lo);
     B2_KV4_PUT(2, lo);
@@ -510,6 +510,7 @@ kv4_chunk_kernel(const Kv4AttentionArgs a, float* __restrict__ partials, const C
         // ---- expansion ----
         registers_down<kExpandRegisters>();
         const bool keys = warp < kValueWarp;
+        const uint32_t k1024 = opaque_1024();
         const uint32_t et = tid - (keys ? kKeyWarp : kValueWarp) * 32u;
         uint64_t* const empty = keys ? bars.k_empty : bars.v_empty;
         uint64_t* const full = keys ? bars.k_full : bars.v_full;
@@ -520,9 +521,9 @@ kv4_chunk_kernel(const Kv4AttentionArgs a, float* __restrict__ partials, const C
             if (use > 0) mbar_wait(&empty[stage], (use - 1u) & 1u, abort);
             mbar_wait(&bars.raw_full[slot], (jb / kRawSlots) & 1u, abort);
             if (keys) {
-                expand_keys<D>(raw32 + slot * L::kRawSlot, k32 + stage * L::kKStage, et, token0, whole, span.begin, span.end);
+                expand_keys<D>(raw32 + slot * L::kRawSlot, k32 + stage * L::kKStage, et, token0, whole, span.begin, span.end, k1024);
             } else {
-                expand_values<D>(raw32 + slot * L::kRawSlot, v32 + stage * L::kVStage, et, token0, whole, span.begin, span.end);
+                expand_values<D>(raw32 + slot * L::kRawSlot, v32 + stage * L::kVStage, et, token0, whole, span.begin, span.end, k1024);
             }
             fence_proxy_async_smem();
             __syncwarp();
@@ -774,8 +775,9 @@ kv4_chunk_merge_kernel(const Kv4AttentionArgs a, const float* __restrict__ parti
     }
     pdl_wait();   // every CTA waits, so that this grid never ends before the one it follows
     if (n_splits <= 1u) return;
-    join_splits<D>(a, partials + out_head * plan.splits * (D + 4u), out_head, n_splits, threadIdx.x * 4u,
-                   mine.end > mine.begin);
+    const float* first = partials + out_head * plan.splits * (D + 4u);
+    const uint32_t c = threadIdx.x * 4u;
+    finish<D>(a, join_run(first, first + (D + 4u), D + 4u, n_splits, c), out_head, c, mine.end > mine.begin);
 }
 
 // One CTA holds an SM. Where the row tiles leave SMs idle, the blocks of each are split over several CTAs, down to

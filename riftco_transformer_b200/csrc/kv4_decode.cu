@@ -53,7 +53,7 @@ __device__ __forceinline__ void ldsm4_trans(uint32_t (&r)[4], uint32_t addr) {
 }
 __device__ __forceinline__ void mma16816(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3,
                                          uint32_t b0, uint32_t b1) {
-    asm volatile(
+    asm(   // not volatile: registers only, free to be scheduled between the loads
         "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
         : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
         : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
@@ -85,15 +85,14 @@ __device__ __forceinline__ void lds_words(uint32_t (&v)[N], uint32_t addr) {
 }
 // Two codes of a word, 16 bits apart, as fp16 numbers code - 8 (exact: 1024 + 16 * 15 fits 11 bits).
 template <int NIBBLE>
-__device__ __forceinline__ uint32_t codes_of(uint32_t word) {
-    constexpr uint32_t k1024 = 0x64006400u;
+__device__ __forceinline__ uint32_t codes_of(uint32_t word, uint32_t k1024) {
     if (NIBBLE >= 2) word >>= 8;
     if (NIBBLE % 2 == 0) {
-        uint32_t x = (word & 0x000F000Fu) | k1024;
+        uint32_t x = codes_1024<0x000F000Fu>(word, k1024);
         const __half2 y = __hadd2(*reinterpret_cast<__half2*>(&x), __half2half2(__ushort_as_half(0xE408)));   // -1032
         return *reinterpret_cast<const uint32_t*>(&y);
     }
-    uint32_t x = (word & 0x00F000F0u) | k1024;
+    uint32_t x = codes_1024<0x00F000F0u>(word, k1024);
     const __half2 y = __hfma2(*reinterpret_cast<__half2*>(&x), __half2half2(__ushort_as_half(0x2C00)),   // 1/16
                               __half2half2(__ushort_as_half(0xD480)));                                    // -72
     return *reinterpret_cast<const uint32_t*>(&y);
@@ -101,36 +100,55 @@ __device__ __forceinline__ uint32_t codes_of(uint32_t word) {
 // The first 11 bits of x; x minus it is exact.
 __device__ __forceinline__ float first_part(float x) { return __uint_as_float(__float_as_uint(x) & 0xFFFFE000u); }
 
-struct SplitPlan {
-    uint32_t splits;          // most splits of a row
-    uint32_t tiles_per_split;
+// How the work is cut. A list is what one K/V head of one row reads for up to HC query heads, in pairs of tiles; the
+// lists of all rows, one behind the other, are cut into equal ranges, one for each CTA, whose partial results
+// (one or two a CTA: of the list its range begins in and of the one it ends in) a second kernel joins. Equal ranges
+// keep the card full whatever the lengths. Where every list is short, or there are so many rows that lists alone fill
+// the card, a CTA takes one whole list and there is nothing to join.
+constexpr uint32_t kMaxRows = 1024;   // rows a CTA finds its range among
+constexpr uint32_t kMinPairs = 8;     // pairs of a range: below two a warp a CTA is mostly set-up
+constexpr uint32_t kMostPairs = 64;   // pairs (were all rows of full length) from which there are more ranges than the
+                                      // card holds at once: the last ones of an SM then overlap less time with too few warps
+struct WorkPlan {
+    uint32_t ctas;
+    uint32_t whole_lists;   // 1: CTA i takes list i
 };
 
+// Where a list's partial results are: those of CTAs first .. last, of the first one number `slot`, of the others 0.
+struct ListParts {
+    uint32_t first, last, slot;
+};
+
+// Pairs of tiles of a row's lists: none for a row that is nobody's, one (of no token) for a row that sees nothing.
+__device__ __forceinline__ uint32_t row_pairs(const RowSpan& span) {
+    if (!span.owned) return 0u;
+    if (span.end <= span.begin) return 1u;
+    const uint32_t tiles = (span.end - 1u) / kKv4Tile + 1u - span.begin / kKv4Tile;
+    return (tiles + kPair - 1u) / kPair;
+}
+// CTAs that share `total` pairs, the first pair of CTA c, and the last CTA whose range begins at or before a pair.
+__device__ __forceinline__ uint32_t live_ctas(const WorkPlan& plan, uint32_t lists, uint32_t total) {
+    return min(plan.ctas, max(lists, (total + kMinPairs - 1u) / kMinPairs));
+}
+__device__ __forceinline__ uint32_t first_pair(uint32_t c, uint32_t total, uint32_t ctas) {
+    return static_cast<uint32_t>(static_cast<uint64_t>(c) * total / ctas);
+}
+__device__ __forceinline__ uint32_t owner_of(uint32_t pair, uint32_t total, uint32_t ctas) {   // c * total / ctas < pair + 1
+    return static_cast<uint32_t>(((static_cast<uint64_t>(pair) + 1u) * ctas - 1u) / total);
+}
+
+// CTAs that an SM's registers are to hold.
+__host__ __device__ constexpr int ctas_of(int d, int hc) { return d == 64 ? (hc == 4 ? 6 : 5) : d == 128 ? (hc == 4 ? 4 : 3) : 2; }
+
 template <int D, int HC>   // HC: query heads of one K/V head worked on together (4 or 8)
-__global__ void __launch_bounds__(kWarps * 32)
-kv4_decode_kernel(const Kv4AttentionArgs a, float* __restrict__ partials, const SplitPlan plan) {
+__global__ void __launch_bounds__(kWarps * 32, ctas_of(D, HC))
+kv4_decode_kernel(const Kv4AttentionArgs a, ListParts* __restrict__ list_parts, float* __restrict__ partials, const WorkPlan plan) {
     using namespace sm100;
     pdl_launch_dependents();
     constexpr int G = D / 64, kChunks = D / 32;
     constexpr int HL = HC / 4;            // heads of a lane in the score layout
     constexpr uint32_t kTileBytes = kv4_tile_bytes(D);
-    constexpr float kWTop = 8192.0f;      // p * scale likewise: p <= 4 keeps it below 65504
-
-    const uint32_t rep = a.q_heads / a.cache.kv_heads;
-    const uint32_t head_chunks = (rep + HC - 1u) / HC;
-    uint32_t block = blockIdx.x;
-    const uint32_t split = block % plan.splits;
-    block /= plan.splits;
-    const uint32_t chunk = block % head_chunks;
-    block /= head_chunks;
-    const uint32_t kvh = block % a.cache.kv_heads;
-    const uint32_t row = block / a.cache.kv_heads;
-
-    const RowSpan span = row_span(a, row);
-    const uint32_t tile0 = span.begin / kKv4Tile;
-    const uint32_t tiles = span.end > span.begin ? (span.end - 1u) / kKv4Tile + 1u - tile0 : 0u;
-    const uint32_t n_splits = max(1u, (tiles + plan.tiles_per_split - 1u) / plan.tiles_per_split);
-    if (split >= n_splits || !span.owned) return;
+    constexpr float kWTop = 8192.0f;      // p * scale is scaled to at most 4 kWTop, below 65504
 
     extern __shared__ __align__(128) uint8_t ring_raw[];
     constexpr int kSlots = slots_of(D);
@@ -139,23 +157,98 @@ kv4_decode_kernel(const Kv4AttentionArgs a, float* __restrict__ partials, const 
     __shared__ uint32_t s_abort;
     __shared__ float s_m[kWarps][HC], s_l[kWarps][HC];
 
+    __shared__ uint32_t s_rows[kMaxRows + 1];   // pairs of one list of all rows before a row
+    __shared__ uint32_t s_scan[kWarps];
+
     const uint32_t lane = threadIdx.x & 31u, warp = threadIdx.x >> 5;
     const uint32_t g = lane >> 2, t = lane & 3u;
-    const uint32_t first_head = kvh * rep + chunk * HC;
-    const uint32_t live_heads = min(static_cast<uint32_t>(HC), rep - chunk * HC);
     volatile uint32_t* abort = &s_abort;
-    uint32_t flags = span.bad ? B2_ATTN_STATUS_BAD_BLOCK : 0u;
+    const uint32_t rep = a.q_heads / a.cache.kv_heads;
+    const uint32_t head_chunks = (rep + HC - 1u) / HC, row_lists = a.cache.kv_heads * head_chunks;
 
     if (threadIdx.x == 0) s_abort = 0;
     if (lane == 0) {
         for (int i = 0; i < kSlots; ++i) mbar_init(&bars[warp][i], 1);
         mbar_fence_init();
     }
-    __syncthreads();
+
+    // ---- this CTA's range of pairs ----
+    uint32_t at = 0, at_end = 0, total = 0, ctas = 0, row = 0;
+    if (plan.whole_lists != 0u) {
+        row = blockIdx.x / row_lists;
+        const uint32_t pairs = row_pairs(row_span(a, row));
+        at = blockIdx.x % row_lists * pairs;
+        at_end = at + pairs;
+        __syncthreads();
+    } else {
+        const uint32_t per = (a.rows + kWarps * 32u - 1u) / (kWarps * 32u);   // rows of a thread
+        const uint32_t r0 = min(a.rows, threadIdx.x * per), r1 = min(a.rows, r0 + per);
+        uint32_t mine = 0;
+        for (uint32_t r = r0; r < r1; ++r) {
+            s_rows[r] = mine;
+            mine += row_pairs(row_span(a, r));
+        }
+        uint32_t before = mine;
+#pragma unroll
+        for (uint32_t o = 1; o < 32u; o <<= 1) {
+            const uint32_t up = __shfl_up_sync(0xFFFFFFFFu, before, o);
+            if (lane >= o) before += up;
+        }
+        if (lane == 31u) s_scan[warp] = before;
+        __syncthreads();
+        uint32_t all = 0;
+        before -= mine;
+#pragma unroll
+        for (uint32_t w = 0; w < kWarps; ++w) {
+            before += w < warp ? s_scan[w] : 0u;
+            all += s_scan[w];
+        }
+        for (uint32_t r = r0; r < r1; ++r) s_rows[r] += before;
+        if (threadIdx.x == 0) s_rows[a.rows] = all;
+        __syncthreads();
+        total = all * row_lists;
+        ctas = live_ctas(plan, a.rows * row_lists, total);
+        if (blockIdx.x >= ctas) return;
+        at = first_pair(blockIdx.x, total, ctas);
+        at_end = first_pair(blockIdx.x + 1u, total, ctas);
+        uint32_t lo = 0, hi = a.rows;   // the row with s_rows[row] * row_lists <= at < s_rows[row + 1] * row_lists
+        while (lo + 1u < hi) {
+            const uint32_t mid = (lo + hi) / 2u;
+            if (s_rows[mid] * row_lists <= at) lo = mid; else hi = mid;
+        }
+        row = lo;
+    }
 
     const uint32_t ring32 = smem_u32(ring_raw) + warp * (kSlots * kPairBytes);
-    const uint32_t my_first = tile0 + split * plan.tiles_per_split + warp * kPair;
-    const uint32_t tile_end = tile0 + min(tiles, (split + 1u) * plan.tiles_per_split);
+    uint32_t used = 0;      // pairs this warp has taken through its ring
+    uint32_t segment = 0;   // lists this CTA has begun
+    uint32_t flags = 0;
+    while (at < at_end) {
+    // ---- the next list of the range: its pairs [pair0, pair1) of `pairs` ----
+    const uint32_t row_first = plan.whole_lists != 0u ? 0u : s_rows[row] * row_lists;
+    const RowSpan span = row_span(a, row);
+    const uint32_t pairs = row_pairs(span);
+    if (at - row_first >= pairs * row_lists) {
+        ++row;
+        continue;
+    }
+    const uint32_t in_row = (at - row_first) / pairs, pair0 = (at - row_first) % pairs;
+    const uint32_t pair1 = min(pairs, pair0 + (at_end - at));
+    const uint32_t slot_of_list = segment == 0u ? 0u : 1u;   // a list that is not whole is the CTA's first or its last
+    if (plan.whole_lists == 0u && pair0 == 0u && threadIdx.x == 0) {
+        list_parts[row * row_lists + in_row] = ListParts{
+            blockIdx.x, pair1 == pairs ? blockIdx.x : owner_of(at + pairs - 1u, total, ctas), slot_of_list};
+    }
+    at += pair1 - pair0;
+    ++segment;
+    const uint32_t kvh = in_row / head_chunks, chunk = in_row % head_chunks;
+    const uint32_t first_head = kvh * rep + chunk * HC;
+    const uint32_t live_heads = min(static_cast<uint32_t>(HC), rep - chunk * HC);
+    if (span.bad) flags |= B2_ATTN_STATUS_BAD_BLOCK;
+    const uint32_t tile0 = span.begin / kKv4Tile;
+    const uint32_t tiles = span.end > span.begin ? (span.end - 1u) / kKv4Tile + 1u - tile0 : 0u;
+    const uint32_t my_first = tile0 + pair0 * kPair + warp * kPair;
+    const uint32_t tile_end = tile0 + min(tiles, pair1 * kPair);
     constexpr uint32_t kStride = kWarps * kPair;
     const uint32_t my_pairs = my_first < tile_end ? (tile_end - my_first + kStride - 1u) / kStride : 0u;
     const uint32_t* table = a.cache.block_tables + static_cast<uint64_t>(span.seq) * a.cache.max_blocks;
@@ -173,10 +266,10 @@ kv4_decode_kernel(const Kv4AttentionArgs a, float* __restrict__ partials, const 
             tile_offset = kv4_tile_offset(a.cache, phys, kvh, tile % a.cache.tiles_per_block);
         }
     };
-    // The whole warp: pair i of its list into slot i % kSlots (lanes 2(i % 16) and the next hold its offsets).
+    // The whole warp: pair i of its list into the next slot (lanes 2(i % 16) and the next hold its offsets).
     auto issue = [&](uint32_t i) {
         if ((i & 15u) == 0u) look_up(i);
-        const uint32_t slot = i % kSlots;
+        const uint32_t slot = (used + i) % kSlots;
         if (lane / kPair == (i & 15u)) {
             const uint32_t which = lane % kPair, tile = my_first + i * kStride + which;
             fence_proxy_async_smem();
@@ -289,6 +382,7 @@ kv4_decode_kernel(const Kv4AttentionArgs a, float* __restrict__ partials, const 
     float scale_top = 0.0f;      // power of two at or above it (0: none yet)
     float weight_factor = 0.0f;  // kWTop / scale_top
 
+    const uint32_t k1024 = opaque_1024();
     // This lane's part of a weight: the first 11 bits (even columns) or the rest (odd ones) of w, as
     // w * part_of + ((w & first 11 bits) ^ part_sign).
     const float part_of = (g & 1u) ? 1.0f : 0.0f;
@@ -296,11 +390,11 @@ kv4_decode_kernel(const Kv4AttentionArgs a, float* __restrict__ partials, const 
 
     for (uint32_t i = 0; i < my_pairs; ++i) {
         const uint32_t token0 = (my_first + i * kStride) * kKv4Tile;
-        const uint32_t slot32 = ring32 + (i % kSlots) * kPairBytes;
+        const uint32_t slot = (used + i) % kSlots, slot32 = ring32 + slot * kPairBytes;
         // Only the first and the last tiles hold tokens that are not seen (or no tile at all).
         const bool whole = token0 >= span.begin && token0 + kPair * kKv4Tile <= span.end &&
                            my_first + i * kStride + kPair <= tile_end;
-        mbar_wait(&bars[warp][i % kSlots], (i / kSlots) & 1u, abort);
+        mbar_wait(&bars[warp][slot], ((used + i) / kSlots) & 1u, abort);
         if (!whole) {
             // Lane l guards token l of the pair: a slot that is not seen may hold anything, NaN included.
             const uint32_t token = token0 + lane;
@@ -337,10 +431,10 @@ kv4_decode_kernel(const Kv4AttentionArgs a, float* __restrict__ partials, const 
                 for (int j = 0; j < 2; ++j)
 #pragma unroll
                     for (int u = 0; u < 2; ++u) {
-                        const uint32_t a0 = u == 0 ? codes_of<0>(r[2 * j]) : codes_of<2>(r[2 * j]);
-                        const uint32_t a1 = u == 0 ? codes_of<0>(r[2 * j + 1]) : codes_of<2>(r[2 * j + 1]);
-                        const uint32_t a2 = u == 0 ? codes_of<1>(r[2 * j]) : codes_of<3>(r[2 * j]);
-                        const uint32_t a3 = u == 0 ? codes_of<1>(r[2 * j + 1]) : codes_of<3>(r[2 * j + 1]);
+                        const uint32_t a0 = u == 0 ? codes_of<0>(r[2 * j], k1024) : codes_of<2>(r[2 * j], k1024);
+                        const uint32_t a1 = u == 0 ? codes_of<0>(r[2 * j + 1], k1024) : codes_of<2>(r[2 * j + 1], k1024);
+                        const uint32_t a2 = u == 0 ? codes_of<1>(r[2 * j], k1024) : codes_of<3>(r[2 * j], k1024);
+                        const uint32_t a3 = u == 0 ? codes_of<1>(r[2 * j + 1], k1024) : codes_of<3>(r[2 * j + 1], k1024);
 #pragma unroll
                         for (int part = 0; part < HL; ++part) {
                             mma16816(c, a0, a1, a2, a3, qf[2 * gr + j][u][0][part], qf[2 * gr + j][u][1][part]);
@@ -508,10 +602,10 @@ kv4_decode_kernel(const Kv4AttentionArgs a, float* __restrict__ partials, const 
 #pragma unroll
                     for (int u = 0; u < 2; ++u) {
                         // rows g and g + 8 are channels 4g + 2u and 4g + 2u + 1 of the chunk
-                        const uint32_t a0 = u == 0 ? codes_of<0>(r[2 * j]) : codes_of<2>(r[2 * j]);
-                        const uint32_t a1 = u == 0 ? codes_of<1>(r[2 * j]) : codes_of<3>(r[2 * j]);
-                        const uint32_t a2 = u == 0 ? codes_of<0>(r[2 * j + 1]) : codes_of<2>(r[2 * j + 1]);
-                        const uint32_t a3 = u == 0 ? codes_of<1>(r[2 * j + 1]) : codes_of<3>(r[2 * j + 1]);
+                        const uint32_t a0 = u == 0 ? codes_of<0>(r[2 * j], k1024) : codes_of<2>(r[2 * j], k1024);
+                        const uint32_t a1 = u == 0 ? codes_of<1>(r[2 * j], k1024) : codes_of<3>(r[2 * j], k1024);
+                        const uint32_t a2 = u == 0 ? codes_of<0>(r[2 * j + 1], k1024) : codes_of<2>(r[2 * j + 1], k1024);
+                        const uint32_t a3 = u == 0 ? codes_of<1>(r[2 * j + 1], k1024) : codes_of<3>(r[2 * j + 1], k1024);
 #pragma unroll
                         for (int part = 0; part < HL; ++part) {
                             mma16816(acc[2 * gr + j][u], a0, a1, a2, a3, b[0][part], b[1][part]);
@@ -524,7 +618,7 @@ kv4_decode_kernel(const Kv4AttentionArgs a, float* __restrict__ partials, const 
     }
 
     // ---- join the warps (the ring is free: it holds their accumulators) ----
-    if (lane == 0 && *abort != 0) flags |= B2_ATTN_STATUS_TIMEOUT;
+    used += my_pairs;
     __syncthreads();
     float* s_acc = reinterpret_cast<float*>(ring_raw);   // [warp][HC][D]
     const float undo = scale_top / kWTop;
@@ -561,8 +655,9 @@ kv4_decode_kernel(const Kv4AttentionArgs a, float* __restrict__ partials, const 
             }
         }
     }
-    if (flags != 0u) kv4_flag(a.status, flags);
     __syncthreads();
+    const bool whole = pair1 - pair0 == pairs;
+    float* const part = partials + static_cast<uint64_t>(blockIdx.x * 2u + slot_of_list) * HC * (D + 4u);
     for (uint32_t i = threadIdx.x; i < live_heads * (D / 4u); i += kWarps * 32u) {
         const uint32_t head = i / (D / 4u), c = (i % (D / 4u)) * 4u;
         float mm = s_m[0][head];
@@ -581,8 +676,8 @@ kv4_decode_kernel(const Kv4AttentionArgs a, float* __restrict__ partials, const 
             o.w = fmaf(x.w, f, o.w);
         }
         const uint64_t out_head = static_cast<uint64_t>(row) * a.q_heads + first_head + head;
-        if (n_splits > 1u) {
-            float* dst = partials + (out_head * plan.splits + split) * (D + 4u);
+        if (!whole) {
+            float* dst = part + head * (D + 4u);
             *reinterpret_cast<float4*>(dst + 4u + c) = o;
             if (c == 0) {
                 dst[0] = mm;
@@ -593,109 +688,158 @@ kv4_decode_kernel(const Kv4AttentionArgs a, float* __restrict__ partials, const 
         if (ll == 0.0f && tiles != 0u && c == 0) kv4_flag(a.status, B2_ATTN_STATUS_ALL_NEG_INF);
         put_context<D>(a, out_head, c, o, ll);
     }
+    if (at < at_end) __syncthreads();   // the ring and the statistics are free again
+    }
+    if (lane == 0 && *abort != 0) flags |= B2_ATTN_STATUS_TIMEOUT;
+    if (flags != 0u) kv4_flag(a.status, flags);
 }
 
-// Joins the splits of every (row, query head) that has more than one.
-template <int D>
-__global__ void __launch_bounds__(D / 4)
-kv4_merge_kernel(const Kv4AttentionArgs a, const float* __restrict__ partials, const SplitPlan plan) {
+// Joins the partial results of every list that more than one CTA worked on: a CTA for each list and head, in which
+// kJoiners groups of threads join a run of them each and then, in order, one another's.
+constexpr uint32_t kJoiners = 8;
+template <int D, int HC>
+__global__ void __launch_bounds__(D / 4 * kJoiners)
+kv4_merge_kernel(const Kv4AttentionArgs a, const ListParts* list_parts, const float* partials) {
     sm100::pdl_launch_dependents();
-    const uint64_t out_head = blockIdx.x;
-    const uint32_t row = static_cast<uint32_t>(out_head / a.q_heads);
-    const RowSpan span = row_span(a, row);   // inputs of the call, not of the kernel before
-    const uint32_t tile0 = span.begin / kKv4Tile;
-    const uint32_t tiles = span.end > span.begin ? (span.end - 1u) / kKv4Tile + 1u - tile0 : 0u;
-    const uint32_t n_splits = max(1u, (tiles + plan.tiles_per_split - 1u) / plan.tiles_per_split);
+    const uint32_t rep = a.q_heads / a.cache.kv_heads;
+    const uint32_t head_chunks = (rep + HC - 1u) / HC, row_lists = a.cache.kv_heads * head_chunks;
+    const uint32_t list = blockIdx.x / HC, head = blockIdx.x % HC;
+    const uint32_t row = list / row_lists, in_row = list % row_lists, chunk = in_row % head_chunks;
+    const bool mine = head < rep - chunk * HC && (a.chunk_starts == nullptr || row_span(a, row).owned);
     sm100::pdl_wait();   // every CTA waits, so that this grid never ends before the one it follows
-    if (n_splits <= 1u || !span.owned) return;
-    join_splits<D>(a, partials + out_head * plan.splits * (D + 4u), out_head, n_splits, threadIdx.x * 4u, true);
+    if (!mine) return;
+    const ListParts parts = list_parts[list];
+    if (parts.first == parts.last) return;
+    const uint32_t n = parts.last - parts.first + 1u;
+    const uint64_t out_head = static_cast<uint64_t>(row) * a.q_heads + in_row / head_chunks * rep + chunk * HC + head;
+    const uint64_t stride = 2ull * HC * (D + 4u);   // between CTAs
+    const float* first = partials + ((parts.first * 2ull + parts.slot) * HC + head) * (D + 4u);
+    const float* rest = partials + ((parts.first + 1ull) * 2u * HC + head) * (D + 4u);
+    const uint32_t c = threadIdx.x % (D / 4u) * 4u, joiner = threadIdx.x / (D / 4u);
+    const uint32_t run = (n + kJoiners - 1u) / kJoiners, i0 = min(n, joiner * run), i1 = min(n, i0 + run);
+    __shared__ __align__(16) float s_part[kJoiners][D + 4];
+    Joined mine_joined = join_run(i0 == 0u ? first : rest + (i0 - 1u) * stride, rest + i0 * stride, stride, i1 - i0, c);
+    *reinterpret_cast<float4*>(&s_part[joiner][4u + c]) = mine_joined.o;
+    if (c == 0u) {
+        s_part[joiner][0] = mine_joined.m;
+        s_part[joiner][1] = mine_joined.l;
+    }
+    __syncthreads();
+    if (joiner != 0u) return;
+    const Joined all = join_run(s_part[0], s_part[1], D + 4u, kJoiners, c);
+    finish<D>(a, all, out_head, c, true);
 }
 
 uint32_t heads_together(uint32_t rep) { return rep <= 4u ? 4u : 8u; }
 
-// Tiles of one CTA. Split finer while the card is not filled (four CTAs for every SM), but never below
-// 16 tiles: a CTA's own set-up and the join cost about as much as four tiles a warp.
-SplitPlan split_plan(int sm_count, uint64_t rows, uint32_t q_heads, uint32_t kv_heads, uint32_t max_seq_len) {
-    const uint32_t rep = q_heads / kv_heads;
-    const uint64_t sms = sm_count > 0 ? static_cast<uint64_t>(sm_count) : 148u;
-    const uint64_t lists = rows * kv_heads * ((rep + heads_together(rep) - 1u) / heads_together(rep));
-    const uint64_t tiles = (static_cast<uint64_t>(max_seq_len) + kKv4Tile - 1u) / kKv4Tile;
-    const uint64_t wanted = 4u * sms;   // CTAs
-    uint64_t per = tiles;
-    if (lists < wanted) per = (tiles * lists + wanted - 1u) / wanted;
-    if (per < 16u) per = 16u;
-    if (per > 128u) per = 128u;
-    per = (per + kPair - 1u) / kPair * kPair;
-    return SplitPlan{static_cast<uint32_t>((tiles + per - 1u) / per), static_cast<uint32_t>(per)};
-}
+constexpr int ring_bytes(int d) { return kWarps * slots_of(d) * kPair * static_cast<int>(kv4_tile_bytes(d)); }
 
+// Configures one form of the kernel on the current device and reports how many of its CTAs an SM holds.
 template <int D, int HC>
-int32_t launch_one(const DeviceContext& ctx, const Kv4AttentionArgs& a, float* partials, const SplitPlan& plan,
-                   unsigned blocks, cudaStream_t stream) {
-    constexpr int kRing = kWarps * slots_of(D) * kPair * static_cast<int>(kv4_tile_bytes(D));
+int32_t resident_ctas(const DeviceContext& ctx, uint32_t* out) {
     static PerDeviceOnce configured;
-    B2_TRY(once_per_device(configured, ctx.device, []() -> int32_t {
-        B2_CUDA_TRY(cudaFuncSetAttribute(kv4_decode_kernel<D, HC>, cudaFuncAttributeMaxDynamicSharedMemorySize, kRing));
+    static uint32_t resident[kMaxDevices];
+    B2_TRY(once_per_device(configured, ctx.device, [&]() -> int32_t {
+        B2_CUDA_TRY(cudaFuncSetAttribute(kv4_decode_kernel<D, HC>, cudaFuncAttributeMaxDynamicSharedMemorySize, ring_bytes(D)));
+        int n = 0;
+        B2_CUDA_TRY(cudaOccupancyMaxActiveBlocksPerMultiprocessor(&n, kv4_decode_kernel<D, HC>, kWarps * 32, ring_bytes(D)));
+        resident[ctx.device] = n > 0 ? static_cast<uint32_t>(n) : 1u;
         return B2_STATUS_OK;
     }));
-    kv4_decode_kernel<D, HC><<<blocks, kWarps * 32, kRing, stream>>>(a, partials, plan);
-    B2_CUDA_TRY(cudaGetLastError());
+    *out = resident[ctx.device];
     return B2_STATUS_OK;
 }
 
-template <int D>
-int32_t launch_merge(const Kv4AttentionArgs& a, const float* partials, const SplitPlan& plan, cudaStream_t stream) {
+struct Sizes {
+    uint32_t d, together;
+    uint64_t lists;
+};
+
+int32_t work_plan(const DeviceContext& ctx, uint64_t rows, uint32_t q_heads, uint32_t kv_heads, uint32_t d,
+                  uint32_t max_seq_len, WorkPlan* plan, Sizes* sizes) {
+    const uint32_t rep = q_heads / kv_heads, together = heads_together(rep);
+    const uint64_t lists = rows * kv_heads * ((rep + together - 1u) / together);
+    if (lists > 0x0FFFFFFFull) return fail(B2_STATUS_OVERFLOW, "paged attention batch too large");
+    *sizes = Sizes{d, together, lists};
+    uint32_t resident = 0;
+    switch (d) {
+    case 64: B2_TRY(together == 4u ? (resident_ctas<64, 4>(ctx, &resident)) : (resident_ctas<64, 8>(ctx, &resident))); break;
+    case 128: B2_TRY(together == 4u ? (resident_ctas<128, 4>(ctx, &resident)) : (resident_ctas<128, 8>(ctx, &resident))); break;
+    default: B2_TRY(together == 4u ? (resident_ctas<256, 4>(ctx, &resident)) : (resident_ctas<256, 8>(ctx, &resident))); break;
+    }
+    // a window's first tile may be cut: one tile more than the tokens alone
+    const uint64_t pairs = (static_cast<uint64_t>(max_seq_len) + kKv4Tile - 1u) / (kKv4Tile * kPair) + 1u;
+    // prefix sums of the pairs are 32-bit numbers
+    if (rows > kMaxRows || pairs <= kMinPairs || lists * pairs > 0xFFFFFFFFull) {
+        *plan = WorkPlan{static_cast<uint32_t>(lists), 1u};
+        return B2_STATUS_OK;
+    }
+    const uint64_t held = (ctx.sm_count > 0 ? static_cast<uint64_t>(ctx.sm_count) : 148u) * resident;
+    uint64_t ctas = (lists * pairs + kMinPairs - 1u) / kMinPairs;
+    if (ctas > held) ctas = held * ((lists * pairs + held * kMostPairs - 1u) / (held * kMostPairs));
+    *plan = WorkPlan{static_cast<uint32_t>(ctas), 0u};
+    return B2_STATUS_OK;
+}
+
+size_t table_bytes(const Sizes& s) { return (static_cast<size_t>(s.lists) * sizeof(ListParts) + 255u) & ~size_t{255}; }
+size_t plan_bytes(const WorkPlan& plan, const Sizes& s) {
+    if (plan.whole_lists != 0u) return 0;
+    return table_bytes(s) + static_cast<size_t>(plan.ctas) * 2u * s.together * (s.d + 4u) * sizeof(float);
+}
+
+template <int D, int HC>
+int32_t launch_one(const Kv4AttentionArgs& a, void* workspace, const WorkPlan& plan, const Sizes& sizes, cudaStream_t stream) {
+    ListParts* lists = static_cast<ListParts*>(workspace);
+    float* partials = workspace == nullptr ? nullptr
+                                           : reinterpret_cast<float*>(static_cast<uint8_t*>(workspace) + table_bytes(sizes));
+    kv4_decode_kernel<D, HC><<<plan.ctas, kWarps * 32, ring_bytes(D), stream>>>(a, lists, partials, plan);
+    B2_CUDA_TRY(cudaGetLastError());
+    if (plan.whole_lists != 0u) return B2_STATUS_OK;
     cudaLaunchConfig_t config{};
-    config.gridDim = dim3(static_cast<unsigned>(static_cast<uint64_t>(a.rows) * a.q_heads));
-    config.blockDim = dim3(D / 4);
+    config.gridDim = dim3(static_cast<unsigned>(sizes.lists * HC));
+    config.blockDim = dim3(D / 4 * kJoiners);
     config.stream = stream;
     cudaLaunchAttribute attribute[1];
     attribute[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
     attribute[0].val.programmaticStreamSerializationAllowed = 1;
     config.attrs = attribute;
     config.numAttrs = 1;
-    B2_CUDA_TRY(cudaLaunchKernelEx(&config, kv4_merge_kernel<D>, a, partials, plan));
+    B2_CUDA_TRY(cudaLaunchKernelEx(&config, kv4_merge_kernel<D, HC>, a, static_cast<const ListParts*>(lists),
+                                   static_cast<const float*>(partials)));
     return B2_STATUS_OK;
 }
 
 }  // namespace
 
-size_t kv4_decode_workspace_bytes(int sm_count, uint64_t rows, uint32_t q_heads, uint32_t kv_heads, uint32_t head_width,
-                                  uint32_t max_seq_len) {
-    const SplitPlan plan = split_plan(sm_count, rows, q_heads, kv_heads, max_seq_len);
-    if (plan.splits <= 1u) return 0;
-    return static_cast<size_t>(rows) * q_heads * plan.splits * (head_width + 4u) * sizeof(float);
+int32_t kv4_decode_workspace_bytes(const DeviceContext& ctx, uint64_t rows, uint32_t q_heads, uint32_t kv_heads,
+                                   uint32_t head_width, uint32_t max_seq_len, size_t* bytes) {
+    WorkPlan plan;
+    Sizes sizes;
+    B2_TRY(work_plan(ctx, rows, q_heads, kv_heads, head_width, max_seq_len, &plan, &sizes));
+    *bytes = plan_bytes(plan, sizes);
+    return B2_STATUS_OK;
 }
 
 int32_t launch_kv4_decode(const DeviceContext& ctx, const Kv4AttentionArgs& a, void* workspace, size_t workspace_bytes,
                           cudaStream_t stream) {
-    const size_t need = kv4_decode_workspace_bytes(ctx.sm_count, a.rows, a.q_heads, a.cache.kv_heads,
-                                                   a.cache.head_width, a.max_seq_len);
+    WorkPlan plan;
+    Sizes sizes;
+    B2_TRY(work_plan(ctx, a.rows, a.q_heads, a.cache.kv_heads, a.cache.head_width, a.max_seq_len, &plan, &sizes));
+    const size_t need = plan_bytes(plan, sizes);
     if (need > workspace_bytes) {
         return fail(B2_STATUS_INVALID_ARGUMENT, "paged attention workspace too small: need %zu bytes, got %zu", need,
                     workspace_bytes);
     }
-    const SplitPlan plan = split_plan(ctx.sm_count, a.rows, a.q_heads, a.cache.kv_heads, a.max_seq_len);
-    const uint32_t rep = a.q_heads / a.cache.kv_heads, together = heads_together(rep);
-    const uint64_t blocks = static_cast<uint64_t>(a.rows) * a.cache.kv_heads * ((rep + together - 1u) / together) *
-                            plan.splits;
-    const uint64_t merges = static_cast<uint64_t>(a.rows) * a.q_heads;
-    if (blocks > 0x7FFFFFFFull || merges > 0x7FFFFFFFull) return fail(B2_STATUS_OVERFLOW, "paged attention batch too large");
-    float* partials = static_cast<float*>(workspace);
-    const unsigned n = static_cast<unsigned>(blocks);
     switch (a.cache.head_width) {
     case 64:
-        B2_TRY(together == 4u ? (launch_one<64, 4>(ctx, a, partials, plan, n, stream))
-                              : (launch_one<64, 8>(ctx, a, partials, plan, n, stream)));
-        return plan.splits > 1u ? launch_merge<64>(a, partials, plan, stream) : B2_STATUS_OK;
+        return sizes.together == 4u ? launch_one<64, 4>(a, workspace, plan, sizes, stream)
+                                    : launch_one<64, 8>(a, workspace, plan, sizes, stream);
     case 128:
-        B2_TRY(together == 4u ? (launch_one<128, 4>(ctx, a, partials, plan, n, stream))
-                              : (launch_one<128, 8>(ctx, a, partials, plan, n, stream)));
-        return plan.splits > 1u ? launch_merge<128>(a, partials, plan, stream) : B2_STATUS_OK;
+        return sizes.together == 4u ? launch_one<128, 4>(a, workspace, plan, sizes, stream)
+                                    : launch_one<128, 8>(a, workspace, plan, sizes, stream);
     default:
-        B2_TRY(together == 4u ? (launch_one<256, 4>(ctx, a, partials, plan, n, stream))
-                              : (launch_one<256, 8>(ctx, a, partials, plan, n, stream)));
-        return plan.splits > 1u ? launch_merge<256>(a, partials, plan, stream) : B2_STATUS_OK;
+        return sizes.together == 4u ? launch_one<256, 4>(a, workspace, plan, sizes, stream)
+                                    : launch_one<256, 8>(a, workspace, plan, sizes, stream);
     }
 }
 
