@@ -22,12 +22,17 @@ namespace {
 
 constexpr int kAppendWarps = 8;
 
-__device__ __forceinline__ float lane_min(float v, int lanes) {
-    for (int o = lanes / 2; o > 0; o >>= 1) v = fminf(v, __shfl_xor_sync(0xFFFFFFFFu, v, o));
+// Over the 8 or 16 lanes that share a group.
+template <int LANES>
+__device__ __forceinline__ float lane_min(float v, uint32_t mask) {
+#pragma unroll
+    for (int o = LANES / 2; o > 0; o >>= 1) v = fminf(v, __shfl_xor_sync(mask, v, o));
     return v;
 }
-__device__ __forceinline__ float lane_max(float v, int lanes) {
-    for (int o = lanes / 2; o > 0; o >>= 1) v = fmaxf(v, __shfl_xor_sync(0xFFFFFFFFu, v, o));
+template <int LANES>
+__device__ __forceinline__ float lane_max(float v, uint32_t mask) {
+#pragma unroll
+    for (int o = LANES / 2; o > 0; o >>= 1) v = fmaxf(v, __shfl_xor_sync(mask, v, o));
     return v;
 }
 
@@ -60,129 +65,95 @@ __device__ __forceinline__ uint32_t code_of(float x, const GroupCode& g) {
     return static_cast<uint32_t>(fminf(fmaxf(c, 0.0f), 15.0f));
 }
 
-// One warp stores one head vector of one token. Lane l holds channels E*l .. E*l + E - 1 of the lower
-// half (`lo`) and of the upper half (`hi`) of the head, E = D / 64: the rotation pairs (c, c + D/2), so
-// both of a pair are in one lane. `half_tile` points at the keys' or the values' 9D bytes of the tile.
+// D / 8 lanes store one head vector of one token. Lane l of them holds channels 4l .. 4l + 3 of the lower half (`lo`)
+// and of the upper half (`hi`) of the head: the rotation pairs (c, c + D/2), so both of a pair are in one lane.
+// `mask`: those lanes. `half_tile` points at the keys' or the values' 9D bytes of the tile.
 template <int D>
-__device__ __forceinline__ void store_vector(const float (&lo)[D / 64], const float (&hi)[D / 64],
-                                             uint8_t* half_tile, uint32_t slot, uint32_t lane) {
-    constexpr int E = D / 64;
-    // Lanes that share a group: D = 64 has one group over both halves; D = 128 one for each half (all 32
-    // lanes); D = 256 two for each half (16 lanes each).
-    constexpr int kLanes = D == 256 ? 16 : 32;
-    float lo_min = lo[0], lo_max = lo[0], hi_min = hi[0], hi_max = hi[0];
-    bool lo_ok = true, hi_ok = true;
-#pragma unroll
-    for (int e = 0; e < E; ++e) {
-        lo_min = fminf(lo_min, lo[e]);
-        lo_max = fmaxf(lo_max, lo[e]);
-        hi_min = fminf(hi_min, hi[e]);
-        hi_max = fmaxf(hi_max, hi[e]);
-        lo_ok = lo_ok && fabsf(lo[e]) < INFINITY;   // false for a NaN too
-        hi_ok = hi_ok && fabsf(hi[e]) < INFINITY;
-    }
+__device__ __forceinline__ void store_vector(const float4& lo, const float4& hi, uint8_t* half_tile, uint32_t slot,
+                                             uint32_t l, uint32_t mask) {
+    // Lanes that share a group: at D = 64 all 8, over both halves; else 16, one group (D = 128) or two in each half.
+    constexpr int kLanes = D == 64 ? 8 : 16;
+    float lo_min = fminf(fminf(lo.x, lo.y), fminf(lo.z, lo.w)), lo_max = fmaxf(fmaxf(lo.x, lo.y), fmaxf(lo.z, lo.w));
+    float hi_min = fminf(fminf(hi.x, hi.y), fminf(hi.z, hi.w)), hi_max = fmaxf(fmaxf(hi.x, hi.y), fmaxf(hi.z, hi.w));
+    // false for a NaN too; infinities the range check below finds
+    bool lo_ok = lo.x == lo.x && lo.y == lo.y && lo.z == lo.z && lo.w == lo.w;
+    bool hi_ok = hi.x == hi.x && hi.y == hi.y && hi.z == hi.z && hi.w == hi.w;
     if (D == 64) {
-        lo_min = hi_min = fminf(lo_min, hi_min);
-        lo_max = hi_max = fmaxf(lo_max, hi_max);
-        lo_ok = hi_ok = lo_ok && hi_ok;
+        lo_min = fminf(lo_min, hi_min);
+        lo_max = fmaxf(lo_max, hi_max);
+        lo_ok = lo_ok && hi_ok;
     }
-    lo_min = lane_min(lo_min, kLanes);
-    lo_max = lane_max(lo_max, kLanes);
-    const uint32_t mine = D == 256 ? (0xFFFFu << (lane & 16u)) : 0xFFFFFFFFu;
-    lo_ok = (__ballot_sync(0xFFFFFFFFu, lo_ok) & mine) == mine;
-    GroupCode gl = group_code(lo_min, lo_max, lo_ok), gh = gl;
+    const uint32_t sharers = D == 256 ? 0xFFFFu << (l & 16u) : mask;
+    lo_min = lane_min<kLanes>(lo_min, mask);
+    lo_max = lane_max<kLanes>(lo_max, mask);
+    lo_ok = (__ballot_sync(mask, lo_ok) & sharers) == sharers;
+    const GroupCode gl = group_code(lo_min, lo_max, lo_ok);
+    GroupCode gh = gl;
     if (D != 64) {
-        hi_min = lane_min(hi_min, kLanes);
-        hi_max = lane_max(hi_max, kLanes);
-        hi_ok = (__ballot_sync(0xFFFFFFFFu, hi_ok) & mine) == mine;
+        hi_min = lane_min<kLanes>(hi_min, mask);
+        hi_max = lane_max<kLanes>(hi_max, mask);
+        hi_ok = (__ballot_sync(mask, hi_ok) & sharers) == sharers;
         gh = group_code(hi_min, hi_max, hi_ok);
     }
-    uint32_t wl = 0, wh = 0;   // E codes each
-#pragma unroll
-    for (int e = 0; e < E; ++e) {
-        wl |= code_of(lo[e], gl) << (4 * e);
-        wh |= code_of(hi[e], gh) << (4 * e);
-    }
-    // gather 8 codes (4 bytes) in every (8 / E)-th lane
-    constexpr int kPerWord = 8 / E;
-    uint32_t shift = 4u * E;
-#pragma unroll
-    for (int o = 1; o < kPerWord; o <<= 1) {
-        wl |= __shfl_down_sync(0xFFFFFFFFu, wl, o) << shift;
-        wh |= __shfl_down_sync(0xFFFFFFFFu, wh, o) << shift;
-        shift <<= 1;
-    }
-    if (lane % kPerWord == 0) {
-        const uint32_t channel = E * lane;   // of 8 codes, inside the half
-        auto put = [&](uint32_t c, uint32_t word) {
-            *reinterpret_cast<uint32_t*>(half_tile + (c / 32u) * 256u + slot * 16u + (c % 32u) / 2u) = word;
+    // 4 codes of each half; of two lanes, one word
+    uint32_t wl = code_of(lo.x, gl) | code_of(lo.y, gl) << 4 | code_of(lo.z, gl) << 8 | code_of(lo.w, gl) << 12;
+    uint32_t wh = code_of(hi.x, gh) | code_of(hi.y, gh) << 4 | code_of(hi.z, gh) << 8 | code_of(hi.w, gh) << 12;
+    wl |= __shfl_down_sync(mask, wl, 1) << 16;
+    wh |= __shfl_down_sync(mask, wh, 1) << 16;
+    if (l % 2u == 0u) {
+        const uint32_t c = 4u * l;
+        auto put = [&](uint32_t channel, uint32_t word) {
+            *reinterpret_cast<uint32_t*>(half_tile + (channel / 32u) * 256u + slot * 16u + (channel % 32u) / 2u) = word;
         };
-        put(channel, wl);
-        put(channel + D / 2, wh);
+        put(c, wl);
+        put(c + D / 2, wh);
     }
-    uint32_t* pairs = reinterpret_cast<uint32_t*>(half_tile + 8u * D) + slot * E;
-    if (D == 64) {
-        if (lane == 0) pairs[0] = gl.pair;
-    } else if (D == 128) {
-        if (lane == 0) pairs[0] = gl.pair;
-        if (lane == 0) pairs[1] = gh.pair;
-    } else if (lane % 16u == 0) {
-        pairs[lane / 16u] = gl.pair;
-        pairs[2 + lane / 16u] = gh.pair;
+    uint32_t* pairs = reinterpret_cast<uint32_t*>(half_tile + 8u * D) + slot * (D / 64);
+    if (l % 16u == 0u) {
+        pairs[l / 16u] = gl.pair;
+        if (D != 64) pairs[D / 128 + l / 16u] = gh.pair;
     }
 }
 
-template <int E>
-__device__ __forceinline__ void load_e(float (&dst)[E], const float* src) {
-    if constexpr (E == 1) {
-        dst[0] = *src;
-    } else if constexpr (E == 2) {
-        const float2 t = *reinterpret_cast<const float2*>(src);
-        dst[0] = t.x;
-        dst[1] = t.y;
-    } else {
-        const float4 t = *reinterpret_cast<const float4*>(src);
-        dst[0] = t.x;
-        dst[1] = t.y;
-        dst[2] = t.z;
-        dst[3] = t.w;
-    }
-}
-template <int E>
-__device__ __forceinline__ void store_e(float* dst, const float (&src)[E]) {
-    if constexpr (E == 1) {
-        *dst = src[0];
-    } else if constexpr (E == 2) {
-        *reinterpret_cast<float2*>(dst) = make_float2(src[0], src[1]);
-    } else {
-        *reinterpret_cast<float4*>(dst) = make_float4(src[0], src[1], src[2], src[3]);
-    }
-}
-
-// Grid (token run, slice). A CTA takes `per_cta` consecutive tokens and, of each, every gridDim.y-th
-// group of warps' heads: q heads are rotated, k heads rotated and stored, v heads stored. The angles of
-// a token are the same for all its heads: the first D/2 threads work them out once (in double: position *
-// theta^(-2c/D) passes 10^5 radians in long contexts, where FP32 has lost the phase) into shared memory.
-// Memory-bound for prompts (12.3 KB of q and k, v per token at 32 / 8 heads of 128 against 4.6 KB of
-// 4-bit pages); a single token is bound by the latency of the double-precision angle.
+// Grid (token run, slice). A CTA takes `per_cta` consecutive tokens and, of each, every gridDim.y-th group of its lanes'
+// head vectors: q heads are rotated, k heads rotated and stored, v heads stored. The angles of a token are the same for
+// all its heads: the first D/2 threads work them out once (in double: position * theta^(-2c/D) passes 10^5 radians
+// in long contexts, where FP32 has lost the phase) into shared memory. A prompt is bound by HBM (24.6 KB of q, k and
+// v in, 16.4 KB of q and 1.2 KB of pages out per token at 32 / 8 heads of 128): 16-byte accesses, and the next
+// vector's loads under way while one is worked on. A single token is bound by the latency of its angle.
 template <int D>
 __global__ void __launch_bounds__(kAppendWarps * 32)
 kv4_append_kernel(const Kv4AppendArgs a, uint32_t per_cta) {
     sm100::pdl_launch_dependents();
-    constexpr int E = D / 64, kHalf = D / 2;
+    constexpr uint32_t kHalf = D / 2, kLanes = D / 8, kVectors = 32u / kLanes * kAppendWarps;   // vectors of a CTA at once
     __shared__ __align__(16) float s_cos[2][kHalf], s_sin[2][kHalf];
-    const uint32_t lane = threadIdx.x & 31u, warp = threadIdx.x >> 5;
-    const uint32_t heads = a.q_heads + 2u * a.cache.kv_heads;
+    const uint32_t l = threadIdx.x % kLanes, first = blockIdx.y * kVectors + threadIdx.x / kLanes;
+    const uint32_t mask = D == 256 ? 0xFFFFFFFFu : ((1u << (kLanes % 32u)) - 1u) << (threadIdx.x % 32u / kLanes * kLanes);
+    const uint32_t heads = a.q_heads + 2u * a.cache.kv_heads, stride = gridDim.y * kVectors;
     double turn = 0.0;
     if (threadIdx.x < kHalf) {
         turn = pow(static_cast<double>(a.theta), static_cast<double>(threadIdx.x) * -2.0 / static_cast<double>(D));
     }
+    struct Vector {
+        float4 lo, hi;
+    };
+    auto source = [&](uint64_t token, uint32_t h) -> const float* {
+        const float* base = h < a.q_heads ? a.q : h < a.q_heads + a.cache.kv_heads ? a.k : a.v;
+        const uint32_t head = h < a.q_heads ? h : h < a.q_heads + a.cache.kv_heads ? h - a.q_heads : h - a.q_heads - a.cache.kv_heads;
+        return base + (token * (h < a.q_heads ? a.q_heads : a.cache.kv_heads) + head) * D + 4u * l;
+    };
+    auto load = [&](uint64_t token, uint32_t h) {   // q_out may be q: a lane reads both halves of its pairs before it writes
+        const float* src = source(token, h);
+        return Vector{*reinterpret_cast<const float4*>(src), *reinterpret_cast<const float4*>(src + kHalf)};
+    };
     uint32_t buffer = 0;
     for (uint32_t i = 0; i < per_cta; ++i) {
         const uint64_t token = static_cast<uint64_t>(blockIdx.x) * per_cta + i;
         if (token >= a.n_tokens) return;
         const uint32_t position = a.positions[token];
         if (position == kKv4Pad) continue;   // the same for every thread: no barrier is skipped by some
+        Vector next;
+        if (first < heads) next = load(token, first);
         float* const cosines = s_cos[buffer];
         float* const sines = s_sin[buffer];
         buffer ^= 1u;
@@ -199,78 +170,69 @@ kv4_append_kernel(const Kv4AppendArgs a, uint32_t per_cta) {
         if (!good && threadIdx.x == 0 && blockIdx.y == 0) kv4_flag(a.status, B2_ATTN_STATUS_BAD_BLOCK);
         // One barrier a token: a buffer is written again two barriers after its readers' own.
         __syncthreads();
-        float cs[E], sn[E];
-#pragma unroll
-        for (int e = 0; e < E; ++e) {
-            cs[e] = cosines[E * lane + e];
-            sn[e] = sines[E * lane + e];
-        }
-        for (uint32_t h = blockIdx.y * kAppendWarps + warp; h < heads; h += gridDim.y * kAppendWarps) {
+        const float4 cs = *reinterpret_cast<const float4*>(cosines + 4u * l), sn = *reinterpret_cast<const float4*>(sines + 4u * l);
+        for (uint32_t h = first; h < heads; h += stride) {
+            Vector x = next;
+            if (h + stride < heads) next = load(token, h + stride);
             const bool is_q = h < a.q_heads, is_k = !is_q && h < a.q_heads + a.cache.kv_heads;
-            if (!is_q && !good) continue;
-            const uint32_t head = is_q ? h : (is_k ? h - a.q_heads : h - a.q_heads - a.cache.kv_heads);
-            const uint64_t at = (token * (is_q ? a.q_heads : a.cache.kv_heads) + head) * D;
-            const float* src = (is_q ? a.q : is_k ? a.k : a.v) + at;
-            float lo[E], hi[E];
-            load_e<E>(lo, src + E * lane);   // q_out may be q: a lane reads both halves of its pairs first
-            load_e<E>(hi, src + kHalf + E * lane);
             if (is_q || is_k) {
-#pragma unroll
-                for (int e = 0; e < E; ++e) {
-                    const float x = lo[e], y = hi[e];
-                    lo[e] = __fsub_rn(__fmul_rn(x, cs[e]), __fmul_rn(y, sn[e]));
-                    hi[e] = __fadd_rn(__fmul_rn(y, cs[e]), __fmul_rn(x, sn[e]));
-                }
+                auto turned = [](float p, float q, float c, float s, float* lo, float* hi) {
+                    *lo = __fsub_rn(__fmul_rn(p, c), __fmul_rn(q, s));
+                    *hi = __fadd_rn(__fmul_rn(q, c), __fmul_rn(p, s));
+                };
+                const Vector y = x;
+                turned(y.lo.x, y.hi.x, cs.x, sn.x, &x.lo.x, &x.hi.x);
+                turned(y.lo.y, y.hi.y, cs.y, sn.y, &x.lo.y, &x.hi.y);
+                turned(y.lo.z, y.hi.z, cs.z, sn.z, &x.lo.z, &x.hi.z);
+                turned(y.lo.w, y.hi.w, cs.w, sn.w, &x.lo.w, &x.hi.w);
             }
             if (is_q) {
-                store_e<E>(a.q_out + at + E * lane, lo);
-                store_e<E>(a.q_out + at + kHalf + E * lane, hi);
-            } else {
-                uint8_t* half_tile = a.cache.pages + kv4_tile_offset(a.cache, phys, head, tile) +
-                                     (is_k ? 0u : kv4_half_bytes(D));
-                store_vector<D>(lo, hi, half_tile, slot, lane);
+                float* dst = a.q_out + (token * a.q_heads + h) * D + 4u * l;
+                *reinterpret_cast<float4*>(dst) = x.lo;
+                *reinterpret_cast<float4*>(dst + kHalf) = x.hi;
+            } else if (good) {
+                const uint32_t head = is_k ? h - a.q_heads : h - a.q_heads - a.cache.kv_heads;
+                uint8_t* half_tile = a.cache.pages + kv4_tile_offset(a.cache, phys, head, tile) + (is_k ? 0u : kv4_half_bytes(D));
+                store_vector<D>(x.lo, x.hi, half_tile, slot, l, mask);
             }
         }
     }
 }
 
-// Eight channels per thread: 4 bytes of codes and one pair in, 32 bytes out.
+// D / 4 threads read one stored vector back, four channels each: 2 bytes of codes and a pair in, 16 bytes out, so that
+// a warp writes 512 bytes in a row.
 template <int D>
 __global__ void __launch_bounds__(256) kv4_read_kernel(const Kv4ReadArgs a) {
-    constexpr uint32_t kParts = D / 8;
-    const uint64_t items = static_cast<uint64_t>(a.n_tokens) * a.cache.kv_heads * 2u * kParts;
-    const uint64_t stride = static_cast<uint64_t>(gridDim.x) * blockDim.x;
-    for (uint64_t i = static_cast<uint64_t>(blockIdx.x) * blockDim.x + threadIdx.x; i < items; i += stride) {
-        const uint32_t part = static_cast<uint32_t>(i % kParts);
-        const uint64_t vector = i / kParts;
-        const uint32_t head = static_cast<uint32_t>(vector % a.cache.kv_heads);
-        const uint64_t half = vector / a.cache.kv_heads;
-        const uint32_t is_v = static_cast<uint32_t>(half & 1u);
-        const uint64_t token = half >> 1;
+    constexpr uint32_t kThreads = D / 4, kVectors = 256u / kThreads;
+    const uint32_t c = threadIdx.x % kThreads * 4u;
+    const uint64_t vectors = static_cast<uint64_t>(a.n_tokens) * a.cache.kv_heads;
+    for (uint64_t i = static_cast<uint64_t>(blockIdx.x) * kVectors + threadIdx.x / kThreads; i < vectors;
+         i += static_cast<uint64_t>(gridDim.x) * kVectors) {
+        const uint32_t token = static_cast<uint32_t>(i / a.cache.kv_heads), head = static_cast<uint32_t>(i % a.cache.kv_heads);
         const uint32_t position = __ldg(a.positions + token);
         if (position == kKv4Pad) continue;
-        const uint32_t seq = a.token_seq != nullptr ? __ldg(a.token_seq + token) : static_cast<uint32_t>(token);
+        const uint32_t seq = a.token_seq != nullptr ? __ldg(a.token_seq + token) : token;
         uint64_t phys;
         uint32_t tile, slot;
         if (!kv4_locate(a.cache, seq, position, &phys, &tile, &slot)) {
-            if (part == 0) kv4_flag(a.status, B2_ATTN_STATUS_BAD_BLOCK);
+            if (c == 0u && head == 0u) kv4_flag(a.status, B2_ATTN_STATUS_BAD_BLOCK);
             continue;
         }
-        const uint8_t* half_tile = a.cache.pages + kv4_tile_offset(a.cache, phys, head, tile) +
-                                   is_v * kv4_half_bytes(D);
-        const uint32_t c = part * 8u;
-        const uint32_t codes = *reinterpret_cast<const uint32_t*>(half_tile + (c / 32u) * 256u + slot * 16u + (c % 32u) / 2u);
-        const __half2 pair = reinterpret_cast<const __half2*>(half_tile + 8u * D)[slot * (D / 64u) + c / kKv4Group];
-        const float scale = __low2float(pair), base = __high2float(pair);
-        float out[8];
+        const uint8_t* tile_base = a.cache.pages + kv4_tile_offset(a.cache, phys, head, tile);
+        uint32_t codes[2], pair[2];
 #pragma unroll
-        for (int e = 0; e < 8; ++e) {
-            // scale * code is exact (11 + 4 bits), so one rounding in all
-            out[e] = fmaf(scale, static_cast<float>((codes >> (4 * e)) & 15u), base);
+        for (uint32_t v = 0; v < 2u; ++v) {
+            const uint8_t* half_tile = tile_base + v * kv4_half_bytes(D);
+            codes[v] = *reinterpret_cast<const uint16_t*>(half_tile + (c / 32u) * 256u + slot * 16u + (c % 32u) / 2u);
+            pair[v] = reinterpret_cast<const uint32_t*>(half_tile + 8u * D)[slot * (D / 64u) + c / kKv4Group];
         }
-        float4* dst = reinterpret_cast<float4*>((is_v ? a.v_out : a.k_out) + (token * a.cache.kv_heads + head) * D + c);
-        dst[0] = make_float4(out[0], out[1], out[2], out[3]);
-        dst[1] = make_float4(out[4], out[5], out[6], out[7]);
+#pragma unroll
+        for (uint32_t v = 0; v < 2u; ++v) {
+            const float scale = low_half(pair[v]), base = high_half(pair[v]);
+            // scale * code is exact (11 + 4 bits), so one rounding in all
+            auto value = [&](int e) { return fmaf(scale, static_cast<float>((codes[v] >> (4 * e)) & 15u), base); };
+            *reinterpret_cast<float4*>((v == 0u ? a.k_out : a.v_out) + i * D + c) = make_float4(value(0), value(1), value(2), value(3));
+        }
     }
 }
 
@@ -279,9 +241,10 @@ __global__ void __launch_bounds__(256) kv4_read_kernel(const Kv4ReadArgs a) {
 int32_t launch_kv4_append(const DeviceContext& ctx, const Kv4AppendArgs& a, cudaStream_t stream) {
     const uint32_t heads = a.q_heads + 2u * a.cache.kv_heads;
     const uint32_t sms = ctx.sm_count > 0 ? static_cast<uint32_t>(ctx.sm_count) : 148u;
-    // Few tokens: a warp per head, spread over CTAs (each repeats the token's angles). Many: one CTA per
-    // run of tokens, so that theta^(-2c/d) is worked out once for the run.
-    uint32_t slices = (heads + kAppendWarps - 1u) / kAppendWarps;
+    const uint32_t vectors = kAppendWarps * 256u / a.cache.head_width;   // a CTA's at once
+    // Few tokens: all vectors at once, spread over CTAs (each repeats the token's angles). Many: one CTA per run of
+    // tokens, so that theta^(-2c/d) is worked out once for the run.
+    uint32_t slices = (heads + vectors - 1u) / vectors;
     const uint64_t wanted = 8ull * sms;
     while (slices > 1u && static_cast<uint64_t>(a.n_tokens) * slices > wanted) slices = (slices + 1u) / 2u;
     uint32_t per_cta = 1u;
@@ -299,10 +262,10 @@ int32_t launch_kv4_append(const DeviceContext& ctx, const Kv4AppendArgs& a, cuda
 }
 
 int32_t launch_kv4_read(const DeviceContext& ctx, const Kv4ReadArgs& a, cudaStream_t stream) {
-    const uint64_t items = static_cast<uint64_t>(a.n_tokens) * a.cache.kv_heads * 2u * (a.cache.head_width / 8u);
     const uint64_t sms = ctx.sm_count > 0 ? static_cast<uint64_t>(ctx.sm_count) : 148u;
-    uint64_t blocks = (items + 255u) / 256u;
-    if (blocks > sms * 16u) blocks = sms * 16u;
+    const uint64_t at_once = 1024u / a.cache.head_width;
+    uint64_t blocks = (static_cast<uint64_t>(a.n_tokens) * a.cache.kv_heads + at_once - 1u) / at_once;
+    if (blocks > sms * 32u) blocks = sms * 32u;
     switch (a.cache.head_width) {
     case 64: kv4_read_kernel<64><<<static_cast<unsigned>(blocks), 256, 0, stream>>>(a); break;
     case 128: kv4_read_kernel<128><<<static_cast<unsigned>(blocks), 256, 0, stream>>>(a); break;

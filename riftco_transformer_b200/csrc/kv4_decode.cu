@@ -107,8 +107,10 @@ __device__ __forceinline__ float first_part(float x) { return __uint_as_float(__
 // the card, a CTA takes one whole list and there is nothing to join.
 constexpr uint32_t kMaxRows = 1024;   // rows a CTA finds its range among
 constexpr uint32_t kMinPairs = 8;     // pairs of a range: below two a warp a CTA is mostly set-up
-constexpr uint32_t kMostPairs = 64;   // pairs (were all rows of full length) from which there are more ranges than the
-                                      // card holds at once: the last ones of an SM then overlap less time with too few warps
+// Pairs of a range (were all rows of full length) from which there are more ranges than the card holds at once. More
+// ranges shorten the time in which an SM's last warps run alone, and cost set-up: 64 sequences of 512 to 8192 tokens take
+// 119, 107, 104, 103 and 106 us with at most 32, 64, 96, 160 and any number of pairs, others are fastest from 160 on.
+constexpr uint32_t kMostPairs = 160;
 struct WorkPlan {
     uint32_t ctas;
     uint32_t whole_lists;   // 1: CTA i takes list i
@@ -756,7 +758,7 @@ struct Sizes {
 };
 
 int32_t work_plan(const DeviceContext& ctx, uint64_t rows, uint32_t q_heads, uint32_t kv_heads, uint32_t d,
-                  uint32_t max_seq_len, WorkPlan* plan, Sizes* sizes) {
+                  uint32_t max_tokens, WorkPlan* plan, Sizes* sizes) {
     const uint32_t rep = q_heads / kv_heads, together = heads_together(rep);
     const uint64_t lists = rows * kv_heads * ((rep + together - 1u) / together);
     if (lists > 0x0FFFFFFFull) return fail(B2_STATUS_OVERFLOW, "paged attention batch too large");
@@ -768,7 +770,7 @@ int32_t work_plan(const DeviceContext& ctx, uint64_t rows, uint32_t q_heads, uin
     default: B2_TRY(together == 4u ? (resident_ctas<256, 4>(ctx, &resident)) : (resident_ctas<256, 8>(ctx, &resident))); break;
     }
     // a window's first tile may be cut: one tile more than the tokens alone
-    const uint64_t pairs = (static_cast<uint64_t>(max_seq_len) + kKv4Tile - 1u) / (kKv4Tile * kPair) + 1u;
+    const uint64_t pairs = (static_cast<uint64_t>(max_tokens) + kKv4Tile - 1u) / (kKv4Tile * kPair) + 1u;
     // prefix sums of the pairs are 32-bit numbers
     if (rows > kMaxRows || pairs <= kMinPairs || lists * pairs > 0xFFFFFFFFull) {
         *plan = WorkPlan{static_cast<uint32_t>(lists), 1u};
@@ -824,7 +826,10 @@ int32_t launch_kv4_decode(const DeviceContext& ctx, const Kv4AttentionArgs& a, v
                           cudaStream_t stream) {
     WorkPlan plan;
     Sizes sizes;
-    B2_TRY(work_plan(ctx, a.rows, a.q_heads, a.cache.kv_heads, a.cache.head_width, a.max_seq_len, &plan, &sizes));
+    // a window bounds what a row sees; fewer tokens never need more workspace
+    uint32_t most = a.max_seq_len;
+    if (a.rules.window != 0u && a.rules.prefix_lens == nullptr && a.rules.window < most) most = a.rules.window;
+    B2_TRY(work_plan(ctx, a.rows, a.q_heads, a.cache.kv_heads, a.cache.head_width, most, &plan, &sizes));
     const size_t need = plan_bytes(plan, sizes);
     if (need > workspace_bytes) {
         return fail(B2_STATUS_INVALID_ARGUMENT, "paged attention workspace too small: need %zu bytes, got %zu", need,
