@@ -4,17 +4,19 @@
 // For one row of head h, over the cached tokens t it sees:
 //   s_t = q . k_t / sqrt(d)      cap:  s = cap * tanh(s / cap)      bias:  s -= slope_h * |position - t|
 //   ctx = sum_t softmax(s)_t v_t
-// A code leaves its packed word as the fp16 number a = code - 8: one AND-OR makes 1024 + code (or 1024 +
-// 16 code of the next nibble) of two codes at once, one fp16 add (or multiply-add) takes the 1032 off, both
-// exact; nine instructions for eight codes. With value = base + scale * code = (base + 8 scale) + scale * a,
-// in groups of 64 channels, both products become products with numbers that a tensor core takes exactly:
-//   q . k_t     = sum_g scale_tg (sum_{c in g} q_c a_tc) + (base_tg + 8 scale_tg) (sum_{c in g} q_c)
-//   sum_t p_t v = sum_t (p_t scale_tg) a_tc + sum_t p_t (base_tg + 8 scale_tg)
-// so no value is ever rounded to 16 bits. Cheaper forms of a lose accuracy, because the tensor core cuts its
-// sums off instead of rounding them: fp16 subnormals (an AND alone, five instructions for eight) are aligned
-// to the nominal exponent and drop ten bits of the accumulator, 4e-5 off; 1 + code / 64 (seven) has an offset
-// whose cut-off part adds up over the tokens, 1.5e-4 off at 2049 tokens of zero mean. Centred, the
-// sums stay small and so does what is cut off. The other operand is an FP32 number (q, or p * scale) split into two fp16 parts,
+// A code leaves its packed word as the fp16 number a = code - o (o = 8, for values 8 and 7 in turn): one AND-OR makes
+// 1024 + code (or 1024 + 16 code of the next nibble) of two codes at once, one fp16 add (or multiply-add) takes the
+// offset off, both exact; nine instructions for eight codes. With value = base + scale * code =
+// (base + o scale) + scale * a, in groups of 64 channels, both products become products with numbers that a tensor core
+// takes exactly:
+//   q . k_t     = sum_g scale_tg (sum_{c in g} q_c a_tc) + (base_tg + o scale_tg) (sum_{c in g} q_c)
+//   sum_t p_t v = sum_t (p_t scale_tg) a_tc + sum_t p_t (base_tg + o scale_tg)
+// so no value is ever rounded to 16 bits. Simpler forms of a lose accuracy, because the tensor core cuts its sums off
+// instead of rounding them: fp16 subnormals (an AND alone, five instructions for eight) are aligned to the nominal
+// exponent and drop ten bits of the accumulator, 4e-5 off; 1 + code / 64 (seven) has an offset whose cut-off part adds
+// up over the tokens, 1.5e-4 off at 2049 tokens of zero mean; and code - 8 throughout leaves half a code on average
+// for values, 8.5e-6 at 29000 tokens. Centred, the sums stay small and so does what is cut off. The other operand
+// is an FP32 number (q, or p * scale) split into two fp16 parts,
 // 22 bits, that sit in adjacent columns of the eight of mma.m16n8k16 (up to four query heads: the second
 // part costs nothing) or in a second instruction (five to eight heads). Scores, softmax statistics and
 // accumulators are FP32, and the result agrees with FP32 arithmetic to about 1e-6.
@@ -83,20 +85,30 @@ __device__ __forceinline__ void lds_words(uint32_t (&v)[N], uint32_t addr) {
         }
     }
 }
-// Two codes of a word, 16 bits apart, as fp16 numbers code - 8 (exact: 1024 + 16 * 15 fits 11 bits).
-template <int NIBBLE>
+// Two codes of a word, 16 bits apart, as fp16 numbers code - LOW (the lower one) and code - HIGH, exactly: 1024 + 16 * 15
+// fits 11 bits.
+__host__ __device__ constexpr uint32_t minus_offsets(int base, int low, int high) {   // -(base + low), -(base + high) in fp16
+    // base 1024: ulp 1 at exponent 10; base 64: ulp 1/16 at exponent 6
+    return base == 1024 ? (0xE400u + low) | (0xE400u + high) << 16 : (0xD400u + 16u * low) | (0xD400u + 16u * high) << 16;
+}
+template <int NIBBLE, int LOW, int HIGH>
 __device__ __forceinline__ uint32_t codes_of(uint32_t word, uint32_t k1024) {
     if (NIBBLE >= 2) word >>= 8;
     if (NIBBLE % 2 == 0) {
-        uint32_t x = codes_1024<0x000F000Fu>(word, k1024);
-        const __half2 y = __hadd2(*reinterpret_cast<__half2*>(&x), __half2half2(__ushort_as_half(0xE408)));   // -1032
+        uint32_t x = codes_1024<0x000F000Fu>(word, k1024), off = minus_offsets(1024, LOW, HIGH);
+        const __half2 y = __hadd2(*reinterpret_cast<__half2*>(&x), *reinterpret_cast<__half2*>(&off));
         return *reinterpret_cast<const uint32_t*>(&y);
     }
-    uint32_t x = codes_1024<0x00F000F0u>(word, k1024);
+    uint32_t x = codes_1024<0x00F000F0u>(word, k1024), off = minus_offsets(64, LOW, HIGH);
     const __half2 y = __hfma2(*reinterpret_cast<__half2*>(&x), __half2half2(__ushort_as_half(0x2C00)),   // 1/16
-                              __half2half2(__ushort_as_half(0xD480)));                                    // -72
+                              *reinterpret_cast<__half2*>(&off));
     return *reinterpret_cast<const uint32_t*>(&y);
 }
+template <int NIBBLE>
+__device__ __forceinline__ uint32_t key_codes(uint32_t word, uint32_t k1024) { return codes_of<NIBBLE, 8, 8>(word, k1024); }
+// The two of a word are an even token's and the next one's: 8 and 7 in turn take their mean of 7.5 off.
+template <int NIBBLE>
+__device__ __forceinline__ uint32_t value_codes(uint32_t word, uint32_t k1024) { return codes_of<NIBBLE, 8, 7>(word, k1024); }
 // The first 11 bits of x; x minus it is exact.
 __device__ __forceinline__ float first_part(float x) { return __uint_as_float(__float_as_uint(x) & 0xFFFFE000u); }
 
@@ -385,6 +397,7 @@ kv4_decode_kernel(const Kv4AttentionArgs a, ListParts* __restrict__ list_parts, 
     float weight_factor = 0.0f;  // kWTop / scale_top
 
     const uint32_t k1024 = opaque_1024();
+    const float value_offset = (g & 1u) ? 7.0f : 8.0f;   // of tokens g and g + 8
     // This lane's part of a weight: the first 11 bits (even columns) or the rest (odd ones) of w, as
     // w * part_of + ((w & first 11 bits) ^ part_sign).
     const float part_of = (g & 1u) ? 1.0f : 0.0f;
@@ -433,10 +446,10 @@ kv4_decode_kernel(const Kv4AttentionArgs a, ListParts* __restrict__ list_parts, 
                 for (int j = 0; j < 2; ++j)
 #pragma unroll
                     for (int u = 0; u < 2; ++u) {
-                        const uint32_t a0 = u == 0 ? codes_of<0>(r[2 * j], k1024) : codes_of<2>(r[2 * j], k1024);
-                        const uint32_t a1 = u == 0 ? codes_of<0>(r[2 * j + 1], k1024) : codes_of<2>(r[2 * j + 1], k1024);
-                        const uint32_t a2 = u == 0 ? codes_of<1>(r[2 * j], k1024) : codes_of<3>(r[2 * j], k1024);
-                        const uint32_t a3 = u == 0 ? codes_of<1>(r[2 * j + 1], k1024) : codes_of<3>(r[2 * j + 1], k1024);
+                        const uint32_t a0 = u == 0 ? key_codes<0>(r[2 * j], k1024) : key_codes<2>(r[2 * j], k1024);
+                        const uint32_t a1 = u == 0 ? key_codes<0>(r[2 * j + 1], k1024) : key_codes<2>(r[2 * j + 1], k1024);
+                        const uint32_t a2 = u == 0 ? key_codes<1>(r[2 * j], k1024) : key_codes<3>(r[2 * j], k1024);
+                        const uint32_t a3 = u == 0 ? key_codes<1>(r[2 * j + 1], k1024) : key_codes<3>(r[2 * j + 1], k1024);
 #pragma unroll
                         for (int part = 0; part < HL; ++part) {
                             mma16816(c, a0, a1, a2, a3, qf[2 * gr + j][u][0][part], qf[2 * gr + j][u][1][part]);
@@ -549,7 +562,7 @@ kv4_decode_kernel(const Kv4AttentionArgs a, ListParts* __restrict__ list_parts, 
         for (int k = 0; k < 2 * kPair; ++k)
 #pragma unroll
             for (int gr = 0; gr < G; ++gr) {
-                const float b = fmaf(8.0f, low_half(vq[k][gr]), high_half(vq[k][gr]));
+                const float b = fmaf(value_offset, low_half(vq[k][gr]), high_half(vq[k][gr]));
 #pragma unroll
                 for (int h = 0; h < HL; ++h) base_acc[h][gr] = fmaf(p[k][h], b, base_acc[h][gr]);
             }
@@ -604,10 +617,10 @@ kv4_decode_kernel(const Kv4AttentionArgs a, ListParts* __restrict__ list_parts, 
 #pragma unroll
                     for (int u = 0; u < 2; ++u) {
                         // rows g and g + 8 are channels 4g + 2u and 4g + 2u + 1 of the chunk
-                        const uint32_t a0 = u == 0 ? codes_of<0>(r[2 * j], k1024) : codes_of<2>(r[2 * j], k1024);
-                        const uint32_t a1 = u == 0 ? codes_of<1>(r[2 * j], k1024) : codes_of<3>(r[2 * j], k1024);
-                        const uint32_t a2 = u == 0 ? codes_of<0>(r[2 * j + 1], k1024) : codes_of<2>(r[2 * j + 1], k1024);
-                        const uint32_t a3 = u == 0 ? codes_of<1>(r[2 * j + 1], k1024) : codes_of<3>(r[2 * j + 1], k1024);
+                        const uint32_t a0 = u == 0 ? value_codes<0>(r[2 * j], k1024) : value_codes<2>(r[2 * j], k1024);
+                        const uint32_t a1 = u == 0 ? value_codes<1>(r[2 * j], k1024) : value_codes<3>(r[2 * j], k1024);
+                        const uint32_t a2 = u == 0 ? value_codes<0>(r[2 * j + 1], k1024) : value_codes<2>(r[2 * j + 1], k1024);
+                        const uint32_t a3 = u == 0 ? value_codes<1>(r[2 * j + 1], k1024) : value_codes<3>(r[2 * j + 1], k1024);
 #pragma unroll
                         for (int part = 0; part < HL; ++part) {
                             mma16816(acc[2 * gr + j][u], a0, a1, a2, a3, b[0][part], b[1][part]);
