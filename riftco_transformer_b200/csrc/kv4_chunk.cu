@@ -72,6 +72,7 @@ struct Barriers {
 
 struct ChunkPlan {
     uint32_t row_tiles;         // CTAs of 256 rows a sequence may need
+    uint32_t paired;            // 1: at most 128 rows, whose blocks the two row tiles take in turn
     uint32_t splits;            // most splits of the blocks of one of them
     uint32_t blocks_per_split;
 };
@@ -325,16 +326,17 @@ __device__ __forceinline__ void tmem_ld_ready(uint32_t* x) {
 }
 __device__ __forceinline__ void tmem_ld_32(uint32_t taddr, uint32_t* x) { tmem_ld_32x32(taddr, *reinterpret_cast<uint32_t(*)[32]>(x)); }
 
-// cap * tanh(x * f) for 64 values. Up to |y| = 0.7, where capped scores mostly are, y times a polynomial in y^2
-// (least-squares fit of tanh y / y, weighted to even out its largest error: 5e-8); beyond, 1 - 2 / (1 + e^2y). On the
-// exponential unit alone a capped block would take three times as long as its matrix products.
+// cap * tanh(x * f) for 64 values. Up to |y| = 0.6, where capped scores mostly are, y times a polynomial in y^2
+// (least-squares fit of tanh y with weights that even out its largest error: 6e-7, for a cap of 50 a thirtieth of what
+// rounding the keys to fp16 moves a score); beyond, 1 - 2 / (1 + e^2y). On the exponential unit alone a capped block
+// would take three times as long as its matrix products.
 __device__ __forceinline__ void cap_scores(uint32_t (&x)[64], float f, float cap) {
     float most = 0.0f;
 #pragma unroll
     for (int e = 0; e < 64; e += 2) {
         most = fmaxf(most, fmaxf(fabsf(__uint_as_float(x[e])), fabsf(__uint_as_float(x[e + 1]))));
     }
-    if (__any_sync(0xFFFFFFFFu, !(most * f <= 0.7f))) {
+    if (__any_sync(0xFFFFFFFFu, !(most * f <= 0.6f))) {
 #pragma unroll
         for (int e = 0; e < 64; ++e) {
             const float y = ex2(__uint_as_float(x[e]) * (f * (2.0f * kLog2e)));
@@ -342,17 +344,17 @@ __device__ __forceinline__ void cap_scores(uint32_t (&x)[64], float f, float cap
         }
         return;
     }
-    const uint64_t f2 = two(f, f), cap2 = two(cap, cap);
-    const float c[6] = {1.0f, -0.3333314061164856f, 0.13328571617603302f, -0.053534939885139465f,
-                        0.020045235753059387f, -0.005105267278850079f};
+    const uint64_t f2 = two(f, f);
+    const float c[4] = {0.9999909996986389f * cap, -0.33298975229263306f * cap, 0.1297455132007599f * cap,
+                        -0.03961123898625374f * cap};
 #pragma unroll
     for (int e = 0; e < 64; e += 2) {
         const uint64_t y = mul2(two(__uint_as_float(x[e]), __uint_as_float(x[e + 1])), f2), z = mul2(y, y);
-        uint64_t r = two(c[5], c[5]);
+        uint64_t r = two(c[3], c[3]);
 #pragma unroll
-        for (int k = 4; k >= 0; --k) r = fma2(r, z, two(c[k], c[k]));
+        for (int k = 2; k >= 0; --k) r = fma2(r, z, two(c[k], c[k]));
         float lo, hi;
-        parts(mul2(mul2(r, y), cap2), lo, hi);
+        parts(mul2(r, y), lo, hi);
         x[e] = __float_as_uint(lo);
         x[e + 1] = __float_as_uint(hi);
     }
@@ -388,7 +390,12 @@ kv4_chunk_kernel(const Kv4AttentionArgs a, float* __restrict__ partials, const C
     const uint32_t n_blocks = min(plan.blocks_per_split, blocks - block0);   // 0 where nothing is seen
     const uint32_t first_tile = tile0 + block0 * kBlockTiles;
     const uint32_t end_tile = min(tile0 + tiles, first_tile + n_blocks * kBlockTiles);
-    const uint32_t n_tiles = rows > 128u ? 2u : 1u;   // row tiles with a live row
+    // Row tiles at work. Paired, both hold the same rows, tile i of them blocks i, i + 2, ..., as two partial results:
+    // a tile's chain of products and softmax is twice as long as its share of either unit, and with one tile nothing else
+    // would run beside it.
+    const bool paired = plan.paired != 0u;
+    const uint32_t n_tiles = paired || rows > 128u ? 2u : 1u, step = paired ? 2u : 1u;
+    const uint32_t parts_per_split = step;
 
     const uint32_t smem32 = (smem_u32(smem_raw) + 1023u) & ~1023u;
     const uint32_t q32 = smem32, k32 = q32 + L::kQ, v32 = k32 + kStages * L::kKStage, raw32 = v32 + kStages * L::kVStage;
@@ -405,8 +412,8 @@ kv4_chunk_kernel(const Kv4AttentionArgs a, float* __restrict__ partials, const C
             for (uint32_t i = 0; i < kStages; ++i) {
                 mbar_init(&bars.k_full[i], kExpandWarps);
                 mbar_init(&bars.v_full[i], kExpandWarps);
-                mbar_init(&bars.k_empty[i], n_tiles);
-                mbar_init(&bars.v_empty[i], n_tiles);
+                mbar_init(&bars.k_empty[i], paired ? 1u : n_tiles);
+                mbar_init(&bars.v_empty[i], paired ? 1u : n_tiles);
             }
             for (uint32_t i = 0; i < 2u; ++i) {
                 for (uint32_t b = 0; b < 2u; ++b) {
@@ -457,7 +464,7 @@ kv4_chunk_kernel(const Kv4AttentionArgs a, float* __restrict__ partials, const C
                 __syncwarp();
             }
         } else if (warp - kIssueWarp < n_tiles) {
-            // ---- tcgen05 issue: round jb makes a tile's scores of block jb, then its P V of block jb - 1 ----
+            // ---- tcgen05 issue: round n makes the scores of a tile's n-th block, then P V of the one before ----
             // One warp for each tile: an issued MMA is hardly queued, so that what one warp spends on its barriers (75
             // cycles a wait) would leave the tensor core idle, were it not for the other's MMAs. Tensor memory starts at
             // column 0, this CTA holds all of it.
@@ -469,27 +476,29 @@ kv4_chunk_kernel(const Kv4AttentionArgs a, float* __restrict__ partials, const C
             mbar_wait(&bars.q_full[i], 0u, abort);
             const uint64_t dq = umma_desc_k_major_sw128(q32 + i * (128u * D * 2u));
             const uint64_t dk = umma_desc_k_major_sw128(k32), dv = umma_desc_k_major_sw128(v32);
-            for (uint32_t jb = 0; jb <= n_blocks && n_blocks != 0u; ++jb) {
-                if (jb < n_blocks) {
-                    const uint32_t stage = jb % kStages;
+            const uint32_t first_block = paired ? i : 0u;
+            const uint32_t mine = n_blocks > first_block ? (n_blocks - first_block + step - 1u) / step : 0u;   // its blocks
+            for (uint32_t n = 0; n <= mine && mine != 0u; ++n) {
+                if (n < mine) {
+                    const uint32_t jb = first_block + n * step, stage = jb % kStages;
                     mbar_wait(&bars.k_full[stage], (jb / kStages) & 1u, abort);
                     tcgen05_fence_after_sync();
                     const uint64_t kb = dk + (stage * L::kKStage >> 4);
-                    const uint32_t d = i * kTmemTile + (jb & 1u) * kBlock;   // its P was read by P V of block jb - 2
+                    const uint32_t d = i * kTmemTile + (n & 1u) * kBlock;   // its P was read by P V two of its blocks ago
                     if (elect_one()) {
 #pragma unroll
                         for (uint32_t kk = 0; kk < D / 16u; ++kk) {
                             umma_ss(d, dq + (kk / 4u) * (16384u >> 4) + (kk % 4u) * 2u,
                                     kb + (kk / 4u) * (kBlock * 128u >> 4) + (kk % 4u) * 2u, idesc_f16(kBlock), kk != 0u ? 1u : 0u);
                         }
-                        umma_commit(&bars.s_full[i][jb & 1u]);
+                        umma_commit(&bars.s_full[i][n & 1u]);
                         umma_commit(&bars.k_empty[stage]);
                     }
                     __syncwarp();
                 }
-                if (jb > 0u) {
-                    const uint32_t before = jb - 1u, stage = before % kStages;
-                    mbar_wait(&bars.v_full[stage], (before / kStages) & 1u, abort);
+                if (n > 0u) {
+                    const uint32_t before = n - 1u, jb = first_block + before * step, stage = jb % kStages;
+                    mbar_wait(&bars.v_full[stage], (jb / kStages) & 1u, abort);
                     mbar_wait(&bars.p_full[i][before & 1u], (before / 2u) & 1u, abort);
                     tcgen05_fence_after_sync();
                     const uint64_t b = dv + (stage * L::kVStage >> 4);
@@ -499,7 +508,7 @@ kv4_chunk_kernel(const Kv4AttentionArgs a, float* __restrict__ partials, const C
                         for (uint32_t kk = 0; kk < kBlock / 16u; ++kk) {
                             umma_ts(i * kTmemTile + kTmemO, w + kk * 8u, b + kk * 2u, idesc_f16(D), kk != 0u ? 1u : before);
                         }
-                        umma_commit(jb == n_blocks ? &bars.o_full[i] : &bars.o_done[i]);
+                        umma_commit(n == mine ? &bars.o_full[i] : &bars.o_done[i]);
                         umma_commit(&bars.v_empty[stage]);
                     }
                     __syncwarp();
@@ -536,7 +545,8 @@ kv4_chunk_kernel(const Kv4AttentionArgs a, float* __restrict__ partials, const C
         // ---- softmax: a thread is a row ----
         registers_up<kSoftmaxRegisters>();
         const uint32_t i = warp / 4u;
-        const uint32_t r = i * 128u + (warp % 4u) * 32u + lane, gr = row0 + r;
+        const uint32_t tile_rows = paired ? 0u : i * 128u;   // rows before the tile's
+        const uint32_t r = tile_rows + (warp % 4u) * 32u + lane, gr = row0 + r;
         const bool live = r < rows;
         const uint32_t lane_base = i * kTmemTile + (((warp % 4u) * 32u) << 16);
         const int64_t position64 = span.position0 + gr / rep;
@@ -556,7 +566,7 @@ kv4_chunk_kernel(const Kv4AttentionArgs a, float* __restrict__ partials, const C
         // its own 32 rows, kChannels8 lanes a row, with all loads of eight steps before their first use.
         const float to_unit = (capped ? 1.0f / a.rules.softcap : kLog2e) / sqrtf(static_cast<float>(D));
         constexpr uint32_t kRowsAtOnce = 32u / kChannels8, kSteps = 32u / kRowsAtOnce;
-        const uint32_t warp_row = i * 128u + (warp % 4u) * 32u, c8 = lane % kChannels8;
+        const uint32_t warp_row = tile_rows + (warp % 4u) * 32u, c8 = lane % kChannels8;
         const uint32_t my_out = static_cast<uint32_t>(gr / rep), my_head = gr % rep;
         float row_factor = 0.0f;
 #pragma unroll 1
@@ -603,10 +613,12 @@ kv4_chunk_kernel(const Kv4AttentionArgs a, float* __restrict__ partials, const C
         if (lane == 0) mbar_arrive(&bars.q_full[i]);
         float m = kNoMax, l = 0.0f;
 
-        for (uint32_t jb = 0; jb < n_blocks; ++jb) {
-            const uint32_t token0 = (first_tile + jb * kBlockTiles) * kKv4Tile;
-            const uint32_t buffer = lane_base + (jb & 1u) * kBlock;
-            mbar_wait(&bars.s_full[i][jb & 1u], (jb / 2u) & 1u, abort);
+        const uint32_t first_block = paired ? i : 0u;
+        const uint32_t mine = n_blocks > first_block ? (n_blocks - first_block + step - 1u) / step : 0u;   // the tile's blocks
+        for (uint32_t n = 0; n < mine; ++n) {
+            const uint32_t token0 = (first_tile + (first_block + n * step) * kBlockTiles) * kKv4Tile;
+            const uint32_t buffer = lane_base + (n & 1u) * kBlock;
+            mbar_wait(&bars.s_full[i][n & 1u], (n / 2u) & 1u, abort);
             tcgen05_fence_after_sync();
             const bool masked = token0 < all_begin || token0 + kBlock > all_end;   // the same for the whole warp
             uint32_t x[64];
@@ -666,8 +678,8 @@ kv4_chunk_kernel(const Kv4AttentionArgs a, float* __restrict__ partials, const C
                 const float shrink = ex2(m - moved);
                 m = moved;
                 l *= shrink;
-                if (jb > 0u) {
-                    mbar_wait(&bars.o_done[i], (jb - 1u) & 1u, abort);   // P V of the block before: O is at rest
+                if (n > 0u) {
+                    mbar_wait(&bars.o_done[i], (n - 1u) & 1u, abort);   // P V of the block before: O is at rest
                     tcgen05_fence_after_sync();
 #pragma unroll 1
                     for (uint32_t c = 0; c < D / 32u; ++c) {
@@ -685,12 +697,12 @@ kv4_chunk_kernel(const Kv4AttentionArgs a, float* __restrict__ partials, const C
             tmem_st_wait();
             tcgen05_fence_before_sync();
             __syncwarp();
-            if (lane == 0) mbar_arrive(&bars.p_full[i][jb & 1u]);
+            if (lane == 0) mbar_arrive(&bars.p_full[i][n & 1u]);
         }
 
         // ---- epilogue ----
         if (live && isnan(l)) flags |= B2_ATTN_STATUS_NAN_OR_POS_INF;
-        if (n_blocks != 0u) {
+        if (mine != 0u) {
             mbar_wait(&bars.o_full[i], 0u, abort);
             tcgen05_fence_after_sync();
         } else {
@@ -698,9 +710,9 @@ kv4_chunk_kernel(const Kv4AttentionArgs a, float* __restrict__ partials, const C
         }
         if (lane == 0 && *abort != 0) flags |= B2_ATTN_STATUS_TIMEOUT;
         const uint64_t out_head = static_cast<uint64_t>(span.first + my_out) * a.q_heads + kvh * rep + my_head;
-        const bool whole = n_splits == 1u;
+        const bool whole = n_splits * parts_per_split == 1u;
         if (whole && live && l == 0.0f && end > begin) flags |= B2_ATTN_STATUS_ALL_NEG_INF;
-        float* part = partials + (out_head * plan.splits + split) * (D + 4u);
+        float* part = partials + ((out_head * plan.splits + split) * parts_per_split + (paired ? i : 0u)) * (D + 4u);
         if (!whole && live) *reinterpret_cast<float2*>(part) = make_float2(m, l);
         const float inv = whole ? (l == 0.0f ? 0.0f : 1.0f / l) : 1.0f;
         // The tile's Q is not needed any more: its 2 D bytes a row take the warp's bf16 rows, so that they leave in whole
@@ -709,7 +721,7 @@ kv4_chunk_kernel(const Kv4AttentionArgs a, float* __restrict__ partials, const C
 #pragma unroll 1
         for (uint32_t c = 0; c < D / 32u; ++c) {
             uint32_t o[32];
-            if (n_blocks != 0u) {
+            if (mine != 0u) {
                 tmem_ld_32(lane_base + kTmemO + c * 32u, o);
                 tmem_ld_ready(o);
             }
@@ -739,10 +751,10 @@ kv4_chunk_kernel(const Kv4AttentionArgs a, float* __restrict__ partials, const C
             __syncwarp();
 #pragma unroll 4
             for (uint32_t n = 0; n < kSteps; ++n) {
-                const uint32_t mine = n * kRowsAtOnce + lane / kChannels8;
-                const uint64_t head = __shfl_sync(0xFFFFFFFFu, out_head, mine);
-                const uint4 v = lds128(stage32 + mine * (D * 2u) + ((c8 ^ (mine & 7u)) << 4));
-                if (warp_row + mine < rows) {
+                const uint32_t which = n * kRowsAtOnce + lane / kChannels8;
+                const uint64_t head = __shfl_sync(0xFFFFFFFFu, out_head, which);
+                const uint4 v = lds128(stage32 + which * (D * 2u) + ((c8 ^ (which & 7u)) << 4));
+                if (warp_row + which < rows) {
                     reinterpret_cast<uint4*>(static_cast<__nv_bfloat16*>(a.ctx16) + head * D)[c8] = v;
                 }
             }
@@ -764,35 +776,53 @@ kv4_chunk_merge_kernel(const Kv4AttentionArgs a, const float* __restrict__ parti
     const uint32_t head = static_cast<uint32_t>(out_head % a.q_heads) % rep;
     const RowSpan mine = row_span(a, row);   // inputs of the call, not of the kernel before
     uint32_t n_splits = 0;
+    bool ours = false;
     if (mine.owned) {
         const uint32_t first = min(__ldg(a.chunk_starts + mine.seq), a.rows);
         const TileSpan span = tile_span(a, mine.seq, rep, ((row - first) * rep + head) / kRows * kRows);
-        if ((row - first) < span.tokens) {
+        ours = row - first < span.tokens;
+        if (ours) {
             const uint32_t tile0 = span.begin / kKv4Tile;
             const uint32_t tiles = span.end > span.begin ? (span.end - 1u) / kKv4Tile + 1u - tile0 : 0u;
             n_splits = ((tiles + kBlockTiles - 1u) / kBlockTiles + plan.blocks_per_split - 1u) / plan.blocks_per_split;
         }
     }
     pdl_wait();   // every CTA waits, so that this grid never ends before the one it follows
-    if (n_splits <= 1u) return;
-    const float* first = partials + out_head * plan.splits * (D + 4u);
+    const uint32_t each = plan.paired != 0u ? 2u : 1u, n = max(n_splits, 1u) * each;   // where nothing is seen one split says so
+    if (!ours || n <= 1u) return;
+    const float* first = partials + out_head * plan.splits * each * (D + 4u);
     const uint32_t c = threadIdx.x * 4u;
-    finish<D>(a, join_run(first, first + (D + 4u), D + 4u, n_splits, c), out_head, c, mine.end > mine.begin);
+    finish<D>(a, join_run(first, first + (D + 4u), D + 4u, n, c), out_head, c, mine.end > mine.begin);
 }
 
-// One CTA holds an SM. Where the row tiles leave SMs idle, the blocks of each are split over several CTAs, down to
-// eight blocks, below which a CTA's own set-up costs as much as its blocks.
-ChunkPlan chunk_plan(int sm_count, uint32_t n_seq, uint32_t q_heads, uint32_t kv_heads, uint32_t max_chunk, uint32_t max_seq_len) {
+// One CTA holds an SM. Where the row tiles are fewer than the SMs, the blocks of each are split over as many CTAs as
+// make the waves shortest: a CTA's set-up and epilogue take about as long as six blocks, joining as four. With more row
+// tiles the longer ones start first and the shorter ones fill in; splitting those too made four chunks of 300 to 700
+// tokens, 192 CTAs, slower (132 against 166 us: the FP32 partial results of so many rows).
+ChunkPlan chunk_plan(int sm_count, uint32_t n_seq, uint32_t q_heads, uint32_t kv_heads, uint32_t max_chunk, uint32_t max_tokens) {
     const uint64_t rep = q_heads / kv_heads;
     const uint64_t sms = sm_count > 0 ? static_cast<uint64_t>(sm_count) : 148u;
     const uint64_t row_tiles = (max_chunk * rep + kRows - 1u) / kRows;
-    const uint64_t blocks = (static_cast<uint64_t>(max_seq_len) + kBlock - 1u) / kBlock + 1u;   // a window may start inside a tile
+    const uint64_t blocks = (static_cast<uint64_t>(max_tokens) + kBlock - 1u) / kBlock + 1u;   // a window may start inside a tile
     const uint64_t ctas = row_tiles * n_seq * kv_heads;
-    uint64_t per = blocks;
-    if (ctas < sms) per = (blocks * ctas + sms - 1u) / sms;
-    if (per < 8u) per = 8u;
-    return ChunkPlan{static_cast<uint32_t>(row_tiles), static_cast<uint32_t>((blocks + per - 1u) / per), static_cast<uint32_t>(per)};
+    uint64_t best = 1;
+    if (ctas < sms) {
+        uint64_t shortest = UINT64_MAX;
+        for (uint64_t splits = 1; splits <= 64u && (splits == 1u || blocks >= 4u * splits); ++splits) {
+            const uint64_t waves = (ctas * splits + sms - 1u) / sms;
+            const uint64_t time = waves * ((blocks + splits - 1u) / splits + 6u) + (splits > 1u ? 4u : 0u);
+            if (time < shortest) {
+                shortest = time;
+                best = splits;
+            }
+        }
+    }
+    const uint64_t per = (blocks + best - 1u) / best;
+    return ChunkPlan{static_cast<uint32_t>(row_tiles), max_chunk * rep <= 128u ? 1u : 0u,
+                     static_cast<uint32_t>((blocks + per - 1u) / per), static_cast<uint32_t>(per)};
 }
+// Partial results of a row: of a split one, or where its tiles are paired two.
+uint32_t parts_of(const ChunkPlan& plan) { return plan.splits * (plan.paired != 0u ? 2u : 1u); }
 
 template <int D>
 int32_t launch_one(const DeviceContext& ctx, const Kv4AttentionArgs& a, float* partials, const ChunkPlan& plan,
@@ -807,7 +837,7 @@ int32_t launch_one(const DeviceContext& ctx, const Kv4AttentionArgs& a, float* p
     if (ctas > 0x7FFFFFFFull || merges > 0x7FFFFFFFull) return fail(B2_STATUS_OVERFLOW, "paged attention batch too large");
     kv4_chunk_kernel<D><<<static_cast<unsigned>(ctas), kThreads, Layout<D>::kTotal, stream>>>(a, partials, plan);
     B2_CUDA_TRY(cudaGetLastError());
-    if (plan.splits <= 1u) return B2_STATUS_OK;
+    if (parts_of(plan) <= 1u) return B2_STATUS_OK;
     cudaLaunchConfig_t config{};
     config.gridDim = dim3(static_cast<unsigned>(merges));
     config.blockDim = dim3(D / 4);
@@ -831,8 +861,8 @@ bool kv4_chunk_supported(uint32_t head_width, uint32_t q_heads, uint32_t kv_head
 size_t kv4_chunk_workspace_bytes(int sm_count, uint32_t n_seq, uint64_t rows, uint32_t q_heads, uint32_t kv_heads,
                                  uint32_t head_width, uint32_t max_chunk, uint32_t max_seq_len) {
     const ChunkPlan plan = chunk_plan(sm_count, n_seq, q_heads, kv_heads, max_chunk, max_seq_len);
-    if (plan.splits <= 1u) return 0;
-    return static_cast<size_t>(rows) * q_heads * plan.splits * (head_width + 4u) * sizeof(float);
+    if (parts_of(plan) <= 1u) return 0;
+    return static_cast<size_t>(rows) * q_heads * parts_of(plan) * (head_width + 4u) * sizeof(float);
 }
 
 int32_t launch_kv4_chunk(const DeviceContext& ctx, const Kv4AttentionArgs& a, void* workspace, size_t workspace_bytes,
