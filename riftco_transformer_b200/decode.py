@@ -1,6 +1,7 @@
 """One decode step of a Llama-shaped decoder assembled from the hot-path
 operators: packed-NF4 linears, RMSNorm, split-half RoPE + KV-page append, paged
-grouped-query attention, SwiGLU, greedy argmax.
+grouped-query attention, SwiGLU, greedy argmax. The K/V pages are FP32
+(``PagedKvPool``, as in the reference) or 4-bit (``PagedKv4Pool``).
 
 The reference has no incremental decode for its Llama/Mistral model
 (include/riftco_transformer/model/llama_mistral_transformer.hpp:77-79); the
@@ -31,6 +32,7 @@ import torch
 from . import _lib
 from ._lib import lib
 from .backend import PackedNf4Weight, PagedKvPool, _check, _stream_ptr
+from .kv4 import PagedKv4Pool, paged_decode_attention_kv4, paged_decode_kv4_workspace_bytes, rope_append_kv4
 
 
 @dataclass
@@ -172,8 +174,12 @@ class CudaOps:
                                    _stream_ptr(None)))
         self.launches += 1
 
-    def rope_append(self, q, k, v, positions, tables, pool: PagedKvPool, theta: float, status) -> None:
+    def rope_append(self, q, k, v, positions, tables, pool: PagedKvPool | PagedKv4Pool, theta: float, status) -> None:
         n_seq, q_heads, d = q.shape
+        if isinstance(pool, PagedKv4Pool):
+            rope_append_kv4(q, k, v, positions, pool, tables, theta, status=status)
+            self.launches += 1
+            return
         _check(lib.b2_rope_append_kv(q.data_ptr(), k.data_ptr(), v.data_ptr(), positions.data_ptr(),
                                      tables.data_ptr(), pool.key_pages.data_ptr(), pool.value_pages.data_ptr(),
                                      n_seq, q_heads, k.shape[1], d, pool.block_size, pool.physical_blocks,
@@ -182,9 +188,15 @@ class CudaOps:
 
     attention_writes_bf16 = True   # `attention` takes `ctx16`: a bf16 copy of the context for the o-projection
 
-    def attention(self, q, pool: PagedKvPool, tables, seq_lens, ctx, max_seq_len: int, status, workspace,
-                  ctx16=None) -> None:
+    def attention(self, q, pool: PagedKvPool | PagedKv4Pool, tables, seq_lens, ctx, max_seq_len: int, status,
+                  workspace, ctx16=None) -> None:
         n_seq, q_heads, d = q.shape
+        if isinstance(pool, PagedKv4Pool):
+            paged_decode_attention_kv4(q, pool, tables, seq_lens, ctx, max_seq_len, status=status, workspace=workspace,
+                                       context_bf16=None if ctx16 is None else ctx16.view(n_seq, q_heads, d))
+            joins = paged_decode_kv4_workspace_bytes(n_seq, q_heads, pool.kv_heads, d, max_seq_len) > 0
+            self.launches += 2 if joins else 1
+            return
         ws = None if workspace is None else workspace.data_ptr()
         ws_bytes = 0 if workspace is None else workspace.numel() * workspace.element_size()
         if ctx16 is None:
@@ -203,6 +215,10 @@ class CudaOps:
 
     def attention_workspace(self, n_seq, q_heads, d, block_size, max_seq_len):
         need = lib.b2_paged_decode_workspace_bytes(n_seq, q_heads, d, block_size, max_seq_len)
+        return torch.empty(max(need, 16), dtype=torch.uint8, device=self.device)
+
+    def attention_workspace_kv4(self, n_seq, q_heads, kv_heads, d, max_seq_len):
+        need = paged_decode_kv4_workspace_bytes(n_seq, q_heads, kv_heads, d, max_seq_len)
         return torch.empty(max(need, 16), dtype=torch.uint8, device=self.device)
 
     def silu_mul(self, gate, up, out, out16=None) -> None:
@@ -294,7 +310,10 @@ class DecodeStep:
         self.next_tokens = e((B,), dtype=torch.int32)
         self.status = ops.empty((1,), dtype=torch.int32)
         self.status.zero_()   # sticky error bits of the attention / append / gather kernels
-        self.workspace = ops.attention_workspace(B, self.hq, hd, cfg.block_size, max_seq_len)
+        if isinstance(pools[0], PagedKv4Pool):
+            self.workspace = ops.attention_workspace_kv4(B, self.hq, self.hkv, hd, max_seq_len)
+        else:
+            self.workspace = ops.attention_workspace(B, self.hq, hd, cfg.block_size, max_seq_len)
         if world > 1:
             widths = {cfg.q_heads * hd // world, d // world, cfg.ffn // world, cfg.vocab // world}
             self.stage = {n_: e((world, B, n_)) for n_ in widths}
@@ -408,7 +427,8 @@ WHOLE_ON_EVERY_RANK = ("wo", "w_down")   # see DecodeStep: replicated rather tha
 
 
 def synthetic_step(cfg: DecoderConfig, batch: int, context: int, rank: int = 0, world: int = 1, device="cuda",
-                   group=None, seed: int = 1234, whole=None, quantized: bool = True) -> tuple[DecodeStep, dict]:
+                   group=None, seed: int = 1234, whole=None, quantized: bool = True,
+                   kv4: bool = False) -> tuple[DecodeStep, dict]:
     """A DecodeStep over a seeded synthetic model for benchmarking and cross-checks.
 
     Every rank builds the SAME global model from the seed - weights ~ N(0, 0.02^2) quantised to NF4
@@ -421,7 +441,8 @@ def synthetic_step(cfg: DecoderConfig, batch: int, context: int, rank: int = 0, 
     of FP32 partial sums inside the linears.
 
     `whole`: names of the layer weights every rank keeps whole (default: WHOLE_ON_EVERY_RANK when
-    world > 1). `quantized=False` draws the payloads directly in the packed domain (cheaper)."""
+    world > 1). `quantized=False` draws the payloads directly in the packed domain (cheaper).
+    `kv4=True` keeps the K/V pages in 4 bits: the same draws as keys and values, appended at their positions."""
     from . import synth
     cfg.shard_check(world)
     if whole is None:
@@ -457,7 +478,23 @@ def synthetic_step(cfg: DecoderConfig, batch: int, context: int, rank: int = 0, 
     tokens = torch.randint(0, cfg.vocab, (batch,), device=device, generator=g, dtype=torch.int32)
     pools = []
     hkv = cfg.kv_heads // world
+    filled = torch.arange(context, device=device)
     for layer in range(cfg.layers):
+        if kv4:
+            pool = PagedKv4Pool.empty(total, hkv, cfg.block_size, cfg.head_dim, device)
+            pool.pages.zero_()   # the spare slots
+            for s in range(batch if context else 0):
+                drawn = []
+                for which in range(2):   # K, V
+                    rows = torch.empty((context, hkv, cfg.head_dim), device=device)
+                    for j in range(hkv):
+                        g.manual_seed(seed + 104729 * (layer + 1) + 31 * (rank * hkv + j) + which + 7919 * s)
+                        rows[:, j] = torch.randn((context, cfg.head_dim), device=device, generator=g)
+                    drawn.append(rows)
+                rope_append_kv4(drawn[0][:, :1].contiguous(), drawn[0], drawn[1], filled.to(torch.int32), pool, tables,
+                                cfg.theta, token_seq=torch.full((context,), s, dtype=torch.int32, device=device))
+            pools.append(pool)
+            continue
         pages = []
         for which in range(2):   # K, V
             pool = torch.empty((total, hkv, cfg.block_size, cfg.head_dim), device=device)
@@ -472,7 +509,8 @@ def synthetic_step(cfg: DecoderConfig, batch: int, context: int, rank: int = 0, 
         "tokens": tokens,
         "positions": torch.full((batch,), context, dtype=torch.int32, device=device),
         "seq_lens": torch.full((batch,), context + 1, dtype=torch.int32, device=device),
-        "kv_bytes_per_step": cfg.layers * batch * (context + 1) * hkv * cfg.head_dim * 4 * 2,
+        "kv_bytes_per_step": cfg.layers * batch * (context + 1) * (
+            pools[0].bytes_per_token() if kv4 else hkv * cfg.head_dim * 4 * 2),
         "lens": lens,
     }
     return step, inputs

@@ -327,6 +327,23 @@ def test_decode_of_query_and_value_magnitudes_beyond_fp16():
     assert status == 0 and rel_l2(got, case.decode()) <= F32_TOL
 
 
+@pytest.mark.parametrize("hq", [4, 12])
+def test_decode_of_long_sums_that_cancel(hq):
+    """Values of zero mean over 30000 tokens: the context is 1/170 of what it is summed from, so that whatever the tensor
+    core cuts off its partial sums instead of rounding would show. The weights' own errors, 2^-22 * sum |q k| / sqrt(d) of
+    random sign, stay relative to the context: 2 * 10^-6 for sums of 10."""
+    rng = np.random.default_rng(hq)
+    case = kv4_cases.Case(hq, [30000], hq, 1, 128, 16)
+    table = case.tables[0]
+    k, _ = kv4_cases.unpack(case.pages[table], 128)
+    v = rng.standard_normal(k.shape).astype(np.float32)
+    case.pages[table] = kv4_cases.pack(np.nan_to_num(k), v)
+    k, v = kv4_cases.unpack(case.pages[table], 128)
+    case.k, case.v = ([a.transpose(1, 0, 2, 3).reshape(1, -1, 128)[:, :30000]] for a in (k, v))
+    got, status = decode(case)
+    assert status == 0 and rel_l2(got, case.decode()) <= 4e-6
+
+
 def test_decode_values_whose_scale_varies_by_orders_of_magnitude():
     rng = np.random.default_rng(14)
     case = kv4_cases.Case(14, [640], 4, 1, 128, 16)
@@ -417,6 +434,57 @@ def test_chunk_score_rules(rules, new, past):
     assert rel_l2(got, case.chunk(new, **want)) <= BF16_TOL
 
 
+@pytest.mark.parametrize("d,hq,hkv,new,route", [(128, 4, 2, [7], "attention_kv4"), (128, 4, 2, [8], "attention_kv4_tiles"),
+                                                (256, 4, 2, [40], "attention_kv4"), (64, 1, 1, [129, 64], "attention_kv4_tiles")])
+def test_chunk_routes(d, hq, hkv, new, route):
+    import riftco_transformer_b200 as b2
+    case = kv4_cases.Case(9, [m + 30 for m in new], hq, hkv, d, 16, rows=sum(new))
+    got, status = chunk(case, new)
+    assert status == 0 and b2.last_route() == route
+    assert rel_l2(got, case.chunk(new)) <= BF16_TOL
+
+
+@pytest.mark.parametrize("new,past", [([20, 3], [5000, 64]), ([300], [6000]), ([1, 1, 1], [4000, 0, 63])])
+def test_chunk_splits_long_contexts(new, past):
+    """Few rows over many tokens: several CTAs, and both row tiles of one, share a row's tokens."""
+    case = kv4_cases.Case(sum(new), [p + m for p, m in zip(past, new)], 32, 2, 128, 16, rows=sum(new), poison=0x7C)
+    got, status = chunk(case, new)
+    assert status == 0 and rel_l2(got, case.chunk(new)) <= BF16_TOL
+    again, _ = chunk(case, new)
+    assert (again == got).all()
+
+
+def test_chunk_scores_near_and_beyond_the_cap():
+    """Both forms of the tanh: scores well below the cap, and far beyond it."""
+    for strength, cap in ((1.0, 50.0), (3.0, 2.0), (20.0, 30.0)):
+        case = kv4_cases.Case(91, [260], 4, 2, 128, 16, rows=90, strength=strength)
+        got, status = chunk(case, [90], softcap=cap)
+        assert status == 0
+        # fp16 keys and queries move a score by 2 * 2^-11 * |s| at most, a capped one by no more than that of the cap
+        tol = BF16_TOL + 2 * 2.0 ** -11 * min(cap, 16.0 * strength)
+        assert rel_l2(got, case.chunk([90], softcap=cap)) <= tol
+
+
+def test_chunk_of_values_that_are_not_finite():
+    """A NaN group makes the context NaN for the rows that see its token, and for no other."""
+    from riftco_transformer_b200 import _lib
+    for half in (0, 9 * 128):   # keys, values
+        case = kv4_cases.Case(17, [150], 4, 1, 128, 16, rows=100)
+        at = 90                  # the token
+        tile = case.pages[case.tables[0, at // 16], 0, 0]
+        tile[half + 8 * 128:half + 9 * 128].reshape(16, -1)[at % 16] = 0xFF
+        got, status = chunk(case, [100])
+        assert status == _lib.ATTN_STATUS_NAN_OR_POS_INF
+        sees = np.arange(50, 150) >= at
+        assert np.isnan(got[sees]).all()
+        assert rel_l2(got[~sees], case.chunk([100])[~sees]) <= BF16_TOL
+        # rows whose window has passed the token do not see it either
+        got, status = chunk(case, [100], window=20)
+        sees = (np.arange(50, 150) >= at) & (np.arange(50, 150) < at + 20)
+        assert np.isnan(got[sees]).all()
+        assert rel_l2(got[~sees], case.chunk([100], window=20)[~sees]) <= BF16_TOL
+
+
 def test_chunk_leaves_rows_behind_the_last_sequence():
     for new in ([4, 3], [140, 60]):
         lens = [20 + m for m in new]
@@ -490,6 +558,47 @@ def test_prompt_then_tokens_against_the_fp32_cache():
         b2.paged_decode_attention(rows[0], flat, table, positions + 1, ref, max(total), status=status)
         assert rel_l2(got.cpu().numpy(), ref.cpu().numpy()) <= 2 * F32_TOL
     assert int(status.item()) == 0
+
+
+@pytest.mark.parametrize("batch,context", [(3, 300), (32, 40)])
+def test_decode_step_on_4_bit_pages(batch, context):
+    """DecodeStep takes 4-bit pools: two steps give the logits of a step on FP32 pages that hold what the 4-bit ones do,
+    the new token's keys and values included. Contexts differ by FP32 rounding; above 16 rows the linears round them
+    to bf16, where that flips one in some thousands by half a step of 2^-8: far below 5e-3 in the logits."""
+    import riftco_transformer_b200 as b2
+    from riftco_transformer_b200.decode import CudaOps, DecodeStep, DecoderConfig, synthetic_step
+    cfg = DecoderConfig(layers=2, d_model=512, q_heads=4, kv_heads=2, head_dim=128, ffn=1024, vocab=2048)
+    dev = torch.device("cuda", 0)
+    step, inputs = synthetic_step(cfg, batch, context, device=dev, kv4=True)
+    lens = inputs["seq_lens"]
+
+    class Mirror(CudaOps):
+        """Appends to a copy of the 4-bit pool and keeps FP32 pages of what it then holds."""
+
+        def rope_append(self, q, k, v, positions, tables, pool, theta, status):
+            small = self.small[id(pool)]
+            b2.rope_append_kv4(q, k, v, positions, small, tables, theta, status=status)
+            kb, vb = torch.empty_like(k), torch.empty_like(v)
+            b2.dequantize_kv4(small, tables, positions, kb, vb, status=status)
+            page = tables[torch.arange(batch, device=dev), positions.long() // cfg.block_size].long()
+            pool.key_pages[page, :, positions.long() % cfg.block_size] = kb
+            pool.value_pages[page, :, positions.long() % cfg.block_size] = vb
+
+    ops = Mirror(dev)
+    flats, ops.small = [], {}
+    for pool in step.pools:
+        k, v = (torch.from_numpy(a).to(dev) for a in kv4_cases.unpack(pool.pages.cpu().numpy(), cfg.head_dim))
+        flat = b2.PagedKvPool(k, v)
+        flats.append(flat)
+        ops.small[id(flat)] = b2.PagedKv4Pool(pool.pages.clone(), cfg.block_size, cfg.head_dim)
+    other = DecodeStep(cfg, ops, step.w, step.norms, step.embedding, flats, step.tables, batch, context + 1)
+    step.ops.launches = 0
+    got_next, got = step.step(inputs["tokens"], inputs["positions"], lens)
+    want_next, want = other.step(inputs["tokens"], inputs["positions"], lens)
+    torch.cuda.synchronize()
+    assert int(step.status.item()) == 0 and int(other.status.item()) == 0 and step.ops.launches > 0
+    assert rel_l2(got.cpu().numpy(), want.cpu().numpy()) <= 5e-3
+    assert inputs["kv_bytes_per_step"] == 2 * batch * (context + 1) * 2 * 144
 
 
 def test_captured_calls_replay_with_new_inputs():
