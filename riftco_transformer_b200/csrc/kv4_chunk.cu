@@ -121,6 +121,11 @@ template <int N>
 __device__ __forceinline__ void registers_up() { asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(N)); }
 template <int N>
 __device__ __forceinline__ void registers_down() { asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(N)); }
+// Named barriers of two warps, one that waits for its turn and one that passes it.
+__device__ __forceinline__ void turn_wait(uint32_t barrier, bool first) {
+    if (!first) asm volatile("bar.sync %0, 64;" ::"r"(barrier) : "memory");
+}
+__device__ __forceinline__ void turn_pass(uint32_t barrier) { asm volatile("bar.arrive %0, 64;" ::"r"(barrier) : "memory"); }
 __device__ __forceinline__ float rcp(float x) {
     float y;
     asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
@@ -615,6 +620,7 @@ kv4_chunk_kernel(const Kv4AttentionArgs a, float* __restrict__ partials, const C
 
         const uint32_t first_block = paired ? i : 0u;
         const uint32_t mine = n_blocks > first_block ? (n_blocks - first_block + step - 1u) / step : 0u;   // the tile's blocks
+        const uint32_t others = paired ? n_blocks - mine : n_blocks;   // the other tile's
         for (uint32_t n = 0; n < mine; ++n) {
             const uint32_t token0 = (first_tile + (first_block + n * step) * kBlockTiles) * kKv4Tile;
             const uint32_t buffer = lane_base + (n & 1u) * kBlock;
@@ -672,7 +678,11 @@ kv4_chunk_kernel(const Kv4AttentionArgs a, float* __restrict__ partials, const C
                 sum = s0 + s1;
                 top = fmaxf(fmaxf(top4[0], top4[1]), fmaxf(top4[2], top4[3])) * factor;
             };
+            // The warps of the two tiles that share a scheduler take turns with their exponentials, so that one's run under
+            // the other's loads and stores instead of both at half speed.
+            if (n_tiles == 2u) turn_wait(2u + (warp % 4u) * 2u + i, i == 0u && n == 0u);
             weigh();
+            if (n_tiles == 2u && (i == 0u ? n < others : n + 1u < others)) turn_pass(2u + (warp % 4u) * 2u + (i ^ 1u));
             if (__any_sync(0xFFFFFFFFu, top > m + kSlack)) {
                 const float moved = fmaxf(m, top);
                 const float shrink = ex2(m - moved);
