@@ -115,86 +115,105 @@ __device__ __forceinline__ void store_vector(const float4& lo, const float4& hi,
     }
 }
 
+constexpr uint32_t kMostTokens = 8;   // of a CTA
+
 // Grid (token run, slice). A CTA takes `per_cta` consecutive tokens and, of each, every gridDim.y-th group of its lanes'
 // head vectors: q heads are rotated, k heads rotated and stored, v heads stored. The angles of a token are the same for
-// all its heads: the first D/2 threads work them out once (in double: position * theta^(-2c/D) passes 10^5 radians
-// in long contexts, where FP32 has lost the phase) into shared memory. A prompt is bound by HBM (24.6 KB of q, k and
-// v in, 16.4 KB of q and 1.2 KB of pages out per token at 32 / 8 heads of 128): 16-byte accesses, and the next
-// vector's loads under way while one is worked on. A single token is bound by the latency of its angle.
+// all its heads: they are worked out once, into shared memory (in double: position * theta^(-2c/D) passes 10^5
+// radians in long contexts, where FP32 has lost the phase). A prompt is bound by HBM (24.6 KB of q, k and v in, 16.4 KB
+// of q and 1.2 KB of pages out per token at 32 / 8 heads of 128): 16-byte accesses, no barrier between the vectors of a
+// run, and the loads of the next two under way while one is worked on: 8191 tokens take 73 us (4.7 TB/s), 85 us with one
+// vector ahead and a barrier per token. A single token, 6 us, is bound by the latency of its angle.
 template <int D>
-__global__ void __launch_bounds__(kAppendWarps * 32)
+__global__ void __launch_bounds__(kAppendWarps * 32, 4)
 kv4_append_kernel(const Kv4AppendArgs a, uint32_t per_cta) {
     sm100::pdl_launch_dependents();
     constexpr uint32_t kHalf = D / 2, kLanes = D / 8, kVectors = 32u / kLanes * kAppendWarps;   // vectors of a CTA at once
-    __shared__ __align__(16) float s_cos[2][kHalf], s_sin[2][kHalf];
-    const uint32_t l = threadIdx.x % kLanes, first = blockIdx.y * kVectors + threadIdx.x / kLanes;
+    __shared__ __align__(16) float s_cos[kMostTokens][kHalf], s_sin[kMostTokens][kHalf];
+    struct Place {
+        uint64_t phys;
+        uint32_t tile, slot, good, real;   // real: not padding
+    };
+    __shared__ Place s_place[kMostTokens];
+    const uint32_t l = threadIdx.x % kLanes;
     const uint32_t mask = D == 256 ? 0xFFFFFFFFu : ((1u << (kLanes % 32u)) - 1u) << (threadIdx.x % 32u / kLanes * kLanes);
-    const uint32_t heads = a.q_heads + 2u * a.cache.kv_heads, stride = gridDim.y * kVectors;
-    double turn = 0.0;
-    if (threadIdx.x < kHalf) {
-        turn = pow(static_cast<double>(a.theta), static_cast<double>(threadIdx.x) * -2.0 / static_cast<double>(D));
-    }
+    const uint32_t heads = a.q_heads + 2u * a.cache.kv_heads;
+    const uint64_t token0 = static_cast<uint64_t>(blockIdx.x) * per_cta;
+    const uint32_t tokens = static_cast<uint32_t>(min(static_cast<uint64_t>(per_cta), a.n_tokens - token0));
+
+    // The CTA's vectors: slice blockIdx.y of every token's heads, one token behind the other.
+    const uint32_t slice_first = blockIdx.y * kVectors, slice_step = gridDim.y * kVectors;
+    const uint32_t slices = slice_first < heads ? (heads - slice_first + slice_step - 1u) / slice_step : 0u;
+    const uint32_t groups = slices * tokens;   // of kVectors vectors
     struct Vector {
         float4 lo, hi;
     };
-    auto source = [&](uint64_t token, uint32_t h) -> const float* {
-        const float* base = h < a.q_heads ? a.q : h < a.q_heads + a.cache.kv_heads ? a.k : a.v;
-        const uint32_t head = h < a.q_heads ? h : h < a.q_heads + a.cache.kv_heads ? h - a.q_heads : h - a.q_heads - a.cache.kv_heads;
-        return base + (token * (h < a.q_heads ? a.q_heads : a.cache.kv_heads) + head) * D + 4u * l;
-    };
-    auto load = [&](uint64_t token, uint32_t h) {   // q_out may be q: a lane reads both halves of its pairs before it writes
-        const float* src = source(token, h);
-        return Vector{*reinterpret_cast<const float4*>(src), *reinterpret_cast<const float4*>(src + kHalf)};
-    };
-    uint32_t buffer = 0;
-    for (uint32_t i = 0; i < per_cta; ++i) {
-        const uint64_t token = static_cast<uint64_t>(blockIdx.x) * per_cta + i;
-        if (token >= a.n_tokens) return;
-        const uint32_t position = a.positions[token];
-        if (position == kKv4Pad) continue;   // the same for every thread: no barrier is skipped by some
-        Vector next;
-        if (first < heads) next = load(token, first);
-        float* const cosines = s_cos[buffer];
-        float* const sines = s_sin[buffer];
-        buffer ^= 1u;
-        if (threadIdx.x < kHalf) {
-            double s_, c_;
-            sincos(static_cast<double>(position) * turn, &s_, &c_);
-            cosines[threadIdx.x] = static_cast<float>(c_);
-            sines[threadIdx.x] = static_cast<float>(s_);
+    auto head_of = [&](uint32_t group) { return slice_first + group % slices * slice_step + threadIdx.x / kLanes; };
+    auto load = [&](uint32_t group) {   // q_out may be q: a lane reads both halves of its pairs before it writes
+        Vector x{make_float4(0.f, 0.f, 0.f, 0.f), make_float4(0.f, 0.f, 0.f, 0.f)};
+        const uint32_t h = head_of(group);
+        if (group < groups && h < heads) {
+            const uint64_t token = token0 + group / slices;
+            const float* base = h < a.q_heads ? a.q : h < a.q_heads + a.cache.kv_heads ? a.k : a.v;
+            const uint32_t head = h < a.q_heads ? h : h < a.q_heads + a.cache.kv_heads ? h - a.q_heads : h - a.q_heads - a.cache.kv_heads;
+            const float* src = base + (token * (h < a.q_heads ? a.q_heads : a.cache.kv_heads) + head) * D + 4u * l;
+            x.lo = *reinterpret_cast<const float4*>(src);
+            x.hi = *reinterpret_cast<const float4*>(src + kHalf);
         }
-        const uint32_t seq = a.token_seq != nullptr ? a.token_seq[token] : static_cast<uint32_t>(token);
-        uint64_t phys;
-        uint32_t tile, slot;
-        const bool good = kv4_locate(a.cache, seq, position, &phys, &tile, &slot);
-        if (!good && threadIdx.x == 0 && blockIdx.y == 0) kv4_flag(a.status, B2_ATTN_STATUS_BAD_BLOCK);
-        // One barrier a token: a buffer is written again two barriers after its readers' own.
-        __syncthreads();
-        const float4 cs = *reinterpret_cast<const float4*>(cosines + 4u * l), sn = *reinterpret_cast<const float4*>(sines + 4u * l);
-        for (uint32_t h = first; h < heads; h += stride) {
-            Vector x = next;
-            if (h + stride < heads) next = load(token, h + stride);
-            const bool is_q = h < a.q_heads, is_k = !is_q && h < a.q_heads + a.cache.kv_heads;
-            if (is_q || is_k) {
-                auto turned = [](float p, float q, float c, float s, float* lo, float* hi) {
-                    *lo = __fsub_rn(__fmul_rn(p, c), __fmul_rn(q, s));
-                    *hi = __fadd_rn(__fmul_rn(q, c), __fmul_rn(p, s));
-                };
-                const Vector y = x;
-                turned(y.lo.x, y.hi.x, cs.x, sn.x, &x.lo.x, &x.hi.x);
-                turned(y.lo.y, y.hi.y, cs.y, sn.y, &x.lo.y, &x.hi.y);
-                turned(y.lo.z, y.hi.z, cs.z, sn.z, &x.lo.z, &x.hi.z);
-                turned(y.lo.w, y.hi.w, cs.w, sn.w, &x.lo.w, &x.hi.w);
-            }
-            if (is_q) {
-                float* dst = a.q_out + (token * a.q_heads + h) * D + 4u * l;
-                *reinterpret_cast<float4*>(dst) = x.lo;
-                *reinterpret_cast<float4*>(dst + kHalf) = x.hi;
-            } else if (good) {
-                const uint32_t head = is_k ? h - a.q_heads : h - a.q_heads - a.cache.kv_heads;
-                uint8_t* half_tile = a.cache.pages + kv4_tile_offset(a.cache, phys, head, tile) + (is_k ? 0u : kv4_half_bytes(D));
-                store_vector<D>(x.lo, x.hi, half_tile, slot, l, mask);
-            }
+        return x;
+    };
+    Vector ahead[2] = {load(0), load(1)};
+
+    {
+        const uint32_t c = threadIdx.x % kHalf;
+        const double turn = pow(static_cast<double>(a.theta), static_cast<double>(c) * -2.0 / static_cast<double>(D));
+        for (uint32_t i = threadIdx.x / kHalf; i < tokens; i += kAppendWarps * 32u / kHalf) {
+            double s_, c_;
+            sincos(static_cast<double>(a.positions[token0 + i]) * turn, &s_, &c_);
+            s_cos[i][c] = static_cast<float>(c_);
+            s_sin[i][c] = static_cast<float>(s_);
+        }
+    }
+    if (threadIdx.x < tokens) {
+        const uint64_t token = token0 + threadIdx.x;
+        const uint32_t position = a.positions[token], seq = a.token_seq != nullptr ? a.token_seq[token] : static_cast<uint32_t>(token);
+        Place p{0, 0, 0, 0, position != kKv4Pad};
+        if (p.real != 0u) {
+            p.good = kv4_locate(a.cache, seq, position, &p.phys, &p.tile, &p.slot) ? 1u : 0u;
+            if (p.good == 0u && blockIdx.y == 0) kv4_flag(a.status, B2_ATTN_STATUS_BAD_BLOCK);
+        }
+        s_place[threadIdx.x] = p;
+    }
+    __syncthreads();
+
+#pragma unroll 2
+    for (uint32_t group = 0; group < groups; ++group) {
+        Vector x = ahead[group % 2u];
+        ahead[group % 2u] = load(group + 2u);
+        const uint32_t h = head_of(group), i = group / slices;
+        const Place place = s_place[i];
+        if (h >= heads || place.real == 0u) continue;   // the same for all lanes of a vector
+        const bool is_q = h < a.q_heads, is_k = !is_q && h < a.q_heads + a.cache.kv_heads;
+        if (is_q || is_k) {
+            const float4 cs = *reinterpret_cast<const float4*>(&s_cos[i][4u * l]), sn = *reinterpret_cast<const float4*>(&s_sin[i][4u * l]);
+            auto turned = [](float p, float q, float c, float s, float* lo, float* hi) {
+                *lo = __fsub_rn(__fmul_rn(p, c), __fmul_rn(q, s));
+                *hi = __fadd_rn(__fmul_rn(q, c), __fmul_rn(p, s));
+            };
+            const Vector y = x;
+            turned(y.lo.x, y.hi.x, cs.x, sn.x, &x.lo.x, &x.hi.x);
+            turned(y.lo.y, y.hi.y, cs.y, sn.y, &x.lo.y, &x.hi.y);
+            turned(y.lo.z, y.hi.z, cs.z, sn.z, &x.lo.z, &x.hi.z);
+            turned(y.lo.w, y.hi.w, cs.w, sn.w, &x.lo.w, &x.hi.w);
+        }
+        if (is_q) {
+            float* dst = a.q_out + ((token0 + i) * a.q_heads + h) * D + 4u * l;
+            *reinterpret_cast<float4*>(dst) = x.lo;
+            *reinterpret_cast<float4*>(dst + kHalf) = x.hi;
+        } else if (place.good != 0u) {
+            const uint32_t head = is_k ? h - a.q_heads : h - a.q_heads - a.cache.kv_heads;
+            uint8_t* half_tile = a.cache.pages + kv4_tile_offset(a.cache, place.phys, head, place.tile) + (is_k ? 0u : kv4_half_bytes(D));
+            store_vector<D>(x.lo, x.hi, half_tile, place.slot, l, mask);
         }
     }
 }
@@ -249,7 +268,7 @@ int32_t launch_kv4_append(const DeviceContext& ctx, const Kv4AppendArgs& a, cuda
     while (slices > 1u && static_cast<uint64_t>(a.n_tokens) * slices > wanted) slices = (slices + 1u) / 2u;
     uint32_t per_cta = 1u;
     if (slices == 1u) per_cta = static_cast<uint32_t>((a.n_tokens + wanted - 1u) / wanted);
-    if (per_cta > 8u) per_cta = 8u;
+    if (per_cta > kMostTokens) per_cta = kMostTokens;
     const dim3 grid((a.n_tokens + per_cta - 1u) / per_cta, slices);
     const unsigned threads = kAppendWarps * 32;
     switch (a.cache.head_width) {
