@@ -85,6 +85,22 @@ __device__ __forceinline__ void lds_words(uint32_t (&v)[N], uint32_t addr) {
         }
     }
 }
+// c = kOffset + a * b in integers, c read as FP32 being kMagic + a * b; or c += a * b.
+constexpr uint32_t kMagicBits = 0x4B400000u;   // 1.5 * 2^23: sums below 2^22 in magnitude keep the exponent
+constexpr float kMagic = 12582912.0f;
+template <bool FIRST>
+__device__ __forceinline__ void mma16832(uint32_t (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3,
+                                         uint32_t b0, uint32_t b1) {
+    if constexpr (FIRST) {
+        asm("mma.sync.aligned.m16n8k32.row.col.s32.u8.s8.s32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%10,%10,%10};"
+            : "=r"(c[0]), "=r"(c[1]), "=r"(c[2]), "=r"(c[3])
+            : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1), "r"(kMagicBits));
+    } else {
+        asm("mma.sync.aligned.m16n8k32.row.col.s32.u8.s8.s32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+            : "+r"(c[0]), "+r"(c[1]), "+r"(c[2]), "+r"(c[3])
+            : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+    }
+}
 // Two codes of a word, 16 bits apart, as fp16 numbers code - LOW (the lower one) and code - HIGH, exactly: 1024 + 16 * 15
 // fits 11 bits.
 __host__ __device__ constexpr uint32_t minus_offsets(int base, int low, int high) {   // -(base + low), -(base + high) in fp16
@@ -104,8 +120,6 @@ __device__ __forceinline__ uint32_t codes_of(uint32_t word, uint32_t k1024) {
                               *reinterpret_cast<__half2*>(&off));
     return *reinterpret_cast<const uint32_t*>(&y);
 }
-template <int NIBBLE>
-__device__ __forceinline__ uint32_t key_codes(uint32_t word, uint32_t k1024) { return codes_of<NIBBLE, 8, 8>(word, k1024); }
 // The two of a word are an even token's and the next one's: 8 and 7 in turn take their mean of 7.5 off.
 template <int NIBBLE>
 __device__ __forceinline__ uint32_t value_codes(uint32_t word, uint32_t k1024) { return codes_of<NIBBLE, 8, 7>(word, k1024); }
@@ -298,14 +312,15 @@ kv4_decode_kernel(const Kv4AttentionArgs a, ListParts* __restrict__ list_parts, 
     };
     for (uint32_t i = 0; i < kSlots && i < my_pairs; ++i) issue(i);
 
-    // ---- q: scaled by a power of two, split into two fp16 parts, in the order the codes come out ----
-    // Column n of the products is head n/2, part n%2 (HC = 4), or head n with the parts in two
-    // instructions (HC = 8). A chunk of 32 channels takes two k16 steps; in step u the lane's four k
-    // positions are channels 8t + 2u, 8t + 2u + 4, then 8t + 2u + 1, 8t + 2u + 5.
+    // ---- q: rounded to 23 bits of its head's largest, split into three signed bytes, in the order the codes come out ----
+    // HC = 4: columns 2h and 2h + 1 of the first product are the two upper bytes of head h, column 2h of the second the
+    // lowest; HC = 8: a product for each byte, column n is head n. Of a chunk of 32 channels the lane's k positions are
+    // channels 8t + 0, 2, 4, 6 (low nibbles), then 8t + 1, 3, 5, 7.
     const uint32_t col_head = HC == 4 ? g >> 1 : g;
     const bool col_live = col_head < live_heads;
     const float* qp = a.q + (static_cast<uint64_t>(row) * a.q_heads + first_head + (col_live ? col_head : 0u)) * D;
-    uint32_t qf[kChunks][2][2][HL];   // [chunk][step][register][part, HC = 8]
+    constexpr int kProducts = HC == 4 ? 2 : 3;
+    uint32_t qf[kChunks][2][kProducts];   // [chunk][register][product]
     float q_unscale;                  // of column head
     float q_sum[G];
     {
@@ -325,11 +340,12 @@ kv4_decode_kernel(const Kv4AttentionArgs a, ListParts* __restrict__ list_parts, 
         }
         top = fmaxf(top, __shfl_xor_sync(0xFFFFFFFFu, top, 1));
         top = fmaxf(top, __shfl_xor_sync(0xFFFFFFFFu, top, 2));
-        // 2^e with top * 2^e in [2^13, 2^14); a head of zeros or beyond 2^113 keeps a bounded factor
-        int e = 13 - (static_cast<int>((__float_as_uint(top) >> 23) & 255u) - 127);
-        e = max(-100, min(100, e));
+        // 2^e with top * 2^e in [2^21, 2^22); a head of zeros keeps a bounded factor
+        int e = 21 - (static_cast<int>((__float_as_uint(top) >> 23) & 255u) - 127);
+        e = min(100, e);
         const float up = __uint_as_float(static_cast<uint32_t>(e + 127) << 23);
-        q_unscale = __uint_as_float(static_cast<uint32_t>(127 - e) << 23);
+        // (an infinite q has no integers; a NaN one makes q_sum, and with it every score, NaN)
+        q_unscale = top < INFINITY ? __uint_as_float(static_cast<uint32_t>(127 - e) << 23) : __uint_as_float(0x7FC00000u);
 #pragma unroll
         for (int gr = 0; gr < G; ++gr) {
             float s = 0.0f;
@@ -341,22 +357,29 @@ kv4_decode_kernel(const Kv4AttentionArgs a, ListParts* __restrict__ list_parts, 
             s += __shfl_xor_sync(0xFFFFFFFFu, s, 2);
             q_sum[gr] = s;
         }
-        const bool second = HC == 4 && (g & 1u) != 0u;
+        const bool odd = HC == 4 && (g & 1u) != 0u;
 #pragma unroll
         for (int j = 0; j < kChunks; ++j)
 #pragma unroll
-            for (int u = 0; u < 2; ++u)
+            for (int w = 0; w < 2; ++w) {
+                uint32_t bytes[3] = {0u, 0u, 0u};   // lowest first, of the four channels
 #pragma unroll
-                for (int w = 0; w < 2; ++w) {
-                    const float v0 = x[j][2 * u + w] * up, v1 = x[j][2 * u + w + 4] * up;
-                    const float h0 = first_part(v0), h1 = first_part(v1);
-                    if (HC == 4) {
-                        qf[j][u][w][0] = second ? pack_half(v0 - h0, v1 - h1) : pack_half(h0, h1);
-                    } else {
-                        qf[j][u][w][0] = pack_half(h0, h1);
-                        qf[j][u][w][HL - 1] = pack_half(v0 - h0, v1 - h1);
-                    }
+                for (int b = 0; b < 4; ++b) {
+                    const int n = __float2int_rn(x[j][2 * b + w] * up);   // n = d2 2^16 + d1 2^8 + d0, -128 <= d0, d1 < 128
+                    const int n1 = (n + 128) >> 8, n2 = (n1 + 128) >> 8;
+                    bytes[0] |= (static_cast<uint32_t>(n) & 255u) << (8 * b);
+                    bytes[1] |= (static_cast<uint32_t>(n1) & 255u) << (8 * b);
+                    bytes[2] |= (static_cast<uint32_t>(n2) & 255u) << (8 * b);
                 }
+                if (HC == 4) {
+                    qf[j][w][0] = odd ? bytes[1] : bytes[2];
+                    qf[j][w][1] = odd ? 0u : bytes[0];
+                } else {
+                    qf[j][w][0] = bytes[2];
+                    qf[j][w][1] = bytes[1];
+                    qf[j][w][kProducts - 1] = bytes[0];
+                }
+            }
     }
     // Score layout: a lane holds tokens g and g + 8 of heads t (HC = 4) or 2t, 2t + 1 (HC = 8).
     const float inv_sqrt = 1.0f / sqrtf(static_cast<float>(D));
@@ -430,49 +453,49 @@ kv4_decode_kernel(const Kv4AttentionArgs a, ListParts* __restrict__ list_parts, 
 #pragma unroll
         for (int w = 0; w < kPair; ++w) {
             const uint32_t k32 = slot32 + w * kTileBytes;
-            float total[4] = {0.0f, 0.0f, 0.0f, 0.0f};
             uint32_t kp0[G], kp1[G];
             lds_words<G>(kp0, k32 + 8u * D + g * (4u * G));
             lds_words<G>(kp1, k32 + 8u * D + (g + 8u) * (4u * G));
-            float base0[HL], base1[HL];
+            float total0[HL], total1[HL], base0[HL], base1[HL];
 #pragma unroll
-            for (int h = 0; h < HL; ++h) base0[h] = base1[h] = 0.0f;
+            for (int h = 0; h < HL; ++h) total0[h] = total1[h] = base0[h] = base1[h] = 0.0f;
 #pragma unroll
             for (int gr = 0; gr < G; ++gr) {
                 uint32_t r[4];   // chunk 2gr: tokens g, g + 8; chunk 2gr + 1: the same
                 ldsm4(r, k32 + gr * 512u + lane * 16u);
-                float c[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+                uint32_t c[kProducts][4];
 #pragma unroll
-                for (int j = 0; j < 2; ++j)
+                for (int j = 0; j < 2; ++j) {
+                    const uint32_t a0 = r[2 * j] & 0x0F0F0F0Fu, a1 = r[2 * j + 1] & 0x0F0F0F0Fu;
+                    const uint32_t a2 = (r[2 * j] >> 4) & 0x0F0F0F0Fu, a3 = (r[2 * j + 1] >> 4) & 0x0F0F0F0Fu;
 #pragma unroll
-                    for (int u = 0; u < 2; ++u) {
-                        const uint32_t a0 = u == 0 ? key_codes<0>(r[2 * j], k1024) : key_codes<2>(r[2 * j], k1024);
-                        const uint32_t a1 = u == 0 ? key_codes<0>(r[2 * j + 1], k1024) : key_codes<2>(r[2 * j + 1], k1024);
-                        const uint32_t a2 = u == 0 ? key_codes<1>(r[2 * j], k1024) : key_codes<3>(r[2 * j], k1024);
-                        const uint32_t a3 = u == 0 ? key_codes<1>(r[2 * j + 1], k1024) : key_codes<3>(r[2 * j + 1], k1024);
-#pragma unroll
-                        for (int part = 0; part < HL; ++part) {
-                            mma16816(c, a0, a1, a2, a3, qf[2 * gr + j][u][0][part], qf[2 * gr + j][u][1][part]);
+                    for (int n = 0; n < kProducts; ++n) {
+                        if (j == 0) {
+                            mma16832<true>(c[n], a0, a1, a2, a3, qf[2 * gr][0][n], qf[2 * gr][1][n]);
+                        } else {
+                            mma16832<false>(c[n], a0, a1, a2, a3, qf[2 * gr + 1][0][n], qf[2 * gr + 1][1][n]);
                         }
                     }
-                const float s0 = low_half(kp0[gr]), s1 = low_half(kp1[gr]);
-                const float k_base0 = fmaf(8.0f, s0, high_half(kp0[gr]));
-                const float k_base1 = fmaf(8.0f, s1, high_half(kp1[gr]));
-                total[0] = fmaf(s0, c[0], total[0]);
-                total[1] = fmaf(s0, c[1], total[1]);
-                total[2] = fmaf(s1, c[2], total[2]);
-                total[3] = fmaf(s1, c[3], total[3]);
+                }
 #pragma unroll
                 for (int h = 0; h < HL; ++h) {
-                    base0[h] = fmaf(k_base0, base_factor[h][gr], base0[h]);
-                    base1[h] = fmaf(k_base1, base_factor[h][gr], base1[h]);
+                    // the three bytes' sums joined; only the last two additions round, to 2^-24 of the largest possible sum
+                    auto joined = [&](uint32_t high, uint32_t mid, uint32_t low) {
+                        const float y = fmaf(__uint_as_float(high), 65536.0f, -kMagic * 65793.0f);   // 2^16 + 2^8 + 1
+                        return fmaf(__uint_as_float(mid), 256.0f, y) + __uint_as_float(low);
+                    };
+                    const float y0 = HC == 4 ? joined(c[0][0], c[0][1], c[1][0]) : joined(c[0][h], c[1][h], c[kProducts - 1][h]);
+                    const float y1 = HC == 4 ? joined(c[0][2], c[0][3], c[1][2]) : joined(c[0][2 + h], c[1][2 + h], c[kProducts - 1][2 + h]);
+                    total0[h] = fmaf(low_half(kp0[gr]), y0, total0[h]);
+                    total1[h] = fmaf(low_half(kp1[gr]), y1, total1[h]);
+                    base0[h] = fmaf(high_half(kp0[gr]), base_factor[h][gr], base0[h]);
+                    base1[h] = fmaf(high_half(kp1[gr]), base_factor[h][gr], base1[h]);
                 }
             }
 #pragma unroll
             for (int h = 0; h < HL; ++h) {
-                // HC = 4: columns 2t, 2t + 1 are the two parts of head t; HC = 8: two heads
-                s[2 * w][h] = fmaf(HC == 4 ? total[0] + total[1] : total[h], code_factor[h], base0[h]);
-                s[2 * w + 1][h] = fmaf(HC == 4 ? total[2] + total[3] : total[2 + h], code_factor[h], base1[h]);
+                s[2 * w][h] = fmaf(total0[h], code_factor[h], base0[h]);
+                s[2 * w + 1][h] = fmaf(total1[h], code_factor[h], base1[h]);
             }
         }
         if (capped) {
