@@ -4,26 +4,33 @@
 // For one row of head h, over the cached tokens t it sees:
 //   s_t = q . k_t / sqrt(d)      cap:  s = cap * tanh(s / cap)      bias:  s -= slope_h * |position - t|
 //   ctx = sum_t softmax(s)_t v_t
-// A code leaves its packed word as the fp16 number a = code - o (o = 8, for values 8 and 7 in turn): one AND-OR makes
-// 1024 + code (or 1024 + 16 code of the next nibble) of two codes at once, one fp16 add (or multiply-add) takes the
-// offset off, both exact; nine instructions for eight codes. With value = base + scale * code =
-// (base + o scale) + scale * a, in groups of 64 channels, both products become products with numbers that a tensor core
-// takes exactly:
-//   q . k_t     = sum_g scale_tg (sum_{c in g} q_c a_tc) + (base_tg + o scale_tg) (sum_{c in g} q_c)
-//   sum_t p_t v = sum_t (p_t scale_tg) a_tc + sum_t p_t (base_tg + o scale_tg)
-// so no value is ever rounded to 16 bits. Simpler forms of a lose accuracy, because the tensor core cuts its sums off
+// With value = base + scale * code in groups of 64 channels,
+//   q . k_t     = sum_g scale_tg (sum_{c in g} q_c code_tc) + base_tg (sum_{c in g} q_c)
+//   sum_t p_t v = sum_t (p_t scale_tg) a_tc + sum_t p_t (base_tg + o scale_tg),   a = code - o
+// both sums over codes are matrix products with numbers that the tensor core takes exactly, and no value is ever rounded
+// to 16 bits.
+//
+// Keys: codes become bytes with one AND (of the word, and of the word shifted by a nibble: three instructions for eight
+// codes) and meet q in integers, mma.m16n8k32. q is rounded to 23 bits of its head's largest and split into three signed
+// bytes, whose sums (exact, below 2^17) are joined in FP32: 41 instructions a tile less than the form that values have.
+//
+// Values cannot do so: the sums of three bytes would need three accumulators for each channel and head, and registers
+// hold two. Their codes become fp16 numbers a = code - o (o = 8 and 7 in turn): one AND-OR makes 1024 + code (or
+// 1024 + 16 code of the next nibble) of two codes at once, one fp16 add (or multiply-add) takes the offset off, both
+// exact; nine instructions for eight codes. Simpler forms of a lose accuracy, because the tensor core cuts its sums off
 // instead of rounding them: fp16 subnormals (an AND alone, five instructions for eight) are aligned to the nominal
 // exponent and drop ten bits of the accumulator, 4e-5 off; 1 + code / 64 (seven) has an offset whose cut-off part adds
-// up over the tokens, 1.5e-4 off at 2049 tokens of zero mean; and code - 8 throughout leaves half a code on average
-// for values, 8.5e-6 at 29000 tokens. Centred, the sums stay small and so does what is cut off. The other operand
-// is an FP32 number (q, or p * scale) split into two fp16 parts,
-// 22 bits, that sit in adjacent columns of the eight of mma.m16n8k16 (up to four query heads: the second
-// part costs nothing) or in a second instruction (five to eight heads). Scores, softmax statistics and
+// up over the tokens, 1.5e-4 off at 2049 tokens of zero mean; and code - 8 throughout leaves half a code on average,
+// 8.5e-6 at 29000 tokens. Centred, the sums stay small and so does what is cut off. The other operand, p * scale, is
+// split into two fp16 parts, 22 bits, that sit in adjacent columns of the eight of mma.m16n8k16 (up to four query heads:
+// the second part costs nothing) or in a second instruction (five to eight heads). Scores, softmax statistics and
 // accumulators are FP32, and the result agrees with FP32 arithmetic to about 1e-6.
 //
-// Bound by HBM: 9d/8 bytes per token and K/V head against 8d of the FP32 cache. mma.sync rather than
-// tcgen05: a row tile has at most 8 live rows, M = 64 or 128 would be idle lanes, and the operands come
-// from registers without a trip through shared or tensor memory.
+// HBM is the floor: 9d/8 bytes per token and K/V head against 8d of the FP32 cache. What bounds it is instructions: 335
+// for 16 tokens of a K/V head at d = 128, issued in 59% of the cycles (16 warps an SM, each a chain of its own; 20 warps
+// spill). One sequence of 131071 tokens at 32 / 8 heads takes 43 us (3.5 TB/s), the loads alone 30 us. mma.sync rather
+// than tcgen05: a row tile has at most 8 live rows, M = 64 or 128 would be idle lanes, and the operands come from
+// registers without a trip through shared or tensor memory.
 #include "kv4.cuh"
 #include "sm100_ptx.cuh"
 
