@@ -35,7 +35,9 @@ namespace {
 
 using namespace sm100;
 
-constexpr uint32_t kRows = 256, kBlock = 64;   // rows of a CTA, tokens of a block
+constexpr uint32_t kBlock = 64;   // tokens of a block
+// Rows of a CTA: two tiles of 128; one where heads of 256 fill tensor memory with its O.
+__host__ __device__ constexpr uint32_t rows_of(uint32_t d) { return d == 256u ? 128u : 256u; }
 constexpr uint32_t kBlockTiles = kBlock / kKv4Tile;
 constexpr uint32_t kExpandWarps = 4;   // for keys and for values each
 constexpr uint32_t kKeyWarp = 8, kValueWarp = 12, kLoadWarp = 16, kIssueWarp = 17;   // and 18
@@ -45,13 +47,17 @@ constexpr uint32_t kThreads = 20 * 32;
 constexpr int kSoftmaxRegisters = 136, kExpandRegisters = 80, kOtherRegisters = 48;
 static_assert(256 * kSoftmaxRegisters + 256 * kExpandRegisters + 128 * kOtherRegisters <= 640 * 96, "more than the launch holds");
 constexpr uint32_t kRawSlots = 3;
-constexpr uint32_t kStages = 4;   // of expanded keys and of values
+__host__ __device__ constexpr uint32_t stages_of(int d) { return d == 256 ? 2u : 4u; }   // of expanded keys and of values
+constexpr uint32_t kMostStages = 4;
 constexpr uint32_t kTmemColumns = 512, kTmemTile = 256, kTmemO = 128;   // a tile's two S (and P) of 64 columns, its O
+constexpr uint32_t kTmemQ = 384;   // heads of 256: Q, for which shared memory has no room, beside the one tile's O
 constexpr float kSlack = 8.0f;
 
 template <int D>
 struct Layout {
-    static constexpr uint32_t kQ = kRows * D * 2, kKStage = kBlock * D * 2, kVStage = kBlock * D * 2;
+    static constexpr bool kQInTmem = D == 256;
+    static constexpr uint32_t kRows = rows_of(D), kStages = stages_of(D);
+    static constexpr uint32_t kQ = kQInTmem ? 0u : kRows * D * 2, kKStage = kBlock * D * 2, kVStage = kBlock * D * 2;
     // 16 bytes apart, so that the same word of four tiles lies in different banks
     static constexpr uint32_t kRawTile = kv4_tile_bytes(D) + 16u;
     static constexpr uint32_t kRawSlot = kBlockTiles * kRawTile;
@@ -60,7 +66,7 @@ struct Layout {
 
 struct Barriers {
     uint64_t raw_full[kRawSlots], raw_empty[kRawSlots];
-    uint64_t k_full[kStages], k_empty[kStages], v_full[kStages], v_empty[kStages];
+    uint64_t k_full[kMostStages], k_empty[kMostStages], v_full[kMostStages], v_empty[kMostStages];
     uint64_t s_full[2][2], p_full[2][2];   // [tile][buffer]
     // P V of a block and of the last one. Whoever waits for o_done knows that the one before has completed (the
     // scores it has seen were issued after it), so that a parity tells; at the end only two before that is known.
@@ -71,13 +77,13 @@ struct Barriers {
 };
 
 struct ChunkPlan {
-    uint32_t row_tiles;         // CTAs of 256 rows a sequence may need
+    uint32_t row_tiles;         // CTAs a sequence's rows may need
     uint32_t paired;            // 1: at most 128 rows, whose blocks the two row tiles take in turn
     uint32_t splits;            // most splits of the blocks of one of them
     uint32_t blocks_per_split;
 };
 
-// What the 256 rows from `row0` of a sequence's n * rep rows see together.
+// What a CTA's rows, from `row0` on, of a sequence's n * rep rows see together.
 struct TileSpan {
     uint32_t first;          // row of q of the sequence's first new token
     uint32_t tokens;         // new tokens n
@@ -88,7 +94,7 @@ struct TileSpan {
     uint32_t begin, end;     // tokens any row sees
     bool bad;
 };
-__device__ __forceinline__ TileSpan tile_span(const Kv4AttentionArgs& a, uint32_t seq, uint32_t rep, uint32_t row0) {
+__device__ __forceinline__ TileSpan tile_span(const Kv4AttentionArgs& a, uint32_t seq, uint32_t rep, uint32_t row0, uint32_t cta_rows) {
     TileSpan s{};
     uint32_t first = __ldg(a.chunk_starts + seq), last = __ldg(a.chunk_starts + seq + 1u);
     first = min(first, a.rows);
@@ -109,7 +115,7 @@ __device__ __forceinline__ TileSpan tile_span(const Kv4AttentionArgs& a, uint32_
     s.position0 = static_cast<int64_t>(s.len) - (last - first);
     s.bad = s.bad || s.position0 < 0;
     s.prefix = a.rules.prefix_lens != nullptr ? min(s.len, __ldg(a.rules.prefix_lens + seq)) : 0u;
-    const uint32_t token_lo = row0 / rep, token_hi = min(s.tokens - 1u, (row0 + kRows - 1u) / rep);
+    const uint32_t token_lo = row0 / rep, token_hi = min(s.tokens - 1u, (row0 + cta_rows - 1u) / rep);
     const int64_t lowest = max(static_cast<int64_t>(0), s.position0 + token_lo), highest = s.position0 + token_hi;
     if (highest < 0) return s;
     s.end = max(static_cast<uint32_t>(highest) + 1u, s.prefix);
@@ -245,8 +251,9 @@ template <int D>
 __device__ __forceinline__ void expand_values(uint32_t raw32, uint32_t stage32, uint32_t tid, uint32_t token0, bool whole,
                                               uint32_t begin, uint32_t end, uint32_t k1024) {
     constexpr uint32_t G = D / 64;
-    if (tid >= D) return;
-    const uint32_t octet = tid % 8u, word = tid / 8u;   // tokens 8 octet.., channels 8 word..
+    const uint32_t octet = tid % 8u;   // tokens 8 octet.., channels 8 word..
+#pragma unroll 1
+    for (uint32_t word = tid / 8u; word < D / 8u; word += kExpandWarps * 4u) {
     const uint32_t j = word / 4u;
     const uint32_t tile32 = raw32 + (octet / 2u) * Layout<D>::kRawTile + kv4_half_bytes(D);
     const uint32_t slot0 = (octet & 1u) * 8u;
@@ -291,6 +298,7 @@ __device__ __forceinline__ void expand_values(uint32_t raw32, uint32_t stage32, 
     B2_KV4_PUT(5, hi);
     B2_KV4_PUT(6, hi);
     B2_KV4_PUT(7, hi);
+    }
 #undef B2_KV4_PUT
 }
 
@@ -369,6 +377,7 @@ template <int D>
 __global__ void __launch_bounds__(kThreads, 1)
 kv4_chunk_kernel(const Kv4AttentionArgs a, float* __restrict__ partials, const ChunkPlan plan) {
     using L = Layout<D>;
+    constexpr uint32_t kRows = L::kRows, kStages = L::kStages;
     constexpr uint32_t kChannels8 = D / 8;
     pdl_launch_dependents();
     extern __shared__ __align__(1024) uint8_t smem_raw[];
@@ -383,7 +392,7 @@ kv4_chunk_kernel(const Kv4AttentionArgs a, float* __restrict__ partials, const C
     const uint32_t seq = block % a.cache.n_seq;
     // the last rows see the most tokens: they start first
     const uint32_t row0 = (plan.row_tiles - 1u - block / a.cache.n_seq) * kRows;
-    const TileSpan span = tile_span(a, seq, rep, row0);
+    const TileSpan span = tile_span(a, seq, rep, row0, kRows);
     if (row0 >= span.rows) return;
     const uint32_t rows = min(kRows, span.rows - row0);
     const uint32_t tile0 = span.begin / kKv4Tile;
@@ -432,8 +441,14 @@ kv4_chunk_kernel(const Kv4AttentionArgs a, float* __restrict__ partials, const C
             bars.abort = 0;
             mbar_fence_init();
         }
+        if (L::kQInTmem) {
+            __syncwarp();
+            tmem_alloc(&bars.tmem_base, kTmemColumns);
+            tcgen05_fence_before_sync();
+        }
     }
     __syncthreads();
+    if (L::kQInTmem) tcgen05_fence_after_sync();
 
     // (a warpgroup's four warps take its registers with one instruction, ahead of their own branches)
     if (warp >= kLoadWarp) {
@@ -474,11 +489,12 @@ kv4_chunk_kernel(const Kv4AttentionArgs a, float* __restrict__ partials, const C
             // cycles a wait) would leave the tensor core idle, were it not for the other's MMAs. Tensor memory starts at
             // column 0, this CTA holds all of it.
             const uint32_t i = warp - kIssueWarp;
-            if (i == 0u) tmem_alloc(&bars.tmem_base, kTmemColumns);
+            if (i == 0u && !L::kQInTmem) tmem_alloc(&bars.tmem_base, kTmemColumns);
             // the other tile's warp must not be ahead of the allocation
             asm volatile("bar.sync 1, %0;" ::"r"(n_tiles * 32u) : "memory");
             tcgen05_fence_after_sync();
             mbar_wait(&bars.q_full[i], 0u, abort);
+            tcgen05_fence_after_sync();
             const uint64_t dq = umma_desc_k_major_sw128(q32 + i * (128u * D * 2u));
             const uint64_t dk = umma_desc_k_major_sw128(k32), dv = umma_desc_k_major_sw128(v32);
             const uint32_t first_block = paired ? i : 0u;
@@ -493,8 +509,12 @@ kv4_chunk_kernel(const Kv4AttentionArgs a, float* __restrict__ partials, const C
                     if (elect_one()) {
 #pragma unroll
                         for (uint32_t kk = 0; kk < D / 16u; ++kk) {
-                            umma_ss(d, dq + (kk / 4u) * (16384u >> 4) + (kk % 4u) * 2u,
-                                    kb + (kk / 4u) * (kBlock * 128u >> 4) + (kk % 4u) * 2u, idesc_f16(kBlock), kk != 0u ? 1u : 0u);
+                            const uint64_t b = kb + (kk / 4u) * (kBlock * 128u >> 4) + (kk % 4u) * 2u;
+                            if (L::kQInTmem) {
+                                umma_ts(d, kTmemQ + kk * 8u, b, idesc_f16(kBlock), kk != 0u ? 1u : 0u);
+                            } else {
+                                umma_ss(d, dq + (kk / 4u) * (16384u >> 4) + (kk % 4u) * 2u, b, idesc_f16(kBlock), kk != 0u ? 1u : 0u);
+                            }
                         }
                         umma_commit(&bars.s_full[i][n & 1u]);
                         umma_commit(&bars.k_empty[stage]);
@@ -574,8 +594,44 @@ kv4_chunk_kernel(const Kv4AttentionArgs a, float* __restrict__ partials, const C
         const uint32_t warp_row = tile_rows + (warp % 4u) * 32u, c8 = lane % kChannels8;
         const uint32_t my_out = static_cast<uint32_t>(gr / rep), my_head = gr % rep;
         float row_factor = 0.0f;
+        // 2^e with a row's largest magnitude * 2^e in [2^9, 2^10), and what takes a product back
+        auto row_scale = [&](float top, float* up, float* down) {
+            int e = 9 - (static_cast<int>((__float_as_uint(top) >> 23) & 255u) - 127);
+            e = max(-100, min(100, e));   // a row of zeros or beyond 2^109 keeps a bounded factor
+            *up = __uint_as_float(static_cast<uint32_t>(e + 127) << 23);
+            *down = __uint_as_float(static_cast<uint32_t>(127 - e) << 23) * to_unit;
+        };
+        if constexpr (L::kQInTmem) {   // a thread's own row into its tensor-memory lane
+            const float4* src = reinterpret_cast<const float4*>(a.q + (static_cast<uint64_t>(span.first + my_out) * a.q_heads + kvh * rep + my_head) * D);
+            float top = 0.0f, up;
+#pragma unroll 8
+            for (uint32_t c = 0; c < D / 4u && live; ++c) {
+                const float4 u = __ldg(src + c);
+                top = fmaxf(fmaxf(fmaxf(top, fabsf(u.x)), fabsf(u.y)), fmaxf(fabsf(u.z), fabsf(u.w)));
+            }
+            row_scale(top, &up, &row_factor);
 #pragma unroll 1
-        for (uint32_t n0 = 0; n0 < kSteps; n0 += 8u) {
+            for (uint32_t c = 0; c < D / 64u; ++c) {
+                uint32_t w[32];
+#pragma unroll
+                for (uint32_t n = 0; n < 8u; ++n) {
+                    float4 u0 = make_float4(0.f, 0.f, 0.f, 0.f), u1 = u0;
+                    if (live) {
+                        u0 = __ldg(src + c * 16u + n * 2u);
+                        u1 = __ldg(src + c * 16u + n * 2u + 1u);
+                    }
+                    w[4 * n] = pack_half(u0.x * up, u1.x * up);
+                    w[4 * n + 1] = pack_half(u0.y * up, u1.y * up);
+                    w[4 * n + 2] = pack_half(u0.z * up, u1.z * up);
+                    w[4 * n + 3] = pack_half(u0.w * up, u1.w * up);
+                }
+                tmem_st_32(lane_base + kTmemQ + c * 32u, w);
+            }
+            tmem_st_wait();
+            tcgen05_fence_before_sync();
+        }
+#pragma unroll 1
+        for (uint32_t n0 = 0; n0 < kSteps && !L::kQInTmem; n0 += 8u) {
             float y[8][8];
 #pragma unroll
             for (uint32_t n = 0; n < 8u; ++n) {
@@ -598,10 +654,8 @@ kv4_chunk_kernel(const Kv4AttentionArgs a, float* __restrict__ partials, const C
                 for (int e = 0; e < 8; ++e) top = fmaxf(top, fabsf(y[n][e]));
 #pragma unroll
                 for (uint32_t o = kChannels8 / 2u; o > 0u; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xFFFFFFFFu, top, o));
-                int e = 9 - (static_cast<int>((__float_as_uint(top) >> 23) & 255u) - 127);
-                e = max(-100, min(100, e));   // a row of zeros or beyond 2^109 keeps a bounded factor
-                const float up = __uint_as_float(static_cast<uint32_t>(e + 127) << 23);
-                const float down = __uint_as_float(static_cast<uint32_t>(127 - e) << 23) * to_unit;
+                float up, down;
+                row_scale(top, &up, &down);
                 // to the lane whose row it is
 #pragma unroll
                 for (uint32_t k = 0; k < kRowsAtOnce; ++k) {
@@ -725,8 +779,9 @@ kv4_chunk_kernel(const Kv4AttentionArgs a, float* __restrict__ partials, const C
         float* part = partials + ((out_head * plan.splits + split) * parts_per_split + (paired ? i : 0u)) * (D + 4u);
         if (!whole && live) *reinterpret_cast<float2*>(part) = make_float2(m, l);
         const float inv = whole ? (l == 0.0f ? 0.0f : 1.0f / l) : 1.0f;
-        // The tile's Q is not needed any more: its 2 D bytes a row take the warp's bf16 rows, so that they leave in whole
-        // rows instead of 16 bytes of 32 different ones.
+        // The tile's Q (heads of 256: the keys' stages) is not needed any more: 2 D bytes a row take the warp's bf16 rows, so
+        // that they leave in whole rows instead of 16 bytes of 32 different ones.
+        static_assert(L::kQ + kStages * L::kKStage >= kRows * D * 2u, "room for the rows");
         const uint32_t stage32 = q32 + i * (128u * D * 2u) + (warp % 4u) * (32u * D * 2u);
 #pragma unroll 1
         for (uint32_t c = 0; c < D / 32u; ++c) {
@@ -789,7 +844,7 @@ kv4_chunk_merge_kernel(const Kv4AttentionArgs a, const float* __restrict__ parti
     bool ours = false;
     if (mine.owned) {
         const uint32_t first = min(__ldg(a.chunk_starts + mine.seq), a.rows);
-        const TileSpan span = tile_span(a, mine.seq, rep, ((row - first) * rep + head) / kRows * kRows);
+        const TileSpan span = tile_span(a, mine.seq, rep, ((row - first) * rep + head) / rows_of(D) * rows_of(D), rows_of(D));
         ours = row - first < span.tokens;
         if (ours) {
             const uint32_t tile0 = span.begin / kKv4Tile;
@@ -809,10 +864,10 @@ kv4_chunk_merge_kernel(const Kv4AttentionArgs a, const float* __restrict__ parti
 // make the waves shortest: a CTA's set-up and epilogue take about as long as six blocks, joining as four. With more row
 // tiles the longer ones start first and the shorter ones fill in; splitting those too made four chunks of 300 to 700
 // tokens, 192 CTAs, slower (132 against 166 us: the FP32 partial results of so many rows).
-ChunkPlan chunk_plan(int sm_count, uint32_t n_seq, uint32_t q_heads, uint32_t kv_heads, uint32_t max_chunk, uint32_t max_tokens) {
+ChunkPlan chunk_plan(int sm_count, uint32_t n_seq, uint32_t q_heads, uint32_t kv_heads, uint32_t head_width, uint32_t max_chunk, uint32_t max_tokens) {
     const uint64_t rep = q_heads / kv_heads;
     const uint64_t sms = sm_count > 0 ? static_cast<uint64_t>(sm_count) : 148u;
-    const uint64_t row_tiles = (max_chunk * rep + kRows - 1u) / kRows;
+    const uint64_t row_tiles = (max_chunk * rep + rows_of(head_width) - 1u) / rows_of(head_width);
     const uint64_t blocks = (static_cast<uint64_t>(max_tokens) + kBlock - 1u) / kBlock + 1u;   // a window may start inside a tile
     const uint64_t ctas = row_tiles * n_seq * kv_heads;
     uint64_t best = 1;
@@ -828,7 +883,7 @@ ChunkPlan chunk_plan(int sm_count, uint32_t n_seq, uint32_t q_heads, uint32_t kv
         }
     }
     const uint64_t per = (blocks + best - 1u) / best;
-    return ChunkPlan{static_cast<uint32_t>(row_tiles), max_chunk * rep <= 128u ? 1u : 0u,
+    return ChunkPlan{static_cast<uint32_t>(row_tiles), rows_of(head_width) == 256u && max_chunk * rep <= 128u ? 1u : 0u,
                      static_cast<uint32_t>((blocks + per - 1u) / per), static_cast<uint32_t>(per)};
 }
 // Partial results of a row: of a split one, or where its tiles are paired two.
@@ -865,12 +920,12 @@ int32_t launch_one(const DeviceContext& ctx, const Kv4AttentionArgs& a, float* p
 
 bool kv4_chunk_supported(uint32_t head_width, uint32_t q_heads, uint32_t kv_heads, uint32_t max_chunk) {
     const uint64_t rows = static_cast<uint64_t>(max_chunk) * (q_heads / kv_heads);
-    return (head_width == 64u || head_width == 128u) && rows >= 16u && rows <= 0x7FFFFF00u;
+    return (head_width == 64u || head_width == 128u || head_width == 256u) && rows >= 16u && rows <= 0x7FFFFF00u;
 }
 
 size_t kv4_chunk_workspace_bytes(int sm_count, uint32_t n_seq, uint64_t rows, uint32_t q_heads, uint32_t kv_heads,
                                  uint32_t head_width, uint32_t max_chunk, uint32_t max_seq_len) {
-    const ChunkPlan plan = chunk_plan(sm_count, n_seq, q_heads, kv_heads, max_chunk, max_seq_len);
+    const ChunkPlan plan = chunk_plan(sm_count, n_seq, q_heads, kv_heads, head_width, max_chunk, max_seq_len);
     if (parts_of(plan) <= 1u) return 0;
     return static_cast<size_t>(rows) * q_heads * parts_of(plan) * (head_width + 4u) * sizeof(float);
 }
@@ -883,10 +938,14 @@ int32_t launch_kv4_chunk(const DeviceContext& ctx, const Kv4AttentionArgs& a, vo
         return fail(B2_STATUS_INVALID_ARGUMENT, "paged attention workspace too small: need %zu bytes, got %zu", need,
                     workspace_bytes);
     }
-    const ChunkPlan plan = chunk_plan(ctx.sm_count, a.cache.n_seq, a.q_heads, a.cache.kv_heads, a.max_chunk, a.max_seq_len);
+    const ChunkPlan plan = chunk_plan(ctx.sm_count, a.cache.n_seq, a.q_heads, a.cache.kv_heads, a.cache.head_width, a.max_chunk,
+                                      a.max_seq_len);
     float* partials = static_cast<float*>(workspace);
-    return a.cache.head_width == 64u ? launch_one<64>(ctx, a, partials, plan, stream)
-                                     : launch_one<128>(ctx, a, partials, plan, stream);
+    switch (a.cache.head_width) {
+        case 64u: return launch_one<64>(ctx, a, partials, plan, stream);
+        case 128u: return launch_one<128>(ctx, a, partials, plan, stream);
+        default: return launch_one<256>(ctx, a, partials, plan, stream);
+    }
 }
 
 }  // namespace b2

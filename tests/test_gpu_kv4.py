@@ -425,9 +425,10 @@ def test_chunk_is_causal_over_the_cache(d, hq, hkv, new, past):
 @pytest.mark.parametrize("rules", [dict(softcap=4.0), dict(window=1), dict(window=50), dict(bias=True),
                                    dict(prefix=[100, 30]), dict(prefix=[1000, 0], window=40, softcap=3.0, bias=True)])
 @pytest.mark.parametrize("new,past", [([5, 2], [90, 20]), ([150, 260], [33, 0])])
-def test_chunk_score_rules(rules, new, past):
+@pytest.mark.parametrize("d", [128, 256])
+def test_chunk_score_rules(rules, new, past, d):
     lens = [p + m for p, m in zip(past, new)]
-    case = kv4_cases.Case(77, lens, 8, 2, 128, 32, rows=sum(new))
+    case = kv4_cases.Case(77, lens, 8, 2, d, 32, rows=sum(new))
     got, status = chunk(case, new, **rules)
     assert status == 0
     want = {("slopes" if k == "bias" else k): (case.slopes if k == "bias" else v) for k, v in rules.items()}
@@ -435,7 +436,7 @@ def test_chunk_score_rules(rules, new, past):
 
 
 @pytest.mark.parametrize("d,hq,hkv,new,route", [(128, 4, 2, [7], "attention_kv4"), (128, 4, 2, [8], "attention_kv4_tiles"),
-                                                (256, 4, 2, [40], "attention_kv4"), (64, 1, 1, [129, 64], "attention_kv4_tiles")])
+                                                (256, 4, 2, [7], "attention_kv4"), (256, 4, 2, [8, 40], "attention_kv4_tiles"), (64, 1, 1, [129, 64], "attention_kv4_tiles")])
 def test_chunk_routes(d, hq, hkv, new, route):
     import riftco_transformer_b200 as b2
     case = kv4_cases.Case(9, [m + 30 for m in new], hq, hkv, d, 16, rows=sum(new))
@@ -445,9 +446,10 @@ def test_chunk_routes(d, hq, hkv, new, route):
 
 
 @pytest.mark.parametrize("new,past", [([20, 3], [5000, 64]), ([300], [6000]), ([1, 1, 1], [4000, 0, 63])])
-def test_chunk_splits_long_contexts(new, past):
+@pytest.mark.parametrize("d", [128, 256])
+def test_chunk_splits_long_contexts(new, past, d):
     """Few rows over many tokens: several CTAs, and both row tiles of one, share a row's tokens."""
-    case = kv4_cases.Case(sum(new), [p + m for p, m in zip(past, new)], 32, 2, 128, 16, rows=sum(new), poison=0x7C)
+    case = kv4_cases.Case(sum(new), [p + m for p, m in zip(past, new)], 32, 2, d, 16, rows=sum(new), poison=0x7C)
     got, status = chunk(case, new)
     assert status == 0 and rel_l2(got, case.chunk(new)) <= BF16_TOL
     again, _ = chunk(case, new)
@@ -465,14 +467,15 @@ def test_chunk_scores_near_and_beyond_the_cap():
         assert rel_l2(got, case.chunk([90], softcap=cap)) <= tol
 
 
-def test_chunk_of_values_that_are_not_finite():
+@pytest.mark.parametrize("d", [128, 256])
+def test_chunk_of_values_that_are_not_finite(d):
     """A NaN group makes the context NaN for the rows that see its token, and for no other."""
     from riftco_transformer_b200 import _lib
-    for half in (0, 9 * 128):   # keys, values
-        case = kv4_cases.Case(17, [150], 4, 1, 128, 16, rows=100)
+    for half in (0, 9 * d):   # keys, values
+        case = kv4_cases.Case(17, [150], 4, 1, d, 16, rows=100)
         at = 90                  # the token
         tile = case.pages[case.tables[0, at // 16], 0, 0]
-        tile[half + 8 * 128:half + 9 * 128].reshape(16, -1)[at % 16] = 0xFF
+        tile[half + 8 * d:half + 9 * d].reshape(16, -1)[at % 16] = 0xFF
         got, status = chunk(case, [100])
         assert status == _lib.ATTN_STATUS_NAN_OR_POS_INF
         sees = np.arange(50, 150) >= at
@@ -486,9 +489,9 @@ def test_chunk_of_values_that_are_not_finite():
 
 
 def test_chunk_leaves_rows_behind_the_last_sequence():
-    for new in ([4, 3], [140, 60]):
+    for new, d in (([4, 3], 128), ([140, 60], 128), ([140, 60], 256)):
         lens = [20 + m for m in new]
-        case = kv4_cases.Case(5, lens, 8, 2, 128, 16, rows=sum(new) + 9)
+        case = kv4_cases.Case(5, lens, 8, 2, d, 16, rows=sum(new) + 9)
         got, status = chunk(case, new, extra_rows=9)
         assert status == 0 and (got[sum(new):] == 7.0).all()
         assert rel_l2(got[:sum(new)], case.chunk(new)) <= BF16_TOL
@@ -496,8 +499,8 @@ def test_chunk_leaves_rows_behind_the_last_sequence():
 
 def test_chunk_longer_than_its_sequence_is_flagged():
     from riftco_transformer_b200 import _lib
-    for new, lens in (([6, 2], [4, 30]), ([200, 2], [150, 230])):
-        case = kv4_cases.Case(6, lens, 8, 2, 128, 16, rows=sum(new))
+    for new, lens, d in (([6, 2], [4, 30], 128), ([200, 2], [150, 230], 128), ([200, 2], [150, 230], 256)):
+        case = kv4_cases.Case(6, lens, 8, 2, d, 16, rows=sum(new))
         got, status = chunk(case, new, max_len=max(lens))
         assert status == _lib.ATTN_STATUS_BAD_BLOCK
         short = new[0] - lens[0]
