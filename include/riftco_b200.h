@@ -322,9 +322,9 @@ B2_API int32_t b2_paged_decode_attention_noalloc(
  *   code = clamp(rint((x - base) * (1 / scale)), 0, 15), 0 where scale is 0
  * A group that holds a NaN, an infinity or a magnitude above 65000 is stored as
  * scale = base = NaN (codes 0): it reads back as NaN. Attention over such keys
- * reports B2_ATTN_STATUS_NAN_OR_POS_INF; over such values the decode form returns
- * NaN in the 64 channels of the group, the chunk form in the whole rows that see
- * the token, which it also reports.
+ * reports B2_ATTN_STATUS_NAN_OR_POS_INF; over such values it returns NaN in the 64
+ * channels of the group, or (chunks as tiles, below) in the whole rows that see the
+ * token, which are then reported as well.
  * head_width is 64, 128 or 256, block_size any multiple of 16.
  */
 typedef struct b2_kv4_cache {
@@ -395,11 +395,11 @@ B2_API int32_t b2_paged_decode_attention_kv4(const b2_kv4_cache* cache, const b2
  * (b2_nf4_linear_forward_multi_bf16). Rows behind chunk_starts[n_seq] are left as
  * they were; a chunk longer than its sequence is flagged BAD_BLOCK and the
  * tokens that would lie before position 0 get zeros; one longer than max_chunk is
- * flagged and its tokens from max_chunk on are left as they were. From 16 rows
- * (max_chunk * q_heads / kv_heads) on with heads of 64 or 128 the products run in
- * fp16 on the tcgen05 tensor cores (q, k, v and the weights are rounded to 2^-12),
- * otherwise token by token as in the decode form. Other errors and the workspace as
- * above. */
+ * flagged and its tokens from max_chunk on may be left as they were. Calls of four
+ * and more tokens a sequence that are not very small run as tiles of rows, in fp16 on
+ * the tcgen05 tensor cores (q, k, v and the weights are rounded to 2^-12), others
+ * token by token as in the decode form; b2_last_route tells. Other errors and the
+ * workspace as above. */
 B2_API size_t b2_paged_chunk_kv4_workspace_bytes(uint32_t n_seq, uint32_t n_tokens, uint32_t q_heads,
                                                  uint32_t kv_heads, uint32_t head_width, uint32_t max_chunk,
                                                  uint32_t max_seq_len);

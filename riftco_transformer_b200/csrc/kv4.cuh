@@ -90,8 +90,8 @@ int32_t kv4_decode_workspace_bytes(const DeviceContext& ctx, uint64_t rows, uint
 int32_t launch_kv4_decode(const DeviceContext& ctx, const Kv4AttentionArgs& args, void* workspace,
                           size_t workspace_bytes, cudaStream_t stream);
 
-// kv4_chunk.cu - tiles of 128 query rows on the tcgen05 tensor cores, bf16 contexts.
-bool kv4_chunk_supported(uint32_t head_width, uint32_t q_heads, uint32_t kv_heads, uint32_t max_chunk);
+// kv4_chunk.cu - tiles of 128 query rows on the tcgen05 tensor cores, bf16 contexts. `pays`: rather than row by row.
+bool kv4_chunk_pays(uint32_t n_seq, uint64_t rows, uint32_t q_heads, uint32_t kv_heads, uint32_t max_chunk, uint32_t max_seq_len);
 size_t kv4_chunk_workspace_bytes(int sm_count, uint32_t n_seq, uint64_t rows, uint32_t q_heads, uint32_t kv_heads,
                                  uint32_t head_width, uint32_t max_chunk, uint32_t max_seq_len);
 int32_t launch_kv4_chunk(const DeviceContext& ctx, const Kv4AttentionArgs& args, void* workspace,

@@ -168,7 +168,7 @@ DeviceContext* query_context(uint32_t rows, uint32_t q_heads, uint32_t kv_heads,
 
 int32_t chunk_workspace(const DeviceContext& ctx, uint32_t n_seq, uint32_t n_tokens, uint32_t q_heads, uint32_t kv_heads,
                         uint32_t head_width, uint32_t max_chunk, uint32_t max_seq_len, size_t* bytes) {
-    if (!kv4_chunk_supported(head_width, q_heads, kv_heads, max_chunk)) {
+    if (!kv4_chunk_pays(n_seq, n_tokens, q_heads, kv_heads, max_chunk, max_seq_len)) {
         return kv4_decode_workspace_bytes(ctx, n_tokens, q_heads, kv_heads, head_width, max_seq_len, bytes);
     }
     *bytes = kv4_chunk_workspace_bytes(ctx.sm_count, n_seq, n_tokens, q_heads, kv_heads, head_width, max_chunk, max_seq_len);
@@ -311,7 +311,7 @@ int32_t b2_paged_chunk_attention_kv4(const b2_kv4_cache* cache, const b2_kv4_sco
     size_t need = 0;
     B2_TRY(chunk_workspace(*ctx, args.cache.n_seq, n_tokens, q_heads, kv_heads, head_width, max_chunk, max_seq_len, &need));
     B2_TRY(take_workspace(ctx, need, &workspace, &workspace_bytes, stream));
-    if (kv4_chunk_supported(head_width, q_heads, kv_heads, max_chunk)) {
+    if (kv4_chunk_pays(args.cache.n_seq, n_tokens, q_heads, kv_heads, max_chunk, max_seq_len)) {
         note_route(B2_ROUTE_ATTENTION_KV4_TILES);
         return launch_kv4_chunk(*ctx, args, workspace, workspace_bytes, stream);
     }

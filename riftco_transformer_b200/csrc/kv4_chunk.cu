@@ -23,6 +23,10 @@
 // 128 tokens, whose S and O fill tensor memory, softmax and products of a tile took turns and a 4096-token prompt
 // 203 us.
 //
+// With heads of 256 there is one row tile (128 rows): O takes 256 columns of tensor memory and Q, as A operand of the
+// first product, 128, since shared memory holds only two stages of K and V of that width. The expansion of a block, about
+// 1900 cycles, then serves half as many rows and is what takes longest.
+//
 // Roles (20 warps): 0-3 and 4-7 softmax and epilogue of the two tiles (thread = row = tensor-memory lane), 8-11
 // and 12-15 expansion of keys and of values, 16 bulk copies of raw tiles, 17 and 18 the tcgen05 issue of a
 // tile each (19 completes the warpgroup whose registers go to the softmax). Every wait is bounded.
@@ -918,9 +922,17 @@ int32_t launch_one(const DeviceContext& ctx, const Kv4AttentionArgs& a, float* p
 
 }  // namespace
 
-bool kv4_chunk_supported(uint32_t head_width, uint32_t q_heads, uint32_t kv_heads, uint32_t max_chunk) {
-    const uint64_t rows = static_cast<uint64_t>(max_chunk) * (q_heads / kv_heads);
-    return (head_width == 64u || head_width == 128u || head_width == 256u) && rows >= 16u && rows <= 0x7FFFFF00u;
+// Row by row every token's lists (kv4_decode.cu) read all it sees, as tiles a sequence's tokens read it together. 16
+// sequences at 2000 tokens, 8 K/V heads of 128: 34, 44, 77 and 138 us row by row for 2, 4, 8 and 16 new tokens, 38 to 40 as
+// tiles; heads of 64 28, 36, 56 and 101 against 36, heads of 256 46, 73, 137 and 242 against 51 to 55. So from four lists
+// a sequence and head on. But a call of tiles takes 15 to 25 us however small it is, and row by row 10 to 12 and what
+// its lists (of 32 tokens a step; each costs eleven steps to begin and end) add: 4 x 16 tokens after 100 (7700
+// steps) take 14 against 20 us, 16 x 16 after nothing (24600) 28 against 20, 1 x 16 after 3000 (13600) 28 against 23.
+bool kv4_chunk_pays(uint32_t n_seq, uint64_t rows, uint32_t q_heads, uint32_t kv_heads, uint32_t max_chunk, uint32_t max_seq_len) {
+    const uint64_t rep = q_heads / kv_heads, chunks = (rep + 7u) / 8u;
+    if (max_chunk * rep > 0x7FFFFF00u) return false;
+    const double lists = static_cast<double>(rows) * static_cast<double>(chunks);   // of a K/V head
+    return lists >= 4.0 * n_seq && lists * kv_heads * (max_seq_len / 32u + 12u) >= 12000.0;
 }
 
 size_t kv4_chunk_workspace_bytes(int sm_count, uint32_t n_seq, uint64_t rows, uint32_t q_heads, uint32_t kv_heads,

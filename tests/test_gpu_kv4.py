@@ -60,7 +60,8 @@ def decode(case, max_len=None, seq_lens=None, bf16=False, workspace=None, **rule
     return out.tensor.cpu().numpy(), int(status.item())
 
 
-def chunk(case, new, max_len=None, extra_rows=0, **rules):
+def chunk(case, new, max_len=None, extra_rows=0, tiles=True, **rules):
+    """`tiles`: rows that are nobody's make the call large enough for the tile kernel, whatever its chunks."""
     import riftco_transformer_b200 as b2
     if rules.pop("bias", False):
         rules["alibi_slopes"] = cuda(case.slopes)
@@ -69,14 +70,20 @@ def chunk(case, new, max_len=None, extra_rows=0, **rules):
     pool = b2.PagedKv4Pool(cuda(case.pages), case.bs, case.d)
     starts = np.concatenate(([0], np.cumsum(new))).astype(np.uint32)
     assert starts[-1] + extra_rows == case.q.shape[0]
-    ctx, check = guarded_bf16(case.q.shape)
+    rows = case.q.shape[0]
+    q = case.q
+    if tiles:
+        q = np.concatenate((q, np.full((max(12000 // (11 * pool.kv_heads), 4 * len(new)), *q.shape[1:]), np.nan, np.float32)))
+    ctx, check = guarded_bf16(q.shape)
     ctx.fill_(7.0)
     status = status_word()
-    b2.paged_chunk_attention_kv4(cuda(case.q), pool, cuda(case.tables), cuda(np.array(case.lens, np.uint32)),
+    b2.paged_chunk_attention_kv4(cuda(q), pool, cuda(case.tables), cuda(np.array(case.lens, np.uint32)),
                                  cuda(starts), ctx, max(new), max(case.lens) if max_len is None else max_len,
                                  status=status, **rules)
     check()
-    return ctx.float().cpu().numpy(), int(status.item())
+    assert not tiles or b2.last_route() == "attention_kv4_tiles"
+    assert bool((ctx[rows:] == 7.0).all())
+    return ctx[:rows].float().cpu().numpy(), int(status.item())
 
 
 # ---- append and read-back ---------------------------------------------------------------------
@@ -414,10 +421,11 @@ def test_decode_offsets_past_32_bits():
 
 @pytest.mark.parametrize("d,hq,hkv", [(64, 4, 2), (128, 8, 2), (128, 6, 3), (128, 5, 1), (128, 2, 2), (256, 4, 2)])
 @pytest.mark.parametrize("new,past", [([1], [0]), ([3, 1, 5], [40, 0, 17]), ([130, 40], [0, 300]), ([33, 1, 0, 200], [5, 77, 9, 0])])
-def test_chunk_is_causal_over_the_cache(d, hq, hkv, new, past):
+@pytest.mark.parametrize("tiles", [False, True])
+def test_chunk_is_causal_over_the_cache(d, hq, hkv, new, past, tiles):
     lens = [p + m for p, m in zip(past, new)]
     case = kv4_cases.Case(d + sum(new), lens, hq, hkv, d, 16, rows=sum(new))
-    got, status = chunk(case, new)
+    got, status = chunk(case, new, tiles=tiles)
     assert status == 0
     assert rel_l2(got, case.chunk(new)) <= BF16_TOL
 
@@ -425,22 +433,25 @@ def test_chunk_is_causal_over_the_cache(d, hq, hkv, new, past):
 @pytest.mark.parametrize("rules", [dict(softcap=4.0), dict(window=1), dict(window=50), dict(bias=True),
                                    dict(prefix=[100, 30]), dict(prefix=[1000, 0], window=40, softcap=3.0, bias=True)])
 @pytest.mark.parametrize("new,past", [([5, 2], [90, 20]), ([150, 260], [33, 0])])
-@pytest.mark.parametrize("d", [128, 256])
-def test_chunk_score_rules(rules, new, past, d):
+@pytest.mark.parametrize("d,tiles", [(128, True), (256, True), (128, False)])
+def test_chunk_score_rules(rules, new, past, d, tiles):
     lens = [p + m for p, m in zip(past, new)]
     case = kv4_cases.Case(77, lens, 8, 2, d, 32, rows=sum(new))
-    got, status = chunk(case, new, **rules)
+    got, status = chunk(case, new, tiles=tiles, **rules)
     assert status == 0
     want = {("slopes" if k == "bias" else k): (case.slopes if k == "bias" else v) for k, v in rules.items()}
     assert rel_l2(got, case.chunk(new, **want)) <= BF16_TOL
 
 
-@pytest.mark.parametrize("d,hq,hkv,new,route", [(128, 4, 2, [7], "attention_kv4"), (128, 4, 2, [8], "attention_kv4_tiles"),
-                                                (256, 4, 2, [7], "attention_kv4"), (256, 4, 2, [8, 40], "attention_kv4_tiles"), (64, 1, 1, [129, 64], "attention_kv4_tiles")])
-def test_chunk_routes(d, hq, hkv, new, route):
+@pytest.mark.parametrize("d,hq,hkv,new,past,route", [
+    (128, 8, 8, [3] * 4, 4000, "attention_kv4"), (128, 8, 8, [4] * 4, 4000, "attention_kv4_tiles"),
+    (256, 8, 8, [1, 1, 1, 13], 4000, "attention_kv4_tiles"), (64, 96, 8, [2] * 4, 6000, "attention_kv4_tiles"),
+    (64, 8, 2, [40, 20], 100, "attention_kv4"), (64, 2, 2, [129, 640], 30, "attention_kv4_tiles")])
+def test_chunk_routes(d, hq, hkv, new, past, route):
+    """Tiles from four lists a sequence on, and not for very little work."""
     import riftco_transformer_b200 as b2
-    case = kv4_cases.Case(9, [m + 30 for m in new], hq, hkv, d, 16, rows=sum(new))
-    got, status = chunk(case, new)
+    case = kv4_cases.Case(9, [m + past for m in new], hq, hkv, d, 16, rows=sum(new))
+    got, status = chunk(case, new, tiles=False)
     assert status == 0 and b2.last_route() == route
     assert rel_l2(got, case.chunk(new)) <= BF16_TOL
 
@@ -648,6 +659,48 @@ def test_two_calls_at_once_on_two_streams():
     torch.cuda.synchronize()
     for case, (_, _, _, _, _, ctx, _) in zip(cases, todo):
         assert rel_l2(ctx.cpu().numpy(), case.decode()) <= F32_TOL
+
+
+@pytest.mark.parametrize("d,new,past", [(128, [20, 9], [3000, 5000]), (256, [150, 4], [900, 4000])])
+def test_chunk_calls_captured_and_on_two_streams(d, new, past):
+    """Split chunks: one call captured and replayed with new inputs, then two at once, a workspace each."""
+    import riftco_transformer_b200 as b2
+    lens = [p + m for p, m in zip(past, new)]
+    cases = [kv4_cases.Case(s, lens, 16, 4, d, 16, rows=sum(new)) for s in (71, 72)]
+    starts, max_len = cuda(np.array([0, new[0], sum(new)], np.uint32)), max(lens)
+    need = b2.paged_chunk_kv4_workspace_bytes(2, sum(new), 16, 4, d, max(new), max_len)
+    assert need > 0
+    todo = []
+    for case in cases:
+        todo.append((torch.cuda.Stream(), b2.PagedKv4Pool(cuda(case.pages), 16, d), cuda(case.q), cuda(case.tables),
+                     cuda(np.array(lens, np.uint32)), torch.empty(case.q.shape, dtype=torch.bfloat16, device="cuda"),
+                     torch.empty(need, dtype=torch.uint8, device="cuda")))
+    torch.cuda.synchronize()
+
+    def call(stream, pool, q, tables, lens, ctx, workspace):
+        b2.paged_chunk_attention_kv4(q, pool, tables, lens, starts, ctx, max(new), max_len, workspace=workspace, stream=stream)
+
+    for _ in range(10):
+        for one in todo:
+            call(*one)
+    torch.cuda.synchronize()
+    assert b2.last_route() == "attention_kv4_tiles"
+    want = [case.chunk(new) for case in cases]
+    for w, one in zip(want, todo):
+        assert rel_l2(one[5].float().cpu().numpy(), w) <= BF16_TOL
+    stream, pool, q, tables, _, ctx, _ = todo[0]
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph, stream=stream):
+        call(*todo[0])
+    for case, w in zip(reversed(cases), reversed(want)):
+        with torch.cuda.stream(stream):
+            pool.pages.copy_(cuda(case.pages))
+            q.copy_(cuda(case.q))
+            tables.copy_(cuda(case.tables))
+            ctx.fill_(float("nan"))
+            graph.replay()
+        stream.synchronize()
+        assert rel_l2(ctx.float().cpu().numpy(), w) <= BF16_TOL
 
 
 # ---- refusals -------------------------------------------------------------------------------------------
