@@ -24,11 +24,12 @@
 // 203 us.
 //
 // With heads of 256 there is one row tile (128 rows): O takes 256 columns of tensor memory and Q, as A operand of the
-// first product, 128, since shared memory holds only two stages of K and V of that width. The expansion of a block, about
-// 1900 cycles, then serves half as many rows and is what takes longest.
+// first product, 128, since shared memory holds only two stages of K and V of that width. The second tile's softmax warps
+// expand too: three groups of four warps take half blocks of keys and values in turn, 147 against 160 us for 2000
+// tokens after 4000 of 16 / 2 heads.
 //
 // Roles (20 warps): 0-3 and 4-7 softmax and epilogue of the two tiles (thread = row = tensor-memory lane), 8-11
-// and 12-15 expansion of keys and of values, 16 bulk copies of raw tiles, 17 and 18 the tcgen05 issue of a
+// and 12-15 expansion (of keys and of values), 16 bulk copies of raw tiles, 17 and 18 the tcgen05 issue of a
 // tile each (19 completes the warpgroup whose registers go to the softmax). Every wait is bounded.
 #include "kv4.cuh"
 
@@ -43,15 +44,15 @@ constexpr uint32_t kBlock = 64;   // tokens of a block
 // Rows of a CTA: two tiles of 128; one where heads of 256 fill tensor memory with its O.
 __host__ __device__ constexpr uint32_t rows_of(uint32_t d) { return d == 256u ? 128u : 256u; }
 constexpr uint32_t kBlockTiles = kBlock / kKv4Tile;
-constexpr uint32_t kExpandWarps = 4;   // for keys and for values each
-constexpr uint32_t kKeyWarp = 8, kValueWarp = 12, kLoadWarp = 16, kIssueWarp = 17;   // and 18
+constexpr uint32_t kExpandWarps = 4;   // of a group
+constexpr uint32_t kExpandWarp = 8, kLoadWarp = 16, kIssueWarp = 17;   // and 18
 constexpr uint32_t kThreads = 20 * 32;
 // Registers of a thread by warpgroup, against 96 at the launch (the most that 20 warps of 640 threads can have):
-// softmax 2 x 128 x 136 + expansion 2 x 128 x 80 + the last 128 x 48 = 640 x 96, what the launch holds.
+// softmax 2 x 128 x 136 + expansion 2 x 128 x 80 + the last 128 x 48 = 640 x 96, what the launch holds; with three
+// warpgroups that expand and one tile's softmax less.
 constexpr int kSoftmaxRegisters = 136, kExpandRegisters = 80, kOtherRegisters = 48;
 static_assert(256 * kSoftmaxRegisters + 256 * kExpandRegisters + 128 * kOtherRegisters <= 640 * 96, "more than the launch holds");
 constexpr uint32_t kRawSlots = 3;
-__host__ __device__ constexpr uint32_t stages_of(int d) { return d == 256 ? 2u : 4u; }   // of expanded keys and of values
 constexpr uint32_t kMostStages = 4;
 constexpr uint32_t kTmemColumns = 512, kTmemTile = 256, kTmemO = 128;   // a tile's two S (and P) of 64 columns, its O
 constexpr uint32_t kTmemQ = 384;   // heads of 256: Q, for which shared memory has no room, beside the one tile's O
@@ -60,12 +61,15 @@ constexpr float kSlack = 8.0f;
 template <int D>
 struct Layout {
     static constexpr bool kQInTmem = D == 256;
-    static constexpr uint32_t kRows = rows_of(D), kStages = stages_of(D);
+    static constexpr uint32_t kRows = rows_of(D), kStages = D == 256 ? 2 : kMostStages;   // of expanded keys and of values
+    // Channels that a group of four warps expands in one go. Heads of 256 have halves, four to a block, which three groups
+    // take in turn; the others one group for keys and one for values.
+    static constexpr uint32_t kPart = D == 256 ? 128 : D, kHalves = D / kPart;
     static constexpr uint32_t kQ = kQInTmem ? 0u : kRows * D * 2, kKStage = kBlock * D * 2, kVStage = kBlock * D * 2;
     // 16 bytes apart, so that the same word of four tiles lies in different banks
     static constexpr uint32_t kRawTile = kv4_tile_bytes(D) + 16u;
     static constexpr uint32_t kRawSlot = kBlockTiles * kRawTile;
-    static constexpr uint32_t kTotal = kQ + kStages * (kKStage + kVStage) + kRawSlots * kRawSlot + 1024u;
+    static constexpr uint32_t kTotal = kQ + kStages * (kKStage + kVStage) + kRawSlots * kRawSlot + (kQInTmem ? 4u * 4096u : 0u) + 1024u;
 };
 
 struct Barriers {
@@ -212,22 +216,23 @@ __device__ __forceinline__ uint32_t not_finite(uint32_t pair) { return ((pair & 
 // A block of keys: 32 channels of one token per step and thread, rows of the tile in token order. `whole`: every
 // one of the tokens is seen by some row.
 template <int D>
-__device__ __forceinline__ void expand_keys(uint32_t raw32, uint32_t stage32, uint32_t tid, uint32_t token0, bool whole,
+__device__ __forceinline__ void expand_keys(uint32_t raw32, uint32_t stage32, uint32_t half, uint32_t tid, uint32_t token0, bool whole,
                                             uint32_t begin, uint32_t end, uint32_t k1024) {
-    constexpr uint32_t G = D / 64, kSteps = kBlock * (D / 32) / (kExpandWarps * 32u);
+    constexpr uint32_t G = D / 64, kSteps = kBlock * (Layout<D>::kPart / 32) / (kExpandWarps * 32u);
+    const uint32_t n0 = half * kSteps;
     const uint32_t tk = tid % kBlock;   // lanes: consecutive tokens
     const uint32_t tile32 = raw32 + (tk / 16u) * Layout<D>::kRawTile;
     const uint32_t row32 = stage32 + tk * 128u;
     uint32_t pair[kSteps];
     uint4 raw[kSteps];
 #pragma unroll
-    for (uint32_t n = 0; n < kSteps; ++n) {   // chunk of 32 channels j = tid / 64 + 2n, group j / 2 = n
-        pair[n] = lds32(tile32 + 8u * D + (tk % 16u) * (4u * G) + n * 4u);
-        raw[n] = lds128(tile32 + (tid / kBlock + 2u * n) * 256u + (tk % 16u) * 16u);
+    for (uint32_t n = 0; n < kSteps; ++n) {   // chunk of 32 channels j = tid / 64 + 2 (n0 + n), group j / 2 = n0 + n
+        pair[n] = lds32(tile32 + 8u * D + (tk % 16u) * (4u * G) + (n0 + n) * 4u);
+        raw[n] = lds128(tile32 + (tid / kBlock + 2u * (n0 + n)) * 256u + (tk % 16u) * 16u);
     }
     // A value that is not finite must not meet the zero weight of a row that does not see it: its group is
     // expanded as zeros (expand_values), and the token's scores, which such a row masks, become NaN.
-    if (tid < kBlock) {
+    if (half == 0u && tid < kBlock) {
 #pragma unroll
         for (uint32_t gr = 0; gr < G; ++gr) {
             if (not_finite(lds32(tile32 + kv4_half_bytes(D) + 8u * D + (tk % 16u) * (4u * G) + gr * 4u))) pair[0] = 0x7FFF7FFFu;
@@ -244,7 +249,7 @@ __device__ __forceinline__ void expand_keys(uint32_t raw32, uint32_t stage32, ui
 #pragma unroll
         for (uint32_t w = 0; w < 4u; ++w) {
             const uint32_t unit = (tid / kBlock) * 4u + w;
-            sts128(row32 + n * (kBlock * 128u) + ((unit ^ (tk & 7u)) << 4), expand<0>(words[w], scale, base, k1024),
+            sts128(row32 + (n0 + n) * (kBlock * 128u) + ((unit ^ (tk & 7u)) << 4), expand<0>(words[w], scale, base, k1024),
                    expand<1>(words[w], scale, base, k1024), expand<2>(words[w], scale, base, k1024), expand<3>(words[w], scale, base, k1024));
         }
     }
@@ -252,12 +257,11 @@ __device__ __forceinline__ void expand_keys(uint32_t raw32, uint32_t stage32, ui
 
 // A block of values, transposed: eight channels of eight tokens per thread, rows of the tile are channels.
 template <int D>
-__device__ __forceinline__ void expand_values(uint32_t raw32, uint32_t stage32, uint32_t tid, uint32_t token0, bool whole,
+__device__ __forceinline__ void expand_values(uint32_t raw32, uint32_t stage32, uint32_t half, uint32_t tid, uint32_t token0, bool whole,
                                               uint32_t begin, uint32_t end, uint32_t k1024) {
     constexpr uint32_t G = D / 64;
-    const uint32_t octet = tid % 8u;   // tokens 8 octet.., channels 8 word..
-#pragma unroll 1
-    for (uint32_t word = tid / 8u; word < D / 8u; word += kExpandWarps * 4u) {
+    if (tid >= Layout<D>::kPart) return;
+    const uint32_t octet = tid % 8u, word = half * (Layout<D>::kPart / 8u) + tid / 8u;   // tokens 8 octet.., channels 8 word..
     const uint32_t j = word / 4u;
     const uint32_t tile32 = raw32 + (octet / 2u) * Layout<D>::kRawTile + kv4_half_bytes(D);
     const uint32_t slot0 = (octet & 1u) * 8u;
@@ -302,7 +306,6 @@ __device__ __forceinline__ void expand_values(uint32_t raw32, uint32_t stage32, 
     B2_KV4_PUT(5, hi);
     B2_KV4_PUT(6, hi);
     B2_KV4_PUT(7, hi);
-    }
 #undef B2_KV4_PUT
 }
 
@@ -425,11 +428,11 @@ kv4_chunk_kernel(const Kv4AttentionArgs a, float* __restrict__ partials, const C
         if (lane == 0) {
             for (uint32_t i = 0; i < kRawSlots; ++i) {
                 mbar_init(&bars.raw_full[i], 1);
-                mbar_init(&bars.raw_empty[i], 2u * kExpandWarps);
+                mbar_init(&bars.raw_empty[i], 2u * L::kHalves * kExpandWarps);
             }
             for (uint32_t i = 0; i < kStages; ++i) {
-                mbar_init(&bars.k_full[i], kExpandWarps);
-                mbar_init(&bars.v_full[i], kExpandWarps);
+                mbar_init(&bars.k_full[i], L::kHalves * kExpandWarps);
+                mbar_init(&bars.v_full[i], L::kHalves * kExpandWarps);
                 mbar_init(&bars.k_empty[i], paired ? 1u : n_tiles);
                 mbar_init(&bars.v_empty[i], paired ? 1u : n_tiles);
             }
@@ -544,30 +547,35 @@ kv4_chunk_kernel(const Kv4AttentionArgs a, float* __restrict__ partials, const C
                 }
             }
         }
-    } else if (warp >= kKeyWarp) {
-        // ---- expansion ----
+    } else if (warp >= kExpandWarp || (L::kQInTmem && warp >= 4u)) {
+        // ---- expansion: part `part` of a block, its keys' (or their halves) before its values' ----
         registers_down<kExpandRegisters>();
-        const bool keys = warp < kValueWarp;
         const uint32_t k1024 = opaque_1024();
-        const uint32_t et = tid - (keys ? kKeyWarp : kValueWarp) * 32u;
-        uint64_t* const empty = keys ? bars.k_empty : bars.v_empty;
-        uint64_t* const full = keys ? bars.k_full : bars.v_full;
-        for (uint32_t jb = 0; jb < n_blocks; ++jb) {
+        constexpr uint32_t kParts = 2u * L::kHalves, kGroups = L::kQInTmem ? 3u : 2u;
+        const uint32_t group = warp >= kExpandWarp ? (warp - kExpandWarp) / kExpandWarps : 2u, et = tid % (kExpandWarps * 32u);
+        for (uint32_t part = group, jb = 0; jb < n_blocks;) {
+            const bool keys = part < L::kHalves;
+            const uint32_t half = part % L::kHalves;
             const uint32_t stage = jb % kStages, use = jb / kStages, slot = jb % kRawSlots;
             const uint32_t token0 = (first_tile + jb * kBlockTiles) * kKv4Tile;
             const bool whole = token0 >= span.begin && token0 + kBlock <= span.end;
-            if (use > 0) mbar_wait(&empty[stage], (use - 1u) & 1u, abort);
+            if (use > 0) mbar_wait(keys ? &bars.k_empty[stage] : &bars.v_empty[stage], (use - 1u) & 1u, abort);
             mbar_wait(&bars.raw_full[slot], (jb / kRawSlots) & 1u, abort);
             if (keys) {
-                expand_keys<D>(raw32 + slot * L::kRawSlot, k32 + stage * L::kKStage, et, token0, whole, span.begin, span.end, k1024);
+                expand_keys<D>(raw32 + slot * L::kRawSlot, k32 + stage * L::kKStage, half, et, token0, whole, span.begin, span.end, k1024);
             } else {
-                expand_values<D>(raw32 + slot * L::kRawSlot, v32 + stage * L::kVStage, et, token0, whole, span.begin, span.end, k1024);
+                expand_values<D>(raw32 + slot * L::kRawSlot, v32 + stage * L::kVStage, half, et, token0, whole, span.begin, span.end, k1024);
             }
             fence_proxy_async_smem();
             __syncwarp();
             if (lane == 0) {
                 mbar_arrive(&bars.raw_empty[slot]);
-                mbar_arrive(&full[stage]);
+                mbar_arrive(keys ? &bars.k_full[stage] : &bars.v_full[stage]);
+            }
+            part += kGroups;
+            if (part >= kParts) {
+                part -= kParts;
+                ++jb;
             }
         }
     } else if (warp / 4u < n_tiles) {
@@ -605,31 +613,62 @@ kv4_chunk_kernel(const Kv4AttentionArgs a, float* __restrict__ partials, const C
             *up = __uint_as_float(static_cast<uint32_t>(e + 127) << 23);
             *down = __uint_as_float(static_cast<uint32_t>(127 - e) << 23) * to_unit;
         };
-        if constexpr (L::kQInTmem) {   // a thread's own row into its tensor-memory lane
-            const float4* src = reinterpret_cast<const float4*>(a.q + (static_cast<uint64_t>(span.first + my_out) * a.q_heads + kvh * rep + my_head) * D);
-            float top = 0.0f, up;
-#pragma unroll 8
-            for (uint32_t c = 0; c < D / 4u && live; ++c) {
-                const float4 u = __ldg(src + c);
-                top = fmaxf(fmaxf(fmaxf(top, fabsf(u.x)), fabsf(u.y)), fmaxf(fabsf(u.z), fabsf(u.w)));
+        if constexpr (L::kQInTmem) {
+            // Into each row's lane of tensor memory, by way of shared memory, 64 channels of the warp's rows at a time: a
+            // thread that read its own row would take 16 bytes of 32 different ones. First the rows' largest magnitudes.
+            float my_up = 0.0f;
+#pragma unroll 1
+            for (uint32_t n0 = 0; n0 < 32u; n0 += 8u) {
+                float top8[8];
+#pragma unroll
+                for (uint32_t n = 0; n < 8u; ++n) {
+                    const uint32_t token = __shfl_sync(0xFFFFFFFFu, my_out, n0 + n), head = __shfl_sync(0xFFFFFFFFu, my_head, n0 + n);
+                    float4 u0 = make_float4(0.f, 0.f, 0.f, 0.f), u1 = u0;
+                    if (warp_row + n0 + n < rows) {
+                        const float* src = a.q + (static_cast<uint64_t>(span.first + token) * a.q_heads + kvh * rep + head) * D + lane * 8u;
+                        u0 = __ldg(reinterpret_cast<const float4*>(src));
+                        u1 = __ldg(reinterpret_cast<const float4*>(src) + 1);
+                    }
+                    top8[n] = fmaxf(fmaxf(fmaxf(fabsf(u0.x), fabsf(u0.y)), fmaxf(fabsf(u0.z), fabsf(u0.w))),
+                                    fmaxf(fmaxf(fabsf(u1.x), fabsf(u1.y)), fmaxf(fabsf(u1.z), fabsf(u1.w))));
+                }
+#pragma unroll
+                for (uint32_t n = 0; n < 8u; ++n) {
+                    const float top = __uint_as_float(__reduce_max_sync(0xFFFFFFFFu, __float_as_uint(top8[n])));   // not negative
+                    float up, down;
+                    row_scale(top, &up, &down);
+                    if (lane == n0 + n) {
+                        my_up = up;
+                        row_factor = down;
+                    }
+                }
             }
-            row_scale(top, &up, &row_factor);
+            const uint32_t turn32 = raw32 + kRawSlots * L::kRawSlot + (warp % 4u) * 4096u;
 #pragma unroll 1
             for (uint32_t c = 0; c < D / 64u; ++c) {
+#pragma unroll
+                for (uint32_t n = 0; n < 8u; ++n) {   // eight lanes a row
+                    const uint32_t which = n * 4u + lane / 8u;
+                    const uint32_t token = __shfl_sync(0xFFFFFFFFu, my_out, which), head = __shfl_sync(0xFFFFFFFFu, my_head, which);
+                    const float up = __shfl_sync(0xFFFFFFFFu, my_up, which);
+                    float4 u0 = make_float4(0.f, 0.f, 0.f, 0.f), u1 = u0;
+                    if (warp_row + which < rows) {
+                        const float* src = a.q + (static_cast<uint64_t>(span.first + token) * a.q_heads + kvh * rep + head) * D + c * 64u + lane % 8u * 8u;
+                        u0 = __ldg(reinterpret_cast<const float4*>(src));
+                        u1 = __ldg(reinterpret_cast<const float4*>(src) + 1);
+                    }
+                    sts128(turn32 + which * 128u + (((lane % 8u) ^ (which & 7u)) << 4), pack_half(u0.x * up, u1.x * up),
+                           pack_half(u0.y * up, u1.y * up), pack_half(u0.z * up, u1.z * up), pack_half(u0.w * up, u1.w * up));
+                }
+                __syncwarp();
                 uint32_t w[32];
 #pragma unroll
                 for (uint32_t n = 0; n < 8u; ++n) {
-                    float4 u0 = make_float4(0.f, 0.f, 0.f, 0.f), u1 = u0;
-                    if (live) {
-                        u0 = __ldg(src + c * 16u + n * 2u);
-                        u1 = __ldg(src + c * 16u + n * 2u + 1u);
-                    }
-                    w[4 * n] = pack_half(u0.x * up, u1.x * up);
-                    w[4 * n + 1] = pack_half(u0.y * up, u1.y * up);
-                    w[4 * n + 2] = pack_half(u0.z * up, u1.z * up);
-                    w[4 * n + 3] = pack_half(u0.w * up, u1.w * up);
+                    const uint4 v = lds128(turn32 + lane * 128u + ((n ^ (lane & 7u)) << 4));
+                    w[4 * n] = v.x; w[4 * n + 1] = v.y; w[4 * n + 2] = v.z; w[4 * n + 3] = v.w;
                 }
                 tmem_st_32(lane_base + kTmemQ + c * 32u, w);
+                __syncwarp();
             }
             tmem_st_wait();
             tcgen05_fence_before_sync();
