@@ -337,7 +337,7 @@ typedef struct b2_kv4_cache {
 
 /* What is done to a score s = q . k / sqrt(head_width) before the softmax, in this
  * order; a NULL pointer or zeros mean plain scores. position is the query's own.
- *   softcap > 0:   s = softcap * tanh(s / softcap)
+ *   softcap > 0:   s = softcap * tanh(s / softcap)   (1e-6 to 1e18)
  *   alibi_slopes:  s -= alibi_slopes[query head] * |position - t|   (device float[q_heads])
  *   window > 0:    token t is seen only if t > position - window */
 typedef struct b2_kv4_score_rules {
@@ -372,7 +372,8 @@ B2_API int32_t b2_kv4_dequantize(const b2_kv4_cache* cache, const uint32_t* posi
  * ctx_bf16 rounded from it (either may be NULL, not both); all 16-byte aligned.
  * q_heads is any multiple of kv_heads. Scores, softmax statistics and sums are FP32,
  * the products exact to 22 bits. A sequence of length 0 sees nothing and gets zeros.
- * Errors go to the status word: NaN or +infinite scores, every score of a head
+ * Errors go to the status word: NaN or +infinite scores (all scores of a query that
+ * holds a NaN or an infinity may count as such), every score of a head
  * -infinite (zeros), a block id outside the pool (its page is read as page 0), a
  * length above max_seq_len (read up to max_seq_len; BAD_BLOCK).
  * Workspace as for b2_paged_decode_attention: at least the bytes below (NULL: the

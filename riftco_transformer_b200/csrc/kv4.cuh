@@ -181,6 +181,7 @@ __device__ __forceinline__ RowSpan row_span(const Kv4AttentionArgs& a, uint32_t 
         r.owned = row >= first && row < last;
         if (!r.owned) return r;
         back = last - 1u - row;
+        r.bad = last - first > a.max_chunk;
     }
     uint32_t len = __ldg(a.seq_lens + r.seq);
     if (len > a.max_seq_len) {

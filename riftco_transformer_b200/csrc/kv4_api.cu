@@ -121,8 +121,9 @@ int32_t attention_args(const AttentionCall& c, Kv4AttentionArgs* args) {
     }
     Kv4ScoreRules rules;
     if (c.rules != nullptr) {
-        if (!std::isfinite(c.rules->softcap) || c.rules->softcap < 0.0f) {
-            return fail(B2_STATUS_INVALID_ARGUMENT, "paged attention score cap must be finite and not negative");
+        // (beyond these 1 / cap or cap * log2(e) and their products with scores leave FP32)
+        if (c.rules->softcap != 0.0f && !(c.rules->softcap >= 1e-6f && c.rules->softcap <= 1e18f)) {
+            return fail(B2_STATUS_INVALID_ARGUMENT, "paged attention score cap must be 0 or between 1e-6 and 1e18");
         }
         if (misaligned(c.rules->alibi_slopes, 4)) {
             return fail(B2_STATUS_INVALID_ARGUMENT, "paged attention slopes must be 4-byte aligned");

@@ -60,7 +60,7 @@ def decode(case, max_len=None, seq_lens=None, bf16=False, workspace=None, **rule
     return out.tensor.cpu().numpy(), int(status.item())
 
 
-def chunk(case, new, max_len=None, extra_rows=0, tiles=True, **rules):
+def chunk(case, new, max_len=None, extra_rows=0, tiles=True, max_chunk=None, **rules):
     """`tiles`: rows that are nobody's make the call large enough for the tile kernel, whatever its chunks."""
     import riftco_transformer_b200 as b2
     if rules.pop("bias", False):
@@ -78,7 +78,8 @@ def chunk(case, new, max_len=None, extra_rows=0, tiles=True, **rules):
     ctx.fill_(7.0)
     status = status_word()
     b2.paged_chunk_attention_kv4(cuda(q), pool, cuda(case.tables), cuda(np.array(case.lens, np.uint32)),
-                                 cuda(starts), ctx, max(new), max(case.lens) if max_len is None else max_len,
+                                 cuda(starts), ctx, max(new) if max_chunk is None else max_chunk,
+                                 max(case.lens) if max_len is None else max_len,
                                  status=status, **rules)
     check()
     assert not tiles or b2.last_route() == "attention_kv4_tiles"
@@ -286,7 +287,7 @@ def test_decode_block_sizes_and_what_unused_slots_hold(bs, poison):
     assert rel_l2(got, case.decode()) <= F32_TOL
 
 
-@pytest.mark.parametrize("rules", [dict(softcap=5.0), dict(window=1), dict(window=16), dict(window=33),
+@pytest.mark.parametrize("rules", [dict(softcap=5.0), dict(softcap=1e-6), dict(softcap=1e18), dict(window=1), dict(window=16), dict(window=33),
                                    dict(window=100000), dict(bias=True), dict(softcap=2.0, window=200, bias=True)])
 @pytest.mark.parametrize("hq", [8, 16])
 def test_decode_score_rules(rules, hq):
@@ -500,19 +501,31 @@ def test_chunk_of_values_that_are_not_finite(d):
 
 
 def test_chunk_leaves_rows_behind_the_last_sequence():
-    for new, d in (([4, 3], 128), ([140, 60], 128), ([140, 60], 256)):
+    for new, d, tiles in (([4, 3], 128, True), ([140, 60], 128, True), ([140, 60], 256, True), ([4, 3], 64, False)):
         lens = [20 + m for m in new]
         case = kv4_cases.Case(5, lens, 8, 2, d, 16, rows=sum(new) + 9)
-        got, status = chunk(case, new, extra_rows=9)
+        got, status = chunk(case, new, extra_rows=9, tiles=tiles)
         assert status == 0 and (got[sum(new):] == 7.0).all()
         assert rel_l2(got[:sum(new)], case.chunk(new)) <= BF16_TOL
 
 
-def test_chunk_longer_than_its_sequence_is_flagged():
+@pytest.mark.parametrize("tiles", [False, True])
+def test_chunk_longer_than_the_bound_is_flagged(tiles):
+    from riftco_transformer_b200 import _lib
+    new = [30, 9]
+    case = kv4_cases.Case(8, [50, 40], 8, 2, 128, 16, rows=39)
+    got, status = chunk(case, new, max_chunk=10, tiles=tiles)
+    assert status == _lib.ATTN_STATUS_BAD_BLOCK
+    want = case.chunk(new)
+    assert rel_l2(got[:10], want[:10]) <= BF16_TOL and rel_l2(got[30:], want[30:]) <= BF16_TOL
+
+
+@pytest.mark.parametrize("tiles", [False, True])
+def test_chunk_longer_than_its_sequence_is_flagged(tiles):
     from riftco_transformer_b200 import _lib
     for new, lens, d in (([6, 2], [4, 30], 128), ([200, 2], [150, 230], 128), ([200, 2], [150, 230], 256)):
         case = kv4_cases.Case(6, lens, 8, 2, d, 16, rows=sum(new))
-        got, status = chunk(case, new, max_len=max(lens))
+        got, status = chunk(case, new, max_len=max(lens), tiles=tiles)
         assert status == _lib.ATTN_STATUS_BAD_BLOCK
         short = new[0] - lens[0]
         assert (got[:short] == 0).all()
@@ -720,7 +733,8 @@ def test_refusals():
         dict(q=q.half()), dict(q=q[:, :7]), dict(q=q.transpose(0, 1)), dict(q=q[:1]), dict(ctx=None), dict(ctx=q),
         dict(ctx=ctx[:1]), dict(lens=lens.float()), dict(lens=lens[:1]), dict(tables=tables.long()),
         dict(max_len=0), dict(max_len=49), dict(max_len=-1), dict(softcap=-1.0), dict(softcap=float("nan")),
-        dict(softcap=float("inf")), dict(window=-1), dict(alibi_slopes=torch.ones(7, device="cuda")),
+        dict(softcap=float("inf")), dict(softcap=1e-7), dict(softcap=2e18), dict(window=-1),
+        dict(alibi_slopes=torch.ones(7, device="cuda")),
         dict(alibi_slopes=torch.ones(8)), dict(context_bf16=torch.empty_like(q)), dict(q=q.cpu()),
         dict(status=torch.zeros(1, device="cuda")), dict(workspace=torch.zeros(16, dtype=torch.uint8)),
         dict(ctx=pool.pages.view(-1)[:q.numel() * 4].view(torch.float32).view(q.shape)),
