@@ -600,7 +600,7 @@ kv4_chunk_kernel(const Kv4AttentionArgs a, float* __restrict__ partials, const C
         const float cap_log2 = a.rules.softcap * kLog2e;
         const float slope = biased && live ? __ldg(a.rules.alibi_slopes + kvh * rep + gr % rep) * kLog2e : 0.0f;
         // Q: scaled to a largest magnitude in [2^9, 2^10) per row, fp16, in the order the codes come out. A warp stages
-        // its own 32 rows, kChannels8 lanes a row, with all loads of eight steps before their first use.
+        // its own 32 rows, four lanes a row, so that two exchanges find a row's largest.
         const float to_unit = (capped ? 1.0f / a.rules.softcap : kLog2e) / sqrtf(static_cast<float>(D));
         constexpr uint32_t kRowsAtOnce = 32u / kChannels8, kSteps = 32u / kRowsAtOnce;
         const uint32_t warp_row = tile_rows + (warp % 4u) * 32u, c8 = lane % kChannels8;
@@ -673,41 +673,48 @@ kv4_chunk_kernel(const Kv4AttentionArgs a, float* __restrict__ partials, const C
             tmem_st_wait();
             tcgen05_fence_before_sync();
         }
+        constexpr uint32_t kUnits = L::kQInTmem ? 1u : D / 32u;   // of eight channels, of a lane
+        constexpr uint32_t kAtOnce = L::kQInTmem ? 1u : 8u / kUnits;   // times eight rows: 64 registers of loads
 #pragma unroll 1
-        for (uint32_t n0 = 0; n0 < kSteps && !L::kQInTmem; n0 += 8u) {
-            float y[8][8];
+        for (uint32_t n0 = 0; n0 < 4u && !L::kQInTmem; n0 += kAtOnce) {
+            float y[kAtOnce][kUnits][8];
 #pragma unroll
-            for (uint32_t n = 0; n < 8u; ++n) {
-                const uint32_t mine = (n0 + n) * kRowsAtOnce + lane / kChannels8;   // of the warp's 32 rows
+            for (uint32_t n = 0; n < kAtOnce; ++n) {
+                const uint32_t mine = (n0 + n) * 8u + lane / 4u;   // of the warp's 32 rows
                 const uint32_t token = __shfl_sync(0xFFFFFFFFu, my_out, mine), head = __shfl_sync(0xFFFFFFFFu, my_head, mine);
-                float4 u0 = make_float4(0.f, 0.f, 0.f, 0.f), u1 = u0;
-                if (warp_row + mine < rows) {
-                    const float* src = a.q + (static_cast<uint64_t>(span.first + token) * a.q_heads + kvh * rep + head) * D + c8 * 8u;
-                    u0 = __ldg(reinterpret_cast<const float4*>(src));
-                    u1 = __ldg(reinterpret_cast<const float4*>(src) + 1);
+                const float* src = a.q + (static_cast<uint64_t>(span.first + token) * a.q_heads + kvh * rep + head) * D + lane % 4u * 8u;
+#pragma unroll
+                for (uint32_t u = 0; u < kUnits; ++u) {
+                    float4 u0 = make_float4(0.f, 0.f, 0.f, 0.f), u1 = u0;
+                    if (warp_row + mine < rows) {
+                        u0 = __ldg(reinterpret_cast<const float4*>(src + u * 32u));
+                        u1 = __ldg(reinterpret_cast<const float4*>(src + u * 32u) + 1);
+                    }
+                    y[n][u][0] = u0.x; y[n][u][1] = u0.y; y[n][u][2] = u0.z; y[n][u][3] = u0.w;
+                    y[n][u][4] = u1.x; y[n][u][5] = u1.y; y[n][u][6] = u1.z; y[n][u][7] = u1.w;
                 }
-                y[n][0] = u0.x; y[n][1] = u0.y; y[n][2] = u0.z; y[n][3] = u0.w;
-                y[n][4] = u1.x; y[n][5] = u1.y; y[n][6] = u1.z; y[n][7] = u1.w;
             }
 #pragma unroll
-            for (uint32_t n = 0; n < 8u; ++n) {
-                const uint32_t mine = (n0 + n) * kRowsAtOnce + lane / kChannels8, tile_row = (warp % 4u) * 32u + mine;
-                float top = 0.0f;
+            for (uint32_t n = 0; n < kAtOnce; ++n) {
+                float top = 0.0f, up, down;
 #pragma unroll
-                for (int e = 0; e < 8; ++e) top = fmaxf(top, fabsf(y[n][e]));
+                for (uint32_t u = 0; u < kUnits; ++u)
 #pragma unroll
-                for (uint32_t o = kChannels8 / 2u; o > 0u; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xFFFFFFFFu, top, o));
-                float up, down;
+                    for (int e = 0; e < 8; ++e) top = fmaxf(top, fabsf(y[n][u][e]));
+                top = fmaxf(top, __shfl_xor_sync(0xFFFFFFFFu, top, 1));
+                top = fmaxf(top, __shfl_xor_sync(0xFFFFFFFFu, top, 2));
                 row_scale(top, &up, &down);
-                // to the lane whose row it is
+                const float f = __shfl_sync(0xFFFFFFFFu, down, lane % 8u * 4u);   // to the lane whose row it is
+                if (lane / 8u == n0 + n) row_factor = f;
+                const uint32_t tile_row = (warp % 4u) * 32u + (n0 + n) * 8u + lane / 4u;
+                const uint32_t dst = q32 + i * (128u * D * 2u) + tile_row * 128u;
 #pragma unroll
-                for (uint32_t k = 0; k < kRowsAtOnce; ++k) {
-                    const float f = __shfl_sync(0xFFFFFFFFu, down, k * kChannels8);
-                    if (lane == (n0 + n) * kRowsAtOnce + k) row_factor = f;
+                for (uint32_t u = 0; u < kUnits; ++u) {
+                    const uint32_t unit = u * 4u + lane % 4u;
+                    const float(&z)[8] = y[n][u];
+                    sts128(dst + (unit / 8u) * 16384u + (((unit % 8u) ^ (tile_row & 7u)) << 4), pack_half(z[0] * up, z[4] * up),
+                           pack_half(z[1] * up, z[5] * up), pack_half(z[2] * up, z[6] * up), pack_half(z[3] * up, z[7] * up));
                 }
-                const uint32_t dst = q32 + i * (128u * D * 2u) + (c8 / 8u) * 16384u + tile_row * 128u + (((c8 % 8u) ^ (tile_row & 7u)) << 4);
-                sts128(dst, pack_half(y[n][0] * up, y[n][4] * up), pack_half(y[n][1] * up, y[n][5] * up),
-                       pack_half(y[n][2] * up, y[n][6] * up), pack_half(y[n][3] * up, y[n][7] * up));
             }
         }
         fence_proxy_async_smem();
