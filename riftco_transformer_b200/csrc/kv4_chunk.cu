@@ -80,6 +80,8 @@ struct Barriers {
     // scores it has seen were issued after it), so that a parity tells; at the end only two before that is known.
     uint64_t o_done[2], o_full[2];
     uint64_t q_full[2];   // a tile's rows of Q are staged
+    uint64_t pair_full;   // paired: the second tile's maxima and sums are in `pair`
+    float2 pair[128];
     uint32_t tmem_base;
     uint32_t abort;
 };
@@ -380,7 +382,12 @@ __device__ __forceinline__ void cap_scores(uint32_t (&x)[64], float f, float cap
     }
 }
 
-template <int D>
+// The softmax loop's speed hangs on what else the kernel holds, so forms that a launch can tell apart are kernels of their
+// own. PAIRED (see below): in one kernel what joins the tiles made a prompt a tenth slower (191 us against 171 before
+// and 166 apart). RULES: score caps or distance biases; without their code drafted tokens take 33 instead of 35 us and
+// heads of 256 36 instead of 39. Unpaired tiles of smaller heads have the one form with it: that loop, as compiled, is the
+// faster one for plain scores too (163 us; without that code 182, or 173 with no turns).
+template <int D, bool PAIRED, bool RULES>
 __global__ void __launch_bounds__(kThreads, 1)
 kv4_chunk_kernel(const Kv4AttentionArgs a, float* __restrict__ partials, const ChunkPlan plan) {
     using L = Layout<D>;
@@ -411,12 +418,12 @@ kv4_chunk_kernel(const Kv4AttentionArgs a, float* __restrict__ partials, const C
     const uint32_t n_blocks = min(plan.blocks_per_split, blocks - block0);   // 0 where nothing is seen
     const uint32_t first_tile = tile0 + block0 * kBlockTiles;
     const uint32_t end_tile = min(tile0 + tiles, first_tile + n_blocks * kBlockTiles);
-    // Row tiles at work. Paired, both hold the same rows, tile i of them blocks i, i + 2, ..., as two partial results:
-    // a tile's chain of products and softmax is twice as long as its share of either unit, and with one tile nothing else
+    // Row tiles at work. Paired, both hold the same rows, tile i of them blocks i, i + 2, ..., joined at the end: a tile's
+    // chain of products and softmax is twice as long as its share of either unit, and with one tile nothing else
     // would run beside it.
-    const bool paired = plan.paired != 0u;
-    const uint32_t n_tiles = paired || rows > 128u ? 2u : 1u, step = paired ? 2u : 1u;
-    const uint32_t parts_per_split = step;
+    constexpr bool paired = PAIRED;
+    constexpr uint32_t step = paired ? 2u : 1u;
+    const uint32_t n_tiles = paired || rows > 128u ? 2u : 1u;
 
     const uint32_t smem32 = (smem_u32(smem_raw) + 1023u) & ~1023u;
     const uint32_t q32 = smem32, k32 = q32 + L::kQ, v32 = k32 + kStages * L::kKStage, raw32 = v32 + kStages * L::kVStage;
@@ -445,6 +452,7 @@ kv4_chunk_kernel(const Kv4AttentionArgs a, float* __restrict__ partials, const C
                 mbar_init(&bars.o_full[i], 1);
                 mbar_init(&bars.q_full[i], 4);
             }
+            mbar_init(&bars.pair_full, 4);
             bars.abort = 0;
             mbar_fence_init();
         }
@@ -596,7 +604,7 @@ kv4_chunk_kernel(const Kv4AttentionArgs a, float* __restrict__ partials, const C
         // every row of the warp sees tokens [all_begin, all_end); rows that are not live do not count
         const uint32_t all_begin = __reduce_max_sync(0xFFFFFFFFu, live ? begin : 0u);
         const uint32_t all_end = __reduce_min_sync(0xFFFFFFFFu, live ? end : 0xFFFFFFFFu);
-        const bool capped = a.rules.softcap != 0.0f, biased = a.rules.alibi_slopes != nullptr;
+        const bool capped = RULES && a.rules.softcap != 0.0f, biased = RULES && a.rules.alibi_slopes != nullptr;
         const float cap_log2 = a.rules.softcap * kLog2e;
         const float slope = biased && live ? __ldg(a.rules.alibi_slopes + kvh * rep + gr % rep) * kLog2e : 0.0f;
         // Q: scaled to a largest magnitude in [2^9, 2^10) per row, fp16, in the order the codes come out. A warp stages
@@ -724,7 +732,7 @@ kv4_chunk_kernel(const Kv4AttentionArgs a, float* __restrict__ partials, const C
 
         const uint32_t first_block = paired ? i : 0u;
         const uint32_t mine = n_blocks > first_block ? (n_blocks - first_block + step - 1u) / step : 0u;   // the tile's blocks
-        const uint32_t others = paired ? n_blocks - mine : n_blocks;   // the other tile's
+        const bool turns = !PAIRED && n_tiles == 2u;
         for (uint32_t n = 0; n < mine; ++n) {
             const uint32_t token0 = (first_tile + (first_block + n * step) * kBlockTiles) * kKv4Tile;
             const uint32_t buffer = lane_base + (n & 1u) * kBlock;
@@ -783,10 +791,11 @@ kv4_chunk_kernel(const Kv4AttentionArgs a, float* __restrict__ partials, const C
                 top = fmaxf(fmaxf(top4[0], top4[1]), fmaxf(top4[2], top4[3])) * factor;
             };
             // The warps of the two tiles that share a scheduler take turns with their exponentials, so that one's run under
-            // the other's loads and stores instead of both at half speed.
-            if (n_tiles == 2u) turn_wait(2u + (warp % 4u) * 2u + i, i == 0u && n == 0u);
+            // the other's loads and stores instead of both at half speed (a 4096-token prompt 163 us, 173 without; tiles of
+            // the same rows, whose blocks come in turn anyway, lose 2 of 33 to it).
+            if (turns) turn_wait(2u + (warp % 4u) * 2u + i, i == 0u && n == 0u);
             weigh();
-            if (n_tiles == 2u && (i == 0u ? n < others : n + 1u < others)) turn_pass(2u + (warp % 4u) * 2u + (i ^ 1u));
+            if (turns && (i == 0u || n + 1u < mine)) turn_pass(2u + (warp % 4u) * 2u + (i ^ 1u));
             if (__any_sync(0xFFFFFFFFu, top > m + kSlack)) {
                 const float moved = fmaxf(m, top);
                 const float shrink = ex2(m - moved);
@@ -816,61 +825,90 @@ kv4_chunk_kernel(const Kv4AttentionArgs a, float* __restrict__ partials, const C
 
         // ---- epilogue ----
         if (live && isnan(l)) flags |= B2_ATTN_STATUS_NAN_OR_POS_INF;
-        if (mine != 0u) {
-            mbar_wait(&bars.o_full[i], 0u, abort);
-            tcgen05_fence_after_sync();
-        } else {
-            mbar_wait(&bars.q_full[i], 0u, abort);   // the other warps' staging, which the rows below are written over
-        }
-        if (lane == 0 && *abort != 0) flags |= B2_ATTN_STATUS_TIMEOUT;
-        const uint64_t out_head = static_cast<uint64_t>(span.first + my_out) * a.q_heads + kvh * rep + my_head;
-        const bool whole = n_splits * parts_per_split == 1u;
-        if (whole && live && l == 0.0f && end > begin) flags |= B2_ATTN_STATUS_ALL_NEG_INF;
-        float* part = partials + ((out_head * plan.splits + split) * parts_per_split + (paired ? i : 0u)) * (D + 4u);
-        if (!whole && live) *reinterpret_cast<float2*>(part) = make_float2(m, l);
-        const float inv = whole ? (l == 0.0f ? 0.0f : 1.0f / l) : 1.0f;
-        // The tile's Q (heads of 256: the keys' stages) is not needed any more: 2 D bytes a row take the warp's bf16 rows, so
-        // that they leave in whole rows instead of 16 bytes of 32 different ones.
-        static_assert(L::kQ + kStages * L::kKStage >= kRows * D * 2u, "room for the rows");
-        const uint32_t stage32 = q32 + i * (128u * D * 2u) + (warp % 4u) * (32u * D * 2u);
-#pragma unroll 1
-        for (uint32_t c = 0; c < D / 32u; ++c) {
-            uint32_t o[32];
-            if (mine != 0u) {
-                tmem_ld_32(lane_base + kTmemO + c * 32u, o);
-                tmem_ld_ready(o);
-            }
-#pragma unroll
-            for (int e = 0; e < 32; ++e) o[e] = l == 0.0f ? 0u : __float_as_uint(__uint_as_float(o[e]) * inv);
-            if (whole) {
-#pragma unroll
-                for (uint32_t e = 0; e < 4u; ++e) {
-                    uint32_t w[4];
-#pragma unroll
-                    for (uint32_t k = 0; k < 4u; ++k) {
-                        const __nv_bfloat162 b = __floats2bfloat162_rn(__uint_as_float(o[8 * e + 2 * k]), __uint_as_float(o[8 * e + 2 * k + 1]));
-                        w[k] = *reinterpret_cast<const uint32_t*>(&b);
-                    }
-                    sts128(stage32 + lane * (D * 2u) + (((c * 4u + e) ^ (lane & 7u)) << 4), w[0], w[1], w[2], w[3]);
-                }
-            } else if (live) {
-                float4* dst = reinterpret_cast<float4*>(part + 4u + c * 32u);
-#pragma unroll
-                for (int e = 0; e < 8; ++e) {
-                    dst[e] = make_float4(__uint_as_float(o[4 * e]), __uint_as_float(o[4 * e + 1]), __uint_as_float(o[4 * e + 2]),
-                                         __uint_as_float(o[4 * e + 3]));
-                }
-            }
-        }
-        if (whole) {
+        if (paired && i == 1u) {   // the first tile's warps join both: they reach the same lanes of tensor memory
+            bars.pair[r] = make_float2(m, l);
             __syncwarp();
+            if (lane == 0) mbar_arrive(&bars.pair_full);
+        } else {
+            const bool both = paired && n_blocks > 1u;   // the second tile had blocks
+            float keep = 1.0f, other = 0.0f;             // factors of the tiles' sums
+            if (mine != 0u) {
+                mbar_wait(&bars.o_full[i], 0u, abort);
+                if (both) {
+                    mbar_wait(&bars.o_full[1], 0u, abort);
+                    mbar_wait(&bars.pair_full, 0u, abort);
+                    const float2 its = bars.pair[r];
+                    const float top = fmaxf(m, its.x);
+                    keep = ex2(m - top);
+                    other = ex2(its.x - top);
+                    m = top;
+                    l = l * keep + its.y * other;
+                }
+                tcgen05_fence_after_sync();
+            } else {
+                mbar_wait(&bars.q_full[i], 0u, abort);   // the other warps' staging, which the rows below are written over
+            }
+            if (lane == 0 && *abort != 0) flags |= B2_ATTN_STATUS_TIMEOUT;
+            const uint64_t out_head = static_cast<uint64_t>(span.first + my_out) * a.q_heads + kvh * rep + my_head;
+            const bool whole = n_splits == 1u;
+            if (whole && live && l == 0.0f && end > begin) flags |= B2_ATTN_STATUS_ALL_NEG_INF;
+            float* part = partials + (out_head * plan.splits + split) * (D + 4u);
+            if (!whole && live) *reinterpret_cast<float2*>(part) = make_float2(m, l);
+            const float inv = whole ? (l == 0.0f ? 0.0f : 1.0f / l) : 1.0f;
+            keep *= inv;
+            other *= inv;
+            // The tile's Q (heads of 256: the keys' stages) is not needed any more: 2 D bytes a row take the warp's bf16 rows, so
+            // that they leave in whole rows instead of 16 bytes of 32 different ones.
+            static_assert(L::kQ + kStages * L::kKStage >= kRows * D * 2u, "room for the rows");
+            const uint32_t stage32 = q32 + i * (128u * D * 2u) + (warp % 4u) * (32u * D * 2u);
+#pragma unroll 1
+            for (uint32_t c = 0; c < D / 32u; ++c) {
+                uint32_t o[32];
+                if (mine != 0u) {
+                    tmem_ld_32(lane_base + kTmemO + c * 32u, o);
+                    tmem_ld_ready(o);
+                }
+#pragma unroll
+                for (int e = 0; e < 32; ++e) o[e] = l == 0.0f ? 0u : __float_as_uint(__uint_as_float(o[e]) * keep);
+                if (both) {
+                    uint32_t its[32];
+                    tmem_ld_32(lane_base + kTmemTile + kTmemO + c * 32u, its);
+                    tmem_ld_ready(its);
+#pragma unroll
+                    for (int e = 0; e < 32; ++e) {
+                        o[e] = l == 0.0f ? 0u : __float_as_uint(fmaf(__uint_as_float(its[e]), other, __uint_as_float(o[e])));
+                    }
+                }
+                if (whole) {
+#pragma unroll
+                    for (uint32_t e = 0; e < 4u; ++e) {
+                        uint32_t w[4];
+#pragma unroll
+                        for (uint32_t k = 0; k < 4u; ++k) {
+                            const __nv_bfloat162 b = __floats2bfloat162_rn(__uint_as_float(o[8 * e + 2 * k]), __uint_as_float(o[8 * e + 2 * k + 1]));
+                            w[k] = *reinterpret_cast<const uint32_t*>(&b);
+                        }
+                        sts128(stage32 + lane * (D * 2u) + (((c * 4u + e) ^ (lane & 7u)) << 4), w[0], w[1], w[2], w[3]);
+                    }
+                } else if (live) {
+                    float4* dst = reinterpret_cast<float4*>(part + 4u + c * 32u);
+#pragma unroll
+                    for (int e = 0; e < 8; ++e) {
+                        dst[e] = make_float4(__uint_as_float(o[4 * e]), __uint_as_float(o[4 * e + 1]), __uint_as_float(o[4 * e + 2]),
+                                             __uint_as_float(o[4 * e + 3]));
+                    }
+                }
+            }
+            if (whole) {
+                __syncwarp();
 #pragma unroll 4
-            for (uint32_t n = 0; n < kSteps; ++n) {
-                const uint32_t which = n * kRowsAtOnce + lane / kChannels8;
-                const uint64_t head = __shfl_sync(0xFFFFFFFFu, out_head, which);
-                const uint4 v = lds128(stage32 + which * (D * 2u) + ((c8 ^ (which & 7u)) << 4));
-                if (warp_row + which < rows) {
-                    reinterpret_cast<uint4*>(static_cast<__nv_bfloat16*>(a.ctx16) + head * D)[c8] = v;
+                for (uint32_t n = 0; n < kSteps; ++n) {
+                    const uint32_t which = n * kRowsAtOnce + lane / kChannels8;
+                    const uint64_t head = __shfl_sync(0xFFFFFFFFu, out_head, which);
+                    const uint4 v = lds128(stage32 + which * (D * 2u) + ((c8 ^ (which & 7u)) << 4));
+                    if (warp_row + which < rows) {
+                        reinterpret_cast<uint4*>(static_cast<__nv_bfloat16*>(a.ctx16) + head * D)[c8] = v;
+                    }
                 }
             }
         }
@@ -903,11 +941,10 @@ kv4_chunk_merge_kernel(const Kv4AttentionArgs a, const float* __restrict__ parti
         }
     }
     pdl_wait();   // every CTA waits, so that this grid never ends before the one it follows
-    const uint32_t each = plan.paired != 0u ? 2u : 1u, n = max(n_splits, 1u) * each;   // where nothing is seen one split says so
-    if (!ours || n <= 1u) return;
-    const float* first = partials + out_head * plan.splits * each * (D + 4u);
+    if (!ours || n_splits <= 1u) return;
+    const float* first = partials + out_head * plan.splits * (D + 4u);
     const uint32_t c = threadIdx.x * 4u;
-    finish<D>(a, join_run(first, first + (D + 4u), D + 4u, n, c), out_head, c, mine.end > mine.begin);
+    finish<D>(a, join_run(first, first + (D + 4u), D + 4u, n_splits, c), out_head, c, mine.end > mine.begin);
 }
 
 // One CTA holds an SM. Where the row tiles are fewer than the SMs, the blocks of each are split over as many CTAs as
@@ -936,23 +973,21 @@ ChunkPlan chunk_plan(int sm_count, uint32_t n_seq, uint32_t q_heads, uint32_t kv
     return ChunkPlan{static_cast<uint32_t>(row_tiles), rows_of(head_width) == 256u && max_chunk * rep <= 128u ? 1u : 0u,
                      static_cast<uint32_t>((blocks + per - 1u) / per), static_cast<uint32_t>(per)};
 }
-// Partial results of a row: of a split one, or where its tiles are paired two.
-uint32_t parts_of(const ChunkPlan& plan) { return plan.splits * (plan.paired != 0u ? 2u : 1u); }
 
-template <int D>
+template <int D, bool PAIRED, bool RULES>
 int32_t launch_one(const DeviceContext& ctx, const Kv4AttentionArgs& a, float* partials, const ChunkPlan& plan,
                    cudaStream_t stream) {
     static PerDeviceOnce configured;
     B2_TRY(once_per_device(configured, ctx.device, []() -> int32_t {
-        B2_CUDA_TRY(cudaFuncSetAttribute(kv4_chunk_kernel<D>, cudaFuncAttributeMaxDynamicSharedMemorySize, Layout<D>::kTotal));
+        B2_CUDA_TRY(cudaFuncSetAttribute(kv4_chunk_kernel<D, PAIRED, RULES>, cudaFuncAttributeMaxDynamicSharedMemorySize, Layout<D>::kTotal));
         return B2_STATUS_OK;
     }));
     const uint64_t ctas = static_cast<uint64_t>(plan.row_tiles) * a.cache.n_seq * a.cache.kv_heads * plan.splits;
     const uint64_t merges = static_cast<uint64_t>(a.rows) * a.q_heads;
     if (ctas > 0x7FFFFFFFull || merges > 0x7FFFFFFFull) return fail(B2_STATUS_OVERFLOW, "paged attention batch too large");
-    kv4_chunk_kernel<D><<<static_cast<unsigned>(ctas), kThreads, Layout<D>::kTotal, stream>>>(a, partials, plan);
+    kv4_chunk_kernel<D, PAIRED, RULES><<<static_cast<unsigned>(ctas), kThreads, Layout<D>::kTotal, stream>>>(a, partials, plan);
     B2_CUDA_TRY(cudaGetLastError());
-    if (parts_of(plan) <= 1u) return B2_STATUS_OK;
+    if (plan.splits <= 1u) return B2_STATUS_OK;
     cudaLaunchConfig_t config{};
     config.gridDim = dim3(static_cast<unsigned>(merges));
     config.blockDim = dim3(D / 4);
@@ -964,6 +999,17 @@ int32_t launch_one(const DeviceContext& ctx, const Kv4AttentionArgs& a, float* p
     config.numAttrs = 1;
     B2_CUDA_TRY(cudaLaunchKernelEx(&config, kv4_chunk_merge_kernel<D>, a, const_cast<const float*>(partials), plan));
     return B2_STATUS_OK;
+}
+
+template <int D>
+int32_t launch_form(const DeviceContext& ctx, const Kv4AttentionArgs& a, float* partials, const ChunkPlan& plan, cudaStream_t stream) {
+    const bool rules = a.rules.softcap != 0.0f || a.rules.alibi_slopes != nullptr;
+    if constexpr (D == 256) {
+        return rules ? launch_one<D, false, true>(ctx, a, partials, plan, stream) : launch_one<D, false, false>(ctx, a, partials, plan, stream);
+    } else {
+        if (plan.paired == 0u) return launch_one<D, false, true>(ctx, a, partials, plan, stream);
+        return rules ? launch_one<D, true, true>(ctx, a, partials, plan, stream) : launch_one<D, true, false>(ctx, a, partials, plan, stream);
+    }
 }
 
 }  // namespace
@@ -984,8 +1030,8 @@ bool kv4_chunk_pays(uint32_t n_seq, uint64_t rows, uint32_t q_heads, uint32_t kv
 size_t kv4_chunk_workspace_bytes(int sm_count, uint32_t n_seq, uint64_t rows, uint32_t q_heads, uint32_t kv_heads,
                                  uint32_t head_width, uint32_t max_chunk, uint32_t max_seq_len) {
     const ChunkPlan plan = chunk_plan(sm_count, n_seq, q_heads, kv_heads, head_width, max_chunk, max_seq_len);
-    if (parts_of(plan) <= 1u) return 0;
-    return static_cast<size_t>(rows) * q_heads * parts_of(plan) * (head_width + 4u) * sizeof(float);
+    if (plan.splits <= 1u) return 0;
+    return static_cast<size_t>(rows) * q_heads * plan.splits * (head_width + 4u) * sizeof(float);
 }
 
 int32_t launch_kv4_chunk(const DeviceContext& ctx, const Kv4AttentionArgs& a, void* workspace, size_t workspace_bytes,
@@ -1000,9 +1046,9 @@ int32_t launch_kv4_chunk(const DeviceContext& ctx, const Kv4AttentionArgs& a, vo
                                       a.max_seq_len);
     float* partials = static_cast<float*>(workspace);
     switch (a.cache.head_width) {
-        case 64u: return launch_one<64>(ctx, a, partials, plan, stream);
-        case 128u: return launch_one<128>(ctx, a, partials, plan, stream);
-        default: return launch_one<256>(ctx, a, partials, plan, stream);
+        case 64u: return launch_form<64>(ctx, a, partials, plan, stream);
+        case 128u: return launch_form<128>(ctx, a, partials, plan, stream);
+        default: return launch_form<256>(ctx, a, partials, plan, stream);
     }
 }
 
