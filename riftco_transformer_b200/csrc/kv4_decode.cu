@@ -142,7 +142,8 @@ constexpr uint32_t kMaxRows = 1024;   // rows a CTA finds its range among
 constexpr uint32_t kMinPairs = 8;     // pairs of a range: below two a warp a CTA is mostly set-up
 // Pairs of a range (were all rows of full length) from which there are more ranges than the card holds at once. More
 // ranges shorten the time in which an SM's last warps run alone, and cost set-up: 64 sequences of 512 to 8192 tokens take
-// 119, 107, 104, 103 and 106 us with at most 32, 64, 96, 160 and any number of pairs, others are fastest from 160 on.
+// 119, 107, 104, 103 and 106 us (96 now, at 160) with at most 32, 64, 96, 160 and any number of pairs, others are fastest
+// from 160 on.
 constexpr uint32_t kMostPairs = 160;
 struct WorkPlan {
     uint32_t ctas;
