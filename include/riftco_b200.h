@@ -396,7 +396,7 @@ B2_API int32_t b2_paged_decode_attention_kv4(const b2_kv4_cache* cache, const b2
  * (b2_nf4_linear_forward_multi_bf16). Rows behind chunk_starts[n_seq] are left as
  * they were; a chunk longer than its sequence is flagged BAD_BLOCK and the
  * tokens that would lie before position 0 get zeros; one longer than max_chunk is
- * flagged and its tokens from max_chunk on may be left as they were. Calls of four
+ * flagged and its tokens from max_chunk on may be left as they were. Calls of three
  * and more tokens a sequence that are not very small run as tiles of rows, in fp16 on
  * the tcgen05 tensor cores (q, k, v and the weights are rounded to 2^-12), others
  * token by token as in the decode form; b2_last_route tells. Other errors and the

@@ -1015,16 +1015,17 @@ int32_t launch_form(const DeviceContext& ctx, const Kv4AttentionArgs& a, float* 
 }  // namespace
 
 // Row by row every token's lists (kv4_decode.cu) read all it sees, as tiles a sequence's tokens read it together. 16
-// sequences at 2000 tokens, 8 K/V heads of 128: 34, 44, 77 and 138 us row by row for 2, 4, 8 and 16 new tokens, 38 to 40 as
-// tiles; heads of 64 28, 36, 56 and 101 against 36, heads of 256 46, 73, 137 and 242 against 51 to 55. So from four lists
-// a sequence and head on. But a call of tiles takes 15 to 25 us however small it is, and row by row 10 to 12 and what
-// its lists (of 32 tokens a step; each costs eleven steps to begin and end) add: 4 x 16 tokens after 100 (7700
-// steps) take 14 against 20 us, 16 x 16 after nothing (24600) 28 against 20, 1 x 16 after 3000 (13600) 28 against 23.
+// sequences at 2000 tokens, 8 query and K/V heads of 128: 34, 40, 44, 77 and 138 us row by row for 2, 3, 4, 8 and 16 new
+// tokens, 34 to 36 as tiles; heads of 64 26, 31, 36, 56 and 101 against 30 to 32, heads of 256 47, 63, 73, 137 and 242
+// against 48 to 55. So from three lists a sequence and K/V head on. But a call of tiles takes 12 to 23 us however small
+// it is, and row by row 10 to 12 and what its lists (of 32 tokens a step; each costs eleven steps to begin and end) add.
+// Over 216 calls of 1 to 64 sequences, 2 to 16 new tokens and up to 8000 cached ones tiles from 6000 steps on give the
+// shortest times (geometric mean 23.4 us; from 0 or from 12000 on 23.8, never 26).
 bool kv4_chunk_pays(uint32_t n_seq, uint64_t rows, uint32_t q_heads, uint32_t kv_heads, uint32_t max_chunk, uint32_t max_seq_len) {
     const uint64_t rep = q_heads / kv_heads, chunks = (rep + 7u) / 8u;
     if (max_chunk * rep > 0x7FFFFF00u) return false;
     const double lists = static_cast<double>(rows) * static_cast<double>(chunks);   // of a K/V head
-    return lists >= 4.0 * n_seq && lists * kv_heads * (max_seq_len / 32u + 12u) >= 12000.0;
+    return lists >= 3.0 * n_seq && lists * kv_heads * (max_seq_len / 32u + 12u) >= 6000.0;
 }
 
 size_t kv4_chunk_workspace_bytes(int sm_count, uint32_t n_seq, uint64_t rows, uint32_t q_heads, uint32_t kv_heads,

@@ -73,7 +73,7 @@ def chunk(case, new, max_len=None, extra_rows=0, tiles=True, max_chunk=None, **r
     rows = case.q.shape[0]
     q = case.q
     if tiles:
-        q = np.concatenate((q, np.full((max(12000 // (11 * pool.kv_heads), 4 * len(new)), *q.shape[1:]), np.nan, np.float32)))
+        q = np.concatenate((q, np.full((max(6000 // (11 * pool.kv_heads), 3 * len(new)), *q.shape[1:]), np.nan, np.float32)))
     ctx, check = guarded_bf16(q.shape)
     ctx.fill_(7.0)
     status = status_word()
@@ -445,11 +445,11 @@ def test_chunk_score_rules(rules, new, past, d, tiles):
 
 
 @pytest.mark.parametrize("d,hq,hkv,new,past,route", [
-    (128, 8, 8, [3] * 4, 4000, "attention_kv4"), (128, 8, 8, [4] * 4, 4000, "attention_kv4_tiles"),
+    (128, 8, 8, [2] * 4, 4000, "attention_kv4"), (128, 8, 8, [3] * 4, 4000, "attention_kv4_tiles"),
     (256, 8, 8, [1, 1, 1, 13], 4000, "attention_kv4_tiles"), (64, 96, 8, [2] * 4, 6000, "attention_kv4_tiles"),
     (64, 8, 2, [40, 20], 100, "attention_kv4"), (64, 2, 2, [129, 640], 30, "attention_kv4_tiles")])
 def test_chunk_routes(d, hq, hkv, new, past, route):
-    """Tiles from four lists a sequence on, and not for very little work."""
+    """Tiles from three lists a sequence on, and not for very little work."""
     import riftco_transformer_b200 as b2
     case = kv4_cases.Case(9, [m + past for m in new], hq, hkv, d, 16, rows=sum(new))
     got, status = chunk(case, new, tiles=False)
