@@ -791,8 +791,8 @@ kv4_chunk_kernel(const Kv4AttentionArgs a, float* __restrict__ partials, const C
                 top = fmaxf(fmaxf(top4[0], top4[1]), fmaxf(top4[2], top4[3])) * factor;
             };
             // The warps of the two tiles that share a scheduler take turns with their exponentials, so that one's run under
-            // the other's loads and stores instead of both at half speed (a 4096-token prompt 163 us, 173 without; tiles of
-            // the same rows, whose blocks come in turn anyway, lose 2 of 33 to it).
+            // the other's loads and stores instead of both at half speed (four capped chunks of 300 to 700 tokens 118 us, 124
+            // without; tiles of the same rows, whose blocks come in turn anyway, lose 1 of 40 to it).
             if (turns) turn_wait(2u + (warp % 4u) * 2u + i, i == 0u && n == 0u);
             weigh();
             if (turns && (i == 0u || n + 1u < mine)) turn_pass(2u + (warp % 4u) * 2u + (i ^ 1u));
@@ -1020,7 +1020,7 @@ int32_t launch_form(const DeviceContext& ctx, const Kv4AttentionArgs& a, float* 
 // against 48 to 55. So from three lists a sequence and K/V head on. But a call of tiles takes 12 to 23 us however small
 // it is, and row by row 10 to 12 and what its lists (of 32 tokens a step; each costs eleven steps to begin and end) add.
 // Over 216 calls of 1 to 64 sequences, 2 to 16 new tokens and up to 8000 cached ones tiles from 6000 steps on give the
-// shortest times (geometric mean 23.4 us; from 0 or from 12000 on 23.8, never 26).
+// shortest times (geometric mean 23.4 us; from 0 or 12000 on 23.8, never 28.6).
 bool kv4_chunk_pays(uint32_t n_seq, uint64_t rows, uint32_t q_heads, uint32_t kv_heads, uint32_t max_chunk, uint32_t max_seq_len) {
     const uint64_t rep = q_heads / kv_heads, chunks = (rep + 7u) / 8u;
     if (max_chunk * rep > 0x7FFFFF00u) return false;

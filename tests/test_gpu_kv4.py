@@ -479,25 +479,26 @@ def test_chunk_scores_near_and_beyond_the_cap():
         assert rel_l2(got, case.chunk([90], softcap=cap)) <= tol
 
 
+@pytest.mark.parametrize("new,at,window", [(100, 90, 20), (20, 137, 5)])
 @pytest.mark.parametrize("d", [128, 256])
-def test_chunk_of_values_that_are_not_finite(d):
-    """A NaN group makes the context NaN for the rows that see its token, and for no other."""
+def test_chunk_of_values_that_are_not_finite(d, new, at, window):
+    """A NaN group of token `at` makes the context NaN for the rows that see it, and for no other."""
     from riftco_transformer_b200 import _lib
+    position = np.arange(150 - new, 150)
     for half in (0, 9 * d):   # keys, values
-        case = kv4_cases.Case(17, [150], 4, 1, d, 16, rows=100)
-        at = 90                  # the token
+        case = kv4_cases.Case(17, [150], 4, 1, d, 16, rows=new)
         tile = case.pages[case.tables[0, at // 16], 0, 0]
         tile[half + 8 * d:half + 9 * d].reshape(16, -1)[at % 16] = 0xFF
-        got, status = chunk(case, [100])
+        got, status = chunk(case, [new])
         assert status == _lib.ATTN_STATUS_NAN_OR_POS_INF
-        sees = np.arange(50, 150) >= at
+        sees = position >= at
         assert np.isnan(got[sees]).all()
-        assert rel_l2(got[~sees], case.chunk([100])[~sees]) <= BF16_TOL
+        assert rel_l2(got[~sees], case.chunk([new])[~sees]) <= BF16_TOL
         # rows whose window has passed the token do not see it either
-        got, status = chunk(case, [100], window=20)
-        sees = (np.arange(50, 150) >= at) & (np.arange(50, 150) < at + 20)
+        got, status = chunk(case, [new], window=window)
+        sees = (position >= at) & (position < at + window)
         assert np.isnan(got[sees]).all()
-        assert rel_l2(got[~sees], case.chunk([100], window=20)[~sees]) <= BF16_TOL
+        assert rel_l2(got[~sees], case.chunk([new], window=window)[~sees]) <= BF16_TOL
 
 
 def test_chunk_leaves_rows_behind_the_last_sequence():
