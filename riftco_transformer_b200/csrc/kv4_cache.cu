@@ -115,14 +115,14 @@ __device__ __forceinline__ void store_vector(const float4& lo, const float4& hi,
     }
 }
 
-constexpr uint32_t kMostTokens = 8;   // of a CTA
+constexpr uint32_t kMostTokens = 16;   // of a CTA
 
 // Grid (token run, slice). A CTA takes `per_cta` consecutive tokens and, of each, every gridDim.y-th group of its lanes'
 // head vectors: q heads are rotated, k heads rotated and stored, v heads stored. The angles of a token are the same for
 // all its heads: they are worked out once, into shared memory (in double: position * theta^(-2c/D) passes 10^5
 // radians in long contexts, where FP32 has lost the phase). A prompt is bound by HBM (24.6 KB of q, k and v in, 16.4 KB
 // of q and 1.2 KB of pages out per token at 32 / 8 heads of 128): 16-byte accesses, no barrier between the vectors of a
-// run, and the loads of the next two under way while one is worked on: 8191 tokens take 73 us (4.7 TB/s), 85 us with one
+// run, and the loads of the next two under way while one is worked on: 8191 tokens take 72 us (4.8 TB/s), 85 us with one
 // vector ahead and a barrier per token. A single token, 6 us, is bound by the latency of its angle.
 template <int D>
 __global__ void __launch_bounds__(kAppendWarps * 32, 4)
@@ -219,7 +219,7 @@ kv4_append_kernel(const Kv4AppendArgs a, uint32_t per_cta) {
 }
 
 // D / 4 threads read one stored vector back, four channels each: 2 bytes of codes and a pair in, 16 bytes out, so that
-// a warp writes 512 bytes in a row.
+// a warp writes 512 bytes in a row. Bound by what HBM takes in: 16000 tokens of 8 heads of 128, 131 MB out, 42 us.
 template <int D>
 __global__ void __launch_bounds__(256) kv4_read_kernel(const Kv4ReadArgs a) {
     constexpr uint32_t kThreads = D / 4, kVectors = 256u / kThreads;
@@ -262,9 +262,10 @@ int32_t launch_kv4_append(const DeviceContext& ctx, const Kv4AppendArgs& a, cuda
     const uint32_t sms = ctx.sm_count > 0 ? static_cast<uint32_t>(ctx.sm_count) : 148u;
     const uint32_t vectors = kAppendWarps * 256u / a.cache.head_width;   // a CTA's at once
     // Few tokens: all vectors at once, spread over CTAs (each repeats the token's angles). Many: one CTA per run of
-    // tokens, so that theta^(-2c/d) is worked out once for the run.
+    // tokens, so that theta^(-2c/d) is worked out once for the run, as many as the card holds (2048 tokens 28 us, 30 with
+    // twice as many, 33 with four times).
     uint32_t slices = (heads + vectors - 1u) / vectors;
-    const uint64_t wanted = 8ull * sms;
+    const uint64_t wanted = 4ull * sms;   // what the card holds at once
     while (slices > 1u && static_cast<uint64_t>(a.n_tokens) * slices > wanted) slices = (slices + 1u) / 2u;
     uint32_t per_cta = 1u;
     if (slices == 1u) per_cta = static_cast<uint32_t>((a.n_tokens + wanted - 1u) / wanted);

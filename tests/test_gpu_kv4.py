@@ -103,7 +103,8 @@ def append(pages, tables, q, k, v, positions, token_seq, bs, theta=1e4, in_place
 
 
 @pytest.mark.parametrize("d", [64, 128, 256])
-@pytest.mark.parametrize("hq,hkv,bs,tokens", [(2, 2, 16, 1), (8, 2, 32, 7), (5, 5, 48, 33), (32, 8, 64, 300)])
+@pytest.mark.parametrize("hq,hkv,bs,tokens", [(2, 2, 16, 1), (8, 2, 32, 7), (5, 5, 48, 33), (32, 8, 64, 300),
+                                              (1, 1, 16, 9500)])
 def test_append_stores_the_defined_bytes(d, hq, hkv, bs, tokens):
     """q's first kv_heads heads carry the same data as k, so q_out is the rotated k the cache has to
     hold: its bytes are then exact whatever the last bit of a sine."""
