@@ -162,9 +162,11 @@ __device__ __forceinline__ uint32_t row_pairs(const RowSpan& span) {
     const uint32_t tiles = (span.end - 1u) / kKv4Tile + 1u - span.begin / kKv4Tile;
     return (tiles + kPair - 1u) / kPair;
 }
-// CTAs that share `total` pairs, the first pair of CTA c, and the last CTA whose range begins at or before a pair.
+// CTAs that share `total` pairs, the first pair of CTA c, and the last CTA whose range begins at or before a pair. Never
+// more CTAs than pairs: `lists` counts rows that are nobody's too, which have no pairs, and a CTA with an empty range
+// between a list's first and last would leave a partial result unwritten that the join reads.
 __device__ __forceinline__ uint32_t live_ctas(const WorkPlan& plan, uint32_t lists, uint32_t total) {
-    return min(plan.ctas, max(lists, (total + kMinPairs - 1u) / kMinPairs));
+    return min(plan.ctas, max(min(lists, total), (total + kMinPairs - 1u) / kMinPairs));
 }
 __device__ __forceinline__ uint32_t first_pair(uint32_t c, uint32_t total, uint32_t ctas) {
     return static_cast<uint32_t>(static_cast<uint64_t>(c) * total / ctas);

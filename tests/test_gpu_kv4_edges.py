@@ -1,0 +1,125 @@
+"""The 4-bit paged K/V cache on the GPU at the edges of what its calls allow: rows and tokens that are nobody's,
+groups whose stored scale is negative, weights far below the largest, queries and bounds of any size.
+
+Tolerances. FP32 contexts and those of the tile kernel as in test_gpu_kv4.py (F32_TOL, BF16_TOL, derived there); a context
+of the row-by-row form is the FP32 one rounded to bf16, half a step of which is 2^-8 of a value: ROW_TOL. Where a test has
+another bound its derivation stands beside it."""
+import ctypes as C
+
+import numpy as np
+import pytest
+import torch
+
+import kv4_cases
+from conftest import rel_l2
+from test_gpu_kv4 import BF16_TOL, F32_TOL, chunk, cuda, decode, guarded_bf16, status_word
+
+pytestmark = pytest.mark.gpu
+
+ROW_TOL = 2.0 ** -8 + F32_TOL
+
+
+class Held(kv4_cases.Case):
+    """A cache that holds given keys and values, [kv_heads, tokens, d] of each sequence, on pages in order."""
+
+    def __init__(self, q, k, v, bs=16):
+        self.hq, (self.hkv, _, self.d), self.bs = q.shape[1], k[0].shape, bs
+        self.q, self.lens = np.asarray(q, np.float32), [x.shape[1] for x in k]
+        need = [-(-n // bs) for n in self.lens]
+        self.tables = np.full((len(k), max(need)), 0xFFFFFFFF, np.uint32)
+        self.k, self.v, pages, at = [], [], [], 0
+        for i, n in enumerate(self.lens):
+            held = []
+            for x in (k[i], v[i]):
+                x = np.concatenate((x, np.zeros((self.hkv, need[i] * bs - n, self.d))), 1).astype(np.float32)
+                held.append(x.reshape(self.hkv, need[i], bs, self.d).swapaxes(0, 1))
+            packed = kv4_cases.pack(*held)
+            for to, x in zip((self.k, self.v), kv4_cases.unpack(packed, self.d)):
+                to.append(x.swapaxes(0, 1).reshape(self.hkv, -1, self.d)[:, :n])
+            pages.append(packed)
+            self.tables[i, :need[i]] = np.arange(at, at + need[i])
+            at += need[i]
+        self.pages = np.concatenate(pages)
+        self.slopes = None
+
+
+# ---- rows behind the last sequence, row by row -------------------------------------------------
+
+PADDED = [   # lengths, new tokens, rows of the call, max_seq_len, q heads, K/V heads
+    ([1000], [1], 64, 1000, 4, 1),
+    ([300] * 4, [1] * 4, 64, 300, 16, 4),
+    ([60] * 10 + [0] * 6, [1] * 10 + [0] * 6, 32, 2048, 32, 8),
+    ([1000] * 2 + [0] * 62, [1] * 2 + [0] * 62, 128, 4096, 32, 8),
+    ([50], [1], 5, 400, 8, 8),
+    ([700, 0, 37], [2, 0, 2], 8, 2500, 24, 2),
+    ([0, 0], [0, 0], 16, 3000, 8, 2),
+]
+
+
+def padded_call(lens, new, rows, max_len, hq, hkv, d, seed=81):
+    """A case, and a function that runs it in a call of `rows` rows and returns (contexts, status)."""
+    import riftco_transformer_b200 as b2
+    case = kv4_cases.Case(seed, lens, hq, hkv, d, 16, rows=sum(new))
+    tables = np.full((len(lens), -(-max_len // 16)), 0xFFFFFFFF, np.uint32)
+    tables[:, :case.tables.shape[1]] = case.tables
+    q = np.concatenate((case.q, np.full((rows - sum(new), hq, d), np.nan, np.float32)))
+    pool, q, tables = b2.PagedKv4Pool(cuda(case.pages), 16, d), cuda(q), cuda(tables)
+    seq_lens, starts = cuda(np.array(lens, np.uint32)), cuda(np.concatenate(([0], np.cumsum(new))).astype(np.uint32))
+    need = b2.paged_chunk_kv4_workspace_bytes(len(lens), rows, hq, hkv, d, max(1, max(new)), max_len)
+    workspace = torch.empty(max(need, 16), dtype=torch.uint8, device="cuda")
+    ctx, check = guarded_bf16((rows, hq, d))
+    status = status_word()
+
+    def launch():
+        b2.paged_chunk_attention_kv4(q, pool, tables, seq_lens, starts, ctx, max(1, max(new)), max_len, status=status,
+                                     workspace=workspace)
+
+    def run(how=launch):
+        workspace.fill_(0xFF)   # NaN: nothing that the call has not written may be joined
+        ctx.fill_(7.0)
+        status.zero_()
+        how()
+        check()
+        assert bool((ctx[sum(new):] == 7.0).all())
+        return ctx[:sum(new)].float().cpu().numpy(), int(status.item())
+    return case, run, launch, (pool, q, tables, seq_lens, starts)
+
+
+@pytest.mark.parametrize("lens,new,rows,max_len,hq,hkv", PADDED)
+@pytest.mark.parametrize("d", [64, 128, 256])
+def test_rows_that_are_nobodys_take_no_part_in_the_join(lens, new, rows, max_len, hq, hkv, d):
+    import riftco_transformer_b200 as b2
+    case, run, _, _ = padded_call(lens, new, rows, max_len, hq, hkv, d)
+    out, status = run()
+    assert b2.last_route() == "attention_kv4" and status == 0
+    if sum(new):
+        assert rel_l2(out, case.chunk(new)) <= ROW_TOL
+
+
+def test_padded_call_captured_once_and_replayed_with_other_batches():
+    """16 slots and 32 rows, from one live token at length 40 to two in every slot at 900."""
+    batches = [([40] + [0] * 15, [1] + [0] * 15), ([900] * 16, [2] * 16), ([7, 900, 0, 333] * 4, [1, 2, 0, 2] * 4),
+               ([0] * 16, [0] * 16), ([1] * 3 + [0] * 13, [1] * 3 + [0] * 13)]
+    cases = [padded_call(lens, new, 32, 2048, 16, 4, 128, seed=90 + i) for i, (lens, new) in enumerate(batches)]
+    # the graph's own buffers, as many pages as the largest batch takes
+    captured = padded_call(*batches[1], 32, 2048, 16, 4, 128, seed=91)
+    _, run, launch, buffers = captured
+    launch()
+    stream, graph = torch.cuda.Stream(), torch.cuda.CUDAGraph()
+    torch.cuda.synchronize()
+    with torch.cuda.graph(graph, stream=stream):
+        launch()
+
+    def replay():
+        torch.cuda.synchronize()
+        graph.replay()
+    for i in (0, 2, 1, 3, 4):
+        case, _, _, (pool, *rest) = cases[i]
+        buffers[0].pages[:pool.pages.shape[0]].copy_(pool.pages)
+        for to, x in zip(buffers[1:], rest):
+            to.copy_(x)
+        live = sum(batches[i][1])
+        out, status = run(replay)
+        assert status == 0 and (out[live:] == 7.0).all()
+        if live:
+            assert rel_l2(out[:live], case.chunk(batches[i][1])) <= ROW_TOL
