@@ -319,7 +319,9 @@ B2_API int32_t b2_paged_decode_attention_noalloc(
  * and value = base + scale * code, one pair for 64 channels of one token. A group
  * x is stored, in FP32 with every operation rounded to nearest even, as
  *   base = f16(min x)   scale = f16((max x - base) / 15)
- *   code = clamp(rint((x - base) * (1 / scale)), 0, 15), 0 where scale is 0
+ *   code = clamp(rint((x - base) * (1 / scale)), 0, 15), 0 where scale <= 0
+ * (scale is below 0 where f16 rounds the smallest value above the largest one: a
+ * group of equal or nearly equal values, which then reads back as base).
  * A group that holds a NaN, an infinity or a magnitude above 65000 is stored as
  * scale = base = NaN (codes 0): it reads back as NaN. Attention over such keys
  * reports B2_ATTN_STATUS_NAN_OR_POS_INF; over such values it returns NaN in the 64

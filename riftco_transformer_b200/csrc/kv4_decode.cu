@@ -428,8 +428,8 @@ kv4_decode_kernel(const Kv4AttentionArgs a, ListParts* __restrict__ list_parts, 
         for (int u = 0; u < 2; ++u)
 #pragma unroll
             for (int c = 0; c < 4; ++c) acc[j][u][c] = 0.0f;
-    // p * scale is brought to fp16's range by a power of two over the largest value scale met so far.
-    float scale_top = 0.0f;      // power of two at or above it (0: none yet)
+    // p * scale is brought to fp16's range by a power of two over the largest magnitude of a value scale met so far.
+    float scale_top = 0.0f;      // power of two at or above it (0: none but zeros yet)
     float weight_factor = 0.0f;  // kWTop / scale_top
 
     const uint32_t k1024 = opaque_1024();
@@ -538,12 +538,12 @@ kv4_decode_kernel(const Kv4AttentionArgs a, ListParts* __restrict__ list_parts, 
 
         // ---- maximum: moved only when a score passes it by kSlack, or a value scale its bound ----
         uint32_t vq[2 * kPair][G];   // pairs of the values of tokens g, g + 8 of both tiles
-        __half2 top2 = __half2half2(__ushort_as_half(0));
+        __half2 top2 = __half2half2(__ushort_as_half(0));   // of magnitudes: a scale is negative where its base was rounded up
 #pragma unroll
         for (int k = 0; k < 2 * kPair; ++k) {
             lds_words<G>(vq[k], slot32 + (k / 2) * kTileBytes + kv4_half_bytes(D) + 8u * D + (g + 8u * (k % 2)) * (4u * G));
 #pragma unroll
-            for (int gr = 0; gr < G; ++gr) top2 = __hmax2(top2, *reinterpret_cast<__half2*>(&vq[k][gr]));
+            for (int gr = 0; gr < G; ++gr) top2 = __hmax2(top2, __habs2(*reinterpret_cast<__half2*>(&vq[k][gr])));
         }
         float scale_max = __low2float(top2);
         bool move = scale_max > scale_top;

@@ -123,3 +123,71 @@ def test_padded_call_captured_once_and_replayed_with_other_batches():
         assert status == 0 and (out[live:] == 7.0).all()
         if live:
             assert rel_l2(out[:live], case.chunk(batches[i][1])) <= ROW_TOL
+
+
+# ---- groups whose fp16 base lies above their largest value -------------------------------------
+
+def rounded_up(kind, d, tokens=300):
+    """Values [1, tokens, d] with constant groups that fp16 rounds up (1.0005 to 1.000977, 1000.3 to 1000.5): their stored
+    scale, (largest - base) / 15, is negative."""
+    rng = np.random.default_rng(d)
+    v = np.full((1, tokens, d), 1.0005)
+    if kind == "large beside small":   # the small one's scale is 1.6e-6
+        v[:] = 1000.3
+        if d == 64:
+            v[:, 1::2] = 0.1
+        else:
+            v[..., 64:128] = 0.1
+    elif kind == "ordinary later":
+        v[:, 200:] = rng.standard_normal((1, tokens - 200, d)) + 0.3
+    elif kind == "ordinary before":
+        v[:, :100] = rng.standard_normal((1, 100, d)) + 0.3
+    return v
+
+
+SCALES = ["constant", "large beside small", "ordinary later", "ordinary before"]
+
+
+@pytest.mark.parametrize("d", [64, 128, 256])
+@pytest.mark.parametrize("hq", [4, 12])
+@pytest.mark.parametrize("kind", SCALES)
+def test_values_of_negative_scale(kind, d, hq):
+    rng = np.random.default_rng(7)
+    v = rounded_up(kind, d)
+    assert (kv4_cases.quantize(v.astype(np.float32))[1] < 0).any()
+    k = 0.5 * rng.standard_normal(v.shape)
+    case = Held(rng.standard_normal((3, hq, d)), [k], [v])
+
+    def check(out, want, tolerance):
+        for group in range(d // 64):   # each by itself: they differ by orders of magnitude
+            part = (..., slice(64 * group, 64 * group + 64))
+            assert rel_l2(out[part], want[part]) <= tolerance
+    want = case.chunk([3])
+    for tiles, tolerance in ((False, ROW_TOL), (True, BF16_TOL)):
+        out, status = chunk(case, [3], tiles=tiles)
+        assert status == 0
+        check(out, want, tolerance)
+    case.q = case.q[2:]
+    out, status = decode(case)
+    assert status == 0
+    check(out, want[2:], F32_TOL)
+
+
+@pytest.mark.parametrize("d", [64, 128, 256])
+def test_append_stores_negative_scales_as_defined(d):
+    """Code 0 and the rounded base: the bytes of the restatement, and read back the base alone."""
+    import riftco_transformer_b200 as b2
+    for kind in SCALES:
+        v = np.ascontiguousarray(rounded_up(kind, d, 304).swapaxes(0, 1), np.float32)   # [tokens, 1, d]
+        q = np.zeros((304, 1, d), np.float32)
+        pool = b2.PagedKv4Pool(torch.zeros((19, 1, 1, 18 * d), dtype=torch.uint8, device="cuda"), 16, d)
+        tables, positions = cuda(np.arange(19, dtype=np.uint32)[None]), cuda(np.arange(304, dtype=np.uint32))
+        owner, status = cuda(np.zeros(304, np.uint32)), status_word()
+        b2.rope_append_kv4(cuda(q), cuda(q), cuda(v), positions, pool, tables, 1e4, token_seq=owner, status=status)
+        by_page = v[:, 0].reshape(19, 1, 16, d)
+        want = kv4_cases.pack(np.zeros_like(by_page), by_page)
+        assert (pool.pages.cpu().numpy()[..., 9 * d:] == want[..., 9 * d:]).all()
+        k_out, v_out = torch.empty((304, 1, d), device="cuda"), torch.empty((304, 1, d), device="cuda")
+        b2.dequantize_kv4(pool, tables, positions, k_out, v_out, token_seq=owner, status=status)
+        codes, scale, base = kv4_cases.quantize(v)
+        assert (v_out.cpu().numpy() == kv4_cases.values(codes, scale, base)).all() and int(status.item()) == 0
