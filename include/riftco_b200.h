@@ -400,9 +400,10 @@ B2_API int32_t b2_paged_decode_attention_kv4(const b2_kv4_cache* cache, const b2
  * tokens that would lie before position 0 get zeros; one longer than max_chunk is
  * flagged and its tokens from max_chunk on may be left as they were. Calls of three
  * and more tokens a sequence that are not very small run as tiles of rows, in fp16 on
- * the tcgen05 tensor cores (q, k, v and the weights are rounded to 2^-12), others
- * token by token as in the decode form; b2_last_route tells. Other errors and the
- * workspace as above. */
+ * the tcgen05 tensor cores (q, k, v and the weights are each off by at most 2^-11 of
+ * themselves, weights below 2^-21 of the row's largest by 2^-32 of that), others token
+ * by token as in the decode form; b2_last_route tells. Other errors and the workspace
+ * as above. */
 B2_API size_t b2_paged_chunk_kv4_workspace_bytes(uint32_t n_seq, uint32_t n_tokens, uint32_t q_heads,
                                                  uint32_t kv_heads, uint32_t head_width, uint32_t max_chunk,
                                                  uint32_t max_seq_len);

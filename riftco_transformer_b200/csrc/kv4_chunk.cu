@@ -12,10 +12,13 @@
 // transposed on the way, since its contraction is over tokens: two tokens' words are merged so that one
 // AND-OR yields two tokens' codes of one channel.
 //
-// Roundings: Q, K, V and P are fp16 (2^-12 of each value; Q is first scaled by a power of two per row), sums,
-// maxima and O are FP32, and the context is bf16 (2^-9), which is the larger error. The maximum m is moved, and O
-// rescaled in tensor memory, only when a score passes it by 8 in log2 units: P may reach 2^8, and a row
-// sum of 2^8 * 10^5 tokens stays far inside FP32.
+// Roundings: Q, K, V and P are fp16 (by at most 2^-11 of each value; Q is first scaled by a power of two per row), sums,
+// maxima and O are FP32, and the context is bf16 (2^-8), which is the larger error. P is measured against m, 7 below the
+// largest score (log2 units) when it is set, and m is moved, and O rescaled in tensor memory, only when a score passes it
+// by 15: P reaches from 2^15, as high as fp16 goes, down to its subnormal step, so that no weight is off by more than
+// 2^-32 of the largest, or 2^-11 of itself. (Against the largest score itself weights below 2^-25 vanished from O but not
+// from the sum: 131071 equal ones under a peak 25 above them were lost.) A row sum of 2^15 * 2^31 tokens stays far inside
+// FP32.
 //
 // What bounds it: per 64 tokens and row tile (D = 128) the two products take 400 + 256 cycles of the tensor core
 // (N = 64 reads Q faster than it multiplies) and the exponentials 512 of the 16-per-cycle unit, that is 1312 and 1024
@@ -56,7 +59,8 @@ constexpr uint32_t kRawSlots = 3;
 constexpr uint32_t kMostStages = 4;
 constexpr uint32_t kTmemColumns = 512, kTmemTile = 256, kTmemO = 128;   // a tile's two S (and P) of 64 columns, its O
 constexpr uint32_t kTmemQ = 384;   // heads of 256: Q, for which shared memory has no room, beside the one tile's O
-constexpr float kSlack = 8.0f;
+constexpr float kHeadroom = 7.0f;   // log2 of the largest weight when the reference m is set, for the sake of the smallest
+constexpr float kSlack = 15.0f;     // P may reach 2^kSlack before m is moved
 
 template <int D>
 struct Layout {
@@ -767,8 +771,8 @@ kv4_chunk_kernel(const Kv4AttentionArgs a, float* __restrict__ partials, const C
                     if (token0 + e < begin || token0 + e >= end) x[e] = 0xFF800000u;   // -infinity
                 }
             }
-            // The weights are made against the maximum so far, while the block's own is found; where it passes that by
-            // more than kSlack (the first block, hardly ever later) they are made again.
+            // The weights are made against the reference so far, while the block's maximum is found; where it passes that
+            // by more than kSlack (the first block, hardly ever later) they are made again.
             uint32_t p[32];
             float sum, top;
             auto weigh = [&]() {
@@ -797,7 +801,7 @@ kv4_chunk_kernel(const Kv4AttentionArgs a, float* __restrict__ partials, const C
             weigh();
             if (turns && (i == 0u || n + 1u < mine)) turn_pass(2u + (warp % 4u) * 2u + (i ^ 1u));
             if (__any_sync(0xFFFFFFFFu, top > m + kSlack)) {
-                const float moved = fmaxf(m, top);
+                const float moved = fmaxf(m, top - kHeadroom);
                 const float shrink = ex2(m - moved);
                 m = moved;
                 l *= shrink;

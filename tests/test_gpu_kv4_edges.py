@@ -191,3 +191,57 @@ def test_append_stores_negative_scales_as_defined(d):
         b2.dequantize_kv4(pool, tables, positions, k_out, v_out, token_seq=owner, status=status)
         codes, scale, base = kv4_cases.quantize(v)
         assert (v_out.cpu().numpy() == kv4_cases.values(codes, scale, base)).all() and int(status.item()) == 0
+
+
+# ---- weights far below the largest -------------------------------------------------------------
+
+def peaked(d, hq, new, tokens, period):
+    """Every `period`-th token has a key that lifts its score 20 to 29 (log2 units, by head) above the others' of zero, and
+    values of zero, so that the context is what the many small weights carry. Queries and keys are exact in fp16 and the
+    product of both with 1 / sqrt(d) is the score: the tile kernel's operands round nothing of it."""
+    rng = np.random.default_rng(d + period)
+    k = np.zeros((1, tokens, d))
+    k[:, ::period] = np.float16(25.5 * np.log(2.0) / np.sqrt(d))
+    v = 1.0 + 0.25 * rng.standard_normal((1, tokens, d))
+    v[:, ::period] = 0.0
+    q = np.ones((new, hq, d)) * (0.8125 + 0.0625 * (np.arange(hq) % 6))[:, None]
+    return Held(q, [k], [v], bs=64)
+
+
+def small_weight_bound(case, want, period):
+    """A weight is fp16 against at least 2^7 at the peak: half a step, 2^-11 of it or 2^-25 / 2^7 = 2^-32 of the largest,
+    `period` of them under each peak; values round by 2^-11 and the context by 2^-8, the exponential and FP32 sums by
+    less than 2^-18."""
+    largest = max(np.abs(v).max() for v in case.v)
+    return period * 2.0 ** -32 * largest + (2.0 ** -8 + 2.0 ** -10 + 2.0 ** -18) * np.abs(want)
+
+
+@pytest.mark.parametrize("d", [64, 128, 256])
+@pytest.mark.parametrize("hq,new", [(4, 5), (4, 40)])   # one tile's rows, and two tiles'
+def test_chunk_small_weights_under_a_peak(d, hq, new):
+    case = peaked(d, hq, new, 5000, 512)
+    out, status = chunk(case, [new])
+    want = case.chunk([new])
+    # (a value's group rounds to 4 bits before; what the cache holds is what `want` averages)
+    assert status == 0
+    assert (np.abs(out - want) <= small_weight_bound(case, want, 512)).all()
+
+
+def test_chunk_peak_over_131071_flat_tokens():
+    """One peak at the context's start, the rest of it read by the same CTA: 148 sequences over the same pages leave no
+    SM to split them for."""
+    import riftco_transformer_b200 as b2
+    n, new, hq, d, seqs = 131072, 4, 4, 128, 148
+    case = peaked(d, hq, new, n, n)
+    pool = b2.PagedKv4Pool(cuda(case.pages), case.bs, d)
+    ctx = torch.empty((seqs * new, hq, d), dtype=torch.bfloat16, device="cuda")
+    status = status_word()
+    assert b2.paged_chunk_kv4_workspace_bytes(seqs, seqs * new, hq, 1, d, new, n) == 0   # not split
+    b2.paged_chunk_attention_kv4(cuda(np.tile(case.q, (seqs, 1, 1))), pool, cuda(np.tile(case.tables, (seqs, 1))),
+                                 cuda(np.full(seqs, n, np.uint32)), cuda(np.arange(0, seqs * new + 1, new, dtype=np.uint32)),
+                                 ctx, new, n, status=status)
+    assert b2.last_route() == "attention_kv4_tiles" and int(status.item()) == 0
+    out = ctx.view(seqs, new, hq, d)
+    assert bool((out == out[:1]).all())
+    want = case.chunk([new])
+    assert (np.abs(out[0].float().cpu().numpy() - want) <= small_weight_bound(case, want, n)).all()
