@@ -61,6 +61,10 @@ constexpr uint32_t kTmemColumns = 512, kTmemTile = 256, kTmemO = 128;   // a til
 constexpr uint32_t kTmemQ = 384;   // heads of 256: Q, for which shared memory has no room, beside the one tile's O
 constexpr float kHeadroom = 7.0f;   // log2 of the largest weight when the reference m is set, for the sake of the smallest
 constexpr float kSlack = 15.0f;     // P may reach 2^kSlack before m is moved
+// From this magnitude of m on (log2 units) a score's rounding counts: the steps of FP32 are 1/8 and more, so that a fused
+// product minus a rounded m may be off by powers of two, and m + kSlack by a step. Such rows' scores are rounded first, the
+// way their maximum is, and m follows every block's.
+constexpr float kFar = 1048576.0f;
 
 template <int D>
 struct Layout {
@@ -733,6 +737,7 @@ kv4_chunk_kernel(const Kv4AttentionArgs a, float* __restrict__ partials, const C
         __syncwarp();
         if (lane == 0) mbar_arrive(&bars.q_full[i]);
         float m = kNoMax, l = 0.0f;
+        float limit = kNoMax;   // largest score for which m stays: m + kSlack, or none
 
         const uint32_t first_block = paired ? i : 0u;
         const uint32_t mine = n_blocks > first_block ? (n_blocks - first_block + step - 1u) / step : 0u;   // the tile's blocks
@@ -800,11 +805,18 @@ kv4_chunk_kernel(const Kv4AttentionArgs a, float* __restrict__ partials, const C
             if (turns) turn_wait(2u + (warp % 4u) * 2u + i, i == 0u && n == 0u);
             weigh();
             if (turns && (i == 0u || n + 1u < mine)) turn_pass(2u + (warp % 4u) * 2u + (i ^ 1u));
-            if (__any_sync(0xFFFFFFFFu, top > m + kSlack)) {
+            if (__any_sync(0xFFFFFFFFu, top > limit)) {
                 const float moved = fmaxf(m, top - kHeadroom);
                 const float shrink = ex2(m - moved);
                 m = moved;
                 l *= shrink;
+                const bool far = m != kNoMax && fabsf(m) > kFar;
+                limit = far ? -INFINITY : m + kSlack;
+                if (__any_sync(0xFFFFFFFFu, far)) {
+#pragma unroll
+                    for (int e = 0; e < 64; ++e) x[e] = __float_as_uint(__fmul_rn(__uint_as_float(x[e]), factor));
+                    factor = 1.0f;
+                }
                 if (n > 0u) {
                     mbar_wait(&bars.o_done[i], (n - 1u) & 1u, abort);   // P V of the block before: O is at rest
                     tcgen05_fence_after_sync();

@@ -245,3 +245,48 @@ def test_chunk_peak_over_131071_flat_tokens():
     assert bool((out == out[:1]).all())
     want = case.chunk([new])
     assert (np.abs(out[0].float().cpu().numpy() - want) <= small_weight_bound(case, want, n)).all()
+
+
+# ---- scores and queries of any finite magnitude ------------------------------------------------
+
+@pytest.mark.parametrize("d", [64, 128, 256])
+@pytest.mark.parametrize("tiles", [False, True])
+@pytest.mark.parametrize("power", [-120, 0, 20, 60, 112])
+def test_chunk_scores_of_any_finite_magnitude(d, tiles, power):
+    """Keys that are constant over a token, one of them the largest, queries 2^power times 1 or 2: large scores (up to 2^119,
+    inside FP32) pick that token, tiny ones weigh all alike. Keys and queries are exact in fp16."""
+    rng = np.random.default_rng(d)
+    n, new, hq = 200, 6, 4
+    k = np.broadcast_to((np.arange(n) % 64 / 64.0 + (np.arange(n) // 64) / 4.0)[None, :, None], (1, n, d))
+    v = rng.standard_normal((1, n, d)) + 0.3
+    q = np.exp2(power) * rng.integers(1, 3, (new, hq, 1)) * np.ones((1, 1, d))
+    case = Held(q, [k], [v])
+    out, status = chunk(case, [new], tiles=tiles)
+    assert status == 0
+    assert rel_l2(out, case.chunk([new])) <= (BF16_TOL if tiles else ROW_TOL)
+
+
+def a_step_apart(d, hq, power):
+    """Scores of about 1.5 * 2^power (log2 units) that rise by 4 every 128 tokens: at 2^25 by one step of FP32, which decides
+    between tokens as it will, but a context is an average of values. Returns a case of 4 rows, and the values' extremes."""
+    n = 3000
+    rng = np.random.default_rng(power)
+    k = np.ones((1, n, d))
+    k[..., 64:] = np.arange(n)[None, :, None] // 128 / 4.0
+    v = rng.standard_normal((1, n, d)) + 0.3
+    unit = np.sqrt(d) / np.log2(np.e) / 64
+    q = np.full((4, hq, d), 0.0)
+    q[..., :64], q[..., 64:128] = 1.5 * 2.0 ** power * unit, 16.0 * unit
+    case = Held(q, [k], [v])
+    return case, case.v[0].min(1)[0], case.v[0].max(1)[0]
+
+
+@pytest.mark.parametrize("d", [128, 256])
+@pytest.mark.parametrize("hq", [4, 8])
+@pytest.mark.parametrize("power", range(18, 31))
+def test_chunk_scores_a_rounding_step_apart(d, hq, power):
+    case, low, high = a_step_apart(d, hq, power)
+    out, status = chunk(case, [4])
+    assert status == 0
+    # 2^-7 covers the context's bf16 and the values' fp16
+    assert (out >= low - 2.0 ** -7 * np.abs(low)).all() and (out <= high + 2.0 ** -7 * np.abs(high)).all()
