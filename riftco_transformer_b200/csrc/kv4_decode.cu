@@ -549,7 +549,8 @@ kv4_decode_kernel(const Kv4AttentionArgs a, ListParts* __restrict__ list_parts, 
         bool move = scale_max > scale_top;
 #pragma unroll
         for (int h = 0; h < HL; ++h) {
-            move = move || fmaxf(fmaxf(s[0][h], s[1][h]), fmaxf(s[2][h], s[3][h])) > m[h] + kSlack;
+            // (the difference of close numbers is exact; m + kSlack may round up past the next score, and p to 2^4)
+            move = move || fmaxf(fmaxf(s[0][h], s[1][h]), fmaxf(s[2][h], s[3][h])) - m[h] > kSlack;
         }
         if (__any_sync(0xFFFFFFFFu, move)) {
             scale_max = fmaxf(scale_max, __shfl_xor_sync(0xFFFFFFFFu, scale_max, 4));

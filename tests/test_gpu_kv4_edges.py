@@ -290,3 +290,17 @@ def test_chunk_scores_a_rounding_step_apart(d, hq, power):
     assert status == 0
     # 2^-7 covers the context's bf16 and the values' fp16
     assert (out >= low - 2.0 ** -7 * np.abs(low)).all() and (out <= high + 2.0 ** -7 * np.abs(high)).all()
+
+
+@pytest.mark.parametrize("d", [128, 256])
+@pytest.mark.parametrize("hq", [4, 8])
+@pytest.mark.parametrize("power", range(18, 31))
+def test_decode_scores_a_rounding_step_apart(d, hq, power):
+    case, low, high = a_step_apart(d, hq, power)
+    out, status = chunk(case, [4], tiles=False)
+    assert status == 0
+    assert (out >= low - ROW_TOL * np.abs(low)).all() and (out <= high + ROW_TOL * np.abs(high)).all()
+    case.q = case.q[-1:]
+    out, status = decode(case)
+    assert status == 0
+    assert (out >= low - F32_TOL * np.abs(low)).all() and (out <= high + F32_TOL * np.abs(high)).all()
