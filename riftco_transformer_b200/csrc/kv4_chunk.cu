@@ -625,7 +625,7 @@ kv4_chunk_kernel(const Kv4AttentionArgs a, float* __restrict__ partials, const C
         // 2^e with a row's largest magnitude * 2^e in [2^9, 2^10), and what takes a product back
         auto row_scale = [&](float top, float* up, float* down) {
             int e = 9 - (static_cast<int>((__float_as_uint(top) >> 23) & 255u) - 127);
-            e = max(-100, min(100, e));   // a row of zeros or beyond 2^109 keeps a bounded factor
+            e = min(100, e);   // a row of zeros keeps a bounded factor; the largest rows have e = -119, still a normal 2^e
             *up = __uint_as_float(static_cast<uint32_t>(e + 127) << 23);
             *down = __uint_as_float(static_cast<uint32_t>(127 - e) << 23) * to_unit;
         };

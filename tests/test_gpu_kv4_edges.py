@@ -304,3 +304,20 @@ def test_decode_scores_a_rounding_step_apart(d, hq, power):
     out, status = decode(case)
     assert status == 0
     assert (out >= low - F32_TOL * np.abs(low)).all() and (out <= high + F32_TOL * np.abs(high)).all()
+
+
+@pytest.mark.parametrize("d", [64, 128, 256])
+@pytest.mark.parametrize("tiles", [True])
+@pytest.mark.parametrize("power", [116, 118, 123])
+def test_chunk_queries_near_the_end_of_fp32(d, tiles, power):
+    """Queries of 2^power and twice that over keys of 2^-14 to 2^-13 (scores up to 2^118): the largest key's token is picked,
+    the queries' size overflows nothing."""
+    rng = np.random.default_rng(d)
+    n, new, hq = 200, 6, 4
+    k = np.broadcast_to(2.0 ** -14 * (1.0 + np.arange(n) % 191 / 256.0)[None, :, None], (1, n, d))
+    v = rng.standard_normal((1, n, d)) + 0.3
+    q = np.exp2(power) * rng.integers(1, 3, (new, hq, 1)) * np.ones((1, 1, d))
+    case = Held(q, [k], [v])
+    out, status = chunk(case, [new], tiles=tiles)
+    assert status == 0
+    assert rel_l2(out, case.chunk([new])) <= (BF16_TOL if tiles else ROW_TOL)
