@@ -375,8 +375,8 @@ B2_API int32_t b2_kv4_dequantize(const b2_kv4_cache* cache, const uint32_t* posi
  * q_heads is any multiple of kv_heads. Scores, softmax statistics and sums are FP32,
  * the products exact to 22 bits. A sequence of length 0 sees nothing and gets zeros.
  * Errors go to the status word: NaN or +infinite scores (all scores of a query that
- * holds a NaN or an infinity may count as such), every score of a head
- * -infinite (zeros), a block id outside the pool (its page is read as page 0), a
+ * holds a NaN, an infinity or a magnitude above 2e37 may count as such), every score of
+ * a head -infinite (zeros), a block id outside the pool (its page is read as page 0), a
  * length above max_seq_len (read up to max_seq_len; BAD_BLOCK).
  * Workspace as for b2_paged_decode_attention: at least the bytes below (NULL: the
  * library's arena), 16-byte aligned, not shared by calls that may overlap on the GPU. */

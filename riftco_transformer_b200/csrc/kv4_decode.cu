@@ -335,7 +335,8 @@ kv4_decode_kernel(const Kv4AttentionArgs a, ListParts* __restrict__ list_parts, 
     constexpr int kProducts = HC == 4 ? 2 : 3;
     uint32_t qf[kChunks][2][kProducts];   // [chunk][register][product]
     float q_unscale;                  // of column head
-    float q_sum[G];
+    constexpr float kSumScale = 0.0078125f;   // 2^-7: the sum of 64 channels stays inside FP32
+    float q_sum[G];                   // times kSumScale
     {
         float x[kChunks][8];
         float top = 0.0f;
@@ -365,7 +366,7 @@ kv4_decode_kernel(const Kv4AttentionArgs a, ListParts* __restrict__ list_parts, 
 #pragma unroll
             for (int j = 2 * gr; j < 2 * gr + 2; ++j)
 #pragma unroll
-                for (int c = 0; c < 8; ++c) s += x[j][c];
+                for (int c = 0; c < 8; ++c) s = fmaf(x[j][c], kSumScale, s);
             s += __shfl_xor_sync(0xFFFFFFFFu, s, 1);
             s += __shfl_xor_sync(0xFFFFFFFFu, s, 2);
             q_sum[gr] = s;
@@ -408,7 +409,7 @@ kv4_decode_kernel(const Kv4AttentionArgs a, ListParts* __restrict__ list_parts, 
         const int src = HC == 4 ? static_cast<int>(t) * 8 : static_cast<int>(2 * t + h) * 4;   // lane of column head
         code_factor[h] = __shfl_sync(0xFFFFFFFFu, q_unscale, src) * (inv_sqrt * unit);
 #pragma unroll
-        for (int gr = 0; gr < G; ++gr) base_factor[h][gr] = __shfl_sync(0xFFFFFFFFu, q_sum[gr], src) * (inv_sqrt * unit);
+        for (int gr = 0; gr < G; ++gr) base_factor[h][gr] = __shfl_sync(0xFFFFFFFFu, q_sum[gr], src) * (inv_sqrt * unit * (1.0f / kSumScale));
         const uint32_t head = HC == 4 ? t : 2 * t + h;
         slope[h] = biased && head < live_heads ? __ldg(a.rules.alibi_slopes + first_head + head) * kLog2e : 0.0f;
     }

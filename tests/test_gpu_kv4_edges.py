@@ -307,7 +307,7 @@ def test_decode_scores_a_rounding_step_apart(d, hq, power):
 
 
 @pytest.mark.parametrize("d", [64, 128, 256])
-@pytest.mark.parametrize("tiles", [True])
+@pytest.mark.parametrize("tiles", [False, True])
 @pytest.mark.parametrize("power", [116, 118, 123])
 def test_chunk_queries_near_the_end_of_fp32(d, tiles, power):
     """Queries of 2^power and twice that over keys of 2^-14 to 2^-13 (scores up to 2^118): the largest key's token is picked,
