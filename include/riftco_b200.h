@@ -398,7 +398,8 @@ B2_API int32_t b2_paged_decode_attention_kv4(const b2_kv4_cache* cache, const b2
  * (b2_nf4_linear_forward_multi_bf16). Rows behind chunk_starts[n_seq] are left as
  * they were; a chunk longer than its sequence is flagged BAD_BLOCK and the
  * tokens that would lie before position 0 get zeros; one longer than max_chunk is
- * flagged and its tokens from max_chunk on may be left as they were. Calls of three
+ * flagged and its tokens from max_chunk on may be left as they were; chunks that end
+ * behind n_tokens are flagged, the rows that are there get their contexts. Calls of three
  * and more tokens a sequence that are not very small run as tiles of rows, in fp16 on
  * the tcgen05 tensor cores (q, k, v and the weights are each off by at most 2^-11 of
  * themselves, weights below 2^-21 of the row's largest by 2^-32 of that), others token

@@ -114,15 +114,12 @@ struct TileSpan {
 };
 __device__ __forceinline__ TileSpan tile_span(const Kv4AttentionArgs& a, uint32_t seq, uint32_t rep, uint32_t row0, uint32_t cta_rows) {
     TileSpan s{};
-    uint32_t first = __ldg(a.chunk_starts + seq), last = __ldg(a.chunk_starts + seq + 1u);
-    first = min(first, a.rows);
-    last = min(last, a.rows);
-    s.first = first;
-    s.tokens = last > first ? last - first : 0u;
-    if (s.tokens > a.max_chunk) {   // the grid holds max_chunk of them
-        s.bad = true;
-        s.tokens = a.max_chunk;
-    }
+    const uint32_t first = __ldg(a.chunk_starts + seq), last = __ldg(a.chunk_starts + seq + 1u);
+    s.first = min(first, a.rows);
+    const uint32_t end_row = min(last, a.rows);
+    s.tokens = end_row > s.first ? end_row - s.first : 0u;   // those that the call has rows for
+    s.bad = last > first && last - first > a.max_chunk;
+    s.tokens = min(s.tokens, a.max_chunk);   // the grid holds max_chunk of them
     s.rows = s.tokens * rep;
     if (row0 >= s.rows) return s;
     s.len = __ldg(a.seq_lens + seq);
@@ -405,6 +402,7 @@ kv4_chunk_kernel(const Kv4AttentionArgs a, float* __restrict__ partials, const C
     extern __shared__ __align__(1024) uint8_t smem_raw[];
     __shared__ __align__(8) Barriers bars;
 
+    check_chunk_starts(a);
     const uint32_t rep = a.q_heads / a.cache.kv_heads;
     uint32_t block = blockIdx.x;
     const uint32_t split = block % plan.splits;

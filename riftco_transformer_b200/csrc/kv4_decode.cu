@@ -186,6 +186,7 @@ __global__ void __launch_bounds__(kWarps * 32, ctas_of(D, HC))
 kv4_decode_kernel(const Kv4AttentionArgs a, ListParts* __restrict__ list_parts, float* __restrict__ partials, const WorkPlan plan) {
     using namespace sm100;
     pdl_launch_dependents();
+    check_chunk_starts(a);
     constexpr int G = D / 64, kChunks = D / 32;
     constexpr int HL = HC / 4;            // heads of a lane in the score layout
     constexpr uint32_t kTileBytes = kv4_tile_bytes(D);

@@ -321,3 +321,26 @@ def test_chunk_queries_near_the_end_of_fp32(d, tiles, power):
     out, status = chunk(case, [new], tiles=tiles)
     assert status == 0
     assert rel_l2(out, case.chunk([new])) <= (BF16_TOL if tiles else ROW_TOL)
+
+
+# ---- chunk starts past the call's rows ----------------------------------------------------------
+
+@pytest.mark.parametrize("d", [64, 128, 256])
+@pytest.mark.parametrize("new,claimed,tiles", [([5, 4], 7, False), ([60, 70], 75, True), ([9, 0], 3, False), ([130, 0], 5, True)])
+def test_chunk_starts_past_the_rows_are_flagged(d, new, claimed, tiles):
+    """The last sequence says it has more new tokens than the call has rows: the rows there are get the contexts of their
+    positions, in both forms, and the call is flagged."""
+    import riftco_transformer_b200 as b2
+    from riftco_transformer_b200 import _lib
+    case = kv4_cases.Case(91, [max(40, new[0]), 150], 8, 8, d, 16, rows=sum(new))
+    ctx, check = guarded_bf16(case.q.shape)
+    status = status_word()
+    b2.paged_chunk_attention_kv4(cuda(case.q), b2.PagedKv4Pool(cuda(case.pages), 16, d), cuda(case.tables),
+                                 cuda(np.array(case.lens, np.uint32)), cuda(np.array([0, new[0], new[0] + claimed], np.uint32)),
+                                 ctx, max(claimed, new[0]), 150, status=status)
+    check()
+    assert b2.last_route() == ("attention_kv4_tiles" if tiles else "attention_kv4")
+    assert int(status.item()) == _lib.ATTN_STATUS_BAD_BLOCK
+    want = [kv4_cases.attend(case.q[i], case.k[0], case.v[0], case.lens[0] - new[0] + i) for i in range(new[0])]
+    want += [kv4_cases.attend(case.q[new[0] + i], case.k[1], case.v[1], 150 - claimed + i) for i in range(new[1])]
+    assert rel_l2(ctx.float().cpu().numpy(), np.stack(want)) <= (BF16_TOL if tiles else ROW_TOL)
