@@ -885,10 +885,13 @@ int32_t launch_kv4_decode(const DeviceContext& ctx, const Kv4AttentionArgs& a, v
                           cudaStream_t stream) {
     WorkPlan plan;
     Sizes sizes;
-    // a window bounds what a row sees; fewer tokens never need more workspace
-    uint32_t most = a.max_seq_len;
-    if (a.rules.window != 0u && a.rules.prefix_lens == nullptr && a.rules.window < most) most = a.rules.window;
-    B2_TRY(work_plan(ctx, a.rows, a.q_heads, a.cache.kv_heads, a.cache.head_width, most, &plan, &sizes));
+    // A window bounds what a row sees. Fewer tokens need no more workspace, but for bounds so large that their pairs pass 32
+    // bits: those are planned as whole lists, in no workspace, and so is their window then.
+    const uint32_t window = a.rules.window != 0u && a.rules.prefix_lens == nullptr ? a.rules.window : UINT32_MAX;
+    B2_TRY(work_plan(ctx, a.rows, a.q_heads, a.cache.kv_heads, a.cache.head_width, a.max_seq_len, &plan, &sizes));
+    if (window < a.max_seq_len && plan.whole_lists == 0u) {
+        B2_TRY(work_plan(ctx, a.rows, a.q_heads, a.cache.kv_heads, a.cache.head_width, window, &plan, &sizes));
+    }
     const size_t need = plan_bytes(plan, sizes);
     if (need > workspace_bytes) {
         return fail(B2_STATUS_INVALID_ARGUMENT, "paged attention workspace too small: need %zu bytes, got %zu", need,

@@ -344,3 +344,31 @@ def test_chunk_starts_past_the_rows_are_flagged(d, new, claimed, tiles):
     want = [kv4_cases.attend(case.q[i], case.k[0], case.v[0], case.lens[0] - new[0] + i) for i in range(new[0])]
     want += [kv4_cases.attend(case.q[new[0] + i], case.k[1], case.v[1], 150 - claimed + i) for i in range(new[1])]
     assert rel_l2(ctx.float().cpu().numpy(), np.stack(want)) <= (BF16_TOL if tiles else ROW_TOL)
+
+
+# ---- a window over a bound at which the sums of all lists pass 32 bits ------------------------
+
+@pytest.mark.parametrize("given", [False, True])
+def test_window_under_the_largest_bound(given):
+    """64 sequences with a capacity of 2^31 - 1 tokens: the size query answers 0, with a window or without, and the call
+    asks for no more."""
+    import riftco_transformer_b200 as b2
+    n, d, bs, max_len = 64, 64, 1 << 20, 0x7FFFFFFF
+    rng = np.random.default_rng(3)
+    k, v = (rng.standard_normal((1, 64, d)) for _ in range(2))
+    case = Held(rng.standard_normal((n, 1, d)), [k] * n, [v] * n)
+    pages = torch.zeros((1, 1, bs // 16, 18 * d), dtype=torch.uint8, device="cuda")
+    pages[0, 0, :4] = cuda(case.pages[:4, 0, 0])
+    pool = b2.PagedKv4Pool(pages, bs, d)
+    tables = torch.zeros((n, 2048), dtype=torch.int32, device="cuda")
+    lens = np.arange(1, n + 1).astype(np.uint32)
+    assert b2.paged_decode_kv4_workspace_bytes(n, 1, 1, d, max_len) == 0
+    workspace = torch.empty(16, dtype=torch.uint8, device="cuda") if given else None
+    out = torch.empty((n, 1, d), device="cuda")
+    for window in (0, 1, 20, 1000, 1 << 30):
+        out.fill_(float("nan"))
+        status = status_word()
+        b2.paged_decode_attention_kv4(cuda(case.q), pool, tables, cuda(lens), out, max_len, window=window, status=status,
+                                      workspace=workspace)
+        want = np.stack([kv4_cases.attend(case.q[i], case.k[i], case.v[i], i, window=window) for i in range(n)])
+        assert int(status.item()) == 0 and rel_l2(out.cpu().numpy(), want) <= F32_TOL
