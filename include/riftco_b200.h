@@ -352,8 +352,9 @@ typedef struct b2_kv4_score_rules {
  * (the same rotation; q_out may be q), and stores rotated k and v in slot
  * positions[t] of sequence token_seq[t], or of sequence t where token_seq is NULL
  * (n_tokens == n_seq then). q, q_out [n_tokens, q_heads, d], k, v [n_tokens, kv_heads, d],
- * FP32, 16-byte aligned. A token with position 0xFFFFFFFF is padding: nothing of it
- * is read or written. A position, sequence or block id outside the cache stores
+ * FP32, 16-byte aligned. A token with position 0xFFFFFFFF is padding: its rows have to
+ * be there, as those of all n_tokens, but may hold anything, and nothing of it is
+ * written. A position, sequence or block id outside the cache stores
  * nothing (q is still rotated) and sets B2_ATTN_STATUS_BAD_BLOCK. The (sequence,
  * position) pairs of one call must be distinct: of two tokens that share a slot,
  * parts of either may be stored. */

@@ -372,3 +372,38 @@ def test_window_under_the_largest_bound(given):
                                       workspace=workspace)
         want = np.stack([kv4_cases.attend(case.q[i], case.k[i], case.v[i], i, window=window) for i in range(n)])
         assert int(status.item()) == 0 and rel_l2(out.cpu().numpy(), want) <= F32_TOL
+
+
+# ---- padding tokens -----------------------------------------------------------------------------
+
+@pytest.mark.parametrize("d", [64, 128, 256])
+@pytest.mark.parametrize("live,padded", [(1, 64), (37, 300), (700, 1400)])
+def test_append_buffers_may_end_before_the_padding(d, live, padded):
+    """Nothing of a padding token is read or written: its rows of q, k and v need not be there. The call goes through the C
+    entry, since the Python one asks for whole tensors; what follows the live rows here belongs to this test, and keeps
+    its pattern."""
+    import riftco_transformer_b200 as b2
+    from riftco_transformer_b200 import _lib
+    rng = np.random.default_rng(live)
+    hq, hkv, bs = 4, 2, 16
+    blocks = -(-live // bs)
+    q = rng.standard_normal((live, hq, d)).astype(np.float32)
+    k, v = (rng.standard_normal((live, hkv, d)).astype(np.float32) for _ in range(2))
+    tables, owner = cuda(np.arange(blocks, dtype=np.uint32)[None]), cuda(np.zeros(padded, np.uint32))
+    positions = cuda(np.concatenate((np.arange(live), np.full(padded - live, 0xFFFFFFFF))).astype(np.uint32))
+
+    def append(n, behind):
+        """The pool's bytes and the rotated queries, from buffers of the live rows and `behind` floats."""
+        pool = b2.PagedKv4Pool(torch.zeros((blocks, hkv, 1, 18 * d), dtype=torch.uint8, device="cuda"), bs, d)
+        held = [cuda(np.concatenate((x.ravel(), np.full(behind, np.nan, np.float32)))) for x in (q, k, v)]
+        status, struct = status_word(), pool.struct(tables)
+        code = _lib.lib.b2_rope_append_kv4(C.byref(struct), held[0].data_ptr(), held[0].data_ptr(), held[1].data_ptr(),
+                                           held[2].data_ptr(), positions.data_ptr(), owner.data_ptr(), n, hq, 1e4,
+                                           status.data_ptr(), torch.cuda.current_stream().cuda_stream)
+        torch.cuda.synchronize()
+        assert code == 0 and int(status.item()) == 0
+        assert all(bool(x[x.numel() - behind:].isnan().all()) for x in held)
+        return pool.pages, held[0][:q.size]
+    want_pages, want_q = append(live, 0)
+    pages, turned = append(padded, 64)
+    assert torch.equal(pages, want_pages) and torch.equal(turned, want_q)
