@@ -53,6 +53,13 @@ def _need(t, what: str, dtypes, shape, device: int) -> int:
 _F32 = (torch.float32,)
 
 
+def _u32(value: int, what: str) -> int:
+    """`value`, which a uint32 of the C ABI has to hold: ctypes would pass on the lower half of a larger one."""
+    if not 0 <= value <= 0xFFFFFFFF:
+        raise ValueError(f"paged attention {what} must be between 0 and 2**32 - 1, got {value}")
+    return value
+
+
 @dataclass
 class PagedKv4Pool:
     """One layer's 4-bit K/V pages: ``pages`` uint8 [physical_blocks, kv_heads,
@@ -160,8 +167,9 @@ def dequantize_kv4(pool: PagedKv4Pool, block_tables: torch.Tensor, positions: to
 def _rules(softcap, window, alibi_slopes, q_heads, device):
     if not softcap and not window and alibi_slopes is None:
         return None
-    if not 0 <= window <= 0xFFFFFFFF:
-        raise ValueError("paged attention window must be between 0 and 2**32 - 1")
+    if softcap != 0 and not 1e-6 <= softcap <= 1e18:   # here too: one below FP32's range would become 0, no cap
+        raise ValueError(f"paged attention score cap must be 0 or between 1e-6 and 1e18, got {softcap}")
+    _u32(window, "window")
     slopes = None if alibi_slopes is None else _need(alibi_slopes, "slopes", _F32, (q_heads,), device)
     return C.byref(Kv4ScoreRulesStruct(softcap, window, slopes))
 
@@ -176,7 +184,9 @@ def _workspace(workspace, device):
 
 def paged_decode_kv4_workspace_bytes(n_seq: int, q_heads: int, kv_heads: int, head_width: int,
                                      max_seq_len: int) -> int:
-    return lib.b2_paged_decode_kv4_workspace_bytes(n_seq, q_heads, kv_heads, head_width, max_seq_len)
+    return lib.b2_paged_decode_kv4_workspace_bytes(_u32(n_seq, "sequences"), _u32(q_heads, "query heads"),
+                                                   _u32(kv_heads, "KV heads"), _u32(head_width, "head width"),
+                                                   _u32(max_seq_len, "max_seq_len"))
 
 
 def paged_decode_attention_kv4(queries: torch.Tensor, pool: PagedKv4Pool, block_tables: torch.Tensor,
@@ -186,6 +196,7 @@ def paged_decode_attention_kv4(queries: torch.Tensor, pool: PagedKv4Pool, block_
                                workspace: torch.Tensor | None = None, stream=None) -> None:
     """One query token per sequence: queries [n_seq, q_heads, d] FP32, ``context`` the same (None
     where only ``context_bf16`` is wanted), seq_lens [n_seq] the lengths with the new token."""
+    _u32(max_seq_len, "max_seq_len")
     cache = pool.struct(block_tables)
     device = pool.device_index
     if queries.dim() != 3:
@@ -205,8 +216,10 @@ def paged_decode_attention_kv4(queries: torch.Tensor, pool: PagedKv4Pool, block_
 
 def paged_chunk_kv4_workspace_bytes(n_seq: int, n_tokens: int, q_heads: int, kv_heads: int, head_width: int,
                                     max_chunk: int, max_seq_len: int) -> int:
-    return lib.b2_paged_chunk_kv4_workspace_bytes(n_seq, n_tokens, q_heads, kv_heads, head_width, max_chunk,
-                                                  max_seq_len)
+    return lib.b2_paged_chunk_kv4_workspace_bytes(_u32(n_seq, "sequences"), _u32(n_tokens, "tokens"),
+                                                  _u32(q_heads, "query heads"), _u32(kv_heads, "KV heads"),
+                                                  _u32(head_width, "head width"), _u32(max_chunk, "max_chunk"),
+                                                  _u32(max_seq_len, "max_seq_len"))
 
 
 def paged_chunk_attention_kv4(queries: torch.Tensor, pool: PagedKv4Pool, block_tables: torch.Tensor,
@@ -218,6 +231,8 @@ def paged_chunk_attention_kv4(queries: torch.Tensor, pool: PagedKv4Pool, block_t
     """Several new tokens per sequence, already appended: queries [n_tokens, q_heads, d] FP32 and
     ``context_bf16`` the same in bf16, ``chunk_starts`` [n_seq + 1] the first row of each sequence's
     tokens, ``prefix_lens`` [n_seq] how much of a sequence is seen from all of it."""
+    _u32(max_chunk, "max_chunk")
+    _u32(max_seq_len, "max_seq_len")
     cache = pool.struct(block_tables)
     device = pool.device_index
     if queries.dim() != 3:
