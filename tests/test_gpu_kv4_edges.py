@@ -374,36 +374,88 @@ def test_window_under_the_largest_bound(given):
         assert int(status.item()) == 0 and rel_l2(out.cpu().numpy(), want) <= F32_TOL
 
 
-# ---- padding tokens -----------------------------------------------------------------------------
+# ---- forms that the other tests reach at one width only ----------------------------------------
 
-@pytest.mark.parametrize("d", [64, 128, 256])
-@pytest.mark.parametrize("live,padded", [(1, 64), (37, 300), (700, 1400)])
-def test_append_buffers_may_end_before_the_padding(d, live, padded):
-    """Nothing of a padding token is read or written: its rows of q, k and v need not be there. The call goes through the C
-    entry, since the Python one asks for whole tensors; what follows the live rows here belongs to this test, and keeps
-    its pattern."""
+RULES = [dict(softcap=5.0), dict(bias=True), dict(softcap=20.0, window=40, bias=True), dict(window=33)]
+
+
+@pytest.mark.parametrize("d", [64, 256])
+@pytest.mark.parametrize("hq", [2, 8, 16])
+@pytest.mark.parametrize("rules", RULES)
+def test_decode_score_rules_at_other_widths(rules, hq, d):
+    case = kv4_cases.Case(101, [1, 16, 33, 700, 3000], hq, 2, d, 16)
+    out, status = decode(case, **rules)
+    rules = dict(rules)
+    if rules.pop("bias", False):
+        rules["slopes"] = case.slopes
+    assert status == 0
+    assert rel_l2(out, case.decode(**rules)) <= F32_TOL
+
+
+@pytest.mark.parametrize("new,past", [([5, 2], [90, 20]), ([150, 260], [33, 0]), ([4], [5000])])
+@pytest.mark.parametrize("rules", RULES + [dict(prefix=[70, 10])])
+def test_chunk_score_rules_with_heads_of_64(rules, new, past):
+    rules = dict(rules)
+    if "prefix" in rules:
+        rules["prefix"] = rules["prefix"][:len(new)]
+    case = kv4_cases.Case(102, [p + m for p, m in zip(past, new)], 4, 2, 64, 16, rows=sum(new))
+    for tiles, tolerance in ((True, BF16_TOL), (False, ROW_TOL)):
+        if not tiles and sum(new) > 16:
+            continue
+        out, status = chunk(case, new, tiles=tiles, **rules)
+        plain = dict(rules)
+        if plain.pop("bias", False):
+            plain["slopes"] = case.slopes
+        assert status == 0
+        assert rel_l2(out, case.chunk(new, **plain)) <= tolerance
+
+
+@pytest.mark.parametrize("hq", [4, 7])
+def test_decode_of_more_rows_than_a_cta_looks_through(hq):
+    lens = [1 + i % 37 for i in range(1100)]
+    lens[7], lens[500], lens[1099] = 2000, 0, 901
+    case = kv4_cases.Case(103, lens, hq, 1, 128, 16)
+    out, status = decode(case)
+    assert status == 0
+    assert rel_l2(out, case.decode()) <= F32_TOL
+
+
+@pytest.mark.parametrize("d,hq,hkv,new,past", [(128, 32, 8, [5, 3, 4], [2000, 1500, 900]), (128, 16, 8, [300], [1000]),
+                                               (64, 8, 2, [40, 7], [3000, 100]), (256, 16, 4, [150], [2000])])
+def test_a_call_repeats_itself_bit_for_bit(d, hq, hkv, new, past):
+    """Partial results are joined in a fixed order, with no atomics on values."""
+    case = kv4_cases.Case(104, [p + m for p, m in zip(past, new)], hq, hkv, d, 16, rows=sum(new))
+    for rules in (dict(), dict(softcap=30.0, bias=True)):
+        first, _ = chunk(case, new, **rules)
+        for _ in range(3):
+            assert (chunk(case, new, **rules)[0] == first).all()
+    rows, case.q = case.q, case.q[:len(new)]
+    first, _ = decode(case)
+    for _ in range(3):
+        assert (decode(case)[0] == first).all()
+    case.q = rows
+
+
+def test_arena_growth_is_refused_inside_a_capture():
+    """Without a workspace a call that needs more than the library's arena holds is refused while its stream is captured;
+    nothing of it is enqueued, and the capture goes on. (The bound below asks for 7 GB, which is never allocated.)"""
     import riftco_transformer_b200 as b2
-    from riftco_transformer_b200 import _lib
-    rng = np.random.default_rng(live)
-    hq, hkv, bs = 4, 2, 16
-    blocks = -(-live // bs)
-    q = rng.standard_normal((live, hq, d)).astype(np.float32)
-    k, v = (rng.standard_normal((live, hkv, d)).astype(np.float32) for _ in range(2))
-    tables, owner = cuda(np.arange(blocks, dtype=np.uint32)[None]), cuda(np.zeros(padded, np.uint32))
-    positions = cuda(np.concatenate((np.arange(live), np.full(padded - live, 0xFFFFFFFF))).astype(np.uint32))
-
-    def append(n, behind):
-        """The pool's bytes and the rotated queries, from buffers of the live rows and `behind` floats."""
-        pool = b2.PagedKv4Pool(torch.zeros((blocks, hkv, 1, 18 * d), dtype=torch.uint8, device="cuda"), bs, d)
-        held = [cuda(np.concatenate((x.ravel(), np.full(behind, np.nan, np.float32)))) for x in (q, k, v)]
-        status, struct = status_word(), pool.struct(tables)
-        code = _lib.lib.b2_rope_append_kv4(C.byref(struct), held[0].data_ptr(), held[0].data_ptr(), held[1].data_ptr(),
-                                           held[2].data_ptr(), positions.data_ptr(), owner.data_ptr(), n, hq, 1e4,
-                                           status.data_ptr(), torch.cuda.current_stream().cuda_stream)
-        torch.cuda.synchronize()
-        assert code == 0 and int(status.item()) == 0
-        assert all(bool(x[x.numel() - behind:].isnan().all()) for x in held)
-        return pool.pages, held[0][:q.size]
-    want_pages, want_q = append(live, 0)
-    pages, turned = append(padded, 64)
-    assert torch.equal(pages, want_pages) and torch.equal(turned, want_q)
+    d, bs = 64, 1 << 20
+    pool = b2.PagedKv4Pool(torch.zeros((1, 1, bs // 16, 18 * d), dtype=torch.uint8, device="cuda"), bs, d)
+    tables = torch.zeros((8, 2048), dtype=torch.int32, device="cuda")
+    q, lens = torch.randn((8, 4, d), device="cuda"), torch.full((8,), 30, dtype=torch.int32, device="cuda")
+    ctx = torch.full_like(q, float("nan"))
+    assert b2.paged_decode_kv4_workspace_bytes(8, 4, 1, d, 0x7FFFFFFF) > 1 << 32
+    b2.paged_decode_attention_kv4(q, pool, tables, lens, ctx, 30)
+    ctx.fill_(float("nan"))
+    refused, graph = None, torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        b2.paged_decode_attention_kv4(q, pool, tables, lens, ctx, 30)
+        try:
+            b2.paged_decode_attention_kv4(q, pool, tables, lens, ctx, 0x7FFFFFFF)
+        except ValueError as e:
+            refused = str(e)
+    assert refused is not None and "stream capture" in refused
+    graph.replay()
+    torch.cuda.synchronize()
+    assert bool((ctx == 0).all())   # pages of zeros hold zeros
