@@ -160,11 +160,11 @@ __device__ __forceinline__ void bulk_load(uint32_t dst32, const void* src, uint3
                  : "memory");
 }
 
-// One thread of the grid: chunks that end behind the call's rows are flagged (chunk_starts rises, its last entry tells).
-__device__ __forceinline__ void check_chunk_starts(const Kv4AttentionArgs& a) {
-    if (blockIdx.x == 0u && threadIdx.x == 0u && a.chunk_starts != nullptr && __ldg(a.chunk_starts + a.cache.n_seq) > a.rows) {
-        kv4_flag(a.status, B2_ATTN_STATUS_BAD_BLOCK);
-    }
+// For one thread of the grid: BAD_BLOCK where chunks end behind the call's rows (chunk_starts rises, its last entry tells).
+// The caller raises it at its end, so that nobody waits for the load.
+__device__ __forceinline__ uint32_t chunk_starts_flag(const Kv4AttentionArgs& a) {
+    if (blockIdx.x != 0u || threadIdx.x != 0u || a.chunk_starts == nullptr) return 0u;
+    return __ldg(a.chunk_starts + a.cache.n_seq) > a.rows ? B2_ATTN_STATUS_BAD_BLOCK : 0u;
 }
 
 // What a row sees: tokens [begin, end) of sequence `seq`, its own position, and whether the caller's

@@ -402,7 +402,7 @@ kv4_chunk_kernel(const Kv4AttentionArgs a, float* __restrict__ partials, const C
     extern __shared__ __align__(1024) uint8_t smem_raw[];
     __shared__ __align__(8) Barriers bars;
 
-    check_chunk_starts(a);
+    const uint32_t starts_flag = chunk_starts_flag(a);
     const uint32_t rep = a.q_heads / a.cache.kv_heads;
     uint32_t block = blockIdx.x;
     const uint32_t split = block % plan.splits;
@@ -413,7 +413,10 @@ kv4_chunk_kernel(const Kv4AttentionArgs a, float* __restrict__ partials, const C
     // the last rows see the most tokens: they start first
     const uint32_t row0 = (plan.row_tiles - 1u - block / a.cache.n_seq) * kRows;
     const TileSpan span = tile_span(a, seq, rep, row0, kRows);
-    if (row0 >= span.rows) return;
+    if (row0 >= span.rows) {
+        if (starts_flag != 0u) kv4_flag(a.status, starts_flag);
+        return;
+    }
     const uint32_t rows = min(kRows, span.rows - row0);
     const uint32_t tile0 = span.begin / kKv4Tile;
     const uint32_t tiles = span.end > span.begin ? (span.end - 1u) / kKv4Tile + 1u - tile0 : 0u;
@@ -435,7 +438,7 @@ kv4_chunk_kernel(const Kv4AttentionArgs a, float* __restrict__ partials, const C
     const uint32_t q32 = smem32, k32 = q32 + L::kQ, v32 = k32 + kStages * L::kKStage, raw32 = v32 + kStages * L::kVStage;
     const uint32_t tid = threadIdx.x, lane = tid & 31u, warp = tid >> 5;
     volatile uint32_t* abort = &bars.abort;
-    uint32_t flags = span.bad ? B2_ATTN_STATUS_BAD_BLOCK : 0u;
+    uint32_t flags = span.bad ? B2_ATTN_STATUS_BAD_BLOCK : starts_flag;
 
     if (warp == kIssueWarp) {
         if (lane == 0) {

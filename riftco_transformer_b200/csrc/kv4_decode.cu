@@ -186,7 +186,7 @@ __global__ void __launch_bounds__(kWarps * 32, ctas_of(D, HC))
 kv4_decode_kernel(const Kv4AttentionArgs a, ListParts* __restrict__ list_parts, float* __restrict__ partials, const WorkPlan plan) {
     using namespace sm100;
     pdl_launch_dependents();
-    check_chunk_starts(a);
+    uint32_t flags = chunk_starts_flag(a);
     constexpr int G = D / 64, kChunks = D / 32;
     constexpr int HL = HC / 4;            // heads of a lane in the score layout
     constexpr uint32_t kTileBytes = kv4_tile_bytes(D);
@@ -250,7 +250,10 @@ kv4_decode_kernel(const Kv4AttentionArgs a, ListParts* __restrict__ list_parts, 
         __syncthreads();
         total = all * row_lists;
         ctas = live_ctas(plan, a.rows * row_lists, total);
-        if (blockIdx.x >= ctas) return;
+        if (blockIdx.x >= ctas) {
+            if (flags != 0u) kv4_flag(a.status, flags);
+            return;
+        }
         at = first_pair(blockIdx.x, total, ctas);
         at_end = first_pair(blockIdx.x + 1u, total, ctas);
         uint32_t lo = 0, hi = a.rows;   // the row with s_rows[row] * row_lists <= at < s_rows[row + 1] * row_lists
@@ -264,7 +267,6 @@ kv4_decode_kernel(const Kv4AttentionArgs a, ListParts* __restrict__ list_parts, 
     const uint32_t ring32 = smem_u32(ring_raw) + warp * (kSlots * kPairBytes);
     uint32_t used = 0;      // pairs this warp has taken through its ring
     uint32_t segment = 0;   // lists this CTA has begun
-    uint32_t flags = 0;
     while (at < at_end) {
     // ---- the next list of the range: its pairs [pair0, pair1) of `pairs` ----
     const uint32_t row_first = plan.whole_lists != 0u ? 0u : s_rows[row] * row_lists;
