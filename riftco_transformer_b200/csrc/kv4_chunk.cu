@@ -24,7 +24,7 @@
 // (N = 64 reads Q faster than it multiplies) and the exponentials 512 of the 16-per-cycle unit, that is 1312 and 1024
 // for the CTA. A row tile has two S buffers, so that the next scores are made while these are weighed: with blocks of
 // 128 tokens, whose S and O fill tensor memory, softmax and products of a tile took turns and a 4096-token prompt
-// 203 us, when it took 179 as it is (now 163 to 174, by clock).
+// 203 us, when it took 179 as it is (now 163 to 178, by clock and card).
 //
 // With heads of 256 there is one row tile (128 rows): O takes 256 columns of tensor memory and Q, as A operand of the
 // first product, 128, since shared memory holds only two stages of K and V of that width. The second tile's softmax warps

@@ -26,7 +26,7 @@
 // the second part costs nothing) or in a second instruction (five to eight heads). Scores, softmax statistics and
 // accumulators are FP32, and the result agrees with FP32 arithmetic to about 1e-6.
 //
-// HBM is the floor: 9d/8 bytes per token and K/V head against 8d of the FP32 cache. What bounds it is instructions: 335
+// HBM is the floor: 9d/8 bytes per token and K/V head against 8d of the FP32 cache. What bounds it is instructions: 330
 // for 16 tokens of a K/V head at d = 128, issued in 59% of the cycles (16 warps an SM, each a chain of its own; 20 warps
 // spill). One sequence of 131071 tokens at 32 / 8 heads takes 43 us (3.5 TB/s), the loads alone 30 us. mma.sync rather
 // than tcgen05: a row tile has at most 8 live rows, M = 64 or 128 would be idle lanes, and the operands come from

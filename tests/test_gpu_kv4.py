@@ -1,8 +1,8 @@
 """The 4-bit paged K/V cache on the GPU: append, read-back and attention against the numpy restatement
 (bytes exactly, attention in 64 bits).
 
-Tolerances. FP32 contexts: each product of q (two fp16 parts, 2^-22) with exact codes is summed in FP32,
-so a score is off by about 2^-22 * sum |q k| / sqrt(d), with sums around 40 here 1e-5; a weight is off by
+Tolerances. FP32 contexts: each product of q (integers, off by at most 2^-22 of their head's largest) with
+exact codes is summed in FP32, so a score is off by about 2^-22 * sum |q k| / sqrt(d), with sums around 40 here 1e-5; a weight is off by
 as much relative to itself, and the context by at most twice that relative to the values it averages:
 rel-L2 2e-5. bf16 contexts: half a step of the rounding, 2^-8 of each value, and the fp16 operands of the
 tile kernel, 2^-11 on keys, queries, weights and values: a score of up to 16 then moves by up to
