@@ -394,7 +394,8 @@ B2_API int32_t b2_paged_decode_attention_kv4(const b2_kv4_cache* cache, const b2
  * them is seq_lens[s]; chunk_starts is uint32[n_seq + 1], rising. The token at
  * position p sees t < max(p + 1, prefix_lens[s]) (prefix_lens may be NULL: causal;
  * a prefix is seen from anywhere in it, the window and the sequence's end still
- * apply). max_chunk and max_seq_len bound the chunk lengths and seq_lens. The
+ * apply). max_chunk and max_seq_len bound the chunk lengths and seq_lens; max_chunk is
+ * at most n_tokens and max_seq_len. The
  * context is written in bf16, the form the output projection reads
  * (b2_nf4_linear_forward_multi_bf16). Rows behind chunk_starts[n_seq] are left as
  * they were; a chunk longer than its sequence is flagged BAD_BLOCK and the

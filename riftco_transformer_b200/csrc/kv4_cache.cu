@@ -6,9 +6,9 @@
 // A group of 64 channels x of a rotated key or of a value is stored as
 //   base = f16(min x)   scale = f16((max x - base) / 15)   code = clamp(rint((x - base) * (1 / scale)), 0, 15)
 // in FP32, every operation rounded to nearest even. Codes are 0 where scale is 0, a constant group, or below 0, where
-// base was rounded up past all of a nearly constant one. The codes are taken against the ROUNDED base and scale, the ones a reader uses, so that rounding them to
-// 11 bits costs at most 15 * scale * 2^-11 at the top of the range, 1/137 of a step, instead of adding
-// to the error of every value. A group that holds a NaN or an infinity, or a magnitude above 65000
+// base was rounded up past all of a nearly constant one. The codes are taken against the ROUNDED base and scale, the ones
+// a reader uses, so that rounding them to 11 bits costs at most 15 * scale * 2^-11 at the top of the range, 1/137 of a
+// step, instead of adding to the error of every value. A group that holds a NaN or an infinity, or a magnitude above 65000
 // (fp16 spans 65504), is stored as scale = base = NaN: it reads back as NaN and the attention over it reports it.
 #include "kv4.cuh"
 #include "sm100_ptx.cuh"
